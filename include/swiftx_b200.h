@@ -412,6 +412,54 @@ int64_t swx_embedding_args_size(void);
 int64_t swx_embedding_bwd_workspace_bytes(int64_t ntok, int64_t vocab, int64_t dim);
 int swx_embedding_bwd(const swx_embedding_args* args, void* stream);
 
+/* Softmax cross entropy of a linear head, without keeping the (tokens, vocab) logits.
+ * It stands in for the head product followed by F.cross_entropy in the language model's
+ * training forward (models/sift_model.py:107-113):
+ *   logit[t, v] = x[t, :] . weight[v, :]
+ *   loss[t] = log(sum_v exp(logit[t, v])) - logit[t, targets[t]],  0 where targets[t] ==
+ *             ignore_index;  reduced by `reduction` (the mean over the tokens that count)
+ * x: (tokens, dim) with row stride x_sr, weight: (vocab, dim) with row stride w_sr, both in
+ * dtype (fp32 or bf16), unit element stride; targets: (tokens,) int64.  Products are summed
+ * in fp32 (fp32 operands as three bf16 pieces, about 2^-23 relative), the softmax
+ * statistics are fp32.  A target outside [0, vocab) that is not ignore_index makes its loss,
+ * and the gradients that it enters, NaN.  Values of x in ignored rows have to be finite
+ * (their products with a zero coefficient enter dweight).
+ * Forward writes loss (tokens values for SWX_XENT_NONE, else one), count (one value, the
+ * tokens that count; not for SWX_XENT_NONE), and row_max, row_rsum (tokens values) for the
+ * backward.  Backward: dloss (as loss) -> dx (tokens, dim) dense in dtype and dweight
+ * (vocab, dim) dense in dw_dtype; either may be NULL.  The vocabulary is walked in pieces;
+ * every sum runs in a fixed order (deterministic).  With no tokens a mean is NaN. */
+#define SWX_XENT_NONE 0
+#define SWX_XENT_MEAN 1
+#define SWX_XENT_SUM 2
+typedef struct swx_xent_args {
+    int64_t tokens, vocab, dim;
+    int32_t dtype;                    /* x, weight, dx: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t dw_dtype;                 /* dweight: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t reduction;                /* SWX_XENT_* */
+    int32_t reserved;
+    int64_t ignore_index;
+    const void* x; int64_t x_sr;
+    const void* weight; int64_t w_sr;
+    const int64_t* targets;
+    float* loss;
+    float* count;
+    float* row_max;
+    float* row_rsum;
+    const float* dloss;               /* backward */
+    void* dx;
+    void* dweight;
+    void* workspace; int64_t workspace_bytes;
+} swx_xent_args;
+
+int64_t swx_xent_args_size(void);
+/* Scratch bytes of the two calls for these sizes, types, strides and x / weight addresses;
+ * a negated status code for arguments that the calls refuse. */
+int64_t swx_xent_fwd_workspace_bytes(const swx_xent_args* args);
+int64_t swx_xent_bwd_workspace_bytes(const swx_xent_args* args);
+int swx_xent_fwd(const swx_xent_args* args, void* stream);
+int swx_xent_bwd(const swx_xent_args* args, void* stream);
+
 /* Diagnostic: y[i] = 2^x[i] computed by the FMA-pipe exponential the scan backward uses
  * for part of its decays (a degree-5 minimax polynomial after rounding x to an integer
  * part; x clamped to [-125, 127]), so its accuracy can be checked on the device.  x, y:

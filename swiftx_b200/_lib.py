@@ -118,6 +118,20 @@ class EmbeddingArgs(ctypes.Structure):
     ]
 
 
+XENT_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
+class XentArgs(ctypes.Structure):
+    """Mirror of ``swx_xent_args``."""
+    _fields_ = [
+        ("tokens", i64), ("vocab", i64), ("dim", i64),
+        ("dtype", i32), ("dw_dtype", i32), ("reduction", i32), ("reserved", i32), ("ignore_index", i64),
+        ("x", vp), ("x_sr", i64), ("weight", vp), ("w_sr", i64), ("targets", vp),
+        ("loss", vp), ("count", vp), ("row_max", vp), ("row_rsum", vp),
+        ("dloss", vp), ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 _lib = None
 
 
@@ -136,7 +150,8 @@ def load():
     lib.swx_status_string.argtypes = [ctypes.c_int]
     for fn, st in (("swx_scan_args_size", ScanArgs), ("swx_conv_args_size", ConvArgs),
                    ("swx_decode_args_size", DecodeArgs), ("swx_linear_scan_args_size", LinearScanArgs),
-                   ("swx_rmsnorm_args_size", RMSNormArgs), ("swx_embedding_args_size", EmbeddingArgs)):
+                   ("swx_rmsnorm_args_size", RMSNormArgs), ("swx_embedding_args_size", EmbeddingArgs),
+                   ("swx_xent_args_size", XentArgs)):
         getattr(lib, fn).restype = i64
         if getattr(lib, fn)() != ctypes.sizeof(st):
             raise RuntimeError(f"{st.__name__} layout mismatch between the library and its binding")
@@ -151,7 +166,8 @@ def load():
                      ("swx_conv1d_bwd", ConvArgs), ("swx_decode_step", DecodeArgs),
                      ("swx_linear_scan_fwd", LinearScanArgs), ("swx_linear_scan_bwd", LinearScanArgs),
                      ("swx_rmsnorm_fwd", RMSNormArgs), ("swx_rmsnorm_bwd", RMSNormArgs),
-                     ("swx_embedding_bwd", EmbeddingArgs)):
+                     ("swx_embedding_bwd", EmbeddingArgs),
+                     ("swx_xent_fwd", XentArgs), ("swx_xent_bwd", XentArgs)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(st), vp]
@@ -175,6 +191,9 @@ def load():
     lib.swx_rmsnorm_bwd_workspace_bytes.argtypes = [i64]
     lib.swx_embedding_bwd_workspace_bytes.restype = i64
     lib.swx_embedding_bwd_workspace_bytes.argtypes = [i64, i64, i64]
+    for fn in ("swx_xent_fwd_workspace_bytes", "swx_xent_bwd_workspace_bytes"):
+        getattr(lib, fn).restype = i64
+        getattr(lib, fn).argtypes = [ctypes.POINTER(XentArgs)]
     lib.swx_conv1d_bwd_workspace_bytes.restype = i64
     lib.swx_conv1d_bwd_workspace_bytes.argtypes = [i64, i64, i64, i64]
     _lib = lib

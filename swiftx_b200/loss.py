@@ -1,0 +1,111 @@
+"""Softmax cross entropy of the language model's head without its logits.
+
+The reference's training forward multiplies the final norm's output with the head's weight
+and hands the fp32 logits to ``F.cross_entropy`` (models/sift_model.py:103-113): two
+(tokens, vocab) tensors, and a third for their gradient.  ``linear_cross_entropy`` computes
+the same loss and gradients from the two operands; it keeps two floats per token, and one
+piece of the vocabulary's logit gradients while the backward runs.
+"""
+import torch
+
+from . import _lib
+
+_DT = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _rows(t):
+    """(n, d) with unit element stride and non-overlapping rows (a copy otherwise)."""
+    return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _args(x, w, targets, ignore_index, reduction):
+    a = _lib.XentArgs()
+    a.tokens, a.dim, a.vocab = x.shape[0], x.shape[1], w.shape[0]
+    a.dtype, a.reduction, a.ignore_index = _DT[x.dtype], reduction, ignore_index
+    a.x, a.x_sr = x.data_ptr(), x.stride(0)
+    a.weight, a.w_sr = w.data_ptr(), w.stride(0)
+    a.targets = targets.data_ptr()
+    return a
+
+
+def _workspace(lib, name, a, device):
+    n = getattr(lib, name)(a)
+    if n < 0:
+        _lib.check(-n, name)
+    ws = torch.empty(max(n, 1), device=device, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    return ws
+
+
+class LinearCrossEntropyFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, ignore_index, reduction):
+        w = weight if weight.dtype == x.dtype else weight.to(x.dtype)
+        x, w, targets = _rows(x), _rows(w), targets.contiguous()
+        none = reduction == _lib.XENT_REDUCTIONS["none"]
+        with torch.cuda.device(x.device):
+            lib = _lib.load()
+            new = lambda *s: torch.empty(s, device=x.device, dtype=torch.float32)  # noqa: E731
+            T = x.shape[0]
+            loss, count, stats = new(T) if none else new(), new(1), new(2, T)
+            a = _args(x, w, targets, ignore_index, reduction)
+            a.loss, a.count, a.row_max, a.row_rsum = loss.data_ptr(), count.data_ptr(), stats[0].data_ptr(), stats[1:].data_ptr()
+            ws = _workspace(lib, "swx_xent_fwd_workspace_bytes", a, x.device)  # noqa: F841
+            _lib.check(lib.swx_xent_fwd(a, _lib.stream_ptr(x.device)), "swx_xent_fwd")
+        ctx.save_for_backward(x, w, targets, stats, count)
+        ctx.opts = (ignore_index, reduction, weight.dtype)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dloss):
+        x, w, targets, stats, count = ctx.saved_tensors
+        ignore_index, reduction, w_dtype = ctx.opts
+        dloss = dloss.float().contiguous()
+        with torch.cuda.device(x.device):
+            lib = _lib.load()
+            dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
+            dw = torch.empty(w.shape, device=x.device, dtype=w_dtype) if ctx.needs_input_grad[1] else None
+            a = _args(x, w, targets, ignore_index, reduction)
+            a.count, a.row_max, a.row_rsum = count.data_ptr(), stats[0].data_ptr(), stats[1:].data_ptr()
+            a.dw_dtype, a.dloss = _DT[w_dtype], dloss.data_ptr()
+            a.dx = dx.data_ptr() if dx is not None else None
+            a.dweight = dw.data_ptr() if dw is not None else None
+            ws = _workspace(lib, "swx_xent_bwd_workspace_bytes", a, x.device)  # noqa: F841
+            _lib.check(lib.swx_xent_bwd(a, _lib.stream_ptr(x.device)), "swx_xent_bwd")
+        return dx, dw, None, None, None
+
+
+def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
+    """``F.cross_entropy(F.linear(x, weight).float(), targets)`` without the logits (CUDA only).
+
+    x (..., d) and weight (vocab, d), fp32 or bf16; targets (...) int64.  Returns the fp32
+    loss: its mean over the tokens that count, their sum, or (reduction "none") one value
+    for each token, 0 at ignored ones.  bf16 operands give the products of bf16 values summed in
+    fp32; fp32 operands keep fp32 accuracy.  With bf16 x an fp32 weight is rounded to bf16 for
+    the products (what autocast's linear does) and its gradient comes back in fp32, not
+    rounded; under bf16 autocast an fp32 x is cast too.  The gradients are deterministic.
+
+    A target outside [0, vocab) other than ignore_index gives a NaN loss (and gradients)
+    instead of a device-side assertion; x has to be finite in ignored rows too."""
+    if reduction not in _lib.XENT_REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction {reduction!r}: one of none, mean, sum expected")
+    if not (x.is_cuda and weight.is_cuda and targets.is_cuda):
+        raise RuntimeError("swiftx_b200 linear_cross_entropy runs on CUDA tensors only (no CPU path)")
+    if x.device != weight.device or x.device != targets.device:
+        raise ValueError(f"linear_cross_entropy: tensors on {x.device}, {weight.device} and {targets.device}")
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise ValueError(f"linear_cross_entropy: x (..., d) and weight (vocab, d) expected, got {tuple(x.shape)} "
+                         f"and {tuple(weight.shape)}")
+    if targets.dtype != torch.int64 or targets.shape != x.shape[:-1]:
+        raise ValueError(f"linear_cross_entropy: int64 targets of shape {tuple(x.shape[:-1])} expected, got "
+                         f"{targets.dtype} {tuple(targets.shape)}")
+    if x.dtype == torch.float32 and torch.is_autocast_enabled("cuda") \
+            and torch.get_autocast_dtype("cuda") == torch.bfloat16:
+        x = x.to(torch.bfloat16)
+    if x.dtype not in _DT or weight.dtype not in _DT or (x.dtype == torch.float32 and weight.dtype != torch.float32):
+        raise ValueError(f"linear_cross_entropy: fp32 x and weight, or bf16 x with a bf16 or fp32 weight expected, got "
+                         f"{x.dtype} and {weight.dtype}")
+    loss = LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, targets.reshape(-1), int(ignore_index),
+                                      _lib.XENT_REDUCTIONS[reduction])
+    return loss.view(targets.shape) if reduction == "none" else loss
