@@ -64,6 +64,9 @@ struct XentGemm {
     const float* dloss; int reduction;
     int planes;                               // bf16 pieces of the dlogit
     // XE_DX / XE_DW
+    // spread: the steps of all tiles are dealt out evenly and a tile's parts are summed in
+    // acc[part][M][N]; else whole tiles go round and the last piece writes the result
+    int spread;
     float* acc; void* out; int out_bf16; int64_t ld; int first, last;
     const float* scale_num; const float* scale_den;   // the result's factor: num / den, either may be absent
 };
@@ -76,6 +79,47 @@ __device__ __forceinline__ int2 piece_pair(int npair, int i) {
     constexpr uint32_t B = 0u | 1u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
     return make_int2((A >> (2 * i)) & 3, (B >> (2 * i)) & 3);
 }
+
+// The work of one CTA pair: runs of contraction steps [k0, k1) of a tile, each summed in one
+// accumulator.  Whole tiles go round the pairs; spread, pair c takes the steps
+// [c S / P, (c + 1) S / P) of the S steps of all tiles, so that a tile can have several parts
+// (numbered from the pair that has the tile's first step).
+struct XentRuns {
+    int64_t cur, end, tile;
+    int nk, ksub, P, k0, k1, part;
+    bool spread, fresh;
+    __device__ __forceinline__ XentRuns(const XentGemm& p, int64_t c, int64_t P_) : nk(p.nk), ksub(p.ksub), P((int)P_), part(0), spread(p.spread) {
+        const int64_t tiles = (int64_t)p.mt * p.nt;
+        cur = spread ? c * (tiles * nk) / P : c;
+        end = spread ? (c + 1) * (tiles * nk) / P : tiles;
+        k1 = nk;
+        fresh = true;
+        tile = -1;
+    }
+    __device__ __forceinline__ bool next(const XentGemm& p) {
+        if (cur >= end) return false;
+        if (spread) {
+            const int64_t t = cur / nk;
+            k0 = (int)(cur - t * nk);
+            k1 = (int)min((int64_t)min(nk, k0 + ksub), k0 + (end - cur));
+            fresh = t != tile;
+            if (fresh) {
+                const int64_t total = (int64_t)p.mt * p.nt * nk;
+                const int64_t c = ((cur + 1) * P - 1) / total, lo = ((t * nk + 1) * P - 1) / total;
+                part = (int)(c - lo);
+            }
+            tile = t;
+            cur += k1 - k0;
+        } else {
+            tile = cur;
+            k0 = k1 < nk ? k1 : 0;
+            fresh = k0 == 0;
+            k1 = min(k0 + ksub, nk);
+            if (k1 == nk) cur += P;
+        }
+        return true;
+    }
+};
 
 // Tile t -> (row tile, column tile).  XE_LSE, XE_PROB: `group` row tiles of x stay in L2
 // while the weight's column tiles pass by; the gradients: a row tile's column tiles together.
@@ -114,7 +158,6 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = cluster_rank();
     const int64_t cluster = blockIdx.x / 2, nclusters = gridDim.x / 2;
-    const int64_t ntiles = (int64_t)p.mt * p.nt;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < XE_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
@@ -136,14 +179,12 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             uint32_t ph = 0;
             int64_t issued = 0;
             bool ok = true;
-            for (int64_t t = cluster; ok && t < ntiles; t += nclusters) {
-                const int2 rc = tile_of<EPI>(p, t);
+            for (XentRuns r(p, cluster, nclusters); ok && r.next(p);) {
+                const int2 rc = tile_of<EPI>(p, r.tile);
                 const int am = p.a0 + rc.x * XE_TILE + (int)rank * 128, bn = p.b0 + rc.y * XE_TILE + (int)rank * 128;
-                for (int k0 = 0; ok && k0 < p.nk; k0 += p.ksub)
                 for (int i = 0; ok && i < p.npair; ++i) {
                     const int2 pl = piece_pair(p.npair, i);
-                    const int k1 = min(k0 + p.ksub, p.nk);
-                    for (int k = k0; k < k1; ++k) {
+                    for (int k = r.k0; k < r.k1; ++k) {
                         if (!mbar_wait_cluster(&empty[s], ph ^ 1, XE_POLLS)) { ok = false; break; }
                         if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * XE_STAGE);
                         const uint32_t bar = map_to_rank(&full[s], 0);
@@ -188,11 +229,10 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             int s = 0, a = 0;
             uint32_t ph = 0, aph = 0;
             bool ok = true;
-            for (int64_t t = cluster; ok && t < ntiles; t += nclusters)
-            for (int k0 = 0; ok && k0 < p.nk; k0 += p.ksub) {
+            for (XentRuns r(p, cluster, nclusters); ok && r.next(p);) {
                 if (!mbar_wait_cluster(&acc_empty[a], aph ^ 1, XE_POLLS)) { ok = false; break; }
                 tc_fence_after();
-                const int steps = min(p.ksub, p.nk - k0) * p.npair;
+                const int steps = (r.k1 - r.k0) * p.npair;
                 for (int i = 0; i < steps; ++i) {
                     if (!mbar_wait_cluster(&full[s], ph, XE_POLLS)) { ok = false; break; }
                     tc_fence_after();
@@ -222,10 +262,9 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             if (p.scale_num) factor = *p.scale_num;
             if (p.scale_den) factor = *p.scale_den > 0.f ? factor / *p.scale_den : 0.f;   // no token counts: no gradient
         }
-        for (int64_t t = cluster; ok && t < ntiles; t += nclusters)
-        for (int k0 = 0; k0 < p.nk; k0 += p.ksub) {
-            const bool first = p.first && k0 == 0, last = p.last && k0 + p.ksub >= p.nk;
-            const int2 rc = tile_of<EPI>(p, t);
+        for (XentRuns r(p, cluster, nclusters); r.next(p);) {
+            const bool first = p.first && r.fresh, last = p.last && !p.spread && r.k1 == p.nk;
+            const int2 rc = tile_of<EPI>(p, r.tile);
             const int row = rc.x * XE_TILE + (int)rank * 128 + sub * 32 + lane;
             const int c0 = rc.y * XE_TILE + half * 128;
             const bool live = row < p.M;
@@ -318,7 +357,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     }
                 } else if (live && cc < p.N) {
                     const int n = min(32, p.N - cc);
-                    float* acc = p.acc + (int64_t)row * p.N + cc;
+                    float* acc = p.acc + ((int64_t)r.part * p.M + row) * p.N + cc;
                     const bool whole = n == 32 && (reinterpret_cast<uintptr_t>(acc) & 15) == 0;
                     if (!first) {
                         if (whole) {
@@ -396,69 +435,136 @@ struct XentJoin {
     int64_t T, V;
     int np;                                   // pieces per row
     const float2* part; const float* hit; const int64_t* target; int64_t ignore;
-    float* row_max; float* row_rsum; float* rows;
+    float* row_max; float* row_rsum;
+    float* rows;                              // SWX_XENT_NONE: the losses
+    double2* sums;                            // otherwise: each CTA's sum and count
     float* loss; float* count; int reduction; int* counter;
 };
 
-constexpr int XJ_SLICES = 16;
+constexpr int XJ_ROWS = 8, XJ_SLICES = 32, XJ_WARPS = XJ_ROWS * XJ_SLICES / 32;
 
-// CTA = 32 rows x 16 slices of the pieces: each thread joins its slice, the slices are
-// joined in order through shared memory; the last CTA to finish sums the rows (fp64, a fixed
-// order whichever CTA it is).
-__global__ void __launch_bounds__(32 * XJ_SLICES) xent_join_kernel(const XentJoin p) {
-    __shared__ float2 sp[XJ_SLICES][32];
+__device__ __forceinline__ void join_pair(float& m, float& s, float2 q) {
+    const float nm = fmaxf(m, q.x), base = nm == -INFINITY ? 0.f : nm;
+    s = s * ex2((m - base) * LOG2E) + q.y * ex2((q.x - base) * LOG2E);
+    m = nm;
+}
+
+// CTA = 8 rows x 32 slices of the pieces (few rows per CTA, so that a short call still has
+// many CTAs): each thread joins its slice, four pieces at a time, then the slices are joined
+// by shuffles and through shared memory, always in the same order.  Each CTA leaves the sum of
+// its rows' losses and the count of its tokens; the last CTA to finish adds those up (fp64, a
+// fixed order whichever CTA it is).
+__global__ void __launch_bounds__(XJ_ROWS * XJ_SLICES) xent_join_kernel(const XentJoin p) {
+    __shared__ float2 sp[XJ_WARPS][XJ_ROWS];
     __shared__ int is_last;
-    __shared__ double red[32 * XJ_SLICES / 32][2];
-    const int lane = threadIdx.x % 32, sl = threadIdx.x / 32;
-    const int64_t row = (int64_t)blockIdx.x * 32 + lane;
+    __shared__ double red[XJ_WARPS][2];
+    const int r = threadIdx.x % XJ_ROWS, sl = threadIdx.x / XJ_ROWS, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int64_t row = (int64_t)blockIdx.x * XJ_ROWS + r;
     float m = -INFINITY, s = 0.f;
     if (row < p.T) {
-#pragma unroll 4
-        for (int i = sl; i < p.np; i += XJ_SLICES) {
-            const float2 q = p.part[(int64_t)i * p.T + row];
-            const float nm = fmaxf(m, q.x), base = nm == -INFINITY ? 0.f : nm;
-            s = s * ex2((m - base) * LOG2E) + q.y * ex2((q.x - base) * LOG2E);
+        for (int i = sl; i < p.np; i += 4 * XJ_SLICES) {
+            float2 q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                q[j] = i + j * XJ_SLICES < p.np ? p.part[(int64_t)(i + j * XJ_SLICES) * p.T + row] : make_float2(-INFINITY, 0.f);
+            const float nm = fmaxf(fmaxf(fmaxf(m, q[0].x), fmaxf(q[1].x, q[2].x)), q[3].x), base = nm == -INFINITY ? 0.f : nm;
+            s *= ex2((m - base) * LOG2E);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s += q[j].y * ex2((q[j].x - base) * LOG2E);
             m = nm;
         }
     }
-    sp[sl][lane] = make_float2(m, s);
+#pragma unroll
+    for (int o = XJ_ROWS; o < 32; o *= 2) {
+        const float2 q = make_float2(__shfl_down_sync(0xffffffffu, m, o), __shfl_down_sync(0xffffffffu, s, o));
+        join_pair(m, s, q);
+    }
+    if (lane < XJ_ROWS) sp[warp][lane] = make_float2(m, s);
     __syncthreads();
-    if (sl == 0 && row < p.T) {
-        for (int i = 1; i < XJ_SLICES; ++i) {
-            const float2 q = sp[i][lane];
-            const float nm = fmaxf(m, q.x), base = nm == -INFINITY ? 0.f : nm;
-            s = s * ex2((m - base) * LOG2E) + q.y * ex2((q.x - base) * LOG2E);
-            m = nm;
+    double sum = 0., n = 0.;
+    if (warp == 0) {
+        if (lane < XJ_ROWS && row < p.T) {
+            m = sp[0][lane].x;
+            s = sp[0][lane].y;
+#pragma unroll
+            for (int i = 1; i < XJ_WARPS; ++i) join_pair(m, s, sp[i][lane]);
+            p.row_max[row] = m;
+            p.row_rsum[row] = 1.f / s;
+            const int64_t y = p.target[row];
+            float loss = 0.f;
+            if (y != p.ignore) {
+                loss = y >= 0 && y < p.V ? logf(s) + (m - p.hit[row]) : __int_as_float(0x7fc00000);
+                n = 1.;
+            }
+            if (p.rows) p.rows[row] = loss;
+            sum = loss;
         }
-        p.row_max[row] = m;
-        p.row_rsum[row] = 1.f / s;
-        const int64_t y = p.target[row];
-        float loss = 0.f;
-        if (y != p.ignore) loss = y >= 0 && y < p.V ? logf(s) + (m - p.hit[row]) : __int_as_float(0x7fc00000);
-        p.rows[row] = loss;
+        for (int o = XJ_ROWS / 2; o > 0; o >>= 1) {
+            sum += __shfl_down_sync(0xffffffffu, sum, o);
+            n += __shfl_down_sync(0xffffffffu, n, o);
+        }
     }
     if (p.reduction == SWX_XENT_NONE) return;
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) is_last = atomicAdd(p.counter, 1) == (int)gridDim.x - 1;
+    if (threadIdx.x == 0) {
+        p.sums[blockIdx.x] = make_double2(sum, n);
+        __threadfence();
+        is_last = atomicAdd(p.counter, 1) == (int)gridDim.x - 1;
+    }
     __syncthreads();
     if (!is_last) return;
     __threadfence();
-    double sum = 0., n = 0.;
-    for (int64_t i = threadIdx.x; i < p.T; i += blockDim.x) {
-        sum += (double)__ldcg(p.rows + i);
-        n += p.target[i] != p.ignore ? 1. : 0.;
+    sum = n = 0.;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < (int)gridDim.x; i += XJ_ROWS * XJ_SLICES) {
+        const double2 q = __ldcg(p.sums + i);
+        sum += q.x;
+        n += q.y;
     }
     for (int o = 16; o > 0; o >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
         n += __shfl_xor_sync(0xffffffffu, n, o);
     }
-    if (lane == 0) { red[sl][0] = sum; red[sl][1] = n; }
+    if (lane == 0) { red[warp][0] = sum; red[warp][1] = n; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int i = 1; i < XJ_SLICES; ++i) { sum += red[i][0]; n += red[i][1]; }
+        for (int i = 1; i < XJ_WARPS; ++i) { sum += red[i][0]; n += red[i][1]; }
         *p.count = (float)n;
         *p.loss = (float)(p.reduction == SWX_XENT_MEAN ? sum / n : sum);
+    }
+}
+
+// ------------------------------------------------------------------ summing a tile's parts
+// out = factor * (parts in order), for the spread gradients; thread = 4 columns of a row.
+__global__ void __launch_bounds__(256) xent_sum_kernel(const XentGemm p, int P) {
+    const int per = (p.N + 3) / 4;
+    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i >= (int64_t)p.M * per) return;
+    const int row = (int)(i / per), c = (int)(i % per) * 4;
+    const int64_t tile = (int64_t)(row / XE_TILE) * p.nt + c / XE_TILE, total = (int64_t)p.mt * p.nt * p.nk;
+    const int parts = (int)((((tile + 1) * p.nk) * P - 1) / total - ((tile * p.nk + 1) * P - 1) / total) + 1;
+    float factor = 1.f;
+    if (p.scale_num) factor = *p.scale_num;
+    if (p.scale_den) factor = *p.scale_den > 0.f ? factor / *p.scale_den : 0.f;
+    const int n = min(4, p.N - c);
+    const float* a = p.acc + (int64_t)row * p.N + c;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    const bool vec = p.N % 4 == 0;
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k, a += (int64_t)p.M * p.N) {
+        if (vec) {
+            const float4 q = *reinterpret_cast<const float4*>(a);
+            v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) if (j < n) v[j] += a[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (j >= n) break;
+        const float o = v[j] * factor;
+        if (p.out_bf16) static_cast<__nv_bfloat16*>(p.out)[(int64_t)row * p.ld + c + j] = __float2bfloat16_rn(o);
+        else static_cast<float*>(p.out)[(int64_t)row * p.ld + c + j] = o;
     }
 }
 
@@ -493,13 +599,34 @@ __global__ void __launch_bounds__(256) xent_pack_kernel(const T* __restrict__ sr
 }
 
 // ------------------------------------------------------------------ host side
+// How a gradient product's tiles are dealt out to the CTA pairs of a 148-SM B200.  Whole
+// tiles where they keep the pairs busy for seven tenths of their rounds or more; otherwise the steps
+// are spread evenly, at least XE_MIN_SHARE per pair, and the parts of a tile (at most `parts`)
+// are summed afterwards.
+struct XentDeal { int spread, pairs, parts; };
+constexpr int XE_PAIRS = 74, XE_MIN_SHARE = 4;
+
+static XentDeal deal(int64_t tiles, int64_t nk) {
+    const int64_t rounds = (tiles + XE_PAIRS - 1) / XE_PAIRS, total = tiles * nk;
+    XentDeal d{0, (int)std::min<int64_t>(tiles, XE_PAIRS), 1};
+    if (tiles * 10 >= rounds * XE_PAIRS * 7) return d;
+    const int64_t P = std::min<int64_t>(XE_PAIRS, std::max<int64_t>(1, total / XE_MIN_SHARE));
+    if (P <= tiles && tiles % P == 0) return XentDeal{0, (int)P, 1};
+    d.spread = 1;
+    d.pairs = (int)P;
+    for (int64_t t = 0; t < tiles; ++t)
+        d.parts = std::max<int>(d.parts, (int)(((t + 1) * nk * P - 1) / total - ((t * nk + 1) * P - 1) / total) + 1);
+    return d;
+}
+
 struct XentPlan {
     int es, planes;                           // bytes of an input value; bf16 pieces
     int64_t dp;                               // padded contraction length of packed operands
     bool pack_x, pack_w;
     int64_t mt, nt, piece;                    // tiles; vocabulary columns per piece of the backward
     int64_t off_x, off_w, off_part, off_hit, off_rows, off_cnt, fwd_total;
-    int64_t off_p, off_acc, ldp, bwd_total;
+    int64_t off_p, off_acc, off_acc_w, ldp, bwd_total;
+    XentDeal dx;
 };
 
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
@@ -508,14 +635,16 @@ static bool direct_ok(const void* p, int64_t sr, int dtype) {
     return dtype == SWX_DTYPE_BF16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && sr % 8 == 0;
 }
 
-// Vocabulary columns per piece of the backward: the piece's dlogit (tokens x columns, 2 bytes
-// for each bf16 piece) is written once and read twice, so it is kept near 72 MB, which
-// stays in the 126 MB L2 beside the operands; with many tokens at least 4096 columns, so that
-// dx's running sum (read and written once per piece) stays small beside the products.
+// Vocabulary columns per piece of the backward: at most 416 MB of dlogit (tokens x columns,
+// 2 bytes for each bf16 piece).  The piece need not stay in the L2: its one write and two reads
+// hide behind the products, while fewer pieces mean fewer launches, fewer rounds that do not
+// fill the GPU and fewer passes over dx's running sum (8192 tokens x 50001 x 1024, forward
+// and backward: pieces of 72 MB 2.92 ms, 160 MB 2.83, 288 MB 2.67, 450 MB 2.61, one piece 2.56).
 static int64_t piece_columns(int64_t T, int64_t V, int planes) {
-    int64_t c = (int64_t(72) << 20) / (2 * planes * std::max<int64_t>(T, 1)) / 256 * 256;
+    int64_t c = (int64_t(416) << 20) / (2 * planes * std::max<int64_t>(T, 1)) / 256 * 256;
     c = std::max<int64_t>(c, 4096);
-    return std::min<int64_t>(c, up256(V));
+    const int64_t n = (V + c - 1) / c;        // pieces of nearly equal size
+    return up256((V + n - 1) / n);
 }
 
 static XentPlan xent_plan(const swx_xent_args* a) {
@@ -534,13 +663,25 @@ static XentPlan xent_plan(const swx_xent_args* a) {
     q.off_part = base;
     q.off_hit = q.off_part + up256(2 * q.nt * T * 8);
     q.off_rows = q.off_hit + up256(T * 4);
-    q.off_cnt = q.off_rows + up256(T * 4);
+    q.off_cnt = q.off_rows + up256((T + XJ_ROWS - 1) / XJ_ROWS * 16);
     q.fwd_total = q.off_cnt + 256;
     q.piece = piece_columns(T, V, q.planes);
     q.ldp = q.piece;
     q.off_p = base;
     q.off_acc = q.off_p + up256((int64_t)q.planes * T * q.ldp * 2);
-    q.bwd_total = q.off_acc + (a->dtype == SWX_DTYPE_BF16 && q.piece < V ? up256(T * d * 4) : 0);
+    // the running sums of dx (bf16 result: in fp32; one for each part of a spread tile), then
+    // the parts of dW, which live for one piece
+    const int64_t dt = (d + XE_TILE - 1) / XE_TILE;
+    const int64_t cl = V - (V - 1) / q.piece * q.piece;      // columns of the last piece
+    q.dx = deal(q.mt * dt, (std::min(q.piece, V) + XE_K - 1) / XE_K);
+    const bool own_acc = q.dx.spread || (a->dtype == SWX_DTYPE_BF16 && q.piece < V);
+    q.off_acc_w = q.off_acc + (own_acc ? up256(q.dx.parts * T * d * 4) : 0);
+    int64_t w = 0;
+    for (const int64_t cw : {std::min<int64_t>(q.piece, V), cl}) {
+        const XentDeal e = deal((cw + XE_TILE - 1) / XE_TILE * dt, (T + XE_K - 1) / XE_K);
+        if (e.spread) w = std::max<int64_t>(w, up256(e.parts * cw * d * 4));
+    }
+    q.bwd_total = q.off_acc_w + w;
     return q;
 }
 
@@ -585,15 +726,18 @@ static Operand operand(const void* src, int64_t sr, int64_t rows, int64_t d, int
 
 template <int EPI, bool A_MN, bool B_MN>
 static cudaError_t launch_gemm(const XentGemm& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mp,
-                               cudaStream_t st) {
+                               int64_t pairs, cudaStream_t st) {
     auto k = xent_gemm_kernel<EPI, A_MN, B_MN>;
     cudaError_t e = allow_smem(k, XE_SMEM);
     if (e != cudaSuccess) return e;
-    int sms = 0, per = 0;
-    e = sm_fit(k, XE_THREADS, XE_SMEM, &sms, &per);
-    if (e != cudaSuccess) return e;
-    const int64_t pairs = std::min<int64_t>((int64_t)p.mt * p.nt, std::max(1, sms / 2));
+    if (!p.spread) pairs = std::min<int64_t>((int64_t)p.mt * p.nt, pairs);
     k<<<(unsigned)(2 * pairs), XE_THREADS, XE_SMEM, st>>>(p, ma, mb, mp);
+    return cudaGetLastError();
+}
+
+static cudaError_t launch_sum(const XentGemm& p, int pairs, cudaStream_t st) {
+    const int64_t n = (int64_t)p.M * ((p.N + 3) / 4);
+    xent_sum_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(p, pairs);
     return cudaGetLastError();
 }
 
@@ -654,13 +798,13 @@ int swx_xent_fwd(const swx_xent_args* a, void* stream) {
     g.part = reinterpret_cast<float2*>(ws + q.off_part);
     g.hit = reinterpret_cast<float*>(ws + q.off_hit);
     g.counter = reinterpret_cast<int*>(ws + q.off_cnt);
-    if (launch_gemm<XE_LSE, false, false>(g, mx, mw, mx, st) != cudaSuccess) return SWX_ERR_CUDA;
+    if (launch_gemm<XE_LSE, false, false>(g, mx, mw, mx, XE_PAIRS, st) != cudaSuccess) return SWX_ERR_CUDA;
     XentJoin j{};
     j.T = a->tokens; j.V = a->vocab; j.np = (int)(2 * q.nt); j.part = g.part; j.hit = g.hit; j.target = a->targets;
     j.ignore = a->ignore_index; j.row_max = a->row_max; j.row_rsum = a->row_rsum;
-    j.rows = none ? a->loss : reinterpret_cast<float*>(ws + q.off_rows);
+    j.rows = none ? a->loss : nullptr; j.sums = reinterpret_cast<double2*>(ws + q.off_rows);
     j.loss = a->loss; j.count = a->count; j.reduction = a->reduction; j.counter = g.counter;
-    xent_join_kernel<<<(unsigned)((a->tokens + 31) / 32), 32 * XJ_SLICES, 0, st>>>(j);
+    xent_join_kernel<<<(unsigned)((a->tokens + XJ_ROWS - 1) / XJ_ROWS), XJ_ROWS * XJ_SLICES, 0, st>>>(j);
     return cudaGetLastError() == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
 }
 
@@ -704,17 +848,21 @@ int swx_xent_bwd(const swx_xent_args* a, void* stream) {
         g.nk = g.ksub = (int)((d + XE_K - 1) / XE_K); g.b0 = (int)c0;
         g.target = a->targets; g.ignore = a->ignore_index; g.col0 = (int)c0; g.vocab = V;
         g.row_max = a->row_max; g.row_rsum = a->row_rsum; g.dloss = a->dloss; g.reduction = a->reduction;
-        if (launch_gemm<XE_PROB, false, false>(g, x_k, w_k, p_st, st) != cudaSuccess) return SWX_ERR_CUDA;
+        if (launch_gemm<XE_PROB, false, false>(g, x_k, w_k, p_st, XE_PAIRS, st) != cudaSuccess) return SWX_ERR_CUDA;
         if (a->dx) {
             XentGemm h{};
             h.status = status; h.npair = npair;
             h.M = (int)T; h.N = (int)d; h.mt = (int)q.mt; h.nt = (int)((d + XE_TILE - 1) / XE_TILE);
-            h.nk = (int)((cw + XE_K - 1) / XE_K); h.ksub = q.planes == 3 ? XE_KSUB : h.nk; h.kb0 = (int)c0;
+            // every piece the same number of steps (a short last one reads zeros), so that a spread
+            // tile has the same parts in each
+            h.nk = (int)((std::min(q.piece, V) + XE_K - 1) / XE_K); h.ksub = q.planes == 3 ? XE_KSUB : h.nk; h.kb0 = (int)c0;
             h.scale_num = num; h.scale_den = den;
             h.first = c0 == 0; h.last = c0 + cw == V; h.out = a->dx; h.ld = d;
             h.out_bf16 = a->dtype == SWX_DTYPE_BF16;
-            h.acc = h.out_bf16 ? reinterpret_cast<float*>(ws + q.off_acc) : static_cast<float*>(a->dx);
-            if (launch_gemm<XE_DX, false, true>(h, p_k, w_mn, p_st, st) != cudaSuccess) return SWX_ERR_CUDA;
+            h.spread = q.dx.spread;
+            h.acc = h.out_bf16 || h.spread ? reinterpret_cast<float*>(ws + q.off_acc) : static_cast<float*>(a->dx);
+            if (launch_gemm<XE_DX, false, true>(h, p_k, w_mn, p_st, q.dx.pairs, st) != cudaSuccess) return SWX_ERR_CUDA;
+            if (h.spread && h.last && launch_sum(h, q.dx.pairs, st) != cudaSuccess) return SWX_ERR_CUDA;
         }
         if (a->dweight) {
             XentGemm h{};
@@ -725,8 +873,12 @@ int swx_xent_bwd(const swx_xent_args* a, void* stream) {
             h.first = h.last = 1; h.ld = d;
             h.out_bf16 = a->dw_dtype == SWX_DTYPE_BF16;
             h.out = static_cast<uint8_t*>(a->dweight) + c0 * d * (h.out_bf16 ? 2 : 4);
-            h.acc = static_cast<float*>(h.out);       // used with fp32 operands, whose gradient is fp32
-            if (launch_gemm<XE_DW, true, true>(h, p_mn, x_mn, p_st, st) != cudaSuccess) return SWX_ERR_CUDA;
+            const XentDeal e = deal((int64_t)h.mt * h.nt, h.nk);
+            h.spread = e.spread;
+            // whole tiles with fp32 operands sum up in the (fp32) result
+            h.acc = e.spread ? reinterpret_cast<float*>(ws + q.off_acc_w) : static_cast<float*>(h.out);
+            if (launch_gemm<XE_DW, true, true>(h, p_mn, x_mn, p_st, e.pairs, st) != cudaSuccess) return SWX_ERR_CUDA;
+            if (e.spread && launch_sum(h, e.pairs, st) != cudaSuccess) return SWX_ERR_CUDA;
         }
     }
     return SWX_OK;
