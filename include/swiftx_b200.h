@@ -460,6 +460,59 @@ int64_t swx_xent_bwd_workspace_bytes(const swx_xent_args* args);
 int swx_xent_fwd(const swx_xent_args* args, void* stream);
 int swx_xent_bwd(const swx_xent_args* args, void* stream);
 
+/* Linear attention with a decay for each head: a recurrence with a (dk x dv) state per head,
+ * the matrix-state counterpart of the selective scan (models/selective_scan.py:34 keeps a
+ * vector of dstate values per channel; it has no reference counterpart of its own):
+ *   S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T,   out_t = scale * S_t^T q_t
+ * q, k: (batch, seqlen, qk_heads, dk), v, dout: (batch, seqlen, heads, dv), in dtype (fp32
+ * or bf16), unit element stride, any batch / token / head strides; heads a multiple of qk_heads
+ * (head h reads q and k of head h / (heads / qk_heads)); dk, dv <= 128.  log_decay: fp32 with
+ * strides (0 broadcasts it over rows or tokens); any value, -inf resets the state.  States are
+ * fp32, dense (batch, heads, dk, dv).  lengths (batch), optional: row i has min(max(lengths[i], 0),
+ * seqlen) tokens; what lies behind them is not used (it may be NaN), gives zeros in out and in the gradients, and
+ * leaves the state as it was.
+ * The sequence is walked in chunks of 64 tokens on the tensor cores; few rows and heads are cut
+ * into swx_linattn_segments(args) segments walked in parallel, whose start states the forward
+ * leaves in seg_states (batch, heads, segments, dk, dv) for the backward (both need the buffer
+ * when there are 2 segments or more).  bf16 inputs: scores are rounded to bf16 once; states and the decay's
+ * gradient keep fp32 accuracy.  fp32 inputs: about 22-bit products.  Deterministic.
+ * Backward outputs are dense: dq, dk_out (batch, seqlen, qk_heads, dk) and dv_out in dtype,
+ * dlog_decay fp32, (batch, seqlen, heads), or (heads) with decay_per_head, where log_decay is one
+ * value per head and the gradient is summed; dinitial_state optional. */
+typedef struct swx_linattn_args {
+    int64_t batch, seqlen, heads, qk_heads, dk, dv;
+    int32_t dtype;                    /* SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t decay_per_head;
+    float scale;
+    int32_t reserved;
+    const void* q; int64_t q_sb, q_sl, q_sh;
+    const void* k; int64_t k_sb, k_sl, k_sh;
+    const void* v; int64_t v_sb, v_sl, v_sh;
+    const float* log_decay; int64_t g_sb, g_sl, g_sh;
+    const int64_t* lengths;           /* optional */
+    const float* initial_state;       /* optional: zero */
+    void* out;                        /* dense (batch, seqlen, heads, dv) in dtype */
+    float* final_state;               /* optional */
+    float* seg_states;
+    const void* dout; int64_t do_sb, do_sl, do_sh;      /* backward */
+    const float* dfinal_state;        /* optional: zero */
+    void* dq; void* dk_out; void* dv_out;
+    float* dlog_decay;
+    float* dinitial_state;            /* optional */
+    void* workspace; int64_t workspace_bytes;
+} swx_linattn_args;
+
+int64_t swx_linattn_args_size(void);
+/* Segments of the sequence for these sizes; a negated status code for sizes that are refused. */
+int swx_linattn_segments(const swx_linattn_args* args);
+int64_t swx_linattn_fwd_workspace_bytes(const swx_linattn_args* args);
+int64_t swx_linattn_bwd_workspace_bytes(const swx_linattn_args* args);
+int swx_linattn_fwd(const swx_linattn_args* args, void* stream);
+int swx_linattn_bwd(const swx_linattn_args* args, void* stream);
+/* One token for every row (seqlen 1; the token strides, lengths and gradients are not read):
+ * the state `final_state` is updated in place and out (batch, heads, dv) read out of it. */
+int swx_linattn_step(const swx_linattn_args* args, void* stream);
+
 /* Diagnostic: y[i] = 2^x[i] computed by the FMA-pipe exponential the scan backward uses
  * for part of its decays (a degree-5 minimax polynomial after rounding x to an integer
  * part; x clamped to [-125, 127]), so its accuracy can be checked on the device.  x, y:

@@ -132,6 +132,22 @@ class XentArgs(ctypes.Structure):
     ]
 
 
+class LinattnArgs(ctypes.Structure):
+    """Mirror of ``swx_linattn_args``."""
+    _fields_ = [
+        ("batch", i64), ("seqlen", i64), ("heads", i64), ("qk_heads", i64), ("dk", i64), ("dv", i64),
+        ("dtype", i32), ("decay_per_head", i32), ("scale", ctypes.c_float), ("reserved", i32),
+        ("q", vp), ("q_sb", i64), ("q_sl", i64), ("q_sh", i64),
+        ("k", vp), ("k_sb", i64), ("k_sl", i64), ("k_sh", i64),
+        ("v", vp), ("v_sb", i64), ("v_sl", i64), ("v_sh", i64),
+        ("log_decay", vp), ("g_sb", i64), ("g_sl", i64), ("g_sh", i64),
+        ("lengths", vp), ("initial_state", vp), ("out", vp), ("final_state", vp), ("seg_states", vp),
+        ("dout", vp), ("do_sb", i64), ("do_sl", i64), ("do_sh", i64),
+        ("dfinal_state", vp), ("dq", vp), ("dk_out", vp), ("dv_out", vp), ("dlog_decay", vp), ("dinitial_state", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 _lib = None
 
 
@@ -151,7 +167,8 @@ def load():
     for fn, st in (("swx_scan_args_size", ScanArgs), ("swx_conv_args_size", ConvArgs),
                    ("swx_decode_args_size", DecodeArgs), ("swx_linear_scan_args_size", LinearScanArgs),
                    ("swx_rmsnorm_args_size", RMSNormArgs), ("swx_embedding_args_size", EmbeddingArgs),
-                   ("swx_xent_args_size", XentArgs)):
+                   ("swx_xent_args_size", XentArgs),
+                   ("swx_linattn_args_size", LinattnArgs)):
         getattr(lib, fn).restype = i64
         if getattr(lib, fn)() != ctypes.sizeof(st):
             raise RuntimeError(f"{st.__name__} layout mismatch between the library and its binding")
@@ -167,7 +184,9 @@ def load():
                      ("swx_linear_scan_fwd", LinearScanArgs), ("swx_linear_scan_bwd", LinearScanArgs),
                      ("swx_rmsnorm_fwd", RMSNormArgs), ("swx_rmsnorm_bwd", RMSNormArgs),
                      ("swx_embedding_bwd", EmbeddingArgs),
-                     ("swx_xent_fwd", XentArgs), ("swx_xent_bwd", XentArgs)):
+                     ("swx_xent_fwd", XentArgs), ("swx_xent_bwd", XentArgs),
+                     ("swx_linattn_fwd", LinattnArgs), ("swx_linattn_bwd", LinattnArgs),
+                     ("swx_linattn_step", LinattnArgs)):
         fn = getattr(lib, name)
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.POINTER(st), vp]
@@ -194,6 +213,11 @@ def load():
     for fn in ("swx_xent_fwd_workspace_bytes", "swx_xent_bwd_workspace_bytes"):
         getattr(lib, fn).restype = i64
         getattr(lib, fn).argtypes = [ctypes.POINTER(XentArgs)]
+    for fn in ("swx_linattn_fwd_workspace_bytes", "swx_linattn_bwd_workspace_bytes"):
+        getattr(lib, fn).restype = i64
+        getattr(lib, fn).argtypes = [ctypes.POINTER(LinattnArgs)]
+    lib.swx_linattn_segments.restype = ctypes.c_int
+    lib.swx_linattn_segments.argtypes = [ctypes.POINTER(LinattnArgs)]
     lib.swx_conv1d_bwd_workspace_bytes.restype = i64
     lib.swx_conv1d_bwd_workspace_bytes.argtypes = [i64, i64, i64, i64]
     _lib = lib

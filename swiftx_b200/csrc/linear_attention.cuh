@@ -1,0 +1,229 @@
+// Shared parts of the chunked linear-attention kernels (forward and backward).
+//
+// For one head, with a_t = exp(g_t) and states S_t (dk x dv):
+//   S_t = a_t S_{t-1} + k_t v_t^T,   o_t = scale * S_t^T q_t.
+// In a chunk of 64 tokens with G_t = g_1 + .. + g_t and M_ts = exp(G_t - G_s) for s <= t:
+//   o_t = scale * (sum_s M_ts (q_t . k_s) v_s + exp(G_t) S_prev^T q_t)
+//   S_next = exp(G_64) S_prev + sum_s exp(G_64 - G_s) k_s v_s^T
+// The chunk's products run on the tensor cores (warp_mma.cuh); the state stays in fp32
+// registers for a whole segment of chunks.  One CTA of four warps walks a segment of one head and
+// 64 columns of v; a v of more than 64 columns is treated as several heads that share q, k and g.
+#pragma once
+#include <cuda_runtime.h>
+
+#include "common.cuh"
+#include "warp_mma.cuh"
+
+namespace swx {
+
+constexpr int LA_C = 64;                  // tokens per chunk
+constexpr int LA_DV = 64;                 // columns of v per CTA
+constexpr int LA_THREADS = 128;
+
+struct LaTensor { const void* p; int64_t sb, sl, sh; bool vec; };
+
+struct LaDev {
+    int b, L, H, Hk, dk, dv, nsl;         // nsl: slices of 64 columns of v
+    int nc, nseg, segc;                   // chunks; segments; chunks per segment
+    LaTensor q, k, v, dout;
+    const float* g; int64_t g_sb, g_sl, g_sh;
+    const int64_t* lengths;
+    float scale;
+    const float* s0;                      // (b, H, dk, dv) or null: zero
+    void* out;                            // (b, L, H, dv)
+    float* s_last;                        // (b, H, dk, dv) or null
+    float* seg;                           // (b, H, nseg, dk, dv): the state at each segment's start
+    float* rseg;                          // the same for the reverse pass: its gradient at each segment's end
+    float* dec;                           // (b, H, nseg): each segment's decay
+    // backward
+    const float* ds;                      // gradient of the last state, or null
+    float* ds0;                           // gradient of the initial state, or null
+    void* dq; void* dk_out; void* dv_out; // dq, dk: (b, L, Hk, dk) in T, or (b, L, H nsl, dk) fp32 when several share
+    bool shared_qk;
+    float* rin;                           // (b, H nsl, L): the inter-chunk part of q . dq
+    float* yseg;                          // (b, H nsl, nseg): <state, its gradient> at each segment's end
+    float* dg; int64_t dg_sb, dg_sl, dg_sh;   // per (row, token, head of H nsl)
+    bool vec_o, vec_qk;                   // 16-byte pieces of v-shaped (q-shaped) results are aligned and whole
+};
+
+template <typename T, int DK>
+struct LaShape {
+    static constexpr int LDK = (DK < 64 ? 64 : DK) + 16 / (int)sizeof(T) * (sizeof(T) == 4 ? 2 : 1);   // rows of q, k
+    static constexpr int LDV = LA_DV + 8;                                                              // rows of v, do, S
+    static constexpr int QK = LA_C * LDK, V = LA_C * LDV, S = DK * LDV;                                // elements
+    // how the four warps share a (dk x 64) state: WM row groups x WN column groups
+    static constexpr int MT = DK / 16, WM = MT < 4 ? MT : 4, WN = 4 / WM, MI = MT / WM, NI = 8 / WN;
+};
+
+// Per-chunk decays.  Sums of g are in fp64 and kept as two floats (in units of log 2), so
+// that differences of far sums keep their precision; g below -1000 (or -inf: a reset) is
+// taken as -1000, whose exponential is 0 as well.
+struct LaGates {
+    float hi[LA_C], lo[LA_C];             // G_t
+    float pre[LA_C];                      // exp(G_t)
+    float post[LA_C];                     // exp(G_64 - G_t)
+    float all;                            // exp(G_64)
+};
+
+struct LaG { float g0, g1; };
+
+__device__ __forceinline__ LaG la_load_g(const LaDev& p, int b, int h, int t0, int len, int lane) {
+    const float* g = p.g + (int64_t)b * p.g_sb + (int64_t)h * p.g_sh;
+    const int t = t0 + 2 * lane;
+    LaG r{0.f, 0.f};
+    if (t < len) r.g0 = g[(int64_t)t * p.g_sl];
+    if (t + 1 < len) r.g1 = g[(int64_t)(t + 1) * p.g_sl];
+    return r;
+}
+
+// One warp; lane holds tokens 2 lane, 2 lane + 1.  Returns the chunk's sum (log 2 units).
+__device__ __forceinline__ double la_gates(LaGates& s, LaG r, int lane) {
+    const double L2E = 1.4426950408889634073599;
+    const double d0 = (r.g0 < -1000.f ? -1000. : (double)r.g0) * L2E, d1 = (r.g1 < -1000.f ? -1000. : (double)r.g1) * L2E;
+    double x = d0 + d1;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const double y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    const double all = __shfl_sync(0xffffffffu, x, 31), g1 = x, g0 = x - d1;
+    const int t = 2 * lane;
+    s.hi[t] = (float)g0; s.hi[t + 1] = (float)g1;
+    s.lo[t] = (float)(g0 - (double)(float)g0); s.lo[t + 1] = (float)(g1 - (double)(float)g1);
+    s.pre[t] = ex2((float)g0); s.pre[t + 1] = ex2((float)g1);
+    s.post[t] = ex2((float)(all - g0)); s.post[t + 1] = ex2((float)(all - g1));
+    if (lane == 0) s.all = ex2((float)all);
+    return all;
+}
+
+// 64 token rows x W columns into s (row length LD), zero past rows / cols; asynchronous when vec.
+template <typename T, int W, int LD>
+__device__ __forceinline__ void la_load(T* s, const LaTensor& x, int b, int t0, int h, int c0, int rows, int cols) {
+    const T* g = static_cast<const T*>(x.p) + (int64_t)b * x.sb + (int64_t)t0 * x.sl + (int64_t)h * x.sh + c0;
+    if (x.vec) {
+        constexpr int E = 16 / sizeof(T), PER = W / E;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < LA_C * PER; i += LA_THREADS) {
+            const int r = i / PER, c = (i % PER) * E;
+            const int n = r < rows ? min(E, max(0, cols - c)) : 0;
+            cp_async16(s + r * LD + c, n > 0 ? g + (int64_t)r * x.sl + c : static_cast<const T*>(x.p), n * (int)sizeof(T));
+        }
+    } else {
+        for (int i = threadIdx.x; i < LA_C * W; i += LA_THREADS) {
+            const int r = i / W, c = i % W;
+            s[r * LD + c] = r < rows && c < cols ? g[(int64_t)r * x.sl + c] : T(0.f);
+        }
+    }
+}
+
+// (dk x dv slice) fp32 matrices in memory <-> the accumulator tiles of a state.
+template <typename T, int DK>
+__device__ __forceinline__ void la_state_read(float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], const float* src,
+                                              const LaDev& p, int c0, int rw, int lane) {
+    using Sh = LaShape<T, DK>;
+    const int m0 = (rw % Sh::WM) * Sh::MI * 16, n0 = (rw / Sh::WM) * Sh::NI * 8;
+#pragma unroll
+    for (int i = 0; i < Sh::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < Sh::NI; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = m0 + 16 * i + (lane >> 2) + 8 * (e >> 1), c = n0 + 8 * j + 2 * (lane & 3) + (e & 1);
+                S[i][j][e] = src && r < p.dk && c0 + c < p.dv ? src[(int64_t)r * p.dv + c0 + c] : 0.f;
+            }
+}
+template <typename T, int DK>
+__device__ __forceinline__ void la_state_write(const float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], float* dst,
+                                               const LaDev& p, int c0, int rw, int lane) {
+    using Sh = LaShape<T, DK>;
+    const int m0 = (rw % Sh::WM) * Sh::MI * 16, n0 = (rw / Sh::WM) * Sh::NI * 8;
+#pragma unroll
+    for (int i = 0; i < Sh::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < Sh::NI; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = m0 + 16 * i + (lane >> 2) + 8 * (e >> 1), c = n0 + 8 * j + 2 * (lane & 3) + (e & 1);
+                if (r < p.dk && c0 + c < p.dv) dst[(int64_t)r * p.dv + c0 + c] = S[i][j][e];
+            }
+}
+
+// S = all * S + sum over the chunk's tokens of (w_s x_s) y_s^T.  The weighted x is kept to 24
+// bits, so that the state, which is carried through the whole sequence, keeps fp32 accuracy.
+template <typename T, int DK>
+__device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], const T* xs, const T* ys,
+                                                const float* w, float all, float scale, int rw, int lane) {
+    using Sh = LaShape<T, DK>;
+    const int m0 = (rw % Sh::WM) * Sh::MI * 16, n0 = (rw / Sh::WM) * Sh::NI * 8;
+#pragma unroll
+    for (int i = 0; i < Sh::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < Sh::NI; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[i][j][e] *= all;
+#pragma unroll
+    for (int k0 = 0; k0 < LA_C; k0 += 16) {
+        const int t = k0 + 2 * (lane & 3);
+        const float w4[4] = {w[t] * scale, w[t + 1] * scale, w[t + 8] * scale, w[t + 9] * scale};
+        FragB<T> y[Sh::NI / 2][2];
+#pragma unroll
+        for (int j = 0; j < Sh::NI / 2; ++j) load_b2_t(y[j], ys, Sh::LDV, n0 + 16 * j, k0, lane);
+#pragma unroll
+        for (int i = 0; i < Sh::MI; ++i) {
+            FragA<T> a;
+            load_a_t(a, xs, Sh::LDK, m0 + 16 * i, k0, lane);
+            ScaledA<T> s;
+            scale_a(s, a, w4);
+#pragma unroll
+            for (int j = 0; j < Sh::NI; ++j) mma(S[i][j], s, y[j / 2][j & 1]);
+        }
+    }
+}
+
+template <typename T, int DK, int PLANES>
+__device__ __forceinline__ void la_state_share(const float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], T* s, int rw, int lane) {
+    using Sh = LaShape<T, DK>;
+    const int m0 = (rw % Sh::WM) * Sh::MI * 16, n0 = (rw / Sh::WM) * Sh::NI * 8;
+#pragma unroll
+    for (int i = 0; i < Sh::MI; ++i)
+#pragma unroll
+        for (int j = 0; j < Sh::NI; ++j) store_tile<PLANES>(s, Sh::LDV, Sh::S, m0 + 16 * i, n0 + 8 * j, S[i][j], lane);
+}
+
+// A warp's 16 finished rows, gathered in its own rows of a tile, to memory: `rows` live ones (later
+// rows up to `all_rows` get zeros), `cols` columns.
+template <typename T, int W, int LD>
+__device__ __forceinline__ void la_store(const T* s, T* g, int64_t sl, int rows, int all_rows, int cols, bool vec, int lane) {
+    __syncwarp();
+    if (vec) {
+        constexpr int E = 16 / sizeof(T), PER = W / E;
+#pragma unroll
+        for (int i = lane; i < 16 * PER; i += 32) {
+            const int r = i / PER, c = (i % PER) * E;
+            if (r < all_rows && c < cols) {
+                const uint4 z = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(g + (int64_t)r * sl + c) = r < rows ? *reinterpret_cast<const uint4*>(s + r * LD + c) : z;
+            }
+        }
+    } else {
+        for (int i = lane; i < 16 * W; i += 32) {
+            const int r = i / W, c = i % W;
+            if (r < all_rows && c < cols) g[(int64_t)r * sl + c] = r < rows ? s[r * LD + c] : T(0.f);
+        }
+    }
+    __syncwarp();
+}
+
+__device__ __forceinline__ int la_len(const LaDev& p, int b) {
+    if (!p.lengths) return p.L;
+    const int64_t n = p.lengths[b];
+    return n < 0 ? 0 : (n < p.L ? (int)n : p.L);
+}
+
+cudaError_t la_launch_fwd(const LaDev& p, int dtype, cudaStream_t st);
+cudaError_t la_launch_bwd(const LaDev& p, int dtype, cudaStream_t st);
+cudaError_t la_launch_state(const LaDev& p, int dtype, bool reverse, cudaStream_t st);
+cudaError_t la_launch_dg_sum(const float* src, float* dst, bool per_head, int b, int64_t L, int H, int nsl, cudaStream_t st);
+cudaError_t la_launch_group_sum(const float* src, void* dst, int dtype, int64_t rows, int Hk, int per, int d, cudaStream_t st);
+
+}  // namespace swx

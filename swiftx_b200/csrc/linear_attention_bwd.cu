@@ -1,0 +1,480 @@
+// Linear attention with a decay for each head, chunked: gradients.
+//
+// With P_ts = scale M_ts q_t . k_s and A_ts = scale M_ts do_t . v_s (s <= t), S_prev the state at
+// the chunk's start and D the gradient of the state at its end:
+//   dq_t = sum_s A_ts k_s + scale exp(G_t) S_prev do_t
+//   dk_s = sum_t A_ts q_t + exp(G_64 - G_s) D v_s
+//   dv_s = sum_t P_ts do_t + exp(G_64 - G_s) D^T k_s
+//   D_prev = exp(G_64) D + sum_t scale exp(G_t) q_t do_t^T
+// A forward walk carries S and gives dq; a reverse walk carries D and gives dk, dv.  The decay's
+// gradient dg_t is the sum of all terms of the result that cross from before t to t or later, so
+// dg_t = dg_{t+1} + q_t . dq_t - k_t . dk_t, from <S, D> at the segment's end.  The dot
+// products are taken from unrounded sums: sum_s A_ts (q_t . k_s) from the two score tiles, and the
+// states' parts with the state kept to 24 bits (three bf16 pieces), so that dg, fp32, has fp32
+// accuracy although dq and dk are rounded to the inputs' type.
+#include "linear_attention.cuh"
+#include "launch_util.cuh"
+
+namespace swx {
+
+template <typename T> struct Planes { static constexpr int N = sizeof(T) == 4 ? 1 : 3; };
+
+// acc[DK / 8] += rows 16 rw of x (16 x 64) times S^T, S in shared memory in full precision.
+template <typename T, int DK>
+__device__ __forceinline__ void la_times_state_t(float (&acc)[DK / 8][4], const T* x, const T* s, int rw, int lane) {
+    using Sh = LaShape<T, DK>;
+#pragma unroll
+    for (int k0 = 0; k0 < LA_DV; k0 += 16) {
+        FragA<T> a;
+        load_a(a, x, Sh::LDV, 16 * rw, k0, lane);
+#pragma unroll
+        for (int j = 0; j < DK / 16; ++j)
+#pragma unroll
+            for (int pl = Planes<T>::N - 1; pl >= 0; --pl) {
+                FragB<T> f[2];
+                load_b2(f, s + pl * Sh::S, Sh::LDV, 16 * j, k0, lane);
+                mma(acc[2 * j], a, f[0]);
+                mma(acc[2 * j + 1], a, f[1]);
+            }
+    }
+}
+
+// Row dot products of an accumulator (16 x DK) with this warp's rows of a tile in shared memory:
+// {row g, row g + 8}, complete in every lane of the quad.
+template <typename T, int DK>
+__device__ __forceinline__ float2 la_row_dot(const float (&acc)[DK / 8][4], const T* x, int ld, int rw, int lane) {
+    float2 r = make_float2(0.f, 0.f);
+    const T* p = x + (16 * rw + (lane >> 2)) * ld + 2 * (lane & 3);
+#pragma unroll
+    for (int j = 0; j < DK / 8; ++j) {
+        r.x += acc[j][0] * Elem<T>::to_f(p[8 * j]) + acc[j][1] * Elem<T>::to_f(p[8 * j + 1]);
+        r.y += acc[j][2] * Elem<T>::to_f(p[8 * ld + 8 * j]) + acc[j][3] * Elem<T>::to_f(p[8 * ld + 8 * j + 1]);
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o *= 2) {
+        r.x += __shfl_xor_sync(0xffffffffu, r.x, o);
+        r.y += __shfl_xor_sync(0xffffffffu, r.y, o);
+    }
+    return r;
+}
+
+// A warp's 16 rows of dq or dk: rounded, through this warp's own rows of `tile`, or the fp32
+// part of this head where several heads share the gradient.
+template <typename T, int DK>
+__device__ __forceinline__ void la_store_qk(const float (&acc)[DK / 8][4], T* tile, void* dst, const LaDev& p, int b, int hk,
+                                            int64_t vhead, int tr, int len, int rw, int lane) {
+    using Sh = LaShape<T, DK>;
+    if (p.shared_qk) {
+        const int64_t sl = (int64_t)p.H * p.nsl * p.dk;
+        float* o = static_cast<float*>(dst) + ((int64_t)b * p.L + tr) * sl + vhead * p.dk;
+#pragma unroll
+        for (int j = 0; j < DK / 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = (lane >> 2) + 8 * (e >> 1), c = 8 * j + 2 * (lane & 3) + (e & 1);
+                if (c < p.dk && tr + r < p.L) o[(int64_t)r * sl + c] = tr + r < len ? acc[j][e] : 0.f;
+            }
+        return;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < DK / 8; ++j) store_tile<1>(tile, Sh::LDK, 0, 16 * rw, 8 * j, acc[j], lane);
+    const int64_t sl = (int64_t)p.Hk * p.dk;
+    la_store<T, DK, Sh::LDK>(tile + 16 * rw * Sh::LDK, static_cast<T*>(dst) + ((int64_t)b * p.L + tr) * sl + (int64_t)hk * p.dk, sl,
+                             len - tr, p.L - tr, p.dk, p.vec_qk, lane);
+}
+
+template <typename T, int DK> struct LaBwd {
+    using Sh = LaShape<T, DK>;
+    static constexpr int SMEM = (int)sizeof(T) * (2 * Sh::QK + 2 * Sh::V + Planes<T>::N * Sh::S);
+};
+
+// ------------------------------------------------------------------ dq: forward walk
+// Warp = 16 tokens t of the chunk and a quarter of the state.
+template <typename T, int DK>
+__global__ void __launch_bounds__(LA_THREADS) la_dq_kernel(const LaDev p) {
+    using Sh = LaShape<T, DK>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    T* q = reinterpret_cast<T*>(smem);
+    T* k = q + Sh::QK;
+    T* v = k + Sh::QK;
+    T* dout = v + Sh::V;
+    T* ss = dout + Sh::V;
+    __shared__ LaGates gt;
+    __shared__ float red[4];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = (warp + blockIdx.x) & 3;
+    const int seg = (int)(blockIdx.x % p.nseg);
+    const int64_t vh = blockIdx.x / p.nseg;
+    const int sl = (int)(vh % p.nsl), h = (int)(vh / p.nsl % p.H), b = (int)(vh / p.nsl / p.H);
+    const int hk = h / (p.H / p.Hk), c0 = sl * LA_DV, cols = min(LA_DV, p.dv - c0), len = la_len(p, b);
+    const int first = seg * p.segc, last = min(first + p.segc, p.nc);
+    const int64_t bh = (int64_t)b * p.H + h, ssz = (int64_t)p.dk * p.dv, vhead = (int64_t)h * p.nsl + sl;
+
+    float S[Sh::MI][Sh::NI][4];
+    la_state_read<T, DK>(S, p.nseg > 1 ? p.seg + (bh * p.nseg + seg) * ssz : (p.s0 ? p.s0 + bh * ssz : nullptr), p, c0, rw, lane);
+    for (int c = first; c < last; ++c) {
+        const int t0 = c * LA_C, rows = min(LA_C, len - t0);
+        __syncthreads();                                     // the last chunk's tiles are done with
+        la_load<T, DK, Sh::LDK>(q, p.q, b, t0, hk, 0, rows, p.dk);
+        la_load<T, DK, Sh::LDK>(k, p.k, b, t0, hk, 0, rows, p.dk);
+        la_load<T, LA_DV, Sh::LDV>(v, p.v, b, t0, h, c0, rows, cols);
+        la_load<T, LA_DV, Sh::LDV>(dout, p.dout, b, t0, h, c0, rows, cols);
+        cp_async_commit();
+        la_state_share<T, DK, Planes<T>::N>(S, ss, rw, lane);
+        if (warp == 0) la_gates(gt, la_load_g(p, b, h, t0, len, lane), lane);
+        cp_async_wait<0>();
+        __syncthreads();
+        const int r0 = 16 * rw + (lane >> 2), tr = t0 + 16 * rw;
+        float dq[DK / 8][4] = {};
+        la_times_state_t<T, DK>(dq, dout, ss, rw, lane);
+        const float e0 = gt.pre[r0] * p.scale, e1 = gt.pre[r0 + 8] * p.scale;
+#pragma unroll
+        for (int j = 0; j < DK / 8; ++j) { dq[j][0] *= e0; dq[j][1] *= e0; dq[j][2] *= e1; dq[j][3] *= e1; }
+        const float2 rd = la_row_dot<T, DK>(dq, q, Sh::LDK, rw, lane);
+        if ((lane & 3) == 0) {
+            float* rin = p.rin + (((int64_t)b * p.H * p.nsl) + vhead) * p.L;
+            const int t = t0 + r0;
+            if (t < p.L) rin[t] = rd.x;
+            if (t + 8 < p.L) rin[t + 8] = rd.y;
+        }
+        float sc[8][4] = {};
+#pragma unroll
+        for (int k0 = 0; k0 < LA_DV; k0 += 16) {
+            FragA<T> a;
+            load_a(a, dout, Sh::LDV, 16 * rw, k0, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j <= rw) {
+                    FragB<T> f[2];
+                    load_b2(f, v, Sh::LDV, 16 * j, k0, lane);
+                    mma(sc[2 * j], a, f[0]);
+                    mma(sc[2 * j + 1], a, f[1]);
+                }
+        }
+        const float h0 = gt.hi[r0], h1 = gt.hi[r0 + 8], l0 = gt.lo[r0], l1 = gt.lo[r0 + 8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j <= rw) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int s = 16 * j + 8 * x + 2 * (lane & 3) + e;
+                        const float hc = gt.hi[s], lc = gt.lo[s];
+                        sc[2 * j + x][e] = s <= r0 ? sc[2 * j + x][e] * (p.scale * ex2((h0 - hc) + (l0 - lc))) : 0.f;
+                        sc[2 * j + x][2 + e] = s <= r0 + 8 ? sc[2 * j + x][2 + e] * (p.scale * ex2((h1 - hc) + (l1 - lc))) : 0.f;
+                    }
+                FragA<T> a;
+                frag_from(a, sc[2 * j], sc[2 * j + 1]);
+#pragma unroll
+                for (int n = 0; n < DK / 16; ++n) {
+                    FragB<T> f[2];
+                    load_b2_t(f, k, Sh::LDK, 16 * n, 16 * j, lane);
+                    mma(dq[2 * n], a, f[0]);
+                    mma(dq[2 * n + 1], a, f[1]);
+                }
+            }
+        la_store_qk<T, DK>(dq, q, p.dq, p, b, hk, vhead, tr, len, rw, lane);
+        la_state_update<T, DK>(S, k, v, gt.post, gt.all, 1.f, rw, lane);
+    }
+    // <state, its gradient> at the segment's end
+    const float* D = p.nseg > 1 ? p.rseg + (bh * p.nseg + seg) * ssz : (p.ds ? p.ds + bh * ssz : nullptr);
+    float y = 0.f;
+    if (D) {
+        float R[Sh::MI][Sh::NI][4];
+        la_state_read<T, DK>(R, D, p, c0, rw, lane);
+#pragma unroll
+        for (int i = 0; i < Sh::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < Sh::NI; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y += S[i][j][e] * R[i][j][e];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (lane == 0) red[rw] = y;
+    __syncthreads();
+    if (threadIdx.x == 0) p.yseg[((int64_t)b * p.H * p.nsl + vhead) * p.nseg + seg] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// ------------------------------------------------------------------ dk, dv, dg: reverse walk
+// Warp = 16 tokens s of the chunk and a quarter of the state's gradient.
+template <typename T, int DK>
+__global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
+    using Sh = LaShape<T, DK>;
+    extern __shared__ __align__(16) uint8_t smem[];
+    T* q = reinterpret_cast<T*>(smem);
+    T* k = q + Sh::QK;
+    T* v = k + Sh::QK;
+    T* dout = v + Sh::V;
+    T* ss = dout + Sh::V;
+    __shared__ LaGates gt;
+    __shared__ float rowsum[4][LA_C], colsum[LA_C];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = (warp + blockIdx.x) & 3;
+    const int seg = (int)(blockIdx.x % p.nseg);
+    const int64_t vh = blockIdx.x / p.nseg;
+    const int sl = (int)(vh % p.nsl), h = (int)(vh / p.nsl % p.H), b = (int)(vh / p.nsl / p.H);
+    const int hk = h / (p.H / p.Hk), c0 = sl * LA_DV, cols = min(LA_DV, p.dv - c0), len = la_len(p, b);
+    const int first = seg * p.segc, last = min(first + p.segc, p.nc);
+    const int64_t bh = (int64_t)b * p.H + h, ssz = (int64_t)p.dk * p.dv, vhead = (int64_t)h * p.nsl + sl;
+
+    float D[Sh::MI][Sh::NI][4];
+    la_state_read<T, DK>(D, p.nseg > 1 ? p.rseg + (bh * p.nseg + seg) * ssz : (p.ds ? p.ds + bh * ssz : nullptr), p, c0, rw, lane);
+    // the running dg (warp 0): tokens behind the row's end change nothing
+    double run = p.yseg[((int64_t)b * p.H * p.nsl + vhead) * p.nseg + seg];
+    const float* rin = p.rin + ((int64_t)b * p.H * p.nsl + vhead) * p.L;
+    for (int c = last - 1; c >= first; --c) {
+        const int t0 = c * LA_C, rows = min(LA_C, len - t0);
+        __syncthreads();
+        la_load<T, DK, Sh::LDK>(q, p.q, b, t0, hk, 0, rows, p.dk);
+        la_load<T, DK, Sh::LDK>(k, p.k, b, t0, hk, 0, rows, p.dk);
+        la_load<T, LA_DV, Sh::LDV>(v, p.v, b, t0, h, c0, rows, cols);
+        la_load<T, LA_DV, Sh::LDV>(dout, p.dout, b, t0, h, c0, rows, cols);
+        cp_async_commit();
+        la_state_share<T, DK, Planes<T>::N>(D, ss, rw, lane);
+        LaG g{};
+        if (warp == 0) {
+            g = la_load_g(p, b, h, t0, len, lane);
+            la_gates(gt, g, lane);
+        }
+        cp_async_wait<0>();
+        __syncthreads();
+        const int r0 = 16 * rw + (lane >> 2), tr = t0 + 16 * rw;
+        // the scores of this warp's tokens s (rows) with the tokens t >= s (columns)
+        float ps[8][4] = {}, as[8][4] = {};
+#pragma unroll
+        for (int k0 = 0; k0 < DK; k0 += 16) {
+            FragA<T> a;
+            load_a(a, k, Sh::LDK, 16 * rw, k0, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j >= rw) {
+                    FragB<T> f[2];
+                    load_b2(f, q, Sh::LDK, 16 * j, k0, lane);
+                    mma(ps[2 * j], a, f[0]);
+                    mma(ps[2 * j + 1], a, f[1]);
+                }
+        }
+#pragma unroll
+        for (int k0 = 0; k0 < LA_DV; k0 += 16) {
+            FragA<T> a;
+            load_a(a, v, Sh::LDV, 16 * rw, k0, lane);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j >= rw) {
+                    FragB<T> f[2];
+                    load_b2(f, dout, Sh::LDV, 16 * j, k0, lane);
+                    mma(as[2 * j], a, f[0]);
+                    mma(as[2 * j + 1], a, f[1]);
+                }
+        }
+        const float h0 = gt.hi[r0], h1 = gt.hi[r0 + 8], l0 = gt.lo[r0], l1 = gt.lo[r0 + 8];
+        float cs0 = 0.f, cs1 = 0.f;                          // sums over t of this lane's two tokens s
+        FragA<T> pf[4], af[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (j >= rw) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int t = 16 * j + 8 * x + 2 * (lane & 3) + e;
+                        const float ht = gt.hi[t], lt = gt.lo[t];
+                        const float m0 = t >= r0 ? p.scale * ex2((ht - h0) + (lt - l0)) : 0.f;
+                        const float m1 = t >= r0 + 8 ? p.scale * ex2((ht - h1) + (lt - l1)) : 0.f;
+                        float& p0 = ps[2 * j + x][e];
+                        float& p1 = ps[2 * j + x][2 + e];
+                        float& a0 = as[2 * j + x][e];
+                        float& a1 = as[2 * j + x][2 + e];
+                        a0 = t >= r0 ? a0 * m0 : 0.f;
+                        a1 = t >= r0 + 8 ? a1 * m1 : 0.f;
+                        const float x0 = t >= r0 ? a0 * p0 : 0.f, x1 = t >= r0 + 8 ? a1 * p1 : 0.f;
+                        cs0 += x0;
+                        cs1 += x1;
+                        float rs = x0 + x1;                  // over this warp's 16 tokens s, for token t
+#pragma unroll
+                        for (int o = 4; o < 32; o *= 2) rs += __shfl_xor_sync(0xffffffffu, rs, o);
+                        if (lane < 4) rowsum[rw][t] = rs;
+                        p0 = t >= r0 ? p0 * m0 : 0.f;
+                        p1 = t >= r0 + 8 ? p1 * m1 : 0.f;
+                    }
+            } else if (lane < 16) {
+                rowsum[rw][16 * j + lane] = 0.f;
+            }
+            frag_from(pf[j], ps[2 * j], ps[2 * j + 1]);
+            frag_from(af[j], as[2 * j], as[2 * j + 1]);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o *= 2) {
+            cs0 += __shfl_xor_sync(0xffffffffu, cs0, o);
+            cs1 += __shfl_xor_sync(0xffffffffu, cs1, o);
+        }
+        const float w0 = gt.post[r0], w1 = gt.post[r0 + 8];
+        {
+            float dv[8][4] = {};
+#pragma unroll
+            for (int k0 = 0; k0 < DK; k0 += 16) {            // D^T k, D rounded once for a result in T
+                FragA<T> a;
+                load_a(a, k, Sh::LDK, 16 * rw, k0, lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    FragB<T> f[2];
+                    load_b2_t(f, ss, Sh::LDV, 16 * j, k0, lane);
+                    mma(dv[2 * j], a, f[0]);
+                    mma(dv[2 * j + 1], a, f[1]);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { dv[j][0] *= w0; dv[j][1] *= w0; dv[j][2] *= w1; dv[j][3] *= w1; }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j >= rw) {
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        FragB<T> f[2];
+                        load_b2_t(f, dout, Sh::LDV, 16 * n, 16 * j, lane);
+                        mma(dv[2 * n], pf[j], f[0]);
+                        mma(dv[2 * n + 1], pf[j], f[1]);
+                    }
+                }
+            // dk's part from the state reads this warp's rows of v first
+            float dk[DK / 8][4] = {};
+            la_times_state_t<T, DK>(dk, v, ss, rw, lane);
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) store_tile<1>(v, Sh::LDV, 0, 16 * rw, 8 * j, dv[j], lane);
+            const int64_t o_sl = (int64_t)p.H * p.dv;
+            la_store<T, LA_DV, Sh::LDV>(v + 16 * rw * Sh::LDV, static_cast<T*>(p.dv_out) + ((int64_t)b * p.L + tr) * o_sl + (int64_t)h * p.dv + c0,
+                                        o_sl, len - tr, p.L - tr, cols, p.vec_o, lane);
+#pragma unroll
+            for (int j = 0; j < DK / 8; ++j) { dk[j][0] *= w0; dk[j][1] *= w0; dk[j][2] *= w1; dk[j][3] *= w1; }
+            const float2 rd = la_row_dot<T, DK>(dk, k, Sh::LDK, rw, lane);
+            if ((lane & 3) == 0) {
+                colsum[r0] = cs0 + rd.x;
+                colsum[r0 + 8] = cs1 + rd.y;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (j >= rw) {
+#pragma unroll
+                    for (int n = 0; n < DK / 16; ++n) {
+                        FragB<T> f[2];
+                        load_b2_t(f, q, Sh::LDK, 16 * n, 16 * j, lane);
+                        mma(dk[2 * n], af[j], f[0]);
+                        mma(dk[2 * n + 1], af[j], f[1]);
+                    }
+                }
+            la_store_qk<T, DK>(dk, k, p.dk_out, p, b, hk, vhead, tr, len, rw, lane);
+        }
+        la_state_update<T, DK>(D, q, dout, gt.pre, gt.all, p.scale, rw, lane);
+        __syncthreads();                                     // the token sums are complete
+        if (warp == 0) {
+            const int ta = 2 * lane;
+            double d[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int t = ta + e;
+                d[e] = t0 + t < len ? (double)rin[t0 + t] + (((double)rowsum[0][t] + rowsum[1][t]) + ((double)rowsum[2][t] + rowsum[3][t])) - colsum[t]
+                                    : 0.;
+            }
+            double x = d[0] + d[1];                          // suffix sums over the chunk
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const double z = __shfl_down_sync(0xffffffffu, x, o);
+                if (lane + o < 32) x += z;
+            }
+            float* dg = p.dg + (int64_t)b * p.dg_sb + vhead * p.dg_sh + (int64_t)t0 * p.dg_sl;
+            // nothing crosses a reset (a decay of 0): no rounding noise there either
+            if (t0 + ta < p.L) dg[(int64_t)ta * p.dg_sl] = t0 + ta < len && !(g.g0 < -1000.f) ? (float)(run + x) : 0.f;
+            if (t0 + ta + 1 < p.L)
+                dg[(int64_t)(ta + 1) * p.dg_sl] = t0 + ta + 1 < len && !(g.g1 < -1000.f) ? (float)(run + x - d[0]) : 0.f;
+            run += __shfl_sync(0xffffffffu, x, 0);
+        }
+    }
+    if (p.ds0 && seg == 0) la_state_write<T, DK>(D, p.ds0 + bh * ssz, p, c0, rw, lane);
+}
+
+// ------------------------------------------------------------------ sums over heads that share
+// dst[row][hk][c] = sum over the group's parts of src[row][part][c], in order.
+template <typename T>
+__global__ void __launch_bounds__(256) la_group_sum_kernel(const float* src, T* dst, int64_t rows, int Hk, int per, int d) {
+    const int64_t n = rows * Hk * d, i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i >= n) return;
+    const int64_t c = i % d, rh = i / d;
+    const float* s = src + rh * per * d + c;
+    float x = 0.f;
+#pragma unroll 4
+    for (int k = 0; k < per; ++k) x += s[(int64_t)k * d];
+    dst[i] = Elem<T>::from_f(x);
+}
+
+// The decay's gradient from the heads' parts [b][H nsl][L]: dst (b, L, H), the slices added in
+// order, or (per_head) dst (H), every row and token added in a fixed order in fp64.
+__global__ void __launch_bounds__(256) la_dg_sum_kernel(const float* src, float* dst, int b, int64_t L, int H, int nsl) {
+    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i >= (int64_t)b * L * H) return;
+    const int64_t t = i % L, bh = i / L;
+    float x = 0.f;
+    for (int k = 0; k < nsl; ++k) x += src[(bh * nsl + k) * L + t];
+    dst[(bh / H * L + t) * H + bh % H] = x;
+}
+__global__ void __launch_bounds__(1024) la_dg_head_kernel(const float* src, float* dst, int b, int64_t L, int H, int nsl) {
+    __shared__ double red[32];
+    const int h = blockIdx.x;
+    double x = 0.;
+    for (int r = 0; r < b; ++r) {
+        const float* s = src + ((int64_t)r * H + h) * nsl * L;
+#pragma unroll 4
+        for (int64_t t = threadIdx.x; t < nsl * L; t += 1024) x += (double)s[t];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        x = red[threadIdx.x];
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (threadIdx.x == 0) dst[h] = (float)x;
+    }
+}
+
+template <typename T, int DK>
+static cudaError_t bwd(const LaDev& p, cudaStream_t st) {
+    constexpr int smem = LaBwd<T, DK>::SMEM;
+    const unsigned grid = (unsigned)((int64_t)p.b * p.H * p.nsl * p.nseg);
+    auto kq = la_dq_kernel<T, DK>;
+    auto kk = la_dkv_kernel<T, DK>;
+    cudaError_t e = allow_smem(kq, smem);
+    if (e == cudaSuccess) e = allow_smem(kk, smem);
+    if (e != cudaSuccess) return e;
+    kq<<<grid, LA_THREADS, smem, st>>>(p);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    kk<<<grid, LA_THREADS, smem, st>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t bwd_dk(const LaDev& p, cudaStream_t st) {
+    return p.dk <= 32 ? bwd<T, 32>(p, st) : p.dk <= 64 ? bwd<T, 64>(p, st) : bwd<T, 128>(p, st);
+}
+
+cudaError_t la_launch_bwd(const LaDev& p, int dtype, cudaStream_t st) {
+    return dtype == SWX_DTYPE_F32 ? bwd_dk<float>(p, st) : bwd_dk<__nv_bfloat16>(p, st);
+}
+
+cudaError_t la_launch_dg_sum(const float* src, float* dst, bool per_head, int b, int64_t L, int H, int nsl, cudaStream_t st) {
+    if (per_head) la_dg_head_kernel<<<(unsigned)H, 1024, 0, st>>>(src, dst, b, L, H, nsl);
+    else la_dg_sum_kernel<<<(unsigned)(((int64_t)b * L * H + 255) / 256), 256, 0, st>>>(src, dst, b, L, H, nsl);
+    return cudaGetLastError();
+}
+
+cudaError_t la_launch_group_sum(const float* src, void* dst, int dtype, int64_t rows, int Hk, int per, int d, cudaStream_t st) {
+    const int64_t n = rows * Hk * d;
+    const unsigned grid = (unsigned)((n + 255) / 256);
+    if (dtype == SWX_DTYPE_F32) la_group_sum_kernel<float><<<grid, 256, 0, st>>>(src, static_cast<float*>(dst), rows, Hk, per, d);
+    else la_group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(src, static_cast<__nv_bfloat16*>(dst), rows, Hk, per, d);
+    return cudaGetLastError();
+}
+
+}  // namespace swx

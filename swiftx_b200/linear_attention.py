@@ -1,0 +1,160 @@
+"""Linear attention with a decay for each head: a recurrence with a matrix state.
+
+Where the selective scan (models/selective_scan.py:34) keeps ``d_state`` values for each
+channel, ``linear_attention`` keeps a (dk, dv) matrix for each head:
+
+    S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T,    out_t = scale * S_t^T q_t
+
+Over a sequence it runs chunked, on the tensor cores, with gradients; ``linear_attention_step``
+is its form for one token per row, on a state that it updates in place.
+"""
+import torch
+
+from . import _lib
+
+MAX_DIM = 128                    # largest dk and dv
+_DT = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _unit(t):
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _check(name, q, k, v, log_decay, state, token):
+    """Shapes, types and devices of an operand set; ``token``: without the sequence dimension."""
+    ts = [t for t in (q, k, v, log_decay, state) if t is not None]
+    if not all(t.is_cuda for t in ts):
+        raise RuntimeError(f"swiftx_b200 {name} runs on CUDA tensors only (no CPU path)")
+    if any(t.device != q.device for t in ts):
+        raise ValueError(f"{name}: tensors on several devices")
+    lead = 1 if token else 2
+    n = lead + 2
+    if q.dim() != n or v.dim() != n or k.shape != q.shape or v.shape[:lead] != q.shape[:lead]:
+        raise ValueError(f"{name}: q, k {'(b, Hk, dk)' if token else '(b, L, Hk, dk)'} and v with its b{'' if token else ', L'} expected, "
+                         f"got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    hk, dk, h, dv = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
+    if hk < 1 or h < 1 or h % hk:
+        raise ValueError(f"{name}: v's {h} heads are not a multiple of q's and k's {hk}")
+    if not (1 <= dk <= MAX_DIM and 1 <= dv <= MAX_DIM):
+        raise ValueError(f"{name}: dk and dv of 1 to {MAX_DIM} expected, got {dk} and {dv}")
+    if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"{name}: q, k and v of one dtype, fp32 or bf16, expected, got {q.dtype}, {k.dtype} and {v.dtype}")
+    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) not in ((h,), tuple(v.shape[:lead]) + (h,)):
+        raise ValueError(f"{name}: fp32 log_decay of shape {(h,)} or {tuple(v.shape[:lead]) + (h,)} expected, got "
+                         f"{log_decay.dtype} {tuple(log_decay.shape)}")
+    want = (v.shape[0], h, dk, dv)
+    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != want):
+        raise ValueError(f"{name}: fp32 state of shape {want} expected, got {state.dtype} {tuple(state.shape)}")
+
+
+def _args(q, k, v, g, scale):
+    a = _lib.LinattnArgs()
+    a.batch, a.seqlen, a.heads, a.dv = v.shape
+    a.qk_heads, a.dk = q.shape[2:]
+    a.dtype, a.scale, a.decay_per_head = _DT[q.dtype], scale, int(g.dim() == 1)
+    a.q, (a.q_sb, a.q_sl, a.q_sh) = q.data_ptr(), q.stride()[:3]
+    a.k, (a.k_sb, a.k_sl, a.k_sh) = k.data_ptr(), k.stride()[:3]
+    a.v, (a.v_sb, a.v_sl, a.v_sh) = v.data_ptr(), v.stride()[:3]
+    a.log_decay = g.data_ptr()
+    a.g_sb, a.g_sl, a.g_sh = (0, 0, g.stride(0)) if g.dim() == 1 else g.stride()
+    return a
+
+
+class LinearAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
+        q, k, v = _unit(q), _unit(k), _unit(v)
+        g = log_decay
+        s0 = initial_state.contiguous() if initial_state is not None else None
+        b, _, h, dv = v.shape
+        dk = q.shape[-1]
+        with torch.cuda.device(v.device):
+            lib = _lib.load()
+            a = _args(q, k, v, g, scale)
+            n = lib.swx_linattn_segments(a)
+            if n < 0:
+                _lib.check(-n, "swx_linattn_segments")
+            f32 = dict(device=v.device, dtype=torch.float32)
+            out = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+            last = torch.empty(b, h, dk, dv, **f32) if want_state else None
+            seg = torch.empty(b, h, n, dk, dv, **f32) if n > 1 else None
+            ws = torch.empty(max(1, lib.swx_linattn_fwd_workspace_bytes(a)), device=v.device, dtype=torch.uint8) if n > 1 else None
+            a.lengths, a.initial_state, a.out, a.final_state, a.seg_states = (
+                t.data_ptr() if t is not None else None for t in (lengths, s0, out, last, seg))
+            if ws is not None:
+                a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+            _lib.check(lib.swx_linattn_fwd(a, _lib.stream_ptr(v.device)), "swx_linattn_fwd")
+        ctx.save_for_backward(q, k, v, g, s0, lengths, seg)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, dlast):
+        q, k, v, g, s0, lengths, seg = ctx.saved_tensors
+        if dout is None:
+            dout = torch.zeros_like(v)
+        dout = _unit(dout.to(v.dtype))
+        dlast = dlast.float().contiguous() if dlast is not None else None
+        with torch.cuda.device(v.device):
+            lib = _lib.load()
+            a = _args(q, k, v, g, ctx.scale)
+            dense = lambda t: torch.empty(t.shape, device=t.device, dtype=t.dtype)  # noqa: E731
+            dq, dk, dv, dg = dense(q), dense(k), dense(v), dense(g)
+            ds0 = dense(s0) if s0 is not None and ctx.needs_input_grad[4] else None
+            ws = torch.empty(max(1, lib.swx_linattn_bwd_workspace_bytes(a)), device=v.device, dtype=torch.uint8)
+            a.lengths, a.initial_state, a.seg_states, a.dout, a.dfinal_state, a.dq, a.dk_out, a.dv_out, a.dlog_decay, a.dinitial_state = (
+                t.data_ptr() if t is not None else None for t in (lengths, s0, seg, dout, dlast, dq, dk, dv, dg, ds0))
+            a.do_sb, a.do_sl, a.do_sh = dout.stride()[:3]
+            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+            _lib.check(lib.swx_linattn_bwd(a, _lib.stream_ptr(v.device)), "swx_linattn_bwd")
+        return dq, dk, dv, dg, ds0, None, None, None
+
+
+def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=None, return_state=False):
+    """out_t = scale * S_t^T q_t with S_t = exp(log_decay_t) S_{t-1} + k_t v_t^T (CUDA only).
+
+    q, k (b, L, Hk, dk) and v (b, L, H, dv), all fp32 or all bf16, dk and dv up to 128, with any strides
+    and a unit one along the last dimension (a copy otherwise); H a multiple of Hk: head h reads
+    q and k of head h // (H // Hk).  log_decay fp32, (b, L, H), or (H,) for fixed decays; 0 keeps
+    the state, -inf resets it.  initial_state fp32 (b, H, dk, dv).  lengths, an int64 (b,) tensor:
+    row i has lengths[i] tokens (clamped to 0..L); what lies behind them is not read, gives zeros in
+    out and in the gradients, and leaves the state.  Returns out (b, L, H, dv), and with return_state the
+    fp32 state after the last token.  Differentiable in q, k, v, log_decay and initial_state;
+    deterministic.  bf16 inputs: the score tiles are rounded to bf16 once, states and log_decay's gradient
+    keep fp32 accuracy."""
+    _check("linear_attention", q, k, v, log_decay, initial_state, token=False)
+    if lengths is not None:
+        if lengths.dtype != torch.int64 or tuple(lengths.shape) != (v.shape[0],) or lengths.device != v.device:
+            raise ValueError(f"linear_attention: int64 lengths of shape {(v.shape[0],)} on {v.device} expected, got "
+                             f"{lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
+        lengths = lengths.contiguous()
+    out, state = LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
+    return (out, state) if return_state else out
+
+
+@torch.no_grad()
+def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
+    """One token of ``linear_attention`` for every row: q, k (b, Hk, dk), v (b, H, dv), log_decay
+    (b, H) or (H,); ``state``, a dense fp32 (b, H, dk, dv) tensor (as linear_attention returns it), is updated
+    in place.  Returns out (b, H, dv) in v's dtype.  Not differentiable."""
+    _check("linear_attention_step", q, k, v, log_decay, state, token=True)
+    if not state.is_contiguous():
+        raise ValueError("linear_attention_step: state must be a dense (b, H, dk, dv) tensor")
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    with torch.cuda.device(v.device):
+        lib = _lib.load()
+        out = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+        a = _lib.LinattnArgs()
+        a.batch, a.heads, a.dv = v.shape
+        a.seqlen, (a.qk_heads, a.dk) = 1, q.shape[1:]
+        a.dtype, a.scale = _DT[q.dtype], scale
+        a.q, (a.q_sb, a.q_sh) = q.data_ptr(), q.stride()[:2]
+        a.k, (a.k_sb, a.k_sh) = k.data_ptr(), k.stride()[:2]
+        a.v, (a.v_sb, a.v_sh) = v.data_ptr(), v.stride()[:2]
+        a.log_decay = log_decay.data_ptr()
+        a.g_sb, a.g_sh = (0, log_decay.stride(0)) if log_decay.dim() == 1 else log_decay.stride()
+        a.out, a.final_state = out.data_ptr(), state.data_ptr()
+        _lib.check(lib.swx_linattn_step(a, _lib.stream_ptr(v.device)), "swx_linattn_step")
+    return out
