@@ -3,6 +3,7 @@
 The shared library is built in-tree (swiftx_b200/libswiftx_b200.so).  Loading
 fails loudly if it is missing: there is no CPU or eager fallback behind it.
 """
+import contextlib
 import ctypes
 import os
 
@@ -241,3 +242,11 @@ def ptr(t):
 
 def stream_ptr(device):
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def on_device(device):
+    """A context in which ``device`` is the current one; nothing to enter when it is already."""
+    return _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+_NOTHING = contextlib.nullcontext()

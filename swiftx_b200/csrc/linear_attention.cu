@@ -16,7 +16,7 @@ __global__ void __launch_bounds__(LA_THREADS) la_state_kernel(const LaDev p) {
     extern __shared__ __align__(16) uint8_t smem[];
     T* xs = reinterpret_cast<T*>(smem);
     T* ys = xs + 2 * Sh::QK;
-    __shared__ LaGates gates[2];
+    __shared__ LaGates gates[LA_RING];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = warp;
     // the last segment's state (reverse: the first one's) is not needed
     const int nrun = p.nseg - 1;
@@ -28,7 +28,6 @@ __global__ void __launch_bounds__(LA_THREADS) la_state_kernel(const LaDev p) {
     const int n = max(0, last - first);
 
     float S[Sh::MI][Sh::NI][4] = {};
-    double total = 0.;
     auto chunk = [&](int i) { return REV ? last - 1 - i : first + i; };
     auto load = [&](int i) {
         const int t0 = chunk(i) * LA_C, rows = min(LA_C, len - t0);
@@ -36,26 +35,25 @@ __global__ void __launch_bounds__(LA_THREADS) la_state_kernel(const LaDev p) {
         la_load<T, LA_DV, Sh::LDV>(ys + (i & 1) * Sh::V, REV ? p.dout : p.v, b, t0, h, c0, rows, cols);
         cp_async_commit();
     };
-    LaG g{};
-    if (n > 0) {
-        load(0);
-        if (warp == 0) g = la_load_g(p, b, h, chunk(0) * LA_C, len, lane);
-    }
+    if (n > 0) load(0);
+    LaGateRing ring;
+    ring.start(gates, p, b, h, len, n, chunk, warp, lane);
+#pragma unroll 1
     for (int i = 0; i < n; ++i) {
-        LaGates& gt = gates[i & 1];
-        if (warp == 0) total += la_gates(gt, g, lane);
         cp_async_wait<0>();
         __syncthreads();
-        if (i + 1 < n) {
-            load(i + 1);
-            if (warp == 0) g = la_load_g(p, b, h, chunk(i + 1) * LA_C, len, lane);
-        }
-        la_state_update<T, DK>(S, xs + (i & 1) * Sh::QK, ys + (i & 1) * Sh::V, REV ? gt.pre : gt.post, gt.all,
-                               REV ? p.scale : 1.f, rw, lane);
+        if (i + 1 < n) load(i + 1);
+        const LaGates& gt = ring.take(p, b, h, len, n, i, chunk, warp, lane);
+        la_state_update<T, DK, REV>(S, xs + (i & 1) * Sh::QK, ys + (i & 1) * Sh::V, gt, p.scale, rw, lane);
+        ring.make(n, i, warp, lane);
     }
+    __shared__ double sums[4];
+    if (lane == 0) sums[warp] = ring.total;
+    __syncthreads();
     float* dst = (REV ? p.rseg : p.seg) + (((int64_t)b * p.H + h) * p.nseg + seg) * p.dk * p.dv;
     la_state_write<T, DK>(S, dst, p, c0, rw, lane);
-    if (threadIdx.x == 0 && sl == 0) p.dec[((int64_t)b * p.H + h) * p.nseg + seg] = ex2((float)total);
+    if (threadIdx.x == 0 && sl == 0) p.dec[((int64_t)b * p.H + h) * p.nseg + seg] =
+            ex2((float)((sums[0] + sums[1]) + (sums[2] + sums[3])));
 }
 
 // Segment sums -> the state at each segment's start (reverse: its gradient at each segment's
@@ -68,12 +66,21 @@ __global__ void __launch_bounds__(256) la_chain_kernel(const LaDev p, bool rev) 
     float run = start ? start[bh * n + e] : 0.f;
     float* s = (rev ? p.rseg : p.seg) + bh * p.nseg * n + e;
     const float* d = p.dec + bh * p.nseg;
-#pragma unroll 4
-    for (int i = 0; i < p.nseg; ++i) {
-        const int k = rev ? p.nseg - 1 - i : i;
-        const float u = i + 1 < p.nseg ? s[k * n] : 0.f, dk = i + 1 < p.nseg ? d[k] : 0.f;
-        s[k * n] = run;
-        run = dk * run + u;
+    for (int i0 = 0; i0 < p.nseg; i0 += 8) {           // eight loads in flight before the first store
+        float u[8], dec[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int k = rev ? p.nseg - 1 - i0 - i : i0 + i;
+            const bool in = i0 + i + 1 < p.nseg;
+            u[i] = in ? s[k * n] : 0.f;
+            dec[i] = in ? d[k] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i0 + i >= p.nseg) break;
+            s[(rev ? p.nseg - 1 - i0 - i : i0 + i) * n] = run;
+            run = dec[i] * run + u[i];
+        }
     }
 }
 
@@ -81,23 +88,21 @@ __global__ void __launch_bounds__(256) la_chain_kernel(const LaDev p, bool rev) 
 // Warp = 16 tokens of the chunk (and a quarter of the state).  Per chunk: the state's part of
 // the output, exp(G_t) S^T q; the decayed scores of the 16 tokens with the tokens up to them
 // (rounded to the inputs' type once, as the second product's operand); their product with v; then the
-// state's update.  Tiles arrive by cp.async one chunk ahead, one block barrier per chunk.
+// state's update.  Tiles arrive by cp.async one chunk ahead.
 template <typename T, int DK> struct LaFwd {
     using Sh = LaShape<T, DK>;
-    static constexpr int SB = sizeof(T) == 4 && DK == 128 ? 1 : 2;     // copies of the shared state
-    static constexpr int SMEM = (int)sizeof(T) * (4 * Sh::QK + 2 * Sh::V + SB * Sh::S);
+    static constexpr int SMEM = (int)sizeof(T) * (4 * Sh::QK + 2 * Sh::V + Sh::S);
 };
 
 template <typename T, int DK>
-__global__ void __launch_bounds__(LA_THREADS) la_fwd_kernel(const LaDev p) {
+__global__ void __launch_bounds__(LA_THREADS, sizeof(T) == 4 ? 1 : DK == 128 ? 2 : 3) la_fwd_kernel(const LaDev p) {
     using Sh = LaShape<T, DK>;
-    using Fw = LaFwd<T, DK>;
     extern __shared__ __align__(16) uint8_t smem[];
     T* qs = reinterpret_cast<T*>(smem);
     T* ks = qs + 2 * Sh::QK;
     T* vs = ks + 2 * Sh::QK;
     T* ss = vs + 2 * Sh::V;
-    __shared__ LaGates gates[2];
+    __shared__ LaGates gates[LA_RING];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int rw = (warp + blockIdx.x) & 3;           // later tokens have more scores: spread them over the SM's quarters
     const int seg = (int)(blockIdx.x % p.nseg);
@@ -118,27 +123,24 @@ __global__ void __launch_bounds__(LA_THREADS) la_fwd_kernel(const LaDev p) {
         la_load<T, LA_DV, Sh::LDV>(vs + u * Sh::V, p.v, b, t0, h, c0, rows, cols);
         cp_async_commit();
     };
-    LaG g{};
-    if (live > first) {
-        load(0);
-        if (warp == 0) g = la_load_g(p, b, h, first * LA_C, len, lane);
-    }
+    const int n = live - first;
+    auto chunk = [&](int i) { return first + i; };
+    if (n > 0) load(0);
+    LaGateRing ring;
+    ring.start(gates, p, b, h, len, n, chunk, warp, lane);
     T* out = static_cast<T*>(p.out);
     const int64_t o_sl = (int64_t)p.H * p.dv;
-    for (int i = 0; i < live - first; ++i) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
         const int u = i & 1, t0 = (first + i) * LA_C;
-        LaGates& gt = gates[u];
-        if (warp == 0) la_gates(gt, g, lane);
         cp_async_wait<0>();
         __syncthreads();
-        if (i + 1 < live - first) {
-            load(i + 1);
-            if (warp == 0) g = la_load_g(p, b, h, t0 + LA_C, len, lane);
-        }
+        if (i + 1 < n) load(i + 1);
+        const LaGates& gt = ring.take(p, b, h, len, n, i, chunk, warp, lane);
         T* q = qs + u * Sh::QK;
         const T* k = ks + u * Sh::QK;
         const T* v = vs + u * Sh::V;
-        const T* s = ss + (Fw::SB == 2 ? u : 0) * Sh::S;
+        const T* s = ss;
         float o[8][4] = {}, sc[8][4] = {};
 #pragma unroll
         for (int k0 = 0; k0 < DK; k0 += 16) {
@@ -161,46 +163,34 @@ __global__ void __launch_bounds__(LA_THREADS) la_fwd_kernel(const LaDev p) {
                 }
         }
         const int r0 = 16 * rw + (lane >> 2);
-        const float e0 = gt.pre[r0], e1 = gt.pre[r0 + 8];
+        const float e0 = gt.pre(r0) * p.scale, e1 = gt.pre(r0 + 8) * p.scale;
 #pragma unroll
         for (int j = 0; j < 8; ++j) { o[j][0] *= e0; o[j][1] *= e0; o[j][2] *= e1; o[j][3] *= e1; }
-        const float h0 = gt.hi[r0], h1 = gt.hi[r0 + 8], l0 = gt.lo[r0], l1 = gt.lo[r0 + 8];
+        const float2 G0 = gt.G[r0], G1 = gt.G[r0 + 8];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j <= rw) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int c = 16 * j + 8 * x + 2 * (lane & 3) + e;
-                        const float hc = gt.hi[c], lc = gt.lo[c];
-                        sc[2 * j + x][e] = c <= r0 ? sc[2 * j + x][e] * ex2((h0 - hc) + (l0 - lc)) : 0.f;
-                        sc[2 * j + x][2 + e] = c <= r0 + 8 ? sc[2 * j + x][2 + e] * ex2((h1 - hc) + (l1 - lc)) : 0.f;
-                    }
+                la_mask_rows(sc[2 * j], sc[2 * j + 1], gt, j, rw, r0, G0, G1, p.scale, lane);
                 FragA<T> a;
                 frag_from(a, sc[2 * j], sc[2 * j + 1]);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int c = 0; c < 4; ++c) {
                     FragB<T> f[2];
-                    load_b2_t(f, v, Sh::LDV, 16 * n, 16 * j, lane);
-                    mma(o[2 * n], a, f[0]);
-                    mma(o[2 * n + 1], a, f[1]);
+                    load_b2_t(f, v, Sh::LDV, 16 * c, 16 * j, lane);
+                    mma(o[2 * c], a, f[0]);
+                    mma(o[2 * c + 1], a, f[1]);
                 }
             }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[j][e] *= p.scale;
-        }
         __syncwarp();
 #pragma unroll
         for (int j = 0; j < 8; ++j) store_tile<1>(q, Sh::LDK, 0, 16 * rw, 8 * j, o[j], lane);   // this warp's own rows of q
         const int tr = t0 + 16 * rw;
         la_store<T, LA_DV, Sh::LDK>(q + 16 * rw * Sh::LDK, out + ((int64_t)b * p.L + tr) * o_sl + (int64_t)h * p.dv + c0, o_sl,
                                     len - tr, p.L - tr, cols, p.vec_o, lane);
-        la_state_update<T, DK>(S, k, v, gt.post, gt.all, 1.f, rw, lane);
-        if (Fw::SB == 1) __syncthreads();
-        la_state_share<T, DK, 1>(S, ss + (Fw::SB == 2 ? (u ^ 1) : 0) * Sh::S, rw, lane);
+        la_state_update<T, DK, false>(S, k, v, gt, 1.f, rw, lane);
+        __syncthreads();                                  // all have read the state that this replaces
+        la_state_share<T, DK, 1>(S, ss, rw, lane);
+        ring.make(n, i, warp, lane);
     }
     // rows behind the row's last token
     for (int t = max(live, first) * LA_C; t < min(last * LA_C, p.L); ++t)

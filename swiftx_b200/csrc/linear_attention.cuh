@@ -40,9 +40,11 @@ struct LaDev {
     float* ds0;                           // gradient of the initial state, or null
     void* dq; void* dk_out; void* dv_out; // dq, dk: (b, L, Hk, dk) in T, or (b, L, H nsl, dk) fp32 when several share
     bool shared_qk;
-    float* rin;                           // (b, H nsl, L): the inter-chunk part of q . dq
+    float* rin;                           // (b, H nsl, L): the states' part of q . dq
+    float* net;                           // (b, H nsl, L): the scores' part of q . dq, less k . dk
     float* yseg;                          // (b, H nsl, nseg): <state, its gradient> at each segment's end
-    float* dg; int64_t dg_sb, dg_sl, dg_sh;   // per (row, token, head of H nsl)
+    float* dg;                            // (b, L, H), or null:
+    double* dg_part;                      // (H, b nseg): each segment's sum
     bool vec_o, vec_qk;                   // 16-byte pieces of v-shaped (q-shaped) results are aligned and whole
 };
 
@@ -59,13 +61,22 @@ struct LaShape {
 // that differences of far sums keep their precision; g below -1000 (or -inf: a reset) is
 // taken as -1000, whose exponential is 0 as well.
 struct LaGates {
-    float hi[LA_C], lo[LA_C];             // G_t
-    float pre[LA_C];                      // exp(G_t)
+    float2 G[LA_C];                       // G_t, high and low part
     float post[LA_C];                     // exp(G_64 - G_t)
+    float in_block[LA_C];                 // exp(G_e - G_t), e the last token of t's block of 16
     float all;                            // exp(G_64)
+    float unused[3];
+    __device__ __forceinline__ float pre(int t) const { return ex2(G[t].x); }      // exp(G_t)
 };
+// exp(G_a - G_b) from the two-float sums
+__device__ __forceinline__ float la_decay(float2 a, float2 b) { return ex2((a.x - b.x) + (a.y - b.y)); }
 
+// The gates of a walk of n chunks, made for four chunks at a time, one chunk by each warp: their
+// scan is a chain of a thousand cycles that would otherwise hold all warps up in every chunk.  The
+// next four are made in the last step of the present four, whose own gates are the ring's fifth.
+// take() after the barrier that starts step i, make() before the barrier that starts step i + 1.
 struct LaG { float g0, g1; };
+constexpr int LA_RING = 5;
 
 __device__ __forceinline__ LaG la_load_g(const LaDev& p, int b, int h, int t0, int len, int lane) {
     const float* g = p.g + (int64_t)b * p.g_sb + (int64_t)h * p.g_sh;
@@ -88,12 +99,58 @@ __device__ __forceinline__ double la_gates(LaGates& s, LaG r, int lane) {
     }
     const double all = __shfl_sync(0xffffffffu, x, 31), g1 = x, g0 = x - d1;
     const int t = 2 * lane;
-    s.hi[t] = (float)g0; s.hi[t + 1] = (float)g1;
-    s.lo[t] = (float)(g0 - (double)(float)g0); s.lo[t + 1] = (float)(g1 - (double)(float)g1);
-    s.pre[t] = ex2((float)g0); s.pre[t + 1] = ex2((float)g1);
+    const double ge = __shfl_sync(0xffffffffu, x, lane | 7);
+    s.G[t] = make_float2((float)g0, (float)(g0 - (double)(float)g0));
+    s.G[t + 1] = make_float2((float)g1, (float)(g1 - (double)(float)g1));
     s.post[t] = ex2((float)(all - g0)); s.post[t + 1] = ex2((float)(all - g1));
+    s.in_block[t] = ex2((float)(ge - g0)); s.in_block[t + 1] = ex2((float)(ge - g1));
     if (lane == 0) s.all = ex2((float)all);
     return all;
+}
+
+struct LaGateRing {
+    LaGates* s;
+    LaG g;
+    double total;                         // this warp's chunks (log 2 units)
+    template <typename F>
+    __device__ __forceinline__ void start(LaGates* slots, const LaDev& p, int b, int h, int len, int n, F chunk, int warp, int lane) {
+        s = slots;
+        total = 0.;
+        if (warp < n) total += la_gates(s[warp], la_load_g(p, b, h, chunk(warp) * LA_C, len, lane), lane);
+    }
+    template <typename F>
+    __device__ __forceinline__ const LaGates& take(const LaDev& p, int b, int h, int len, int n, int i, F chunk, int warp, int lane) {
+        if ((i & 3) == 3 && i + 1 + warp < n) g = la_load_g(p, b, h, chunk(i + 1 + warp) * LA_C, len, lane);
+        return s[i % LA_RING];
+    }
+    __device__ __forceinline__ void make(int n, int i, int warp, int lane) {
+        if ((i & 3) == 3 && i + 1 + warp < n) total += la_gates(s[(i + 1 + warp) % LA_RING], g, lane);
+    }
+};
+
+// Scores of the rows r0, r0 + 8 of block rw (G0, G1 their sums) with the 16 tokens of block j:
+// times scale exp(G_t - G_s), 0 for s > t.  Off the diagonal the exponential is split at the
+// end of block j, exp(G_t - G_e) exp(G_e - G_s), both at most 1 for decays at most 1: two products
+// a value instead of a difference and an exponential.
+__device__ __forceinline__ void la_mask_rows(float (&c0)[4], float (&c1)[4], const LaGates& gt, int j, int rw, int r0, float2 G0,
+                                             float2 G1, float scale, int lane) {
+    const int s0 = 16 * j + 2 * (lane & 3);
+    if (j < rw) {
+        const float2 Ge = gt.G[16 * j + 15];
+        const float f0 = scale * la_decay(G0, Ge), f1 = scale * la_decay(G1, Ge);
+        const float2 x = *reinterpret_cast<const float2*>(gt.in_block + s0), y = *reinterpret_cast<const float2*>(gt.in_block + s0 + 8);
+        c0[0] *= f0 * x.x; c0[1] *= f0 * x.y; c0[2] *= f1 * x.x; c0[3] *= f1 * x.y;
+        c1[0] *= f0 * y.x; c1[1] *= f0 * y.y; c1[2] *= f1 * y.x; c1[3] *= f1 * y.y;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const float2 a = gt.G[s0 + e], b = gt.G[s0 + 8 + e];
+            c0[e] = s0 + e <= r0 ? c0[e] * (scale * la_decay(G0, a)) : 0.f;
+            c0[2 + e] *= scale * la_decay(G1, a);
+            c1[e] = 0.f;
+            c1[2 + e] = s0 + e <= r0 ? c1[2 + e] * (scale * la_decay(G1, b)) : 0.f;
+        }
+    }
 }
 
 // 64 token rows x W columns into s (row length LD), zero past rows / cols; asynchronous when vec.
@@ -101,12 +158,22 @@ template <typename T, int W, int LD>
 __device__ __forceinline__ void la_load(T* s, const LaTensor& x, int b, int t0, int h, int c0, int rows, int cols) {
     const T* g = static_cast<const T*>(x.p) + (int64_t)b * x.sb + (int64_t)t0 * x.sl + (int64_t)h * x.sh + c0;
     if (x.vec) {
-        constexpr int E = 16 / sizeof(T), PER = W / E;
-#pragma unroll 4
-        for (int i = threadIdx.x; i < LA_C * PER; i += LA_THREADS) {
-            const int r = i / PER, c = (i % PER) * E;
-            const int n = r < rows ? min(E, max(0, cols - c)) : 0;
-            cp_async16(s + r * LD + c, n > 0 ? g + (int64_t)r * x.sl + c : static_cast<const T*>(x.p), n * (int)sizeof(T));
+        // this thread's column and rows r, r + STEP, ..
+        constexpr int E = 16 / sizeof(T), PER = W / E, STEP = LA_THREADS / PER;
+        const int r = threadIdx.x / PER, c = (threadIdx.x % PER) * E;
+        const int n = min(E, max(0, cols - c)) * (int)sizeof(T);
+        const T* src = g + (int64_t)r * x.sl + c;
+        const int64_t step = STEP * x.sl;
+        T* dst = s + r * LD + c;
+        if (rows >= LA_C && n > 0) {
+#pragma unroll
+            for (int i = 0; i < LA_C / STEP; ++i) cp_async16(dst + i * STEP * LD, src + i * step, n);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LA_C / STEP; ++i) {
+                const bool in = r + i * STEP < rows && n > 0;
+                cp_async16(dst + i * STEP * LD, in ? src + i * step : static_cast<const T*>(x.p), in ? n : 0);
+            }
         }
     } else {
         for (int i = threadIdx.x; i < LA_C * W; i += LA_THREADS) {
@@ -148,11 +215,12 @@ __device__ __forceinline__ void la_state_write(const float (&S)[LaShape<T, DK>::
             }
 }
 
-// S = all * S + sum over the chunk's tokens of (w_s x_s) y_s^T.  The weighted x is kept to 24
+// S = exp(G_64) S + sum over the chunk's tokens of (w_s x_s) y_s^T, w_s = exp(G_64 - G_s) or (PRE)
+// scale exp(G_s).  The weighted x is kept to 24
 // bits, so that the state, which is carried through the whole sequence, keeps fp32 accuracy.
-template <typename T, int DK>
+template <typename T, int DK, bool PRE>
 __device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], const T* xs, const T* ys,
-                                                const float* w, float all, float scale, int rw, int lane) {
+                                                const LaGates& gt, float scale, int rw, int lane) {
     using Sh = LaShape<T, DK>;
     const int m0 = (rw % Sh::WM) * Sh::MI * 16, n0 = (rw / Sh::WM) * Sh::NI * 8;
 #pragma unroll
@@ -160,11 +228,16 @@ __device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][L
 #pragma unroll
         for (int j = 0; j < Sh::NI; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[i][j][e] *= all;
+            for (int e = 0; e < 4; ++e) S[i][j][e] *= gt.all;
 #pragma unroll
     for (int k0 = 0; k0 < LA_C; k0 += 16) {
         const int t = k0 + 2 * (lane & 3);
-        const float w4[4] = {w[t] * scale, w[t + 1] * scale, w[t + 8] * scale, w[t + 9] * scale};
+        float w4[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int s = t + (x & 1) + (x >> 1) * 8;
+            w4[x] = PRE ? scale * gt.pre(s) : gt.post[s];
+        }
         FragB<T> y[Sh::NI / 2][2];
 #pragma unroll
         for (int j = 0; j < Sh::NI / 2; ++j) load_b2_t(y[j], ys, Sh::LDV, n0 + 16 * j, k0, lane);
@@ -174,8 +247,7 @@ __device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][L
             load_a_t(a, xs, Sh::LDK, m0 + 16 * i, k0, lane);
             ScaledA<T> s;
             scale_a(s, a, w4);
-#pragma unroll
-            for (int j = 0; j < Sh::NI; ++j) mma(S[i][j], s, y[j / 2][j & 1]);
+            mma_row(S[i], s, y);
         }
     }
 }
@@ -223,7 +295,7 @@ __device__ __forceinline__ int la_len(const LaDev& p, int b) {
 cudaError_t la_launch_fwd(const LaDev& p, int dtype, cudaStream_t st);
 cudaError_t la_launch_bwd(const LaDev& p, int dtype, cudaStream_t st);
 cudaError_t la_launch_state(const LaDev& p, int dtype, bool reverse, cudaStream_t st);
-cudaError_t la_launch_dg_sum(const float* src, float* dst, bool per_head, int b, int64_t L, int H, int nsl, cudaStream_t st);
+cudaError_t la_launch_dg_head(const double* part, float* dst, int H, int n, cudaStream_t st);
 cudaError_t la_launch_group_sum(const float* src, void* dst, int dtype, int64_t rows, int Hk, int per, int d, cudaStream_t st);
 
 }  // namespace swx

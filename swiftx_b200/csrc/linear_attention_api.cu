@@ -84,16 +84,16 @@ __global__ void __launch_bounds__(LS_THREADS) la_step_kernel(const LaStep p) {
 // ------------------------------------------------------------------ plans
 struct LaPlan { int nsl, nc, nseg, segc; };
 
-// One CTA walks a segment of one head's sequence.  The heads alone are enough when they fill the SMs;
-// otherwise the sequence is cut so that about three CTAs (two with dk > 64) sit on each of 148
-// SMs, with at least two chunks per segment: the states at the segments' starts cost one more
-// reading of k and v.
+// One CTA walks a segment of one head's sequence.  Where the heads leave SMs idle the sequence is
+// cut, so that the CTAs fill, and do not exceed, one round of three CTAs (two with dk > 64) on each
+// of 148 SMs, with at least two chunks per segment: the states at the segments' starts cost one
+// more reading of k and v.
 static LaPlan la_plan(const swx_linattn_args* a) {
     LaPlan q{};
     q.nsl = (int)((a->dv + LA_DV - 1) / LA_DV);
     q.nc = (int)((a->seqlen + LA_C - 1) / LA_C);
     const int64_t heads = a->batch * a->heads * q.nsl, target = 148 * (a->dk > 64 ? 2 : 3);
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>((target + heads / 2) / heads, q.nc / 2));
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(target / heads, q.nc / 2));
     q.segc = (int)((q.nc + n - 1) / n);
     q.nseg = (q.nc + q.segc - 1) / std::max(1, q.segc);
     return q;
@@ -109,7 +109,7 @@ static int la_check(const swx_linattn_args* a) {
     return SWX_OK;
 }
 
-struct LaWs { int64_t dec, rseg, rin, yseg, dg, dq, dk, total; };
+struct LaWs { int64_t dec, rseg, rin, net, yseg, dg, dq, dk, total; };
 
 static int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
@@ -123,8 +123,9 @@ static LaWs la_ws(const swx_linattn_args* a, const LaPlan& q) {
     w.dec = take(bh * q.nseg);
     w.rseg = take(q.nseg > 1 ? bh * q.nseg * a->dk * a->dv : 0);
     w.rin = take(bv * a->seqlen);
-    w.yseg = take(bv * std::max(1, q.nseg));
-    w.dg = take(q.nsl > 1 || a->decay_per_head ? bv * a->seqlen : 0);
+    w.net = take(bv * a->seqlen);
+    w.yseg = take(bv * q.nseg);
+    w.dg = take(a->decay_per_head ? 2 * bh * q.nseg : 0);
     w.dq = take(la_shared(a, q) ? bv * a->seqlen * a->dk : 0);
     w.dk = take(la_shared(a, q) ? bv * a->seqlen * a->dk : 0);
     w.total = o;
@@ -229,23 +230,20 @@ int swx_linattn_bwd(const swx_linattn_args* a, void* stream) {
     p.dq = p.shared_qk ? at(w.dq) : a->dq;
     p.dk_out = p.shared_qk ? at(w.dk) : a->dk_out;
     p.dv_out = a->dv_out;
-    const int64_t L = a->seqlen, V = a->heads * q.nsl;
-    const bool parts = q.nsl > 1 || a->decay_per_head;
-    p.dg = parts ? at(w.dg) : a->dlog_decay;
-    p.dg_sb = parts ? V * L : L * a->heads;
-    p.dg_sl = parts ? 1 : a->heads;
-    p.dg_sh = parts ? L : 1;
+    p.net = at(w.net);
+    p.dg = a->decay_per_head ? nullptr : a->dlog_decay;
+    p.dg_part = reinterpret_cast<double*>(ws + w.dg);
     auto whole = [a](const void* o, int64_t d) {
         return (reinterpret_cast<uintptr_t>(o) & 15) == 0 && (d * (a->dtype == SWX_DTYPE_F32 ? 4 : 2)) % 16 == 0;
     };
     p.vec_o = whole(a->dv_out, a->dv);
     if (q.nseg > 1 && la_launch_state(p, a->dtype, true, st) != cudaSuccess) return SWX_ERR_CUDA;
     if (la_launch_bwd(p, a->dtype, st) != cudaSuccess) return SWX_ERR_CUDA;
-    if (parts && la_launch_dg_sum(p.dg, a->dlog_decay, a->decay_per_head != 0, p.b, L, p.H, q.nsl, st) != cudaSuccess) return SWX_ERR_CUDA;
+    if (a->decay_per_head && la_launch_dg_head(p.dg_part, a->dlog_decay, p.H, p.b * p.nseg, st) != cudaSuccess) return SWX_ERR_CUDA;
     if (p.shared_qk) {
         const int per = (int)(a->heads / a->qk_heads) * q.nsl;
-        if (la_launch_group_sum(static_cast<float*>(p.dq), a->dq, a->dtype, a->batch * L, p.Hk, per, p.dk, st) != cudaSuccess ||
-            la_launch_group_sum(static_cast<float*>(p.dk_out), a->dk_out, a->dtype, a->batch * L, p.Hk, per, p.dk, st) != cudaSuccess)
+        if (la_launch_group_sum(static_cast<float*>(p.dq), a->dq, a->dtype, a->batch * a->seqlen, p.Hk, per, p.dk, st) != cudaSuccess ||
+            la_launch_group_sum(static_cast<float*>(p.dk_out), a->dk_out, a->dtype, a->batch * a->seqlen, p.Hk, per, p.dk, st) != cudaSuccess)
             return SWX_ERR_CUDA;
     }
     return SWX_OK;

@@ -28,9 +28,9 @@ __device__ __forceinline__ void la_times_state_t(float (&acc)[DK / 8][4], const 
         FragA<T> a;
         load_a(a, x, Sh::LDV, 16 * rw, k0, lane);
 #pragma unroll
-        for (int j = 0; j < DK / 16; ++j)
+        for (int pl = Planes<T>::N - 1; pl >= 0; --pl)
 #pragma unroll
-            for (int pl = Planes<T>::N - 1; pl >= 0; --pl) {
+            for (int j = 0; j < DK / 16; ++j) {
                 FragB<T> f[2];
                 load_b2(f, s + pl * Sh::S, Sh::LDV, 16 * j, k0, lane);
                 mma(acc[2 * j], a, f[0]);
@@ -92,19 +92,16 @@ template <typename T, int DK> struct LaBwd {
 // ------------------------------------------------------------------ dq: forward walk
 // Warp = 16 tokens t of the chunk and a quarter of the state.
 template <typename T, int DK>
-__global__ void __launch_bounds__(LA_THREADS) la_dq_kernel(const LaDev p) {
+__device__ __forceinline__ void la_dq_walk(const LaDev& p, int64_t block, uint8_t* smem, LaGates* gates, float* red) {
     using Sh = LaShape<T, DK>;
-    extern __shared__ __align__(16) uint8_t smem[];
     T* q = reinterpret_cast<T*>(smem);
     T* k = q + Sh::QK;
     T* v = k + Sh::QK;
     T* dout = v + Sh::V;
     T* ss = dout + Sh::V;
-    __shared__ LaGates gt;
-    __shared__ float red[4];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = (warp + blockIdx.x) & 3;
-    const int seg = (int)(blockIdx.x % p.nseg);
-    const int64_t vh = blockIdx.x / p.nseg;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = (int)(warp + block) & 3;
+    const int seg = (int)(block % p.nseg);
+    const int64_t vh = block / p.nseg;
     const int sl = (int)(vh % p.nsl), h = (int)(vh / p.nsl % p.H), b = (int)(vh / p.nsl / p.H);
     const int hk = h / (p.H / p.Hk), c0 = sl * LA_DV, cols = min(LA_DV, p.dv - c0), len = la_len(p, b);
     const int first = seg * p.segc, last = min(first + p.segc, p.nc);
@@ -112,8 +109,13 @@ __global__ void __launch_bounds__(LA_THREADS) la_dq_kernel(const LaDev p) {
 
     float S[Sh::MI][Sh::NI][4];
     la_state_read<T, DK>(S, p.nseg > 1 ? p.seg + (bh * p.nseg + seg) * ssz : (p.s0 ? p.s0 + bh * ssz : nullptr), p, c0, rw, lane);
-    for (int c = first; c < last; ++c) {
-        const int t0 = c * LA_C, rows = min(LA_C, len - t0);
+    const int n = last - first;
+    auto chunk = [&](int i) { return first + i; };
+    LaGateRing ring;
+    ring.start(gates, p, b, h, len, n, chunk, warp, lane);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const int t0 = chunk(i) * LA_C, rows = min(LA_C, len - t0);
         __syncthreads();                                     // the last chunk's tiles are done with
         la_load<T, DK, Sh::LDK>(q, p.q, b, t0, hk, 0, rows, p.dk);
         la_load<T, DK, Sh::LDK>(k, p.k, b, t0, hk, 0, rows, p.dk);
@@ -121,13 +123,13 @@ __global__ void __launch_bounds__(LA_THREADS) la_dq_kernel(const LaDev p) {
         la_load<T, LA_DV, Sh::LDV>(dout, p.dout, b, t0, h, c0, rows, cols);
         cp_async_commit();
         la_state_share<T, DK, Planes<T>::N>(S, ss, rw, lane);
-        if (warp == 0) la_gates(gt, la_load_g(p, b, h, t0, len, lane), lane);
         cp_async_wait<0>();
         __syncthreads();
+        const LaGates& gt = ring.take(p, b, h, len, n, i, chunk, warp, lane);
         const int r0 = 16 * rw + (lane >> 2), tr = t0 + 16 * rw;
         float dq[DK / 8][4] = {};
         la_times_state_t<T, DK>(dq, dout, ss, rw, lane);
-        const float e0 = gt.pre[r0] * p.scale, e1 = gt.pre[r0 + 8] * p.scale;
+        const float e0 = gt.pre(r0) * p.scale, e1 = gt.pre(r0 + 8) * p.scale;
 #pragma unroll
         for (int j = 0; j < DK / 8; ++j) { dq[j][0] *= e0; dq[j][1] *= e0; dq[j][2] *= e1; dq[j][3] *= e1; }
         const float2 rd = la_row_dot<T, DK>(dq, q, Sh::LDK, rw, lane);
@@ -151,31 +153,24 @@ __global__ void __launch_bounds__(LA_THREADS) la_dq_kernel(const LaDev p) {
                     mma(sc[2 * j + 1], a, f[1]);
                 }
         }
-        const float h0 = gt.hi[r0], h1 = gt.hi[r0 + 8], l0 = gt.lo[r0], l1 = gt.lo[r0 + 8];
+        const float2 G0 = gt.G[r0], G1 = gt.G[r0 + 8];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (j <= rw) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const int s = 16 * j + 8 * x + 2 * (lane & 3) + e;
-                        const float hc = gt.hi[s], lc = gt.lo[s];
-                        sc[2 * j + x][e] = s <= r0 ? sc[2 * j + x][e] * (p.scale * ex2((h0 - hc) + (l0 - lc))) : 0.f;
-                        sc[2 * j + x][2 + e] = s <= r0 + 8 ? sc[2 * j + x][2 + e] * (p.scale * ex2((h1 - hc) + (l1 - lc))) : 0.f;
-                    }
+                la_mask_rows(sc[2 * j], sc[2 * j + 1], gt, j, rw, r0, G0, G1, p.scale, lane);
                 FragA<T> a;
                 frag_from(a, sc[2 * j], sc[2 * j + 1]);
 #pragma unroll
-                for (int n = 0; n < DK / 16; ++n) {
+                for (int c = 0; c < DK / 16; ++c) {
                     FragB<T> f[2];
-                    load_b2_t(f, k, Sh::LDK, 16 * n, 16 * j, lane);
-                    mma(dq[2 * n], a, f[0]);
-                    mma(dq[2 * n + 1], a, f[1]);
+                    load_b2_t(f, k, Sh::LDK, 16 * c, 16 * j, lane);
+                    mma(dq[2 * c], a, f[0]);
+                    mma(dq[2 * c + 1], a, f[1]);
                 }
             }
         la_store_qk<T, DK>(dq, q, p.dq, p, b, hk, vhead, tr, len, rw, lane);
-        la_state_update<T, DK>(S, k, v, gt.post, gt.all, 1.f, rw, lane);
+        la_state_update<T, DK, false>(S, k, v, gt, 1.f, rw, lane);
+        ring.make(n, i, warp, lane);
     }
     // <state, its gradient> at the segment's end
     const float* D = p.nseg > 1 ? p.rseg + (bh * p.nseg + seg) * ssz : (p.ds ? p.ds + bh * ssz : nullptr);
@@ -200,19 +195,17 @@ __global__ void __launch_bounds__(LA_THREADS) la_dq_kernel(const LaDev p) {
 // ------------------------------------------------------------------ dk, dv, dg: reverse walk
 // Warp = 16 tokens s of the chunk and a quarter of the state's gradient.
 template <typename T, int DK>
-__global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
+__device__ __forceinline__ void la_dkv_walk(const LaDev& p, int64_t block, uint8_t* smem, LaGates* gates, float (&rowsum)[4][LA_C],
+                                            float (&colsum)[LA_C]) {
     using Sh = LaShape<T, DK>;
-    extern __shared__ __align__(16) uint8_t smem[];
     T* q = reinterpret_cast<T*>(smem);
     T* k = q + Sh::QK;
     T* v = k + Sh::QK;
     T* dout = v + Sh::V;
     T* ss = dout + Sh::V;
-    __shared__ LaGates gt;
-    __shared__ float rowsum[4][LA_C], colsum[LA_C];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = (warp + blockIdx.x) & 3;
-    const int seg = (int)(blockIdx.x % p.nseg);
-    const int64_t vh = blockIdx.x / p.nseg;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, rw = (int)(warp + block) & 3;
+    const int seg = (int)(block % p.nseg);
+    const int64_t vh = block / p.nseg;
     const int sl = (int)(vh % p.nsl), h = (int)(vh / p.nsl % p.H), b = (int)(vh / p.nsl / p.H);
     const int hk = h / (p.H / p.Hk), c0 = sl * LA_DV, cols = min(LA_DV, p.dv - c0), len = la_len(p, b);
     const int first = seg * p.segc, last = min(first + p.segc, p.nc);
@@ -220,11 +213,14 @@ __global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
 
     float D[Sh::MI][Sh::NI][4];
     la_state_read<T, DK>(D, p.nseg > 1 ? p.rseg + (bh * p.nseg + seg) * ssz : (p.ds ? p.ds + bh * ssz : nullptr), p, c0, rw, lane);
-    // the running dg (warp 0): tokens behind the row's end change nothing
-    double run = p.yseg[((int64_t)b * p.H * p.nsl + vhead) * p.nseg + seg];
-    const float* rin = p.rin + ((int64_t)b * p.H * p.nsl + vhead) * p.L;
-    for (int c = last - 1; c >= first; --c) {
-        const int t0 = c * LA_C, rows = min(LA_C, len - t0);
+    float* net = p.net + ((int64_t)b * p.H * p.nsl + vhead) * p.L;
+    const int n = last - first;
+    auto chunk = [&](int i) { return last - 1 - i; };
+    LaGateRing ring;
+    ring.start(gates, p, b, h, len, n, chunk, warp, lane);
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const int t0 = chunk(i) * LA_C, rows = min(LA_C, len - t0);
         __syncthreads();
         la_load<T, DK, Sh::LDK>(q, p.q, b, t0, hk, 0, rows, p.dk);
         la_load<T, DK, Sh::LDK>(k, p.k, b, t0, hk, 0, rows, p.dk);
@@ -232,13 +228,9 @@ __global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
         la_load<T, LA_DV, Sh::LDV>(dout, p.dout, b, t0, h, c0, rows, cols);
         cp_async_commit();
         la_state_share<T, DK, Planes<T>::N>(D, ss, rw, lane);
-        LaG g{};
-        if (warp == 0) {
-            g = la_load_g(p, b, h, t0, len, lane);
-            la_gates(gt, g, lane);
-        }
         cp_async_wait<0>();
         __syncthreads();
+        const LaGates& gt = ring.take(p, b, h, len, n, i, chunk, warp, lane);
         const int r0 = 16 * rw + (lane >> 2), tr = t0 + 16 * rw;
         // the scores of this warp's tokens s (rows) with the tokens t >= s (columns)
         float ps[8][4] = {}, as[8][4] = {};
@@ -268,36 +260,55 @@ __global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
                     mma(as[2 * j + 1], a, f[1]);
                 }
         }
-        const float h0 = gt.hi[r0], h1 = gt.hi[r0 + 8], l0 = gt.lo[r0], l1 = gt.lo[r0 + 8];
+        const float2 G0 = gt.G[r0], G1 = gt.G[r0 + 8];
+        const float2 Ge = gt.G[16 * rw + 15];
+        const float f0 = p.scale * gt.in_block[r0], f1 = p.scale * gt.in_block[r0 + 8];
         float cs0 = 0.f, cs1 = 0.f;                          // sums over t of this lane's two tokens s
         FragA<T> pf[4], af[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (j >= rw) {
+                float rs[4];                                 // this lane's two tokens s, for tokens t = 2t', 2t'+1, +8, +9
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const int t = 16 * j + 8 * x + 2 * (lane & 3) + e;
-                        const float ht = gt.hi[t], lt = gt.lo[t];
-                        const float m0 = t >= r0 ? p.scale * ex2((ht - h0) + (lt - l0)) : 0.f;
-                        const float m1 = t >= r0 + 8 ? p.scale * ex2((ht - h1) + (lt - l1)) : 0.f;
-                        float& p0 = ps[2 * j + x][e];
-                        float& p1 = ps[2 * j + x][2 + e];
-                        float& a0 = as[2 * j + x][e];
-                        float& a1 = as[2 * j + x][2 + e];
-                        a0 = t >= r0 ? a0 * m0 : 0.f;
-                        a1 = t >= r0 + 8 ? a1 * m1 : 0.f;
-                        const float x0 = t >= r0 ? a0 * p0 : 0.f, x1 = t >= r0 + 8 ? a1 * p1 : 0.f;
+                        const int tb = 8 * x + 2 * (lane & 3) + e, sb = lane >> 2;     // within the blocks
+                        const float2 Gt = gt.G[16 * j + tb];
+                        float m0, m1;                        // scale exp(G_t - G_s), split at the end of s's block
+                        if (j > rw) {
+                            const float d = la_decay(Gt, Ge);
+                            m0 = f0 * d;
+                            m1 = f1 * d;
+                        } else {
+                            m0 = tb >= sb ? p.scale * la_decay(Gt, G0) : 0.f;
+                            m1 = tb >= sb + 8 ? p.scale * la_decay(Gt, G1) : 0.f;
+                        }
+                        float p0 = ps[2 * j + x][e], p1 = ps[2 * j + x][2 + e], a0 = as[2 * j + x][e], a1 = as[2 * j + x][2 + e];
+                        if (j == rw) {                       // no value of a later token s comes in
+                            if (tb < sb) p0 = a0 = 0.f;
+                            if (tb < sb + 8) p1 = a1 = 0.f;
+                        }
+                        a0 *= m0;
+                        a1 *= m1;
+                        const float x0 = a0 * p0, x1 = a1 * p1;
                         cs0 += x0;
                         cs1 += x1;
-                        float rs = x0 + x1;                  // over this warp's 16 tokens s, for token t
-#pragma unroll
-                        for (int o = 4; o < 32; o *= 2) rs += __shfl_xor_sync(0xffffffffu, rs, o);
-                        if (lane < 4) rowsum[rw][t] = rs;
-                        p0 = t >= r0 ? p0 * m0 : 0.f;
-                        p1 = t >= r0 + 8 ? p1 * m1 : 0.f;
+                        rs[2 * x + e] = x0 + x1;
+                        as[2 * j + x][e] = a0;
+                        as[2 * j + x][2 + e] = a1;
+                        ps[2 * j + x][e] = p0 * m0;
+                        ps[2 * j + x][2 + e] = p1 * m1;
                     }
+                // over the 8 lanes that hold the same tokens t: half of the values each time
+                const bool up = lane & 16, mid = lane & 8;
+                float u0 = up ? rs[2] : rs[0], u1 = up ? rs[3] : rs[1];
+                u0 += __shfl_xor_sync(0xffffffffu, up ? rs[0] : rs[2], 16);
+                u1 += __shfl_xor_sync(0xffffffffu, up ? rs[1] : rs[3], 16);
+                float w = mid ? u1 : u0;
+                w += __shfl_xor_sync(0xffffffffu, mid ? u0 : u1, 8);
+                w += __shfl_xor_sync(0xffffffffu, w, 4);
+                if (!(lane & 4)) rowsum[rw][16 * j + (up ? 8 : 0) + 2 * (lane & 3) + (mid ? 1 : 0)] = w;
             } else if (lane < 16) {
                 rowsum[rw][16 * j + lane] = 0.f;
             }
@@ -330,11 +341,11 @@ __global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
             for (int j = 0; j < 4; ++j)
                 if (j >= rw) {
 #pragma unroll
-                    for (int n = 0; n < 4; ++n) {
+                    for (int c = 0; c < 4; ++c) {
                         FragB<T> f[2];
-                        load_b2_t(f, dout, Sh::LDV, 16 * n, 16 * j, lane);
-                        mma(dv[2 * n], pf[j], f[0]);
-                        mma(dv[2 * n + 1], pf[j], f[1]);
+                        load_b2_t(f, dout, Sh::LDV, 16 * c, 16 * j, lane);
+                        mma(dv[2 * c], pf[j], f[0]);
+                        mma(dv[2 * c + 1], pf[j], f[1]);
                     }
                 }
             // dk's part from the state reads this warp's rows of v first
@@ -357,39 +368,21 @@ __global__ void __launch_bounds__(LA_THREADS) la_dkv_kernel(const LaDev p) {
             for (int j = 0; j < 4; ++j)
                 if (j >= rw) {
 #pragma unroll
-                    for (int n = 0; n < DK / 16; ++n) {
+                    for (int c = 0; c < DK / 16; ++c) {
                         FragB<T> f[2];
-                        load_b2_t(f, q, Sh::LDK, 16 * n, 16 * j, lane);
-                        mma(dk[2 * n], af[j], f[0]);
-                        mma(dk[2 * n + 1], af[j], f[1]);
+                        load_b2_t(f, q, Sh::LDK, 16 * c, 16 * j, lane);
+                        mma(dk[2 * c], af[j], f[0]);
+                        mma(dk[2 * c + 1], af[j], f[1]);
                     }
                 }
             la_store_qk<T, DK>(dk, k, p.dk_out, p, b, hk, vhead, tr, len, rw, lane);
         }
-        la_state_update<T, DK>(D, q, dout, gt.pre, gt.all, p.scale, rw, lane);
+        la_state_update<T, DK, true>(D, q, dout, gt, p.scale, rw, lane);
+        ring.make(n, i, warp, lane);
         __syncthreads();                                     // the token sums are complete
-        if (warp == 0) {
-            const int ta = 2 * lane;
-            double d[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int t = ta + e;
-                d[e] = t0 + t < len ? (double)rin[t0 + t] + (((double)rowsum[0][t] + rowsum[1][t]) + ((double)rowsum[2][t] + rowsum[3][t])) - colsum[t]
-                                    : 0.;
-            }
-            double x = d[0] + d[1];                          // suffix sums over the chunk
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-                const double z = __shfl_down_sync(0xffffffffu, x, o);
-                if (lane + o < 32) x += z;
-            }
-            float* dg = p.dg + (int64_t)b * p.dg_sb + vhead * p.dg_sh + (int64_t)t0 * p.dg_sl;
-            // nothing crosses a reset (a decay of 0): no rounding noise there either
-            if (t0 + ta < p.L) dg[(int64_t)ta * p.dg_sl] = t0 + ta < len && !(g.g0 < -1000.f) ? (float)(run + x) : 0.f;
-            if (t0 + ta + 1 < p.L)
-                dg[(int64_t)(ta + 1) * p.dg_sl] = t0 + ta + 1 < len && !(g.g1 < -1000.f) ? (float)(run + x - d[0]) : 0.f;
-            run += __shfl_sync(0xffffffffu, x, 0);
-        }
+        const int t = threadIdx.x;
+        if (t < LA_C && t0 + t < p.L)
+            net[t0 + t] = ((rowsum[0][t] + rowsum[1][t]) + (rowsum[2][t] + rowsum[3][t])) - colsum[t];
     }
     if (p.ds0 && seg == 0) la_state_write<T, DK>(D, p.ds0 + bh * ssz, p, c0, rw, lane);
 }
@@ -408,49 +401,89 @@ __global__ void __launch_bounds__(256) la_group_sum_kernel(const float* src, T* 
     dst[i] = Elem<T>::from_f(x);
 }
 
-// The decay's gradient from the heads' parts [b][H nsl][L]: dst (b, L, H), the slices added in
-// order, or (per_head) dst (H), every row and token added in a fixed order in fp64.
-__global__ void __launch_bounds__(256) la_dg_sum_kernel(const float* src, float* dst, int b, int64_t L, int H, int nsl) {
-    const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-    if (i >= (int64_t)b * L * H) return;
-    const int64_t t = i % L, bh = i / L;
-    float x = 0.f;
-    for (int k = 0; k < nsl; ++k) x += src[(bh * nsl + k) * L + t];
-    dst[(bh / H * L + t) * H + bh % H] = x;
-}
-__global__ void __launch_bounds__(1024) la_dg_head_kernel(const float* src, float* dst, int b, int64_t L, int H, int nsl) {
-    __shared__ double red[32];
-    const int h = blockIdx.x;
-    double x = 0.;
-    for (int r = 0; r < b; ++r) {
-        const float* s = src + ((int64_t)r * H + h) * nsl * L;
-#pragma unroll 4
-        for (int64_t t = threadIdx.x; t < nsl * L; t += 1024) x += (double)s[t];
+// ------------------------------------------------------------------ dg
+// One CTA per segment of one head, from the segment's end: dg_t = <S, D> at the end + the sum of
+// q . dq - k . dk over the tokens from t on (fp64), v's slices added up; or, for a decay per
+// head, the segment's sum of it.
+constexpr int LG_THREADS = 256;
+
+__global__ void __launch_bounds__(LG_THREADS) la_dg_kernel(const LaDev p) {
+    __shared__ double ws[LG_THREADS / 32];
+    const int seg = blockIdx.x % p.nseg, h = blockIdx.x / p.nseg % p.H, b = blockIdx.x / p.nseg / p.H;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, len = la_len(p, b);
+    const int lo = seg * p.segc * LA_C, hi = min(p.L, (seg + 1) * p.segc * LA_C);
+    const int64_t v0 = ((int64_t)b * p.H + h) * p.nsl;
+    double run = 0., all = 0.;
+    for (int s = 0; s < p.nsl; ++s) run += (double)p.yseg[(v0 + s) * p.nseg + seg];
+    const float* g = p.g + (int64_t)b * p.g_sb + (int64_t)h * p.g_sh;
+    for (int t0 = hi; t0 > lo; t0 -= LG_THREADS) {
+        const int t = t0 - 1 - (int)threadIdx.x;             // thread 0: the last token
+        double x = 0.;
+        float gt = 0.f;
+        if (t >= lo && t < len) {
+            gt = g[(int64_t)t * p.g_sl];
+            for (int s = 0; s < p.nsl; ++s) x += (double)p.rin[(v0 + s) * p.L + t] + (double)p.net[(v0 + s) * p.L + t];
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const double z = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += z;
+        }
+        __syncthreads();
+        if (lane == 31) ws[warp] = x;
+        __syncthreads();
+        double before = run;
+        for (int w = 0; w < LG_THREADS / 32; ++w) {
+            if (w < warp) before += ws[w];
+            run += ws[w];
+        }
+        if (t >= lo) {
+            // nothing crosses a reset (a decay of 0): no rounding noise there either
+            const float d = t < len && !(gt < -1000.f) ? (float)(before + x) : 0.f;
+            if (p.dg) p.dg[((int64_t)b * p.L + t) * p.H + h] = d;
+            all += (double)d;
+        }
     }
+    if (p.dg) return;
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) all += __shfl_xor_sync(0xffffffffu, all, o);
+    __syncthreads();
+    if (lane == 0) ws[warp] = all;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < LG_THREADS / 32; ++w) all += ws[w];
+        p.dg_part[((int64_t)h * p.b + b) * p.nseg + seg] = all;
+    }
+}
+__global__ void __launch_bounds__(32) la_dg_head_kernel(const double* part, float* dst, int n) {
+    const double* s = part + (int64_t)blockIdx.x * n;
+    double x = 0.;
+    for (int i = threadIdx.x; i < n; i += 32) x += s[i];
 #pragma unroll
     for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
-    if (threadIdx.x % 32 == 0) red[threadIdx.x / 32] = x;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        x = red[threadIdx.x];
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (threadIdx.x == 0) dst[h] = (float)x;
-    }
+    if (threadIdx.x == 0) dst[blockIdx.x] = (float)x;
+}
+
+// Both walks in one launch, the longer ones (dk, dv) first.
+template <typename T, int DK>
+__global__ void __launch_bounds__(LA_THREADS, sizeof(T) == 4 ? 1 : DK == 128 ? 2 : 3) la_bwd_kernel(const LaDev p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ LaGates gates[LA_RING];
+    __shared__ float rowsum[4][LA_C], colsum[LA_C];
+    const int64_t half = gridDim.x / 2;
+    if (blockIdx.x < half) la_dkv_walk<T, DK>(p, blockIdx.x, smem, gates, rowsum, colsum);
+    else la_dq_walk<T, DK>(p, blockIdx.x - half, smem, gates, colsum);
 }
 
 template <typename T, int DK>
 static cudaError_t bwd(const LaDev& p, cudaStream_t st) {
     constexpr int smem = LaBwd<T, DK>::SMEM;
-    const unsigned grid = (unsigned)((int64_t)p.b * p.H * p.nsl * p.nseg);
-    auto kq = la_dq_kernel<T, DK>;
-    auto kk = la_dkv_kernel<T, DK>;
-    cudaError_t e = allow_smem(kq, smem);
-    if (e == cudaSuccess) e = allow_smem(kk, smem);
+    auto k = la_bwd_kernel<T, DK>;
+    cudaError_t e = allow_smem(k, smem);
     if (e != cudaSuccess) return e;
-    kq<<<grid, LA_THREADS, smem, st>>>(p);
+    k<<<(unsigned)((int64_t)p.b * p.H * p.nsl * p.nseg * 2), LA_THREADS, smem, st>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    kk<<<grid, LA_THREADS, smem, st>>>(p);
+    la_dg_kernel<<<(unsigned)(p.b * p.H * p.nseg), LG_THREADS, 0, st>>>(p);
     return cudaGetLastError();
 }
 
@@ -463,9 +496,8 @@ cudaError_t la_launch_bwd(const LaDev& p, int dtype, cudaStream_t st) {
     return dtype == SWX_DTYPE_F32 ? bwd_dk<float>(p, st) : bwd_dk<__nv_bfloat16>(p, st);
 }
 
-cudaError_t la_launch_dg_sum(const float* src, float* dst, bool per_head, int b, int64_t L, int H, int nsl, cudaStream_t st) {
-    if (per_head) la_dg_head_kernel<<<(unsigned)H, 1024, 0, st>>>(src, dst, b, L, H, nsl);
-    else la_dg_sum_kernel<<<(unsigned)(((int64_t)b * L * H + 255) / 256), 256, 0, st>>>(src, dst, b, L, H, nsl);
+cudaError_t la_launch_dg_head(const double* part, float* dst, int H, int n, cudaStream_t st) {
+    la_dg_head_kernel<<<(unsigned)H, 32, 0, st>>>(part, dst, n);
     return cudaGetLastError();
 }
 

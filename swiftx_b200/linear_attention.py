@@ -20,31 +20,32 @@ def _unit(t):
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _check(name, q, k, v, log_decay, state, token):
-    """Shapes, types and devices of an operand set; ``token``: without the sequence dimension."""
-    ts = [t for t in (q, k, v, log_decay, state) if t is not None]
-    if not all(t.is_cuda for t in ts):
+def _check(name, q, k, v, log_decay, state, lead):
+    """Shapes, types and devices of an operand set; ``lead``: the dimensions before the heads, (b) or (b, L)."""
+    dev = q.device
+    if dev.type != "cuda" or k.device != dev or v.device != dev or log_decay.device != dev \
+            or (state is not None and state.device != dev):
+        if all(t is None or t.is_cuda for t in (q, k, v, log_decay, state)):
+            raise ValueError(f"{name}: tensors on several devices")
         raise RuntimeError(f"swiftx_b200 {name} runs on CUDA tensors only (no CPU path)")
-    if any(t.device != q.device for t in ts):
-        raise ValueError(f"{name}: tensors on several devices")
-    lead = 1 if token else 2
-    n = lead + 2
-    if q.dim() != n or v.dim() != n or k.shape != q.shape or v.shape[:lead] != q.shape[:lead]:
-        raise ValueError(f"{name}: q, k {'(b, Hk, dk)' if token else '(b, L, Hk, dk)'} and v with its b{'' if token else ', L'} expected, "
-                         f"got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    hk, dk, h, dv = q.shape[-2], q.shape[-1], v.shape[-2], v.shape[-1]
+    qs, vs = q.shape, v.shape
+    if len(qs) != lead + 2 or len(vs) != lead + 2 or k.shape != qs or vs[:lead] != qs[:lead]:
+        raise ValueError(f"{name}: q, k {'(b, Hk, dk)' if lead == 1 else '(b, L, Hk, dk)'} and v with its b"
+                         f"{'' if lead == 1 else ', L'} expected, got {tuple(qs)}, {tuple(k.shape)} and {tuple(vs)}")
+    hk, dk = qs[lead:]
+    h, dv = vs[lead:]
     if hk < 1 or h < 1 or h % hk:
         raise ValueError(f"{name}: v's {h} heads are not a multiple of q's and k's {hk}")
     if not (1 <= dk <= MAX_DIM and 1 <= dv <= MAX_DIM):
         raise ValueError(f"{name}: dk and dv of 1 to {MAX_DIM} expected, got {dk} and {dv}")
     if q.dtype not in _DT or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError(f"{name}: q, k and v of one dtype, fp32 or bf16, expected, got {q.dtype}, {k.dtype} and {v.dtype}")
-    if log_decay.dtype != torch.float32 or tuple(log_decay.shape) not in ((h,), tuple(v.shape[:lead]) + (h,)):
-        raise ValueError(f"{name}: fp32 log_decay of shape {(h,)} or {tuple(v.shape[:lead]) + (h,)} expected, got "
-                         f"{log_decay.dtype} {tuple(log_decay.shape)}")
-    want = (v.shape[0], h, dk, dv)
-    if state is not None and (state.dtype != torch.float32 or tuple(state.shape) != want):
-        raise ValueError(f"{name}: fp32 state of shape {want} expected, got {state.dtype} {tuple(state.shape)}")
+    gs = log_decay.shape
+    if log_decay.dtype != torch.float32 or (gs != vs[:-1] and gs != vs[lead:-1]):
+        raise ValueError(f"{name}: fp32 log_decay of shape {(h,)} or {tuple(vs[:-1])} expected, got "
+                         f"{log_decay.dtype} {tuple(gs)}")
+    if state is not None and (state.dtype != torch.float32 or state.shape != (vs[0], h, dk, dv)):
+        raise ValueError(f"{name}: fp32 state of shape {(vs[0], h, dk, dv)} expected, got {state.dtype} {tuple(state.shape)}")
 
 
 def _args(q, k, v, g, scale):
@@ -60,31 +61,37 @@ def _args(q, k, v, g, scale):
     return a
 
 
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _forward(q, k, v, g, s0, lengths, scale, want_state):
+    """(out, the last state or None, the segments' start states or None) of checked operands."""
+    b, _, h, dv = v.shape
+    dk = q.shape[-1]
+    with _lib.on_device(v.device):
+        lib = _lib.load()
+        a = _args(q, k, v, g, scale)
+        n = lib.swx_linattn_segments(a)
+        if n < 0:
+            _lib.check(-n, "swx_linattn_segments")
+        out = v.new_empty(v.shape)
+        last = g.new_empty((b, h, dk, dv)) if want_state else None
+        seg = None
+        if n > 1:
+            seg = g.new_empty((b, h, n, dk, dv))
+            ws = g.new_empty(lib.swx_linattn_fwd_workspace_bytes(a) // 4)
+            a.seg_states, a.workspace, a.workspace_bytes = seg.data_ptr(), ws.data_ptr(), 4 * ws.numel()
+        a.lengths, a.initial_state, a.out, a.final_state = _ptr(lengths), _ptr(s0), out.data_ptr(), _ptr(last)
+        _lib.check(lib.swx_linattn_fwd(a, _lib.stream_ptr(v.device)), "swx_linattn_fwd")
+    return out, last, seg
+
+
 class LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
-        q, k, v = _unit(q), _unit(k), _unit(v)
-        g = log_decay
-        s0 = initial_state.contiguous() if initial_state is not None else None
-        b, _, h, dv = v.shape
-        dk = q.shape[-1]
-        with torch.cuda.device(v.device):
-            lib = _lib.load()
-            a = _args(q, k, v, g, scale)
-            n = lib.swx_linattn_segments(a)
-            if n < 0:
-                _lib.check(-n, "swx_linattn_segments")
-            f32 = dict(device=v.device, dtype=torch.float32)
-            out = torch.empty(v.shape, device=v.device, dtype=v.dtype)
-            last = torch.empty(b, h, dk, dv, **f32) if want_state else None
-            seg = torch.empty(b, h, n, dk, dv, **f32) if n > 1 else None
-            ws = torch.empty(max(1, lib.swx_linattn_fwd_workspace_bytes(a)), device=v.device, dtype=torch.uint8) if n > 1 else None
-            a.lengths, a.initial_state, a.out, a.final_state, a.seg_states = (
-                t.data_ptr() if t is not None else None for t in (lengths, s0, out, last, seg))
-            if ws is not None:
-                a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
-            _lib.check(lib.swx_linattn_fwd(a, _lib.stream_ptr(v.device)), "swx_linattn_fwd")
-        ctx.save_for_backward(q, k, v, g, s0, lengths, seg)
+        out, last, seg = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+        ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths, seg)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return out, last
@@ -93,21 +100,19 @@ class LinearAttentionFn(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, dlast):
         q, k, v, g, s0, lengths, seg = ctx.saved_tensors
-        if dout is None:
-            dout = torch.zeros_like(v)
-        dout = _unit(dout.to(v.dtype))
+        dout = torch.zeros_like(v) if dout is None else _unit(dout.to(v.dtype))
         dlast = dlast.float().contiguous() if dlast is not None else None
-        with torch.cuda.device(v.device):
+        with _lib.on_device(v.device):
             lib = _lib.load()
             a = _args(q, k, v, g, ctx.scale)
-            dense = lambda t: torch.empty(t.shape, device=t.device, dtype=t.dtype)  # noqa: E731
-            dq, dk, dv, dg = dense(q), dense(k), dense(v), dense(g)
-            ds0 = dense(s0) if s0 is not None and ctx.needs_input_grad[4] else None
-            ws = torch.empty(max(1, lib.swx_linattn_bwd_workspace_bytes(a)), device=v.device, dtype=torch.uint8)
-            a.lengths, a.initial_state, a.seg_states, a.dout, a.dfinal_state, a.dq, a.dk_out, a.dv_out, a.dlog_decay, a.dinitial_state = (
-                t.data_ptr() if t is not None else None for t in (lengths, s0, seg, dout, dlast, dq, dk, dv, dg, ds0))
-            a.do_sb, a.do_sl, a.do_sh = dout.stride()[:3]
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+            dq, dk, dv, dg = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), g.new_empty(g.shape)
+            ds0 = s0.new_empty(s0.shape) if s0 is not None and ctx.needs_input_grad[4] else None
+            ws = g.new_empty(lib.swx_linattn_bwd_workspace_bytes(a) // 4)
+            a.lengths, a.initial_state, a.seg_states, a.dfinal_state = _ptr(lengths), _ptr(s0), _ptr(seg), _ptr(dlast)
+            a.dout, (a.do_sb, a.do_sl, a.do_sh) = dout.data_ptr(), dout.stride()[:3]
+            a.dq, a.dk_out, a.dv_out, a.dlog_decay = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), dg.data_ptr()
+            a.dinitial_state = _ptr(ds0)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), 4 * ws.numel()
             _lib.check(lib.swx_linattn_bwd(a, _lib.stream_ptr(v.device)), "swx_linattn_bwd")
         return dq, dk, dv, dg, ds0, None, None, None
 
@@ -124,28 +129,34 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
     fp32 state after the last token.  Differentiable in q, k, v, log_decay and initial_state;
     deterministic.  bf16 inputs: the score tiles are rounded to bf16 once, states and log_decay's gradient
     keep fp32 accuracy."""
-    _check("linear_attention", q, k, v, log_decay, initial_state, token=False)
+    _check("linear_attention", q, k, v, log_decay, initial_state, 2)
     if lengths is not None:
         if lengths.dtype != torch.int64 or tuple(lengths.shape) != (v.shape[0],) or lengths.device != v.device:
             raise ValueError(f"linear_attention: int64 lengths of shape {(v.shape[0],)} on {v.device} expected, got "
                              f"{lengths.dtype} {tuple(lengths.shape)} on {lengths.device}")
         lengths = lengths.contiguous()
-    out, state = LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    if initial_state is not None:
+        initial_state = initial_state.contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
+                                    or (initial_state is not None and initial_state.requires_grad)):
+        out, state = LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
+    else:
+        out, state, _ = _forward(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
     return (out, state) if return_state else out
 
 
-@torch.no_grad()
 def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
     """One token of ``linear_attention`` for every row: q, k (b, Hk, dk), v (b, H, dv), log_decay
     (b, H) or (H,); ``state``, a dense fp32 (b, H, dk, dv) tensor (as linear_attention returns it), is updated
     in place.  Returns out (b, H, dv) in v's dtype.  Not differentiable."""
-    _check("linear_attention_step", q, k, v, log_decay, state, token=True)
+    _check("linear_attention_step", q, k, v, log_decay, state, 1)
     if not state.is_contiguous():
         raise ValueError("linear_attention_step: state must be a dense (b, H, dk, dv) tensor")
     q, k, v = _unit(q), _unit(k), _unit(v)
-    with torch.cuda.device(v.device):
+    with _lib.on_device(v.device):
         lib = _lib.load()
-        out = torch.empty(v.shape, device=v.device, dtype=v.dtype)
+        out = v.new_empty(v.shape)
         a = _lib.LinattnArgs()
         a.batch, a.heads, a.dv = v.shape
         a.seqlen, (a.qk_heads, a.dk) = 1, q.shape[1:]

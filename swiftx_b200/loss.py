@@ -28,13 +28,30 @@ def _args(x, w, targets, ignore_index, reduction):
     return a
 
 
-def _workspace(lib, name, a, device):
+def _workspace(lib, name, a, like):
     n = getattr(lib, name)(a)
     if n < 0:
         _lib.check(-n, name)
-    ws = torch.empty(max(n, 1), device=device, dtype=torch.uint8)
+    ws = like.new_empty(n // 4 + 1)
     a.workspace, a.workspace_bytes = ws.data_ptr(), n
     return ws
+
+
+def _forward(x, w, targets, ignore_index, reduction):
+    """(loss, (row maxima, reciprocal row sums, count) in one buffer) of checked operands."""
+    T = x.shape[0]
+    with _lib.on_device(x.device):
+        lib = _lib.load()
+        none = reduction == _lib.XENT_REDUCTIONS["none"]
+        loss = x.new_empty((T,) if none else (), dtype=torch.float32)
+        stats = loss.new_empty(2 * T + 1)
+        a = _args(x, w, targets, ignore_index, reduction)
+        a.loss = loss.data_ptr()
+        a.row_max = stats.data_ptr()
+        a.row_rsum, a.count = a.row_max + 4 * T, a.row_max + 8 * T
+        ws = _workspace(lib, "swx_xent_fwd_workspace_bytes", a, loss)  # noqa: F841
+        _lib.check(lib.swx_xent_fwd(a, _lib.stream_ptr(x.device)), "swx_xent_fwd")
+    return loss, stats
 
 
 class LinearCrossEntropyFn(torch.autograd.Function):
@@ -42,36 +59,28 @@ class LinearCrossEntropyFn(torch.autograd.Function):
     def forward(ctx, x, weight, targets, ignore_index, reduction):
         w = weight if weight.dtype == x.dtype else weight.to(x.dtype)
         x, w, targets = _rows(x), _rows(w), targets.contiguous()
-        none = reduction == _lib.XENT_REDUCTIONS["none"]
-        with torch.cuda.device(x.device):
-            lib = _lib.load()
-            new = lambda *s: torch.empty(s, device=x.device, dtype=torch.float32)  # noqa: E731
-            T = x.shape[0]
-            loss, count, stats = new(T) if none else new(), new(1), new(2, T)
-            a = _args(x, w, targets, ignore_index, reduction)
-            a.loss, a.count, a.row_max, a.row_rsum = loss.data_ptr(), count.data_ptr(), stats[0].data_ptr(), stats[1:].data_ptr()
-            ws = _workspace(lib, "swx_xent_fwd_workspace_bytes", a, x.device)  # noqa: F841
-            _lib.check(lib.swx_xent_fwd(a, _lib.stream_ptr(x.device)), "swx_xent_fwd")
-        ctx.save_for_backward(x, w, targets, stats, count)
+        loss, stats = _forward(x, w, targets, ignore_index, reduction)
+        ctx.save_for_backward(x, w, targets, stats)
         ctx.opts = (ignore_index, reduction, weight.dtype)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, w, targets, stats, count = ctx.saved_tensors
+        x, w, targets, stats = ctx.saved_tensors
         ignore_index, reduction, w_dtype = ctx.opts
         dloss = dloss.float().contiguous()
-        with torch.cuda.device(x.device):
+        with _lib.on_device(x.device):
             lib = _lib.load()
-            dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if ctx.needs_input_grad[0] else None
-            dw = torch.empty(w.shape, device=x.device, dtype=w_dtype) if ctx.needs_input_grad[1] else None
+            dx = x.new_empty(x.shape) if ctx.needs_input_grad[0] else None
+            dw = w.new_empty(w.shape, dtype=w_dtype) if ctx.needs_input_grad[1] else None
             a = _args(x, w, targets, ignore_index, reduction)
-            a.count, a.row_max, a.row_rsum = count.data_ptr(), stats[0].data_ptr(), stats[1:].data_ptr()
+            a.row_max = stats.data_ptr()
+            a.row_rsum, a.count = a.row_max + 4 * x.shape[0], a.row_max + 8 * x.shape[0]
             a.dw_dtype, a.dloss = _DT[w_dtype], dloss.data_ptr()
             a.dx = dx.data_ptr() if dx is not None else None
             a.dweight = dw.data_ptr() if dw is not None else None
-            ws = _workspace(lib, "swx_xent_bwd_workspace_bytes", a, x.device)  # noqa: F841
+            ws = _workspace(lib, "swx_xent_bwd_workspace_bytes", a, stats)  # noqa: F841
             _lib.check(lib.swx_xent_bwd(a, _lib.stream_ptr(x.device)), "swx_xent_bwd")
         return dx, dw, None, None, None
 
@@ -106,6 +115,10 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     if x.dtype not in _DT or weight.dtype not in _DT or (x.dtype == torch.float32 and weight.dtype != torch.float32):
         raise ValueError(f"linear_cross_entropy: fp32 x and weight, or bf16 x with a bf16 or fp32 weight expected, got "
                          f"{x.dtype} and {weight.dtype}")
-    loss = LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, targets.reshape(-1), int(ignore_index),
-                                      _lib.XENT_REDUCTIONS[reduction])
+    args = (x.reshape(-1, x.shape[-1]), weight, targets.reshape(-1), int(ignore_index), _lib.XENT_REDUCTIONS[reduction])
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        loss = LinearCrossEntropyFn.apply(*args)
+    else:
+        x, weight, targets_1d = _rows(args[0]), _rows(weight.to(x.dtype)), args[2].contiguous()
+        loss = _forward(x, weight, targets_1d, *args[3:])[0]
     return loss.view(targets.shape) if reduction == "none" else loss
