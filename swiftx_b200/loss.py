@@ -56,8 +56,8 @@ def _forward(x, w, targets, ignore_index, reduction):
 
 class LinearCrossEntropyFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, targets, ignore_index, reduction):
-        w = weight if weight.dtype == x.dtype else weight.to(x.dtype)
+    def forward(ctx, x, weight, targets, ignore_index, reduction, weight16=None):
+        w = weight if weight.dtype == x.dtype else weight.to(x.dtype) if weight16 is None else weight16
         x, w, targets = _rows(x), _rows(w), targets.contiguous()
         loss, stats = _forward(x, w, targets, ignore_index, reduction)
         ctx.save_for_backward(x, w, targets, stats)
@@ -82,21 +82,22 @@ class LinearCrossEntropyFn(torch.autograd.Function):
             a.dweight = dw.data_ptr() if dw is not None else None
             ws = _workspace(lib, "swx_xent_bwd_workspace_bytes", a, stats)  # noqa: F841
             _lib.check(lib.swx_xent_bwd(a, _lib.stream_ptr(x.device)), "swx_xent_bwd")
-        return dx, dw, None, None, None
+        return dx, dw, None, None, None, None
 
 
-def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
+def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean", weight16=None):
     """``F.cross_entropy(F.linear(x, weight).float(), targets)`` without the logits (CUDA only).
 
     x (..., d) and weight (vocab, d), fp32 or bf16; targets (...) int64.  Returns the fp32
     loss: its mean over the tokens that count, their sum, or (reduction "none") one value
     for each token, 0 at ignored ones.  bf16 operands give the products of bf16 values summed in
-    fp32; fp32 operands keep fp32 accuracy.  With bf16 x an fp32 weight is rounded to bf16 for
+    fp32; fp32 operands keep fp32 accuracy and have to be finite (an infinity gives NaN).  With bf16 x an fp32 weight is rounded to bf16 for
     the products (what autocast's linear does) and its gradient comes back in fp32, not
     rounded; under bf16 autocast an fp32 x is cast too.  The gradients are deterministic.
 
     A target outside [0, vocab) other than ignore_index gives a NaN loss (and gradients)
-    instead of a device-side assertion; x has to be finite in ignored rows too."""
+    instead of a device-side assertion; x has to be finite in ignored rows too.  weight16: a bf16
+    copy of an fp32 weight that the caller keeps (used with bf16 x instead of rounding again)."""
     if reduction not in _lib.XENT_REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r}: one of none, mean, sum expected")
     if not (x.is_cuda and weight.is_cuda and targets.is_cuda):
@@ -115,10 +116,13 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     if x.dtype not in _DT or weight.dtype not in _DT or (x.dtype == torch.float32 and weight.dtype != torch.float32):
         raise ValueError(f"linear_cross_entropy: fp32 x and weight, or bf16 x with a bf16 or fp32 weight expected, got "
                          f"{x.dtype} and {weight.dtype}")
-    args = (x.reshape(-1, x.shape[-1]), weight, targets.reshape(-1), int(ignore_index), _lib.XENT_REDUCTIONS[reduction])
+    if weight16 is not None and (weight16.dtype != torch.bfloat16 or weight16.shape != weight.shape or weight16.device != x.device):
+        raise ValueError(f"linear_cross_entropy: weight16 is a bf16 copy of the {tuple(weight.shape)} weight, got {weight16.dtype} "
+                         f"{tuple(weight16.shape)}")
+    x2, t1, opts = x.reshape(-1, x.shape[-1]), targets.reshape(-1), (int(ignore_index), _lib.XENT_REDUCTIONS[reduction])
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        loss = LinearCrossEntropyFn.apply(*args)
+        loss = LinearCrossEntropyFn.apply(x2, weight, t1, *opts, weight16)
     else:
-        x, weight, targets_1d = _rows(args[0]), _rows(weight.to(x.dtype)), args[2].contiguous()
-        loss = _forward(x, weight, targets_1d, *args[3:])[0]
+        w = weight if weight.dtype == x.dtype else weight.to(x.dtype) if weight16 is None else weight16
+        loss = _forward(_rows(x2), _rows(w), t1.contiguous(), *opts)[0]
     return loss.view(targets.shape) if reduction == "none" else loss

@@ -36,6 +36,7 @@ from . import embedding as embedding_kernels
 from . import norm as norm_kernels
 from .conv import causal_conv1d_fn, conv1d_backward, conv1d_forward
 from .decode import decode_conv_step, decode_layer_step, decode_ssm_step
+from .loss import linear_cross_entropy
 from .selective_scan import scan_backward, scan_forward, selective_scan_fn
 
 
@@ -510,6 +511,25 @@ class SiftLM(nn.Module):
         the head's are cast to bf16 once per forward, in two launches, and the projections
         run through _Bf16Linear: the same bf16 GEMMs as autocast, without its per-call
         weight casts, and with fp32 weight gradients from the GEMM itself."""
+        logits = self._run(idx, lambda h: _linear(h, self.lm_head.weight, self.lm_head.bias))
+        loss = None
+        if targets is not None:
+            loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)).float(), targets.reshape(-1))
+        return logits, loss
+
+    def loss(self, idx, targets):
+        """forward(idx, targets)[1] without the logits: the head's product and the cross
+        entropy through ``linear_cross_entropy``, which keeps two floats per token instead of
+        (tokens, vocab) logits and their gradient.  Under bf16 autocast the gradients are of
+        the fp32 softmax (forward's pass through bf16 logits), the head's weight gradient in fp32."""
+        w = self.lm_head.weight
+        if not (w.is_cuda and self.lm_head.bias is None and w.dtype in (torch.float32, torch.bfloat16)):
+            return self(idx, targets)[1]
+        return self._run(idx, lambda h: linear_cross_entropy(
+            h, w, targets, weight16=_W16.get(id(w)) if _W16 is not None and w.dtype == torch.float32 else None))
+
+    def _run(self, idx, head):
+        """head(the final norm's output), with the bf16 weight copies of forward."""
         global _W16
         w = self.embedding.weight
         if embedding_kernels.supported(idx, w) and torch.is_grad_enabled():
@@ -523,13 +543,9 @@ class SiftLM(nn.Module):
             if ws is not None:
                 _W16 = _bf16_copies(ws)
         try:
-            logits = _linear(self.backbone(x), self.lm_head.weight, self.lm_head.bias)
+            return head(self.backbone(x))
         finally:
             _W16 = prev
-        loss = None
-        if targets is not None:
-            loss = F.cross_entropy(logits.reshape(-1, logits.size(-1)).float(), targets.reshape(-1))
-        return logits, loss
 
     def projection_weights(self):
         """The fp32 weights that have bf16 copies under bf16 autocast: every block's
