@@ -471,10 +471,10 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  * fp32, dense (batch, heads, dk, dv).  lengths (batch), optional: row i has min(max(lengths[i], 0),
  * seqlen) tokens; what lies behind them is not used (it may be NaN), gives zeros in out and in the gradients, and
  * leaves the state as it was.
- * The sequence is walked in chunks of 64 tokens on the tensor cores; few rows and heads are cut
- * into swx_linattn_segments(args) segments walked in parallel, whose start states the forward
- * leaves in seg_states (batch, heads, segments, dk, dv) for the backward (both need the buffer
- * when there are 2 segments or more).  bf16 inputs: scores are rounded to bf16 once; states and the decay's
+ * The sequence is walked in chunks of 64 or 128 tokens on the tensor cores, cut into segments that are
+ * walked in parallel where there are few rows and heads.  The forward leaves the states at the start of the
+ * backward's swx_linattn_segments(args) segments in seg_states, fp32 (batch, heads, segments, dk,
+ * dv), when it is given; the backward needs them where there are 2 segments or more.  bf16 inputs: scores are rounded to bf16 once; states and the decay's
  * gradient keep fp32 accuracy.  fp32 inputs: about 22-bit products.  Deterministic.
  * Backward outputs are dense: dq, dk_out (batch, seqlen, qk_heads, dk) and dv_out in dtype,
  * dlog_decay fp32, (batch, seqlen, heads), or (heads) with decay_per_head, where log_decay is one
@@ -503,7 +503,7 @@ typedef struct swx_linattn_args {
 } swx_linattn_args;
 
 int64_t swx_linattn_args_size(void);
-/* Segments of the sequence for these sizes; a negated status code for sizes that are refused. */
+/* Segments of the backward for these sizes; a negated status code for sizes that are refused. */
 int swx_linattn_segments(const swx_linattn_args* args);
 int64_t swx_linattn_fwd_workspace_bytes(const swx_linattn_args* args);
 int64_t swx_linattn_bwd_workspace_bytes(const swx_linattn_args* args);

@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(LA_THREADS, sizeof(T) == 4 ? 1 : DK == 128 ? 2
 #pragma unroll 1
     for (int i = 0; i < n; ++i) {
         const int u = i & 1, t0 = (first + i) * LA_C;
+        la_state_save<T, DK>(S, p, bh, first + i, c0, rw, lane);
         cp_async_wait<0>();
         __syncthreads();
         if (i + 1 < n) load(i + 1);
@@ -193,8 +194,8 @@ __global__ void __launch_bounds__(LA_THREADS, sizeof(T) == 4 ? 1 : DK == 128 ? 2
         ring.make(n, i, warp, lane);
     }
     // rows behind the row's last token
-    for (int t = max(live, first) * LA_C; t < min(last * LA_C, p.L); ++t)
-        for (int c = threadIdx.x; c < cols; c += LA_THREADS) out[((int64_t)b * p.L + t) * o_sl + (int64_t)h * p.dv + c0 + c] = T(0.f);
+    for (int c = live; c < last; ++c) la_state_save<T, DK>(S, p, bh, c, c0, rw, lane);
+    la_zero_rows<T>(p, b, h, c0, cols, live * LA_C, min(last * LA_C, p.L), threadIdx.x, LA_THREADS);
     if (p.s_last && seg == p.nseg - 1) la_state_write<T, DK>(S, p.s_last + bh * ssz, p, c0, rw, lane);
 }
 
@@ -216,9 +217,6 @@ static cudaError_t state(const LaDev& p, cudaStream_t st) {
     cudaError_t e = allow_smem(k, smem);
     if (e != cudaSuccess) return e;
     k<<<(unsigned)((int64_t)p.b * p.H * p.nsl * (p.nseg - 1)), LA_THREADS, smem, st>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    const int64_t per = ((int64_t)p.dk * p.dv + 255) / 256;
-    la_chain_kernel<<<(unsigned)((int64_t)p.b * p.H * per), 256, 0, st>>>(p, REV);
     return cudaGetLastError();
 }
 
@@ -232,11 +230,21 @@ static cudaError_t state_dk(const LaDev& p, cudaStream_t st) {
 }
 
 cudaError_t la_launch_fwd(const LaDev& p, int dtype, cudaStream_t st) {
-    return dtype == SWX_DTYPE_F32 ? fwd_dk<float>(p, st) : fwd_dk<__nv_bfloat16>(p, st);
+    if (dtype == SWX_DTYPE_F32) return fwd_dk<float>(p, st);
+    bool taken = false;
+    const cudaError_t e = lt_launch_fwd(p, &taken, st);
+    return taken ? e : fwd_dk<__nv_bfloat16>(p, st);
 }
 cudaError_t la_launch_state(const LaDev& p, int dtype, bool reverse, cudaStream_t st) {
-    if (dtype == SWX_DTYPE_F32) return reverse ? state_dk<float, true>(p, st) : state_dk<float, false>(p, st);
-    return reverse ? state_dk<__nv_bfloat16, true>(p, st) : state_dk<__nv_bfloat16, false>(p, st);
+    cudaError_t e;
+    bool taken = false;
+    if (dtype == SWX_DTYPE_F32) e = reverse ? state_dk<float, true>(p, st) : state_dk<float, false>(p, st);
+    else if ((e = lt_launch_state(p, reverse, &taken, st)), !taken)
+        e = reverse ? state_dk<__nv_bfloat16, true>(p, st) : state_dk<__nv_bfloat16, false>(p, st);
+    if (e != cudaSuccess) return e;
+    const int64_t per = ((int64_t)p.dk * p.dv + 255) / 256;
+    la_chain_kernel<<<(unsigned)((int64_t)p.b * p.H * per), 256, 0, st>>>(p, reverse);
+    return cudaGetLastError();
 }
 
 }  // namespace swx

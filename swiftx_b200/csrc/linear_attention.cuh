@@ -24,7 +24,8 @@ struct LaTensor { const void* p; int64_t sb, sl, sh; bool vec; };
 
 struct LaDev {
     int b, L, H, Hk, dk, dv, nsl;         // nsl: slices of 64 columns of v
-    int nc, nseg, segc;                   // chunks; segments; chunks per segment
+    int nc, nseg, segc;                   // chunks; segments; chunks per segment (even)
+    bool tc;                              // the pipelined kernels, where the tensors allow it
     LaTensor q, k, v, dout;
     const float* g; int64_t g_sb, g_sl, g_sh;
     const int64_t* lengths;
@@ -33,6 +34,8 @@ struct LaDev {
     void* out;                            // (b, L, H, dv)
     float* s_last;                        // (b, H, dk, dv) or null
     float* seg;                           // (b, H, nseg, dk, dv): the state at each segment's start
+    float* save;                          // the forward for the backward: (b, H, save_n, dk, dv), the state at
+    int save_n, save_c;                   // each save_c-th chunk's start, or null
     float* rseg;                          // the same for the reverse pass: its gradient at each segment's end
     float* dec;                           // (b, H, nseg): each segment's decay
     // backward
@@ -252,6 +255,14 @@ __device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][L
     }
 }
 
+// The state before chunk c, kept for the backward's segment that starts there.
+template <typename T, int DK>
+__device__ __forceinline__ void la_state_save(const float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], const LaDev& p, int64_t bh, int c,
+                                              int c0, int rw, int lane) {
+    if (p.save && c % p.save_c == 0)
+        la_state_write<T, DK>(S, p.save + (bh * p.save_n + c / p.save_c) * p.dk * p.dv, p, c0, rw, lane);
+}
+
 template <typename T, int DK, int PLANES>
 __device__ __forceinline__ void la_state_share(const float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], T* s, int rw, int lane) {
     using Sh = LaShape<T, DK>;
@@ -286,12 +297,30 @@ __device__ __forceinline__ void la_store(const T* s, T* g, int64_t sl, int rows,
     __syncwarp();
 }
 
+// Tokens t0 .. t1 - 1 of one head's output columns: zeros, by `threads` threads of which this is `tid`.
+template <typename T>
+__device__ __forceinline__ void la_zero_rows(const LaDev& p, int b, int h, int c0, int cols, int t0, int t1, int tid, int threads) {
+    const int64_t sl = (int64_t)p.H * p.dv;
+    T* out = static_cast<T*>(p.out) + ((int64_t)b * p.L + t0) * sl + (int64_t)h * p.dv + c0;
+    if (p.vec_o) {
+        constexpr int E = 16 / sizeof(T);
+        const int per = cols / E;
+        for (int i = tid; i < (t1 - t0) * per; i += threads)
+            *reinterpret_cast<uint4*>(out + (int64_t)(i / per) * sl + i % per * E) = make_uint4(0, 0, 0, 0);
+    } else {
+        for (int i = tid; i < (t1 - t0) * cols; i += threads) out[(int64_t)(i / cols) * sl + i % cols] = T(0.f);
+    }
+}
+
 __device__ __forceinline__ int la_len(const LaDev& p, int b) {
     if (!p.lengths) return p.L;
     const int64_t n = p.lengths[b];
     return n < 0 ? 0 : (n < p.L ? (int)n : p.L);
 }
 
+// linear_attention_tc.cu, bf16: *taken says whether it ran
+cudaError_t lt_launch_fwd(const LaDev& p, bool* taken, cudaStream_t st);
+cudaError_t lt_launch_state(const LaDev& p, bool reverse, bool* taken, cudaStream_t st);
 cudaError_t la_launch_fwd(const LaDev& p, int dtype, cudaStream_t st);
 cudaError_t la_launch_bwd(const LaDev& p, int dtype, cudaStream_t st);
 cudaError_t la_launch_state(const LaDev& p, int dtype, bool reverse, cudaStream_t st);

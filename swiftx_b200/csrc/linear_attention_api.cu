@@ -82,20 +82,37 @@ __global__ void __launch_bounds__(LS_THREADS) la_step_kernel(const LaStep p) {
 }
 
 // ------------------------------------------------------------------ plans
-struct LaPlan { int nsl, nc, nseg, segc; };
+// Segments of one direction: `nseg` of `segc` chunks of 64 tokens (an even number).
+struct LaCut { int nseg, segc; };
+struct LaPlan { int nsl, nc; bool tc; LaCut fwd, bwd; };
+
+static LaCut la_cut(int nc, int64_t n) {
+    n = std::max<int64_t>(1, std::min<int64_t>(n, nc / 2));
+    LaCut c;
+    c.segc = (int)((nc + n - 1) / n + 1) / 2 * 2;
+    c.nseg = (nc + c.segc - 1) / std::max(1, c.segc);
+    return c;
+}
 
 // One CTA walks a segment of one head's sequence.  Where the heads leave SMs idle the sequence is
-// cut, so that the CTAs fill, and do not exceed, one round of three CTAs (two with dk > 64) on each
-// of 148 SMs, with at least two chunks per segment: the states at the segments' starts cost one
-// more reading of k and v.
+// cut, so that the CTAs fill, and do not exceed, one round on 148 SMs; the states at the segments'
+// starts cost one more reading of k and v.
+// The pipelined kernels (linear_attention_tc.cu, one CTA per SM, chunks of 128 tokens) need a few
+// chunks to fill; they are taken from 4 chunks a walk (8 where the heads alone take several rounds) and
+// 256 chunks in all.  us, theirs against the other kernels', forward, heads of 64: 144 heads x 512
+// tokens 26 / 42, x 4096 101 / 168; 64 heads x 2048 56 / 62; 256 heads x 1024 63 / 68, x 512
+// 37 / 37; 640 heads x 512 90 / 79; 1 head x 16384 (128 chunks) 40 / 33.
+// The other kernels have three CTAs on an SM (two with dk > 64 or fp32); the backward runs two walks at
+// once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).
 static LaPlan la_plan(const swx_linattn_args* a) {
     LaPlan q{};
     q.nsl = (int)((a->dv + LA_DV - 1) / LA_DV);
     q.nc = (int)((a->seqlen + LA_C - 1) / LA_C);
-    const int64_t heads = a->batch * a->heads * q.nsl, target = 148 * (a->dk > 64 ? 2 : 3);
-    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(target / heads, q.nc / 2));
-    q.segc = (int)((q.nc + n - 1) / n);
-    q.nseg = (q.nc + q.segc - 1) / std::max(1, q.segc);
+    const int64_t heads = a->batch * a->heads * q.nsl, chunks = (q.nc + 1) / 2;
+    q.tc = a->dtype == SWX_DTYPE_BF16 && a->dk <= 64 && chunks >= (heads > 148 ? 8 : 4) && heads * chunks >= 256;
+    const int64_t slots = 148 * (a->dk > 64 || a->dtype == SWX_DTYPE_F32 ? 2 : 3);
+    q.fwd = la_cut(q.nc, q.tc ? std::min<int64_t>(148 / heads, chunks / 4) : slots / heads);
+    q.bwd = la_cut(q.nc, slots / heads);
     return q;
 }
 
@@ -109,23 +126,24 @@ static int la_check(const swx_linattn_args* a) {
     return SWX_OK;
 }
 
-struct LaWs { int64_t dec, rseg, rin, net, yseg, dg, dq, dk, total; };
+struct LaWs { int64_t dec, seg, rin, net, yseg, dg, dq, dk, total; };
 
 static int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
 
 static bool la_shared(const swx_linattn_args* a, const LaPlan& q) { return a->heads != a->qk_heads || q.nsl > 1; }
 
+// The backward's scratch: `seg` holds the gradient of the state at each segment's end.
 static LaWs la_ws(const swx_linattn_args* a, const LaPlan& q) {
     LaWs w{};
     const int64_t bh = a->batch * a->heads, bv = bh * q.nsl;
     int64_t o = 0;
     auto take = [&](int64_t floats) { const int64_t at = o; o += up(floats * 4); return at; };
-    w.dec = take(bh * q.nseg);
-    w.rseg = take(q.nseg > 1 ? bh * q.nseg * a->dk * a->dv : 0);
+    w.dec = take(bh * q.bwd.nseg);
+    w.seg = take(q.bwd.nseg > 1 ? bh * q.bwd.nseg * a->dk * a->dv : 0);
     w.rin = take(bv * a->seqlen);
     w.net = take(bv * a->seqlen);
-    w.yseg = take(bv * q.nseg);
-    w.dg = take(a->decay_per_head ? 2 * bh * q.nseg : 0);
+    w.yseg = take(bv * q.bwd.nseg);
+    w.dg = take(a->decay_per_head ? 2 * bh * q.bwd.nseg : 0);
     w.dq = take(la_shared(a, q) ? bv * a->seqlen * a->dk : 0);
     w.dk = take(la_shared(a, q) ? bv * a->seqlen * a->dk : 0);
     w.total = o;
@@ -138,18 +156,18 @@ static LaTensor la_tensor(const void* p, int64_t sb, int64_t sl, int64_t sh, int
     return t;
 }
 
-static LaDev la_pack(const swx_linattn_args* a, const LaPlan& q) {
+static LaDev la_pack(const swx_linattn_args* a, const LaPlan& q, const LaCut& c) {
     LaDev p{};
     const int es = a->dtype == SWX_DTYPE_F32 ? 4 : 2;
     p.b = (int)a->batch; p.L = (int)a->seqlen; p.H = (int)a->heads; p.Hk = (int)a->qk_heads; p.dk = (int)a->dk; p.dv = (int)a->dv;
-    p.nsl = q.nsl; p.nc = q.nc; p.nseg = q.nseg; p.segc = q.segc;
+    p.nsl = q.nsl; p.tc = q.tc; p.nc = q.nc; p.nseg = c.nseg; p.segc = c.segc;
     p.q = la_tensor(a->q, a->q_sb, a->q_sl, a->q_sh, a->batch, a->seqlen, a->qk_heads, es);
     p.k = la_tensor(a->k, a->k_sb, a->k_sl, a->k_sh, a->batch, a->seqlen, a->qk_heads, es);
     p.v = la_tensor(a->v, a->v_sb, a->v_sl, a->v_sh, a->batch, a->seqlen, a->heads, es);
     p.dout = la_tensor(a->dout, a->do_sb, a->do_sl, a->do_sh, a->batch, a->seqlen, a->heads, es);
     p.g = a->log_decay; p.g_sb = a->g_sb; p.g_sl = a->g_sl; p.g_sh = a->g_sh;
     p.lengths = a->lengths; p.scale = a->scale; p.s0 = a->initial_state; p.out = a->out; p.s_last = a->final_state;
-    p.seg = a->seg_states; p.ds = a->dfinal_state; p.ds0 = a->dinitial_state;
+    p.ds = a->dfinal_state; p.ds0 = a->dinitial_state;
     auto whole = [es](const void* o, int64_t d) { return (reinterpret_cast<uintptr_t>(o) & 15) == 0 && (d * es) % 16 == 0; };
     p.vec_o = whole(a->out, a->dv) && whole(a->dv_out, a->dv);
     p.vec_qk = whole(a->dq, a->dk) && whole(a->dk_out, a->dk);
@@ -167,13 +185,15 @@ int64_t swx_linattn_args_size(void) { return (int64_t)sizeof(swx_linattn_args); 
 int swx_linattn_segments(const swx_linattn_args* a) {
     const int c = la_check(a);
     if (c != SWX_OK) return -c;
-    return a->batch * a->seqlen == 0 ? 1 : la_plan(a).nseg;
+    return a->batch * a->seqlen == 0 ? 1 : la_plan(a).bwd.nseg;
 }
 
 int64_t swx_linattn_fwd_workspace_bytes(const swx_linattn_args* a) {
     const int c = la_check(a);
     if (c != SWX_OK) return -c;
-    return a->batch * a->seqlen == 0 ? 0 : up(a->batch * a->heads * la_plan(a).nseg * 4);
+    if (a->batch * a->seqlen == 0) return 0;
+    const int64_t n = la_plan(a).fwd.nseg;
+    return n > 1 ? up(a->batch * a->heads * n * 4) + up(a->batch * a->heads * n * a->dk * a->dv * 4) : 0;
 }
 
 int64_t swx_linattn_bwd_workspace_bytes(const swx_linattn_args* a) {
@@ -196,11 +216,14 @@ int swx_linattn_fwd(const swx_linattn_args* a, void* stream) {
     }
     if (!a->q || !a->k || !a->v || !a->log_decay || !a->out) return SWX_ERR_INVALID_ARG;
     const LaPlan q = la_plan(a);
-    if (q.nseg > 1 && (!a->seg_states || !a->workspace || a->workspace_bytes < swx_linattn_fwd_workspace_bytes(a)))
-        return SWX_ERR_INVALID_ARG;
-    LaDev p = la_pack(a, q);
+    if (q.fwd.nseg > 1 && (!a->workspace || a->workspace_bytes < swx_linattn_fwd_workspace_bytes(a))) return SWX_ERR_INVALID_ARG;
+    LaDev p = la_pack(a, q, q.fwd);
     p.dec = static_cast<float*>(a->workspace);
-    if (q.nseg > 1 && la_launch_state(p, a->dtype, false, st) != cudaSuccess) return SWX_ERR_CUDA;
+    p.seg = p.dec + up(a->batch * a->heads * q.fwd.nseg * 4) / 4;
+    p.save = q.bwd.nseg > 1 ? a->seg_states : nullptr;
+    p.save_n = q.bwd.nseg;
+    p.save_c = q.bwd.segc;
+    if (q.fwd.nseg > 1 && la_launch_state(p, a->dtype, false, st) != cudaSuccess) return SWX_ERR_CUDA;
     return la_launch_fwd(p, a->dtype, st) == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
 }
 
@@ -221,11 +244,13 @@ int swx_linattn_bwd(const swx_linattn_args* a, void* stream) {
         return SWX_ERR_INVALID_ARG;
     const LaPlan q = la_plan(a);
     const LaWs w = la_ws(a, q);
-    if (a->workspace_bytes < w.total || (q.nseg > 1 && !a->seg_states)) return SWX_ERR_INVALID_ARG;
+    if (a->workspace_bytes < w.total || (q.bwd.nseg > 1 && !a->seg_states)) return SWX_ERR_INVALID_ARG;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     auto at = [ws](int64_t o) { return reinterpret_cast<float*>(ws + o); };
-    LaDev p = la_pack(a, q);
-    p.dec = at(w.dec); p.rseg = at(w.rseg); p.rin = at(w.rin); p.yseg = at(w.yseg);
+    LaDev p = la_pack(a, q, q.bwd);
+    p.tc = p.tc && q.bwd.segc >= 16;
+    p.seg = a->seg_states;
+    p.dec = at(w.dec); p.rseg = at(w.seg); p.rin = at(w.rin); p.yseg = at(w.yseg);
     p.shared_qk = la_shared(a, q);
     p.dq = p.shared_qk ? at(w.dq) : a->dq;
     p.dk_out = p.shared_qk ? at(w.dk) : a->dk_out;
@@ -237,7 +262,7 @@ int swx_linattn_bwd(const swx_linattn_args* a, void* stream) {
         return (reinterpret_cast<uintptr_t>(o) & 15) == 0 && (d * (a->dtype == SWX_DTYPE_F32 ? 4 : 2)) % 16 == 0;
     };
     p.vec_o = whole(a->dv_out, a->dv);
-    if (q.nseg > 1 && la_launch_state(p, a->dtype, true, st) != cudaSuccess) return SWX_ERR_CUDA;
+    if (q.bwd.nseg > 1 && la_launch_state(p, a->dtype, true, st) != cudaSuccess) return SWX_ERR_CUDA;
     if (la_launch_bwd(p, a->dtype, st) != cudaSuccess) return SWX_ERR_CUDA;
     if (a->decay_per_head && la_launch_dg_head(p.dg_part, a->dlog_decay, p.H, p.b * p.nseg, st) != cudaSuccess) return SWX_ERR_CUDA;
     if (p.shared_qk) {

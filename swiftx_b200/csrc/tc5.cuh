@@ -1,5 +1,5 @@
-// Thin wrappers of the fifth-generation tensor core (tcgen05) instructions for CTA pairs
-// (cta_group::2): two CTAs of a cluster share one 256-row tile, each holding half of the
+// Thin wrappers of the fifth-generation tensor core (tcgen05) instructions, for one CTA
+// (cta_group::1) and for CTA pairs (cta_group::2): two CTAs of a cluster share one 256-row tile, each holding half of the
 // rows of A and of B in its shared memory and half of the accumulator rows in its tensor
 // memory; the even CTA (the leader) issues the products for both.
 #pragma once
@@ -36,6 +36,23 @@ __device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity
     }
     return false;
 }
+// Announces bytes without arriving.
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" :: "r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// A bounded wait whose tries let the thread sleep up to 20 us each (fewer polls in the other
+// warps' issue slots); 2^16 tries are about a second.
+__device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity, uint32_t limit) {
+    for (uint32_t i = 0; i < limit; ++i) {
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred P;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 P, [%1], %2, %3;\n\t"
+                     "selp.b32 %0, 1, 0, P;\n\t}"
+                     : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
 // A tile into this CTA's shared memory whose bytes are counted on a barrier of either CTA
 // of the pair (bar: an address of the cluster's shared window).
 __device__ __forceinline__ void tma_load_3d_pair(void* sdst, const void* map, int x, int y, int z, uint32_t bar) {
@@ -50,6 +67,18 @@ __device__ __forceinline__ void tma_store_3d(const void* map, const void* ssrc, 
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+// A 4-D tile into this CTA's shared memory, completing on this CTA's barrier.
+__device__ __forceinline__ void tma_load_4d(void* sdst, const void* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+                 "[%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 :: "r"(smem_u32(sdst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tma_prefetch_4d(const void* map, int x, int y, int z, int w) {
+    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];"
+                 :: "l"(map), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
 
 // ---------------------------------------------------------------- tensor memory
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* sdst, uint32_t cols) {      // one warp of each CTA
@@ -97,6 +126,27 @@ __device__ __forceinline__ void mma_bf16_pair(uint32_t d, uint64_t a, uint64_t b
     asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.u32 P, %4, 0;\n\t"
                  "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, P;\n\t}"
                  :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
+}
+// The same for one CTA alone (cta_group::1).
+__device__ __forceinline__ void tmem_alloc(uint32_t* sdst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 :: "r"(smem_u32(sdst)), "r"(cols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(cols));
+}
+// For a whole warp to call, converged: one elected lane issues.  (The operands then stay in uniform
+// registers; inside a branch of one lane each product took about 96 cycles to issue.)
+__device__ __forceinline__ void mma_bf16_cta(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred P, E;\n\tsetp.ne.u32 P, %4, 0;\n\telect.sync _|E, 0xffffffff;\n\t"
+                 "@E tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, P;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("{\n\t.reg .pred E;\n\telect.sync _|E, 0xffffffff;\n\t"
+                 "@E tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                 :: "r"(smem_u32(bar)) : "memory");
 }
 // Arrives on the barrier at this offset in both CTAs once the products issued so far are done.
 __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {

@@ -61,27 +61,36 @@ def _args(q, k, v, g, scale):
     return a
 
 
+def _dense(t):
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _forward(q, k, v, g, s0, lengths, scale, want_state):
-    """(out, the last state or None, the segments' start states or None) of checked operands."""
+def _forward(q, k, v, g, s0, lengths, scale, want_state, save):
+    """(out, the last state or None, the states at the backward's segments' starts or None: with
+    ``save``, where there are several) of checked operands."""
     b, _, h, dv = v.shape
     dk = q.shape[-1]
     with _lib.on_device(v.device):
         lib = _lib.load()
         a = _args(q, k, v, g, scale)
-        n = lib.swx_linattn_segments(a)
+        n = lib.swx_linattn_fwd_workspace_bytes(a)
         if n < 0:
-            _lib.check(-n, "swx_linattn_segments")
-        out = v.new_empty(v.shape)
+            _lib.check(-n, "swx_linattn_fwd")
+        out = _dense(v)
         last = g.new_empty((b, h, dk, dv)) if want_state else None
         seg = None
-        if n > 1:
-            seg = g.new_empty((b, h, n, dk, dv))
-            ws = g.new_empty(lib.swx_linattn_fwd_workspace_bytes(a) // 4)
-            a.seg_states, a.workspace, a.workspace_bytes = seg.data_ptr(), ws.data_ptr(), 4 * ws.numel()
+        if n > 0:
+            ws = g.new_empty(n // 4)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), n
+        if save:
+            m = lib.swx_linattn_segments(a)
+            if m > 1:
+                seg = g.new_empty((b, h, m, dk, dv))
+                a.seg_states = seg.data_ptr()
         a.lengths, a.initial_state, a.out, a.final_state = _ptr(lengths), _ptr(s0), out.data_ptr(), _ptr(last)
         _lib.check(lib.swx_linattn_fwd(a, _lib.stream_ptr(v.device)), "swx_linattn_fwd")
     return out, last, seg
@@ -90,7 +99,7 @@ def _forward(q, k, v, g, s0, lengths, scale, want_state):
 class LinearAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, log_decay, initial_state, lengths, scale, want_state):
-        out, last, seg = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state)
+        out, last, seg = _forward(q, k, v, log_decay, initial_state, lengths, scale, want_state, True)
         ctx.save_for_backward(q, k, v, log_decay, initial_state, lengths, seg)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
@@ -105,8 +114,8 @@ class LinearAttentionFn(torch.autograd.Function):
         with _lib.on_device(v.device):
             lib = _lib.load()
             a = _args(q, k, v, g, ctx.scale)
-            dq, dk, dv, dg = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), g.new_empty(g.shape)
-            ds0 = s0.new_empty(s0.shape) if s0 is not None and ctx.needs_input_grad[4] else None
+            dq, dk, dv, dg = _dense(q), _dense(k), _dense(v), _dense(g)
+            ds0 = _dense(s0) if s0 is not None and ctx.needs_input_grad[4] else None
             ws = g.new_empty(lib.swx_linattn_bwd_workspace_bytes(a) // 4)
             a.lengths, a.initial_state, a.seg_states, a.dfinal_state = _ptr(lengths), _ptr(s0), _ptr(seg), _ptr(dlast)
             a.dout, (a.do_sb, a.do_sl, a.do_sh) = dout.data_ptr(), dout.stride()[:3]
@@ -142,7 +151,7 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
                                     or (initial_state is not None and initial_state.requires_grad)):
         out, state = LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
     else:
-        out, state, _ = _forward(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
+        out, state, _ = _forward(q, k, v, log_decay, initial_state, lengths, float(scale), return_state, False)
     return (out, state) if return_state else out
 
 
@@ -156,7 +165,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
     q, k, v = _unit(q), _unit(k), _unit(v)
     with _lib.on_device(v.device):
         lib = _lib.load()
-        out = v.new_empty(v.shape)
+        out = _dense(v)
         a = _lib.LinattnArgs()
         a.batch, a.heads, a.dv = v.shape
         a.seqlen, (a.qk_heads, a.dk) = 1, q.shape[1:]

@@ -72,7 +72,7 @@ class LinearCrossEntropyFn(torch.autograd.Function):
         dloss = dloss.float().contiguous()
         with _lib.on_device(x.device):
             lib = _lib.load()
-            dx = x.new_empty(x.shape) if ctx.needs_input_grad[0] else None
+            dx = torch.empty_like(x, memory_format=torch.contiguous_format) if ctx.needs_input_grad[0] else None
             dw = w.new_empty(w.shape, dtype=w_dtype) if ctx.needs_input_grad[1] else None
             a = _args(x, w, targets, ignore_index, reduction)
             a.row_max = stats.data_ptr()
@@ -119,10 +119,13 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     if weight16 is not None and (weight16.dtype != torch.bfloat16 or weight16.shape != weight.shape or weight16.device != x.device):
         raise ValueError(f"linear_cross_entropy: weight16 is a bf16 copy of the {tuple(weight.shape)} weight, got {weight16.dtype} "
                          f"{tuple(weight16.shape)}")
-    x2, t1, opts = x.reshape(-1, x.shape[-1]), targets.reshape(-1), (int(ignore_index), _lib.XENT_REDUCTIONS[reduction])
+    # (a reshape that changes nothing would still be a node of the autograd graph)
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    t1 = targets if targets.dim() == 1 else targets.reshape(-1)
+    opts = (int(ignore_index), _lib.XENT_REDUCTIONS[reduction])
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         loss = LinearCrossEntropyFn.apply(x2, weight, t1, *opts, weight16)
     else:
         w = weight if weight.dtype == x.dtype else weight.to(x.dtype) if weight16 is None else weight16
         loss = _forward(_rows(x2), _rows(w), t1.contiguous(), *opts)[0]
-    return loss.view(targets.shape) if reduction == "none" else loss
+    return loss.view(targets.shape) if reduction == "none" and targets.dim() != 1 else loss

@@ -123,6 +123,44 @@ def test_forward_and_gradients(b, L, H, Hk, dk, dv, dtype, decay, state):
     _check(got, _oracle(t, do, ds, scale, None), _oracle(t, do, ds, scale, None, True), t, L)
 
 
+@pytest.mark.parametrize("b,L,H,Hk,dk,dv,decay,state", [
+    (16, 520, 8, 8, 64, 64, "token", False),       # five chunks of 128, the last with 8 tokens; one walk a head
+    (3, 2100, 6, 3, 40, 72, "token", True),        # a slice of 8 columns, shared heads, four segments
+    (1, 4200, 8, 2, 64, 64, "head", True),         # eight segments; the backward's are others
+    (20, 1030, 8, 1, 24, 64, "token", True),       # more heads than SMs
+])
+def test_pipelined_kernels(b, L, H, Hk, dk, dv, decay, state):
+    """Sizes that the pipelined bf16 kernels take (chunks of 128 tokens, a ring of three)."""
+    t, do, ds = _inputs(b, L, H, Hk, dk, dv, torch.bfloat16, decay, state, seed=L)
+    got = _run(t, do, ds, 0.2, None)
+    _check(got, _oracle(t, do, ds, 0.2, None), _oracle(t, do, ds, 0.2, None, True), t, L)
+    assert _lib.load().swx_device_wait_status() == _lib.SWX_OK
+    with torch.no_grad():                          # without the backward's states: the same values
+        out, last = linear_attention(t["q"], t["k"], t["v"], t["g"], initial_state=t["s0"], scale=0.2, return_state=True)
+    assert torch.equal(out, got["out"]) and torch.equal(last, got["state"])
+
+
+def test_pipelined_padded_steep_and_reset_rows():
+    """Lengths on and off the chunks' borders with NaN behind them; resets, decays too steep for the split
+    exponentials (2^-60 inside 16 tokens), and decays of 0, in the pipelined kernels."""
+    b, L, H, dk, dv = 8, 700, 16, 64, 64
+    t, do, ds = _inputs(b, L, H, H, dk, dv, torch.bfloat16, seed=17)
+    t["g"][0, 130, :8] = -float("inf")
+    t["g"][1, :, 3] = -30.0
+    t["g"][2] = 0.0
+    t["g"][3, 200:260, 5] = -200.0
+    n = torch.tensor([700, 0, 1, 128, 129, 640, 699, 5000], device=DEV)
+    got = _run(t, do, ds, 0.125, n)
+    _check(got, _oracle(t, do, ds, 0.125, n), _oracle(t, do, ds, 0.125, n, True), t, L)
+    behind = torch.arange(L, device=DEV)[None, :] >= n[:, None]
+    for k in ("q", "k", "v", "g"):
+        t[k][behind] = float("nan")
+    dirty = _run(t, do, ds, 0.125, n)
+    for k in got:
+        assert torch.equal(got[k], dirty[k]), k
+    assert torch.count_nonzero(got["out"][behind]) == 0
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lengths", [[0, 1, 64, 65], [200, 199, 5, 130], [-3, 1000, 128, 0]])
 def test_padded_rows(dtype, lengths):
@@ -376,8 +414,8 @@ def test_short_buffers_are_refused_on_the_host():
     a.batch, a.seqlen, a.heads, a.qk_heads, a.dk, a.dv, a.dtype = 1, 1000, 2, 2, 64, 64, 1
     a.q = a.k = t["q"].data_ptr()
     a.v, a.log_decay, a.out = t["v"].data_ptr(), t["g"].data_ptr(), t["v"].data_ptr()
-    assert lib.swx_linattn_segments(a) > 1
-    assert lib.swx_linattn_fwd(a, None) == _lib.SWX_ERR_INVALID_ARG            # no seg_states, no workspace
+    assert lib.swx_linattn_segments(a) > 1 and lib.swx_linattn_fwd_workspace_bytes(a) > 0
+    assert lib.swx_linattn_fwd(a, None) == _lib.SWX_ERR_INVALID_ARG            # no workspace
     a.seg_states = a.workspace = t["g"].data_ptr()
     a.workspace_bytes = lib.swx_linattn_fwd_workspace_bytes(a) - 4
     assert lib.swx_linattn_fwd(a, None) == _lib.SWX_ERR_INVALID_ARG
