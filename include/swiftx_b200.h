@@ -467,8 +467,9 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  * q, k: (batch, seqlen, qk_heads, dk), v, dout: (batch, seqlen, heads, dv), in dtype (fp32
  * or bf16), unit element stride, any batch / token / head strides; heads a multiple of qk_heads
  * (head h reads q and k of head h / (heads / qk_heads)); dk, dv <= 128.  log_decay: fp32 with
- * strides (0 broadcasts it over rows or tokens); any value, -inf resets the state.  States are
- * fp32, dense (batch, heads, dk, dv).  lengths (batch), optional: row i has min(max(lengths[i], 0),
+ * strides (0 broadcasts it over rows or tokens), at most 0 as a rule; -inf resets the state, and
+ * growth (above 0) is taken as it is while its exponentials over 128 tokens stay finite.  States are
+ * fp32, dense (batch, heads, dk, dv); final_state, seg_states and workspace start on 16 bytes.  lengths (batch), optional: row i has min(max(lengths[i], 0),
  * seqlen) tokens; what lies behind them is not used (it may be NaN), gives zeros in out and in the gradients, and
  * leaves the state as it was.
  * The sequence is walked in chunks of 64 or 128 tokens on the tensor cores, cut into segments that are

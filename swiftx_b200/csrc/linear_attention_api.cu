@@ -126,6 +126,11 @@ static int la_check(const swx_linattn_args* a) {
     return SWX_OK;
 }
 
+// The buffers that the caller makes for the states and the scratch start on 16 bytes.
+static bool la_aligned(const swx_linattn_args* a) {
+    return ((reinterpret_cast<uintptr_t>(a->final_state) | reinterpret_cast<uintptr_t>(a->seg_states) | reinterpret_cast<uintptr_t>(a->workspace)) & 15) == 0;
+}
+
 struct LaWs { int64_t dec, seg, rin, net, yseg, dg, dq, dk, total; };
 
 static int64_t up(int64_t v) { return (v + 255) / 256 * 256; }
@@ -215,6 +220,7 @@ int swx_linattn_fwd(const swx_linattn_args* a, void* stream) {
         return e == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
     }
     if (!a->q || !a->k || !a->v || !a->log_decay || !a->out) return SWX_ERR_INVALID_ARG;
+    if (!la_aligned(a)) return SWX_ERR_INVALID_ARG;
     const LaPlan q = la_plan(a);
     if (q.fwd.nseg > 1 && (!a->workspace || a->workspace_bytes < swx_linattn_fwd_workspace_bytes(a))) return SWX_ERR_INVALID_ARG;
     LaDev p = la_pack(a, q, q.fwd);
@@ -244,6 +250,7 @@ int swx_linattn_bwd(const swx_linattn_args* a, void* stream) {
         return SWX_ERR_INVALID_ARG;
     const LaPlan q = la_plan(a);
     const LaWs w = la_ws(a, q);
+    if (!la_aligned(a)) return SWX_ERR_INVALID_ARG;
     if (a->workspace_bytes < w.total || (q.bwd.nseg > 1 && !a->seg_states)) return SWX_ERR_INVALID_ARG;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     auto at = [ws](int64_t o) { return reinterpret_cast<float*>(ws + o); };
@@ -267,8 +274,8 @@ int swx_linattn_bwd(const swx_linattn_args* a, void* stream) {
     if (a->decay_per_head && la_launch_dg_head(p.dg_part, a->dlog_decay, p.H, p.b * p.nseg, st) != cudaSuccess) return SWX_ERR_CUDA;
     if (p.shared_qk) {
         const int per = (int)(a->heads / a->qk_heads) * q.nsl;
-        if (la_launch_group_sum(static_cast<float*>(p.dq), a->dq, a->dtype, a->batch * a->seqlen, p.Hk, per, p.dk, st) != cudaSuccess ||
-            la_launch_group_sum(static_cast<float*>(p.dk_out), a->dk_out, a->dtype, a->batch * a->seqlen, p.Hk, per, p.dk, st) != cudaSuccess)
+        if (la_launch_group_sum(static_cast<float*>(p.dq), static_cast<float*>(p.dk_out), a->dq, a->dk_out, a->dtype, a->batch * a->seqlen, p.Hk,
+                                per, p.dk, st) != cudaSuccess)
             return SWX_ERR_CUDA;
     }
     return SWX_OK;

@@ -23,7 +23,7 @@ template <typename T> struct Planes { static constexpr int N = sizeof(T) == 4 ? 
 template <typename T, int DK>
 __device__ __forceinline__ void la_times_state_t(float (&acc)[DK / 8][4], const T* x, const T* s, int rw, int lane) {
     using Sh = LaShape<T, DK>;
-#pragma unroll
+#pragma unroll LA_UNROLL<T>
     for (int k0 = 0; k0 < LA_DV; k0 += 16) {
         FragA<T> a;
         load_a(a, x, Sh::LDV, 16 * rw, k0, lane);
@@ -140,7 +140,7 @@ __device__ __forceinline__ void la_dq_walk(const LaDev& p, int64_t block, uint8_
             if (t + 8 < p.L) rin[t + 8] = rd.y;
         }
         float sc[8][4] = {};
-#pragma unroll
+#pragma unroll LA_UNROLL<T>
         for (int k0 = 0; k0 < LA_DV; k0 += 16) {
             FragA<T> a;
             load_a(a, dout, Sh::LDV, 16 * rw, k0, lane);
@@ -234,7 +234,7 @@ __device__ __forceinline__ void la_dkv_walk(const LaDev& p, int64_t block, uint8
         const int r0 = 16 * rw + (lane >> 2), tr = t0 + 16 * rw;
         // the scores of this warp's tokens s (rows) with the tokens t >= s (columns)
         float ps[8][4] = {}, as[8][4] = {};
-#pragma unroll
+#pragma unroll LA_UNROLL<T>
         for (int k0 = 0; k0 < DK; k0 += 16) {
             FragA<T> a;
             load_a(a, k, Sh::LDK, 16 * rw, k0, lane);
@@ -247,7 +247,7 @@ __device__ __forceinline__ void la_dkv_walk(const LaDev& p, int64_t block, uint8
                     mma(ps[2 * j + 1], a, f[1]);
                 }
         }
-#pragma unroll
+#pragma unroll LA_UNROLL<T>
         for (int k0 = 0; k0 < LA_DV; k0 += 16) {
             FragA<T> a;
             load_a(a, v, Sh::LDV, 16 * rw, k0, lane);
@@ -323,7 +323,7 @@ __device__ __forceinline__ void la_dkv_walk(const LaDev& p, int64_t block, uint8
         const float w0 = gt.post[r0], w1 = gt.post[r0 + 8];
         {
             float dv[8][4] = {};
-#pragma unroll
+#pragma unroll LA_UNROLL<T>
             for (int k0 = 0; k0 < DK; k0 += 16) {            // D^T k, D rounded once for a result in T
                 FragA<T> a;
                 load_a(a, k, Sh::LDK, 16 * rw, k0, lane);
@@ -388,17 +388,32 @@ __device__ __forceinline__ void la_dkv_walk(const LaDev& p, int64_t block, uint8
 }
 
 // ------------------------------------------------------------------ sums over heads that share
-// dst[row][hk][c] = sum over the group's parts of src[row][part][c], in order.
-template <typename T>
-__global__ void __launch_bounds__(256) la_group_sum_kernel(const float* src, T* dst, int64_t rows, int Hk, int per, int d) {
-    const int64_t n = rows * Hk * d, i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    const int64_t c = i % d, rh = i / d;
+// dst[row][hk][c] = sum over the group's parts of src[row][part][c], in order, for dq and dk in one
+// launch; thread = VEC values.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) la_group_sum_kernel(const float* src_q, const float* src_k, T* dst_q, T* dst_k, int64_t rows, int Hk,
+                                                           int per, int d) {
+    const int64_t n = rows * Hk * (d / VEC);
+    int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+    if (i >= 2 * n) return;
+    const float* src = i < n ? src_q : src_k;
+    T* dst = i < n ? dst_q : dst_k;
+    i %= n;
+    const int c = (int)(i % (d / VEC)) * VEC;
+    const int64_t rh = i / (d / VEC);
     const float* s = src + rh * per * d + c;
-    float x = 0.f;
-#pragma unroll 4
-    for (int k = 0; k < per; ++k) x += s[(int64_t)k * d];
-    dst[i] = Elem<T>::from_f(x);
+    float x[VEC] = {};
+#pragma unroll 8
+    for (int k = 0; k < per; ++k) {
+        if constexpr (VEC == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(s + (int64_t)k * d);
+            x[0] += q.x; x[1] += q.y; x[2] += q.z; x[3] += q.w;
+        } else {
+            x[0] += s[(int64_t)k * d];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) dst[rh * d + c + j] = Elem<T>::from_f(x[j]);
 }
 
 // ------------------------------------------------------------------ dg
@@ -501,11 +516,18 @@ cudaError_t la_launch_dg_head(const double* part, float* dst, int H, int n, cuda
     return cudaGetLastError();
 }
 
-cudaError_t la_launch_group_sum(const float* src, void* dst, int dtype, int64_t rows, int Hk, int per, int d, cudaStream_t st) {
-    const int64_t n = rows * Hk * d;
-    const unsigned grid = (unsigned)((n + 255) / 256);
-    if (dtype == SWX_DTYPE_F32) la_group_sum_kernel<float><<<grid, 256, 0, st>>>(src, static_cast<float*>(dst), rows, Hk, per, d);
-    else la_group_sum_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(src, static_cast<__nv_bfloat16*>(dst), rows, Hk, per, d);
+template <typename T>
+static void group_sum(const float* sq, const float* sk, void* dq, void* dk, int64_t rows, int Hk, int per, int d, cudaStream_t st) {
+    const int vec = d % 4 == 0 ? 4 : 1;                          // the parts are 256-byte aligned
+    const unsigned grid = (unsigned)((2 * rows * Hk * (d / vec) + 255) / 256);
+    if (vec == 4) la_group_sum_kernel<T, 4><<<grid, 256, 0, st>>>(sq, sk, static_cast<T*>(dq), static_cast<T*>(dk), rows, Hk, per, d);
+    else la_group_sum_kernel<T, 1><<<grid, 256, 0, st>>>(sq, sk, static_cast<T*>(dq), static_cast<T*>(dk), rows, Hk, per, d);
+}
+
+cudaError_t la_launch_group_sum(const float* sq, const float* sk, void* dq, void* dk, int dtype, int64_t rows, int Hk, int per, int d,
+                                cudaStream_t st) {
+    if (dtype == SWX_DTYPE_F32) group_sum<float>(sq, sk, dq, dk, rows, Hk, per, d, st);
+    else group_sum<__nv_bfloat16>(sq, sk, dq, dk, rows, Hk, per, d, st);
     return cudaGetLastError();
 }
 

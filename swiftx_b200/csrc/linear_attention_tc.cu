@@ -146,10 +146,14 @@ __device__ __forceinline__ void lt_state_read(float (&S)[32], const float* src, 
 }
 __device__ __forceinline__ void lt_state_write(const float (&S)[32], float* dst, const LaDev& p, int row, int c0, int half) {
     if (row < 0 || row >= p.dk) return;
+    float* d = dst + (int64_t)row * p.dv + c0 + 32 * half;
+    const int n = p.dv - c0 - 32 * half;
+    if (p.dv % 4 == 0 && n >= 32) {                              // states are 16-byte aligned
 #pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        const int c = 32 * half + j;
-        if (c0 + c < p.dv) dst[(int64_t)row * p.dv + c0 + c] = S[j];
+        for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(d)[j] = make_float4(S[4 * j], S[4 * j + 1], S[4 * j + 2], S[4 * j + 3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) if (j < n) d[j] = S[j];
     }
 }
 __device__ __forceinline__ void lt_state_save(const float (&S)[32], const LaDev& p, int64_t bh, int c, int row, int c0, int half) {
