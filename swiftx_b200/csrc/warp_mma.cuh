@@ -49,7 +49,11 @@ __device__ __forceinline__ uint32_t to_tf32(float x) {
 __device__ __forceinline__ void mma(float (&c)[4], const FragA<__nv_bfloat16>& a, const FragB<__nv_bfloat16>& b) {
     mma_bf16(c, a.r, b.r);
 }
+// The small products are summed by themselves and added in fp32: the tensor core cuts the low bits of
+// each addition off, and with six additions a step to the large sum, linear attention's decay gradient was 1.3e-6
+// off where it is 8.7e-7 now (2 x 777 x 6 heads; 110 -> 117 us).
 __device__ __forceinline__ void mma(float (&c)[4], const FragA<float>& a, const FragB<float>& b) {
+    float small[4] = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const float av[4] = {a.v[4 * h], a.v[4 * h + 2], a.v[4 * h + 1], a.v[4 * h + 3]};
@@ -64,10 +68,12 @@ __device__ __forceinline__ void mma(float (&c)[4], const FragA<float>& a, const 
             bh[i] = to_tf32(b.v[2 * h + i]);
             bl[i] = to_tf32(b.v[2 * h + i] - __uint_as_float(bh[i]));
         }
-        mma_tf32(c, al, bh);
-        mma_tf32(c, ah, bl);
+        mma_tf32(small, al, bh);
+        mma_tf32(small, ah, bl);
         mma_tf32(c, ah, bh);
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] += small[i];
 }
 
 // ---------------------------------------------------------------- operands from shared memory
