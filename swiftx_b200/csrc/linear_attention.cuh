@@ -94,7 +94,7 @@ __device__ __forceinline__ LaG la_load_g(const LaDev& p, int b, int h, int t0, i
 }
 
 // One warp; lane holds tokens 2 lane, 2 lane + 1.  Returns the chunk's sum (log 2 units).
-__device__ __forceinline__ double la_gates(LaGates& s, LaG r, int lane) {
+static __device__ __noinline__ double la_gates(LaGates& s, LaG r, int lane) {
     const double L2E = 1.4426950408889634073599;
     const double d0 = (r.g0 < -1000.f ? -1000. : (double)r.g0) * L2E, d1 = (r.g1 < -1000.f ? -1000. : (double)r.g1) * L2E;
     double x = d0 + d1;
@@ -159,6 +159,23 @@ __device__ __forceinline__ void la_mask_rows(float (&c0)[4], float (&c1)[4], con
     }
 }
 
+// Paths that aligned tensors do not take stay out of line: the walks' code has to fit the instruction caches.
+template <typename T>
+__device__ __noinline__ void la_load_scalar(T* s, int ld, int width, const T* g, int64_t sl, int rows, int cols) {
+    for (int i = threadIdx.x; i < LA_C * width; i += LA_THREADS) {
+        const int r = i / width, c = i % width;
+        s[r * ld + c] = r < rows && c < cols ? g[(int64_t)r * sl + c] : T(0.f);
+    }
+}
+template <typename T>
+__device__ __noinline__ void la_store_scalar(const T* s, int ld, T* g, int64_t sl, int rows, int all_rows, int cols, int lane) {
+    const int n = 16 * cols;
+    for (int i = lane; i < n; i += 32) {
+        const int r = i / cols, c = i % cols;
+        if (r < all_rows) g[(int64_t)r * sl + c] = r < rows ? s[r * ld + c] : T(0.f);
+    }
+}
+
 // 64 token rows x W columns into s (row length LD), zero past rows / cols; asynchronous when vec.
 template <typename T, int W, int LD>
 __device__ __forceinline__ void la_load(T* s, const LaTensor& x, int b, int t0, int h, int c0, int rows, int cols) {
@@ -171,21 +188,13 @@ __device__ __forceinline__ void la_load(T* s, const LaTensor& x, int b, int t0, 
         const T* src = g + (int64_t)r * x.sl + c;
         const int64_t step = STEP * x.sl;
         T* dst = s + r * LD + c;
-        if (rows >= LA_C && n > 0) {
 #pragma unroll
-            for (int i = 0; i < LA_C / STEP; ++i) cp_async16(dst + i * STEP * LD, src + i * step, n);
-        } else {
-#pragma unroll
-            for (int i = 0; i < LA_C / STEP; ++i) {
-                const bool in = r + i * STEP < rows && n > 0;
-                cp_async16(dst + i * STEP * LD, in ? src + i * step : static_cast<const T*>(x.p), in ? n : 0);
-            }
+        for (int i = 0; i < LA_C / STEP; ++i) {
+            const bool in = r + i * STEP < rows && n > 0;
+            cp_async16(dst + i * STEP * LD, in ? src + i * step : static_cast<const T*>(x.p), in ? n : 0);
         }
     } else {
-        for (int i = threadIdx.x; i < LA_C * W; i += LA_THREADS) {
-            const int r = i / W, c = i % W;
-            s[r * LD + c] = r < rows && c < cols ? g[(int64_t)r * x.sl + c] : T(0.f);
-        }
+        la_load_scalar(s, LD, W, g, x.sl, rows, cols);
     }
 }
 
@@ -292,10 +301,7 @@ __device__ __forceinline__ void la_store(const T* s, T* g, int64_t sl, int rows,
             }
         }
     } else {
-        for (int i = lane; i < 16 * W; i += 32) {
-            const int r = i / W, c = i % W;
-            if (r < all_rows && c < cols) g[(int64_t)r * sl + c] = r < rows ? s[r * LD + c] : T(0.f);
-        }
+        la_store_scalar(s, LD, g, sl, rows, all_rows, cols, lane);
     }
     __syncwarp();
 }
