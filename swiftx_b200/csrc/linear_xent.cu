@@ -221,8 +221,8 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
         }
         __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            // ---- products, for both CTAs
+        if (rank == 0) {
+            // ---- products, for both CTAs (the whole warp, one lane of it issuing)
             constexpr uint32_t idesc = mma_bf16_idesc(XE_TILE, XE_TILE, A_MN, B_MN);
             // 16 contraction steps further: 32 bytes along a K-major row, 16 rows of 128 bytes otherwise
             constexpr uint64_t da = (A_MN ? 2048 : 32) >> 4, db = (B_MN ? 2048 : 32) >> 4;

@@ -122,9 +122,12 @@ constexpr uint32_t mma_bf16_idesc(int m, int n, bool a_mn, bool b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
            ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
+// The products and commits below are for a whole warp to call, converged: one elected lane issues.
+// (The operands then stay in uniform registers; inside a branch of one lane each product took about
+// 96 cycles to issue.)
 __device__ __forceinline__ void mma_bf16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred P;\n\tsetp.ne.u32 P, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, P;\n\t}"
+    asm volatile("{\n\t.reg .pred P, E;\n\tsetp.ne.u32 P, %4, 0;\n\telect.sync _|E, 0xffffffff;\n\t"
+                 "@E tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, P;\n\t}"
                  :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
 }
 // The same for one CTA alone (cta_group::1).
@@ -136,8 +139,6 @@ __device__ __forceinline__ void tmem_alloc(uint32_t* sdst, uint32_t cols) {
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(cols));
 }
-// For a whole warp to call, converged: one elected lane issues.  (The operands then stay in uniform
-// registers; inside a branch of one lane each product took about 96 cycles to issue.)
 __device__ __forceinline__ void mma_bf16_cta(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
     asm volatile("{\n\t.reg .pred P, E;\n\tsetp.ne.u32 P, %4, 0;\n\telect.sync _|E, 0xffffffff;\n\t"
                  "@E tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, P;\n\t}"
@@ -151,7 +152,8 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 // Arrives on the barrier at this offset in both CTAs once the products issued so far are done.
 __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
     const uint16_t both = 3;
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+    asm volatile("{\n\t.reg .pred E;\n\telect.sync _|E, 0xffffffff;\n\t"
+                 "@E tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
                  :: "r"(smem_u32(bar)), "h"(both) : "memory");
 }
 
