@@ -640,11 +640,23 @@ static bool direct_ok(const void* p, int64_t sr, int dtype) {
 // hide behind the products, while fewer pieces mean fewer launches, fewer rounds that do not
 // fill the GPU and fewer passes over dx's running sum (8192 tokens x 50001 x 1024, forward
 // and backward: pieces of 72 MB 2.92 ms, 160 MB 2.83, 288 MB 2.67, 450 MB 2.61, one piece 2.56).
-static int64_t piece_columns(int64_t T, int64_t V, int planes) {
-    int64_t c = (int64_t(416) << 20) / (2 * planes * std::max<int64_t>(T, 1)) / 256 * 256;
-    c = std::max<int64_t>(c, 4096);
-    const int64_t n = (V + c - 1) / c;        // pieces of nearly equal size
-    return up256((V + n - 1) / n);
+//
+// Among the sizes near that, the one whose dW tiles take the fewest rounds of the CTA pairs over
+// all pieces (196 x 4 tiles: pieces of 104 and 92 column tiles 11 rounds, two of 98 12).
+static int64_t piece_columns(int64_t T, int64_t V, int64_t d, int planes) {
+    const int64_t vt = (V + XE_TILE - 1) / XE_TILE, dt = (d + XE_TILE - 1) / XE_TILE;
+    const int64_t most = std::max<int64_t>((int64_t(416) << 20) / (2 * planes * std::max<int64_t>(T, 1)), 4096) / XE_TILE;
+    if (vt <= most) return vt * XE_TILE;
+    auto rounds = [dt](int64_t tiles) { return (tiles * dt + XE_PAIRS - 1) / XE_PAIRS; };
+    int64_t best = most, least = INT64_MAX;
+    for (int64_t c = most; c >= most * 3 / 4 && c > 0; --c) {
+        const int64_t n = vt / c * rounds(c) + rounds(vt % c);
+        if (n < least) {
+            least = n;
+            best = c;
+        }
+    }
+    return best * XE_TILE;
 }
 
 static XentPlan xent_plan(const swx_xent_args* a) {
@@ -665,7 +677,7 @@ static XentPlan xent_plan(const swx_xent_args* a) {
     q.off_rows = q.off_hit + up256(T * 4);
     q.off_cnt = q.off_rows + up256((T + XJ_ROWS - 1) / XJ_ROWS * 16);
     q.fwd_total = q.off_cnt + 256;
-    q.piece = piece_columns(T, V, q.planes);
+    q.piece = piece_columns(T, V, d, q.planes);
     q.ldp = q.piece;
     q.off_p = base;
     q.off_acc = q.off_p + up256((int64_t)q.planes * T * q.ldp * 2);
@@ -853,9 +865,9 @@ int swx_xent_bwd(const swx_xent_args* a, void* stream) {
             XentGemm h{};
             h.status = status; h.npair = npair;
             h.M = (int)T; h.N = (int)d; h.mt = (int)q.mt; h.nt = (int)((d + XE_TILE - 1) / XE_TILE);
-            // every piece the same number of steps (a short last one reads zeros), so that a spread
+            // spread: every piece the same number of steps (a short last one reads zeros), so that a
             // tile has the same parts in each
-            h.nk = (int)((std::min(q.piece, V) + XE_K - 1) / XE_K); h.ksub = q.planes == 3 ? XE_KSUB : h.nk; h.kb0 = (int)c0;
+            h.nk = (int)(((q.dx.spread ? std::min(q.piece, V) : cw) + XE_K - 1) / XE_K); h.ksub = q.planes == 3 ? XE_KSUB : h.nk; h.kb0 = (int)c0;
             h.scale_num = num; h.scale_den = den;
             h.first = c0 == 0; h.last = c0 + cw == V; h.out = a->dx; h.ld = d;
             h.out_bf16 = a->dtype == SWX_DTYPE_BF16;
