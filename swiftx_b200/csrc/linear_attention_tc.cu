@@ -8,10 +8,10 @@
 //   issuer    all products
 //   8 warps A k weighted by exp(G_end - G_s), as three bf16 pieces (24 bits), in the tile's own
 //             (swizzled) layout; U = weighted k^T v; S = exp(G_end) S + U in fp32 registers, shared in bf16
-//   8 warps B P = masked, decayed scores (bf16), written over q and k of the chunk, which are done
-//             with; o = scale exp(G_t) q S + P v, to memory
+//   8 warps B P = masked, decayed scores (bf16), written over the scores in tensor memory, where the
+//             product with v reads them; o = scale exp(G_t) q S + P v, to memory
 // The weighted tile has one buffer in two halves of 64 tokens: one half is made while the other's
-// products run.  The scores, q S and P v, and U have two places each in tensor memory.
+// products run.  The scores and U have two places each in tensor memory.
 // Warp w of a role works on rows 32 (w % 4) .. and, of their columns, on half w / 4.
 #include "linear_attention.cuh"
 #include "launch_util.cuh"
@@ -337,9 +337,9 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
     extern __shared__ uint8_t smem_raw[];
     __shared__ LtGates gates[LT_RING];
     // full: a chunk's tiles have landed.  weighed[half], products[half][parity of the chunk]: of the weighted
-    // tile.  shared[parity]: S is there.  scored[parity]: the scores and q S.  masked[parity]: P is there.
-    // mixed[place of the ring]: P v, and with it every product of the chunk.  read: by B, all of its tensor
-    // memory.  A barrier has as many places as a fast warp can be phases ahead of the slowest that waits or arrives.
+    // tile.  shared[parity]: S is there.  scored[parity]: the scores.  masked[parity]: P is there.
+    // mixed[place of the ring]: q S and P v, and with them every product of the chunk.  read: both, by B.
+    //   A barrier has as many places as a fast warp can be phases ahead of the slowest that waits or arrives.
     __shared__ __align__(8) uint64_t full[LF_RING], weighed[2], products[2][2], shared[2], scored[2], masked[2], mixed[LF_RING], read;
     __shared__ uint32_t tmem_base;
     uint8_t* tiles = smem_raw + (((smem_u32(smem_raw) + 1023) & ~1023u) - smem_u32(smem_raw));
@@ -377,8 +377,8 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    // tensor memory: scores (P v over them, later), q S, U, each for chunks of either parity
-    const uint32_t t_sc = tmem_base, t_qs = t_sc + 256, t_u = t_sc + 384, lanes = (uint32_t)(32 * quarter) << 16;
+    // tensor memory: scores (P over them, later) and U for chunks of either parity, q S, P v
+    const uint32_t t_sc = tmem_base, t_u = t_sc + 256, t_qs = t_sc + 384, t_pv = t_sc + 448, lanes = (uint32_t)(32 * quarter) << 16;
     bool ok = true;
     if (warp == LT_A + LT_B) {                                   // loader
         LtG g = lt_load_g(p, b, h, first * LT_C, n > 0 ? len : 0, lane);
@@ -401,19 +401,29 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
         for (int i = max(0, n - LF_RING); i < n; ++i) lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok);   // all have landed
     } else if (warp == LT_A + LT_B + 1) {                        // issuer
         constexpr uint32_t id_s = mma_bf16_idesc(LT_C, LT_C, false, false), id_o = mma_bf16_idesc(LT_C, 64, false, true);
-        auto mix = [&](int i) {                                  // P v, P over q and k
+        auto mix = [&](int i) {                                  // q S and P v
             lt_wait(&masked[i & 1], (i >> 1) & 1, ok);
+            lt_wait(&shared[i & 1], (i >> 1) & 1, ok);
+            if (i > 0) lt_wait(&read, (i - 1) & 1, ok);
             tc_fence_after();
-            const uint64_t pd = operand_desc(tile(i, 0), 16), vd = operand_desc(tile(i, 2), 16);
+            const uint64_t qd = operand_desc(tile(i, 0), 16), sd = operand_desc(ss + (i & 1) * 64 * 128, 16), vd = operand_desc(tile(i, 2), 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_bf16_cta(t_qs, qd + k * 2, sd + k * (2048 >> 4), id_o, k > 0);
 #pragma unroll
             for (int k = 0; k < LT_C / 16; ++k)
-                mma_bf16_cta(t_sc + 128 * (i & 1), pd + (k / 4) * (LT_BOX >> 4) + (k % 4) * 2, vd + k * (2048 >> 4), id_o, k > 0);
+                mma_bf16_cta_ta(t_pv, t_sc + 128 * (i & 1) + 32 * (k / 2) + 8 * (k % 2), vd + k * (2048 >> 4), id_o, k > 0);
             mma_commit(&mixed[i % LF_RING]);
         };
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
             const uint32_t u = t_u + 64 * (i & 1);
             lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok);
+            if (i >= 2) lt_wait(&mixed[(i - 2) % LF_RING], ((i - 2) / LF_RING) & 1, ok);      // P of two chunks ago has been read
+            tc_fence_after();
+            const uint64_t qd = operand_desc(tile(i, 0), 16), kd = operand_desc(tile(i, 1), 16);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_bf16_cta(t_sc + 128 * (i & 1), qd + k * 2, kd + k * 2, id_s, k > 0);
+            mma_commit(&scored[i & 1]);
             lt_wait(&weighed[0], i & 1, ok);
             tc_fence_after();
             lt_issue_u<0, 4>(u, planes, tile(i, 2));
@@ -422,15 +432,6 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
             tc_fence_after();
             lt_issue_u<4, 8>(u, planes, tile(i, 2));
             mma_commit(&products[1][i & 1]);
-            lt_wait(&shared[i & 1], (i >> 1) & 1, ok);
-            if (i >= 2) lt_wait(&read, i & 1, ok);
-            tc_fence_after();
-            const uint64_t qd = operand_desc(tile(i, 0), 16), kd = operand_desc(tile(i, 1), 16), sd = operand_desc(ss + (i & 1) * 64 * 128, 16);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_bf16_cta(t_sc + 128 * (i & 1), qd + k * 2, kd + k * 2, id_s, k > 0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_bf16_cta(t_qs + 64 * (i & 1), qd + k * 2, sd + k * (2048 >> 4), id_o, k > 0);
-            mma_commit(&scored[i & 1]);
             if (i > 0) mix(i - 1);
         }
         if (n > 0) mix(n - 1);
@@ -457,7 +458,7 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
             }
             all = gt.all;
             lt_state_save(S, p, bh, 2 * chunk(i), srow, c0, half);
-            if (i >= 2) lt_wait(&scored[i & 1], ((i - 2) >> 1) & 1, ok);        // q S of two chunks ago has read this place
+            if (i >= 2) lt_wait(&mixed[(i - 2) % LF_RING], ((i - 2) / LF_RING) & 1, ok);      // q S of two chunks ago has read this place
             lt_state_share(S, ss + (i & 1) * 64 * 128, srow, half);
             fence_proxy_async_smem();
             tc_fence_before();
@@ -480,8 +481,8 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
             lt_wait(&mixed[i % LF_RING], (i / LF_RING) & 1, ok);
             tc_fence_after();
             float o[32], pv[32];
-            tmem_ld32(t_qs + 64 * (i & 1) + lanes + 32 * half, o);
-            tmem_ld32(t_sc + 128 * (i & 1) + lanes + 32 * half, pv);
+            tmem_ld32(t_qs + lanes + 32 * half, o);
+            tmem_ld32(t_pv + lanes + 32 * half, pv);
             tmem_ld_wait();
             tc_fence_before();
             lt_arrive(&read, lane);
@@ -528,12 +529,9 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
                     lt_mask(x, gt, 32 * c, row, G, p.scale);
                     if (row < rows) lt_pack32(w, x);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<uint4*>(tile(i, c >> 1) + lt_at(row, 4 * (c & 1) + j)) =
-                        make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                tmem_st16(t_sc + 128 * (i & 1) + lanes + 32 * c, w);     // over the scores that it came from
             }
-            fence_proxy_async_smem();
+            tmem_st_wait();
             tc_fence_before();
             lt_arrive(&masked[i & 1], lane);
             if (i > 0) finish(i - 1, before);

@@ -106,6 +106,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                 "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+                 :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+                    "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // ---------------------------------------------------------------- products
@@ -143,6 +150,12 @@ __device__ __forceinline__ void mma_bf16_cta(uint32_t d, uint64_t a, uint64_t b,
     asm volatile("{\n\t.reg .pred P, E;\n\tsetp.ne.u32 P, %4, 0;\n\telect.sync _|E, 0xffffffff;\n\t"
                  "@E tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, P;\n\t}"
                  :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
+}
+// The same with A in tensor memory: 16 steps of the contraction in 8 columns, two bf16 values each.
+__device__ __forceinline__ void mma_bf16_cta_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred P, E;\n\tsetp.ne.u32 P, %4, 0;\n\telect.sync _|E, 0xffffffff;\n\t"
+                 "@E tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, P;\n\t}"
+                 :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add ? 1u : 0u) : "memory");
 }
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
     asm volatile("{\n\t.reg .pred E;\n\telect.sync _|E, 0xffffffff;\n\t"
