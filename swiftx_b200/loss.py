@@ -22,8 +22,9 @@ def _args(x, w, targets, ignore_index, reduction):
     a = _lib.XentArgs()
     a.tokens, a.dim, a.vocab = x.shape[0], x.shape[1], w.shape[0]
     a.dtype, a.reduction, a.ignore_index = _DT[x.dtype], reduction, ignore_index
-    a.x, a.x_sr = x.data_ptr(), x.stride(0)
-    a.weight, a.w_sr = w.data_ptr(), w.stride(0)
+    # a single row's stride may be anything
+    a.x, a.x_sr = x.data_ptr(), x.stride(0) if a.tokens != 1 else a.dim
+    a.weight, a.w_sr = w.data_ptr(), w.stride(0) if a.vocab != 1 else a.dim
     a.targets = targets.data_ptr()
     return a
 

@@ -173,6 +173,19 @@ def test_layouts_and_partial_gradients():
         assert torch.equal(linear_cross_entropy(x, w, y), base[0])
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_single_rows_of_any_stride(dtype):
+    """One token and one word, as views whose row stride is 0 or less than the row."""
+    x, w, y = _inputs(1, 9, 24, dtype, ignored=0)
+    base = _run(x, w, y)
+    for stride in (0, 7):
+        for a, b in zip(base, _run(x.as_strided((1, 24), (stride, 1)), w, y)):
+            assert torch.equal(a, b)
+    one = w[:1].as_strided((1, 24), (0, 1))
+    loss, dx, dw = _run(x, one, torch.zeros_like(y))
+    assert float(loss) == 0.0 and not dx.any() and not dw.any()
+
+
 def test_fp32_weight_with_bf16_input_and_autocast():
     """The weight is rounded to bf16 for the products; its gradient comes back in fp32, not rounded again."""
     x, w, y = _inputs(260, 900, 80, FP, seed=4)
