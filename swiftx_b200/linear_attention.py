@@ -134,7 +134,8 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
     q and k of head h // (H // Hk).  log_decay fp32, (b, L, H), or (H,) for fixed decays; 0 keeps
     the state, -inf resets it.  initial_state fp32 (b, H, dk, dv).  lengths, an int64 (b,) tensor:
     row i has lengths[i] tokens (clamped to 0..L); what lies behind them is not read, gives zeros in
-    out and in the gradients, and leaves the state.  Returns out (b, L, H, dv), and with return_state the
+    out and in the gradients, and leaves the state; up to there q, k and v have to be finite (an infinity or
+    NaN at one token can reach the outputs of the chunk's earlier tokens).  Returns out (b, L, H, dv), and with return_state the
     fp32 state after the last token.  Differentiable in q, k, v, log_decay and initial_state;
     deterministic.  bf16 inputs: the score tiles are rounded to bf16 once, states and log_decay's gradient
     keep fp32 accuracy."""
@@ -158,10 +159,13 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
 def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
     """One token of ``linear_attention`` for every row: q, k (b, Hk, dk), v (b, H, dv), log_decay
     (b, H) or (H,); ``state``, a dense fp32 (b, H, dk, dv) tensor (as linear_attention returns it), is updated
-    in place.  Returns out (b, H, dv) in v's dtype.  Not differentiable."""
+    in place.  Returns out (b, H, dv) in v's dtype.  Not differentiable: operands that require
+    gradients are refused unless they are disabled."""
     _check("linear_attention_step", q, k, v, log_decay, state, 1)
     if not state.is_contiguous():
         raise ValueError("linear_attention_step: state must be a dense (b, H, dk, dv) tensor")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
+        raise RuntimeError("linear_attention_step is not differentiable: call it under no_grad, or linear_attention on one token")
     q, k, v = _unit(q), _unit(k), _unit(v)
     with _lib.on_device(v.device):
         lib = _lib.load()
@@ -169,7 +173,7 @@ def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
         a = _lib.LinattnArgs()
         a.batch, a.heads, a.dv = v.shape
         a.seqlen, (a.qk_heads, a.dk) = 1, q.shape[1:]
-        a.dtype, a.scale = _DT[q.dtype], scale
+        a.dtype, a.scale = _DT[q.dtype], float(scale)
         a.q, (a.q_sb, a.q_sh) = q.data_ptr(), q.stride()[:2]
         a.k, (a.k_sb, a.k_sh) = k.data_ptr(), k.stride()[:2]
         a.v, (a.v_sb, a.v_sh) = v.data_ptr(), v.stride()[:2]
@@ -177,4 +181,5 @@ def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
         a.g_sb, a.g_sh = (0, log_decay.stride(0)) if log_decay.dim() == 1 else log_decay.stride()
         a.out, a.final_state = out.data_ptr(), state.data_ptr()
         _lib.check(lib.swx_linattn_step(a, _lib.stream_ptr(v.device)), "swx_linattn_step")
+    torch.autograd.graph.increment_version(state)      # a backward that saved this state must not use the new one
     return out

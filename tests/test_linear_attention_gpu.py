@@ -206,6 +206,20 @@ def test_resets_and_extreme_decays(dtype):
     assert torch.equal(again["out"][:, 70:, 0], got["out"][:, 70:, 0])
 
 
+@pytest.mark.parametrize("b,L,H,dtype", [(1, 190, 4, torch.bfloat16), (2, 190, 4, torch.float32), (32, 520, 4, torch.bfloat16)])
+def test_growing_states(b, L, H, dtype):
+    """Positive log decays: sums that swing by 4 either way, a rise and fall by 36 inside 24 tokens, and one by 50 in
+    20 (beyond what the pipelined kernel's split exponentials take).  The terms' errors are as with decays below 0."""
+    t, do, ds = _inputs(b, L, H, H, 32, 40, dtype, seed=4)
+    at = torch.arange(L, device=DEV)
+    t["g"][..., 0] = 0.4 * torch.cos(at * (2 * torch.pi / 64))
+    t["g"][..., 1] += 0.01
+    t["g"][:, 100:112, 2], t["g"][:, 112:124, 2] = 3.0, -3.0
+    t["g"][:, 130:140, 3], t["g"][:, 140:150, 3] = 5.0, -5.0
+    got = _run(t, do, ds, 0.2, None)
+    _check(got, _oracle(t, do, ds, 0.2, None), _oracle(t, do, ds, 0.2, None, True), t, L)
+
+
 def test_strided_operands():
     """Column slices of one projection's output, a transposed head layout, a broadcast decay and gradient."""
     b, L, H, d = 2, 150, 4, 64
@@ -423,3 +437,22 @@ def test_short_buffers_are_refused_on_the_host():
     a.dlog_decay = t["g"].data_ptr()
     a.workspace_bytes = lib.swx_linattn_bwd_workspace_bytes(a) - 4
     assert lib.swx_linattn_bwd(a, None) == _lib.SWX_ERR_INVALID_ARG
+
+
+def test_step_and_autograd():
+    """A step takes no operand that a gradient is asked of, and a backward that saved the state before it raises."""
+    t, do, _ = _inputs(1, 3, 2, 2, 16, 16, torch.float32)
+    one = [t[n][:, 0] for n in ("q", "k", "v", "g")]
+    for i in range(5):
+        x = [*one, t["s0"].clone()]
+        x[i] = x[i].detach().requires_grad_()
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            linear_attention_step(*x)
+        with torch.no_grad():
+            linear_attention_step(*x)
+    q = t["q"].detach().requires_grad_()
+    state = t["s0"].clone()
+    out = linear_attention(q, t["k"], t["v"], t["g"], initial_state=state)
+    linear_attention_step(*one, state)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(do)
