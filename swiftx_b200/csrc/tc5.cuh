@@ -75,11 +75,6 @@ __device__ __forceinline__ void tma_load_4d(void* sdst, const void* map, int x, 
                  :: "r"(smem_u32(sdst)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ void tma_prefetch_4d(const void* map, int x, int y, int z, int w) {
-    asm volatile("cp.async.bulk.prefetch.tensor.4d.L2.global.tile [%0, {%1, %2, %3, %4}];"
-                 :: "l"(map), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
-
 // ---------------------------------------------------------------- tensor memory
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* sdst, uint32_t cols) {      // one warp of each CTA
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
