@@ -424,7 +424,7 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll
             for (int k = 0; k < 4; ++k) mma_bf16_cta(t_sc + 128 * (i & 1), qd + k * 2, kd + k * 2, id_s, k > 0);
             mma_commit(&scored[i & 1]);
-            if (i > 0) lt_wait(&shared[(i - 1) & 1], ((i - 1) >> 1) & 1, ok);        // every warp of A has read U of two chunks ago
+            if (i > 0) mix(i - 1);        // (and every warp of A has read U of two chunks ago)
             lt_wait(&weighed[0], i & 1, ok);
             tc_fence_after();
             lt_issue_u<0, 4>(u, planes, tile(i, 2));
@@ -433,7 +433,6 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
             tc_fence_after();
             lt_issue_u<4, 8>(u, planes, tile(i, 2));
             mma_commit(&products[1][i & 1]);
-            if (i > 0) mix(i - 1);
         }
         if (n > 0) mix(n - 1);
     } else if (warp < LT_A) {                                    // A
