@@ -96,12 +96,17 @@ static LaCut la_cut(int nc, int64_t n) {
 
 // One CTA walks a segment of one head's sequence.  Where the heads leave SMs idle the sequence is
 // cut, so that the CTAs fill, and do not exceed, one round on 148 SMs; the states at the segments'
-// starts cost one more reading of k and v.
-// The pipelined kernels (linear_attention_tc.cu, one CTA per SM, chunks of 128 tokens) need a few
-// chunks to fill; they are taken from 4 chunks a walk (8 where the heads alone take several rounds) and
-// 256 chunks in all.  us, theirs against the other kernels', forward, heads of 64: 144 heads x 512
-// tokens 26 / 42, x 4096 101 / 168; 64 heads x 2048 56 / 62; 256 heads x 1024 63 / 68, x 512
-// 37 / 37; 640 heads x 512 90 / 79; 1 head x 16384 (128 chunks) 40 / 33.
+// starts cost one more reading of k and v, and two launches.
+//
+// The pipelined kernels (linear_attention_tc.cu, one CTA per SM, chunks of 128 tokens) take bf16 heads of up to 64
+// from 65 tokens on, and from 4 chunks on where the heads alone take several rounds.  us, theirs / the other
+// kernels', forward, heads of 64: 8 heads x 64 tokens 8.2 / 6.5, x 100 8.3 / 9.3, x 512 14.3 / 17.0; 128 heads x 256
+// 11.9 / 24.0, x 4096 97 / 176; 512 heads x 128 30 / 21, x 256 40 / 35, x 512 68 / 74, x 4096 373 / 549.
+// An uncut walk takes them 6 us and 2 for each chunk; a cut one 14 and 3 for each chunk of a segment, with the states
+// and their chain; more than 64 segments make the chain longer than what they save (1 head x 16384
+// tokens: 128 segments 28.3 us, 64 25.2, 32 29.3; 8 heads x 1024: uncut 22, segments of 4 chunks 27.3, of 2
+// 21.0, of 1 18.0; x 512: uncut 14.3, cut 18.0).
+//
 // The other kernels have three CTAs on an SM (two with dk > 64 or fp32); the backward runs two walks at
 // once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).
 static LaPlan la_plan(const swx_linattn_args* a) {
@@ -109,9 +114,10 @@ static LaPlan la_plan(const swx_linattn_args* a) {
     q.nsl = (int)((a->dv + LA_DV - 1) / LA_DV);
     q.nc = (int)((a->seqlen + LA_C - 1) / LA_C);
     const int64_t heads = a->batch * a->heads * q.nsl, chunks = (q.nc + 1) / 2;
-    q.tc = a->dtype == SWX_DTYPE_BF16 && a->dk <= 64 && chunks >= (heads > 148 ? 8 : 4) && heads * chunks >= 256;
+    q.tc = a->dtype == SWX_DTYPE_BF16 && a->dk <= 64 && (heads > 148 ? chunks >= 4 : q.nc >= 2);
     const int64_t slots = 148 * (a->dk > 64 || a->dtype == SWX_DTYPE_F32 ? 2 : 3);
-    q.fwd = la_cut(q.nc, q.tc ? std::min<int64_t>(148 / heads, chunks / 4) : slots / heads);
+    const int64_t n = std::max<int64_t>(1, std::min<int64_t>(148 / heads, 64)), segment = (chunks + n - 1) / n;
+    q.fwd = la_cut(q.nc, !q.tc ? slots / heads : 2 * chunks > 3 * segment + 8 ? n : 1);
     q.bwd = la_cut(q.nc, slots / heads);
     return q;
 }
@@ -255,6 +261,8 @@ int swx_linattn_bwd(const swx_linattn_args* a, void* stream) {
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     auto at = [ws](int64_t o) { return reinterpret_cast<float*>(ws + o); };
     LaDev p = la_pack(a, q, q.bwd);
+    // the reverse states: 64 heads of 8192 tokens (22 chunks a segment) 619 us with the pipelined kernel, 625 with
+    // the other one; 64 x 2048 (6 chunks) 199 and 198
     p.tc = p.tc && q.bwd.segc >= 16;
     p.seg = a->seg_states;
     p.dec = at(w.dec); p.rseg = at(w.seg); p.rin = at(w.rin); p.yseg = at(w.yseg);
