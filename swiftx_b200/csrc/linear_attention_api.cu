@@ -108,7 +108,9 @@ static LaCut la_cut(int nc, int64_t n) {
 // 21.0, of 1 18.0; x 512: uncut 14.3, cut 18.0).
 //
 // The other kernels have three CTAs on an SM (two with dk > 64 or fp32); the backward runs two walks at
-// once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).
+// once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).  Where its
+// last segment would be less than half of the others, all are made shorter by two chunks (forward and
+// backward, 64 heads x 2048 tokens 194 -> 191 us, x 1664 166 -> 153, 80 x 2100 238 -> 218).
 static LaPlan la_plan(const swx_linattn_args* a) {
     LaPlan q{};
     q.nsl = (int)((a->dv + LA_DV - 1) / LA_DV);
@@ -119,6 +121,10 @@ static LaPlan la_plan(const swx_linattn_args* a) {
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>(148 / heads, 64)), segment = (chunks + n - 1) / n;
     q.fwd = la_cut(q.nc, !q.tc ? slots / heads : 2 * chunks > 3 * segment + 8 ? n : 1);
     q.bwd = la_cut(q.nc, slots / heads);
+    if (q.bwd.nseg > 1 && 2 * (q.nc - (q.bwd.nseg - 1) * q.bwd.segc) < q.bwd.segc) {       // a short last segment
+        q.bwd.segc -= 2;
+        q.bwd.nseg = (q.nc + q.bwd.segc - 1) / q.bwd.segc;
+    }
     return q;
 }
 
