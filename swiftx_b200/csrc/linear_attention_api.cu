@@ -12,6 +12,7 @@ namespace swx {
 // S = exp(g) S + k v^T in place, out = scale S^T q.  Reads and writes 8 bytes per state value and
 // little else, so it is bound by HBM: one CTA per (row, head), thread = VEC columns of every
 // R-th row of the state with four loads in flight, column sums joined through shared memory.
+// 256 rows x 32 heads of 64 x 64: 41 to 45 us, 272 MB, 92 to 100 % of the copy rate; 1 x 8: 4 us, a launch.
 struct LaStep {
     int H, Hk, dk, dv;
     float scale;
@@ -159,7 +160,7 @@ static LaWs la_ws(const swx_linattn_args* a, const LaPlan& q) {
     w.seg = take(q.bwd.nseg > 1 ? bh * q.bwd.nseg * a->dk * a->dv : 0);
     w.rin = take(bv * a->seqlen);
     w.net = take(bv * a->seqlen);
-    w.yseg = take(bv * q.bwd.nseg);
+    w.yseg = take(bv * (q.bwd.nseg + 1));
     w.dg = take(a->decay_per_head ? 2 * bh * q.bwd.nseg : 0);
     w.dq = take(la_shared(a, q) ? bv * a->seqlen * a->dk : 0);
     w.dk = take(la_shared(a, q) ? bv * a->seqlen * a->dk : 0);

@@ -21,8 +21,8 @@ template <typename T> struct Planes { static constexpr int N = sizeof(T) == 4 ? 
 
 // acc[DK / 8] += rows 16 rw of x (16 x 64) times S^T, S in shared memory in full precision.
 // The small pieces of S come first: the tensor core cuts the low bits of each addition off, and with 12 additions at the
-// sum's full size instead of 4 a decay gradient for each head was 1.4e-6 off where it is 7e-7 now (16 x 512 x 16 heads,
-// dk 128; the walks 1 % slower for the operand's repeated reads).
+// sum's full size instead of 4 the decay's gradient is up to twice as far off (16 x 512 x 16 heads, dk 128, a decay for each:
+// 2.7e-6 and 1.4e-6; the walks 1 % slower for the operand's repeated reads).
 template <typename T, int DK>
 __device__ __forceinline__ void la_times_state_t(float (&acc)[DK / 8][4], const T* x, const T* s, int rw, int lane) {
     using Sh = LaShape<T, DK>;
@@ -85,6 +85,29 @@ __device__ __forceinline__ void la_store_qk(const float (&acc)[DK / 8][4], T* ti
     const int64_t sl = (int64_t)p.Hk * p.dk;
     la_store<T, DK, Sh::LDK>(tile + 16 * rw * Sh::LDK, static_cast<T*>(dst) + ((int64_t)b * p.L + tr) * sl + (int64_t)hk * p.dk, sl,
                              len - tr, p.L - tr, p.dk, p.vec_qk, lane);
+}
+
+// <a state in registers, one in memory (null: zero)> to `dst`, by the whole CTA; red: 4 floats that no one uses now.
+template <typename T, int DK>
+__device__ __forceinline__ void la_state_dot(const float (&S)[LaShape<T, DK>::MI][LaShape<T, DK>::NI][4], const float* other, float* dst,
+                                             const LaDev& p, int c0, int rw, int lane, float* red) {
+    using Sh = LaShape<T, DK>;
+    float y = 0.f;
+    if (other) {
+        float R[Sh::MI][Sh::NI][4];
+        la_state_read<T, DK>(R, other, p, c0, rw, lane);
+#pragma unroll
+        for (int i = 0; i < Sh::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < Sh::NI; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y += S[i][j][e] * R[i][j][e];
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
+    if (lane == 0) red[rw] = y;
+    __syncthreads();
+    if (threadIdx.x == 0) *dst = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 template <typename T, int DK> struct LaBwd {
@@ -176,23 +199,8 @@ __device__ __forceinline__ void la_dq_walk(const LaDev& p, int64_t block, uint8_
         ring.make(n, i, warp, lane);
     }
     // <state, its gradient> at the segment's end
-    const float* D = p.nseg > 1 ? p.rseg + (bh * p.nseg + seg) * ssz : (p.ds ? p.ds + bh * ssz : nullptr);
-    float y = 0.f;
-    if (D) {
-        float R[Sh::MI][Sh::NI][4];
-        la_state_read<T, DK>(R, D, p, c0, rw, lane);
-#pragma unroll
-        for (int i = 0; i < Sh::MI; ++i)
-#pragma unroll
-            for (int j = 0; j < Sh::NI; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y += S[i][j][e] * R[i][j][e];
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o /= 2) y += __shfl_xor_sync(0xffffffffu, y, o);
-    if (lane == 0) red[rw] = y;
-    __syncthreads();
-    if (threadIdx.x == 0) p.yseg[((int64_t)b * p.H * p.nsl + vhead) * p.nseg + seg] = (red[0] + red[1]) + (red[2] + red[3]);
+    la_state_dot<T, DK>(S, p.nseg > 1 ? p.rseg + (bh * p.nseg + seg) * ssz : (p.ds ? p.ds + bh * ssz : nullptr),
+                        p.yseg + ((int64_t)b * p.H * p.nsl + vhead) * (p.nseg + 1) + seg + 1, p, c0, rw, lane, red);
 }
 
 // ------------------------------------------------------------------ dk, dv, dg: reverse walk
@@ -387,12 +395,18 @@ __device__ __forceinline__ void la_dkv_walk(const LaDev& p, int64_t block, uint8
         if (t < LA_C && t0 + t < p.L)
             net[t0 + t] = ((rowsum[0][t] + rowsum[1][t]) + (rowsum[2][t] + rowsum[3][t])) - colsum[t];
     }
-    if (p.ds0 && seg == 0) la_state_write<T, DK>(D, p.ds0 + bh * ssz, p, c0, rw, lane);
+    if (seg == 0) {
+        if (p.ds0) la_state_write<T, DK>(D, p.ds0 + bh * ssz, p, c0, rw, lane);
+        __syncthreads();
+        la_state_dot<T, DK>(D, p.s0 ? p.s0 + bh * ssz : nullptr, p.yseg + ((int64_t)b * p.H * p.nsl + vhead) * (p.nseg + 1), p, c0, rw, lane,
+                            colsum);
+    }
 }
 
 // ------------------------------------------------------------------ sums over heads that share
 // dst[row][hk][c] = sum over the group's parts of src[row][part][c], in order, for dq and dk in one
-// launch; thread = VEC values.
+// launch; thread = VEC values.  A stream over the parts: 16 x 512 tokens x 16 heads of 128 in 23 us, 134 MB, most of it
+// still in L2.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) la_group_sum_kernel(const float* src_q, const float* src_k, T* dst_q, T* dst_k, int64_t rows, int Hk,
                                                            int per, int d) {
@@ -422,26 +436,64 @@ __global__ void __launch_bounds__(256) la_group_sum_kernel(const float* src_q, c
 // ------------------------------------------------------------------ dg
 // One CTA per segment of one head, from the segment's end: dg_t = <S, D> at the end + the sum of
 // q . dq - k . dk over the tokens from t on (fp64), v's slices added up; or, for a decay per
-// head, the segment's sum of it.
+// head, the segment's sum of it.  At the segment's first token the sum has to arrive at <S, D> of its start.  What it
+// is off by there, mostly the low bits that the tensor core cuts off, all the same way, is taken out over the
+// segment in proportion to the terms' sizes (5 x 1009 x 2 heads, a decay for each head: 3.0e-6 -> 1.1e-6 off; 8 x 2048 x 8
+// heads 6.2e-7 -> 4.4e-7; 4 us either way).
 constexpr int LG_THREADS = 256;
 
 __global__ void __launch_bounds__(LG_THREADS) la_dg_kernel(const LaDev p) {
-    __shared__ double ws[LG_THREADS / 32];
+    __shared__ double ws[LG_THREADS / 32], wm[LG_THREADS / 32];
     const int seg = blockIdx.x % p.nseg, h = blockIdx.x / p.nseg % p.H, b = blockIdx.x / p.nseg / p.H;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, len = la_len(p, b);
     const int lo = seg * p.segc * LA_C, hi = min(p.L, (seg + 1) * p.segc * LA_C);
     const int64_t v0 = ((int64_t)b * p.H + h) * p.nsl;
-    double run = 0., all = 0.;
-    for (int s = 0; s < p.nsl; ++s) run += (double)p.yseg[(v0 + s) * p.nseg + seg];
+    double run = 0., all = 0., start = 0.;
+    for (int s = 0; s < p.nsl; ++s) {
+        start += (double)p.yseg[(v0 + s) * (p.nseg + 1) + seg];
+        run += (double)p.yseg[(v0 + s) * (p.nseg + 1) + seg + 1];
+    }
     const float* g = p.g + (int64_t)b * p.g_sb + (int64_t)h * p.g_sh;
+    auto term = [&](int t, double& size) {                   // a token's q . dq - k . dk
+        double x = 0.;
+        size = 0.;
+        if (t < lo || t >= len) return x;
+        for (int s = 0; s < p.nsl; ++s) {
+            const float a = p.rin[(v0 + s) * p.L + t], c = p.net[(v0 + s) * p.L + t];
+            x += (double)a + (double)c;
+            size += (double)fabsf(a) + (double)fabsf(c);
+        }
+        return x;
+    };
+    // what the sum is off by at the segment's start, for each unit of the terms' sizes
+    double sum = 0., sizes = 0.;
+    for (int t = hi - 1 - (int)threadIdx.x; t >= lo; t -= LG_THREADS) {
+        double m;
+        sum += term(t, m);
+        sizes += m;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        sizes += __shfl_xor_sync(0xffffffffu, sizes, o);
+    }
+    if (lane == 0) {
+        ws[warp] = sum;
+        wm[warp] = sizes;
+    }
+    __syncthreads();
+    sum = sizes = 0.;
+    for (int w = 0; w < LG_THREADS / 32; ++w) {
+        sum += ws[w];
+        sizes += wm[w];
+    }
+    double off = sizes > 0. ? (run + sum - start) / sizes : 0.;
+    if (!(fabs(off) < 1e-3)) off = 0.;                       // not a matter of rounding (values that are not finite)
     for (int t0 = hi; t0 > lo; t0 -= LG_THREADS) {
         const int t = t0 - 1 - (int)threadIdx.x;             // thread 0: the last token
-        double x = 0.;
-        float gt = 0.f;
-        if (t >= lo && t < len) {
-            gt = g[(int64_t)t * p.g_sl];
-            for (int s = 0; s < p.nsl; ++s) x += (double)p.rin[(v0 + s) * p.L + t] + (double)p.net[(v0 + s) * p.L + t];
-        }
+        double m, x = term(t, m);
+        const float gt = t >= lo && t < len ? g[(int64_t)t * p.g_sl] : 0.f;
+        x -= off * m;
 #pragma unroll
         for (int o = 1; o < 32; o *= 2) {
             const double z = __shfl_up_sync(0xffffffffu, x, o);
@@ -482,7 +534,10 @@ __global__ void __launch_bounds__(32) la_dg_head_kernel(const double* part, floa
     if (threadIdx.x == 0) dst[blockIdx.x] = (float)x;
 }
 
-// Both walks in one launch, the longer ones (dk, dv) first.
+// Both walks in one launch, the longer ones (dk, dv) first.  Bound by latency and issue (8 x 2048 x 8 heads of 64, bf16:
+// 120 us, a warp issues in 40 % of a quarter's cycles, mma.sync busy in 35 %, three warps to a quarter: 64 KB of
+// shared memory and 168 registers a thread leave no fourth CTA); of 17 products of 64^3 a chunk, 8 are the second and
+// third pieces that keep the states and the decay's gradient to fp32.
 template <typename T, int DK>
 __global__ void __launch_bounds__(LA_THREADS, sizeof(T) == 4 ? 1 : DK == 128 ? 2 : 3) la_bwd_kernel(const LaDev p) {
     extern __shared__ __align__(16) uint8_t smem[];

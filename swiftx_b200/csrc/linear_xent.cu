@@ -13,7 +13,11 @@
 // Every product runs on the same kernel: a persistent grid of CTA pairs, 256 x 256 tiles,
 // operands staged by TMA into a ring, tcgen05 products issued by one thread per pair into
 // two alternating accumulators in tensor memory, and eight warps per CTA that read an
-// accumulator while the next tile is computed.
+// accumulator while the next tile is computed.  The tensor pipe bounds it: 4096 tokens x 32768 x 1024 bf16, cold,
+// forward 178 us (88 % of the SM's active cycles on products, 1547 TFLOP/s), dlogit 199 us (79 %; it writes 268 MB), dx 190
+// (93 %, on 64 of 74 pairs); 8192 x 50001 x 1024 0.51, 0.57, 0.58 and 0.60 ms, where a library
+// product of the same size alone takes 0.56 to 0.61.  The logits' epilogue (an exponential for each) fits behind a
+// tile's products from about 512 values of the contraction on; below that it bounds the forward.
 //
 // fp32 operands are split into three bf16 pieces (24 bits) and multiplied as the six
 // products of pieces above 2^-24, smallest first, on the same kernel.
@@ -451,7 +455,8 @@ __device__ __forceinline__ void join_pair(float& m, float& s, float2 q) {
 
 // CTA = 8 rows x 32 slices of the pieces (few rows per CTA, so that a short call still has
 // many CTAs): each thread joins its slice, four pieces at a time, then the slices are joined
-// by shuffles and through shared memory, always in the same order.  Each CTA leaves the sum of
+// by shuffles and through shared memory, always in the same order.  A few microseconds whatever the size
+// (512 tokens x 392 pieces 4.4 us, 8192 x 2 6.8), latency.  Each CTA leaves the sum of
 // its rows' losses and the count of its tokens; the last CTA to finish adds those up (fp64, a
 // fixed order whichever CTA it is).
 __global__ void __launch_bounds__(XJ_ROWS * XJ_SLICES) xent_join_kernel(const XentJoin p) {
@@ -534,7 +539,8 @@ __global__ void __launch_bounds__(XJ_ROWS * XJ_SLICES) xent_join_kernel(const Xe
 }
 
 // ------------------------------------------------------------------ summing a tile's parts
-// out = factor * (parts in order), for the spread gradients; thread = 4 columns of a row.
+// out = factor * (parts in order), for the spread gradients; thread = 4 columns of a row.  The parts
+// come from L2 (1003 tokens x 10007 x 200 fp32, dx and dW: 15 us of 235).
 __global__ void __launch_bounds__(256) xent_sum_kernel(const XentGemm p, int P) {
     const int per = (p.N + 3) / 4;
     const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
