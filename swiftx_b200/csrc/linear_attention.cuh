@@ -241,19 +241,21 @@ __device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][L
                                                 const LaGates& gt, float scale, int rw, int lane) {
     using Sh = LaShape<T, DK>;
     const int m0 = (rw % Sh::WM) * Sh::MI * 16, n0 = (rw / Sh::WM) * Sh::NI * 8;
+    auto weights = [&](float (&w4)[4], int k0) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int s = k0 + 2 * (lane & 3) + (x & 1) + (x >> 1) * 8;
+            w4[x] = PRE ? scale * gt.pre(s) : gt.post[s];
+        }
+    };
     if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int i = 0; i < Sh::MI; ++i) {
             float u[Sh::NI][4] = {}, lo[Sh::NI][4] = {};
 #pragma unroll LA_UNROLL<T>
             for (int k0 = 0; k0 < LA_C; k0 += 16) {
-                const int t = k0 + 2 * (lane & 3);
                 float w4[4];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const int s = t + (x & 1) + (x >> 1) * 8;
-                    w4[x] = PRE ? scale * gt.pre(s) : gt.post[s];
-                }
+                weights(w4, k0);
                 FragA<T> a;
                 load_a_t(a, xs, Sh::LDK, m0 + 16 * i, k0, lane);
                 ScaledA<T> s;
@@ -273,33 +275,29 @@ __device__ __forceinline__ void la_state_update(float (&S)[LaShape<T, DK>::MI][L
 #pragma unroll
                 for (int e = 0; e < 4; ++e) S[i][j][e] = fmaf(gt.all, S[i][j][e], u[j][e] + lo[j][e]);
         }
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int i = 0; i < Sh::MI; ++i)
+        for (int i = 0; i < Sh::MI; ++i)
 #pragma unroll
-        for (int j = 0; j < Sh::NI; ++j)
+            for (int j = 0; j < Sh::NI; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[i][j][e] *= gt.all;
+                for (int e = 0; e < 4; ++e) S[i][j][e] *= gt.all;
 #pragma unroll LA_UNROLL<T>
-    for (int k0 = 0; k0 < LA_C; k0 += 16) {
-        const int t = k0 + 2 * (lane & 3);
-        float w4[4];
+        for (int k0 = 0; k0 < LA_C; k0 += 16) {
+            float w4[4];
+            weights(w4, k0);
+            FragB<T> y[Sh::NI / 2][2];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int s = t + (x & 1) + (x >> 1) * 8;
-            w4[x] = PRE ? scale * gt.pre(s) : gt.post[s];
-        }
-        FragB<T> y[Sh::NI / 2][2];
+            for (int j = 0; j < Sh::NI / 2; ++j) load_b2_t(y[j], ys, Sh::LDV, n0 + 16 * j, k0, lane);
 #pragma unroll
-        for (int j = 0; j < Sh::NI / 2; ++j) load_b2_t(y[j], ys, Sh::LDV, n0 + 16 * j, k0, lane);
+            for (int i = 0; i < Sh::MI; ++i) {
+                FragA<T> a;
+                load_a_t(a, xs, Sh::LDK, m0 + 16 * i, k0, lane);
+                ScaledA<T> s;
+                scale_a(s, a, w4);
 #pragma unroll
-        for (int i = 0; i < Sh::MI; ++i) {
-            FragA<T> a;
-            load_a_t(a, xs, Sh::LDK, m0 + 16 * i, k0, lane);
-            ScaledA<T> s;
-            scale_a(s, a, w4);
-            mma_row(S[i], s, y);
+                for (int j = 0; j < Sh::NI; ++j) mma(S[i][j], s.p, y[j / 2][j & 1]);
+            }
         }
     }
 }

@@ -178,21 +178,6 @@ __device__ __forceinline__ void scale_a(ScaledA<float>& o, const FragA<float>& a
 #pragma unroll
     for (int i = 0; i < 8; ++i) o.p.v[i] = a.v[i] * w[(i >> 2) * 2 + (i & 1)];
 }
-// Times N column tiles; the pieces outermost, so that products that follow one another add to
-// different accumulators.
-template <int N>
-__device__ __forceinline__ void mma_row(float (&c)[N][4], const ScaledA<__nv_bfloat16>& a, const FragB<__nv_bfloat16> (&b)[N / 2][2]) {
-#pragma unroll
-    for (int q = 2; q >= 0; --q)
-#pragma unroll
-        for (int j = 0; j < N; ++j) mma_bf16(c[j], a.p[q].r, b[j / 2][j & 1].r);
-}
-template <int N>
-__device__ __forceinline__ void mma_row(float (&c)[N][4], const ScaledA<float>& a, const FragB<float> (&b)[N / 2][2]) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) mma(c[j], a.p, b[j / 2][j & 1]);
-}
-
 // An accumulator tile into shared memory at s[row * ld + column] (row0, col0: the tile's
 // first), as PLANES bf16 pieces `plane` elements apart, or as fp32.
 template <int PLANES>
