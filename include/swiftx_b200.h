@@ -428,7 +428,8 @@ int swx_embedding_bwd(const swx_embedding_args* args, void* stream);
  * tokens that count; not for SWX_XENT_NONE), and row_max, row_rsum (tokens values) for the
  * backward.  Backward: dloss (as loss) -> dx (tokens, dim) dense in dtype and dweight
  * (vocab, dim) dense in dw_dtype; either may be NULL.  The vocabulary is walked in pieces;
- * every sum runs in a fixed order (deterministic).  With no tokens a mean is NaN. */
+ * every sum runs in a fixed order (deterministic).  With no tokens a mean is NaN.  The
+ * workspace starts on 16 bytes. */
 #define SWX_XENT_NONE 0
 #define SWX_XENT_MEAN 1
 #define SWX_XENT_SUM 2

@@ -637,8 +637,10 @@ struct XentPlan {
 
 static int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
+static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 static bool direct_ok(const void* p, int64_t sr, int dtype) {
-    return dtype == SWX_DTYPE_BF16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && sr % 8 == 0;
+    return dtype == SWX_DTYPE_BF16 && aligned16(p) && sr % 8 == 0;
 }
 
 // Vocabulary columns per piece of the backward: at most 416 MB of dlogit (tokens x columns,
@@ -795,7 +797,7 @@ int swx_xent_fwd(const swx_xent_args* a, void* stream) {
     if (a->tokens > 0 && (!a->x || !a->weight || !a->targets || !a->row_max || !a->row_rsum || !a->workspace || (none && !a->loss)))
         return SWX_ERR_INVALID_ARG;
     const XentPlan q = xent_plan(a);
-    if (a->tokens > 0 && a->workspace_bytes < q.fwd_total) return SWX_ERR_INVALID_ARG;
+    if (a->tokens > 0 && (a->workspace_bytes < q.fwd_total || !aligned16(a->workspace))) return SWX_ERR_INVALID_ARG;
     if (a->tokens == 0) {
         if (none) return SWX_OK;
         // no token: a sum of 0, a mean of 0 / 0
@@ -842,7 +844,7 @@ int swx_xent_bwd(const swx_xent_args* a, void* stream) {
         (a->reduction == SWX_XENT_MEAN && !a->count))
         return SWX_ERR_INVALID_ARG;
     const XentPlan q = xent_plan(a);
-    if (a->workspace_bytes < q.bwd_total) return SWX_ERR_INVALID_ARG;
+    if (a->workspace_bytes < q.bwd_total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
     const Operand x = operand(a->x, a->x_sr, T, d, a->dtype, q.pack_x, q, ws, q.off_x, st);

@@ -96,6 +96,14 @@ def test_loss_buffers():
     assert lib.swx_xent_bwd(f, None) == UNSUPPORTED
 
 
+def test_loss_workspace_off_its_alignment_is_refused():
+    lib = _lib.load()
+    a = _xent()
+    a.loss = a.count = a.targets = a.row_max = a.row_rsum = a.dloss = a.dx = 4096
+    a.workspace, a.workspace_bytes = 4096 + 8, 1 << 30
+    assert lib.swx_xent_fwd(a, None) == INVALID and lib.swx_xent_bwd(a, None) == INVALID
+
+
 def test_loss_workspace_does_not_hold_the_logits():
     lib = _lib.load()
     T, V, d = 65536, 131072, 64
