@@ -211,7 +211,7 @@ __device__ __forceinline__ void xent_emit(const XentGemm& p, float (&v)[32], int
 }
 
 // SUMS: the steps of a tile come in several accumulators (fp32 operands); their sum stays in registers until the tile (or
-// this pair's part of it) is complete: through memory each time, 1003 tokens x 10007 x 200 took 232 us, 219 now.
+// this pair's part of it) is complete: through memory each time, 1003 tokens x 10007 x 200 took 232 us, 219 with the registers.
 template <int EPI, bool A_MN, bool B_MN, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1)
 xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -568,7 +568,7 @@ __global__ void __launch_bounds__(XJ_ROWS * XJ_SLICES) xent_join_kernel(const Xe
 
 // ------------------------------------------------------------------ summing a tile's parts
 // out = factor * (parts in order), for the spread gradients; thread = 4 columns of a row.  The parts
-// come from L2 (1003 tokens x 10007 x 200 fp32, dx and dW: 15 us of 235).
+// come from L2 (1003 tokens x 10007 x 200 fp32, dx and dW: 15 us of 216).
 __global__ void __launch_bounds__(256) xent_sum_kernel(const XentGemm p, int P) {
     const int per = (p.N + 3) / 4;
     const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
@@ -606,15 +606,19 @@ __global__ void __launch_bounds__(256) xent_sum_kernel(const XentGemm p, int P) 
 // (rows, d) with any row stride -> dense bf16 pieces (planes, rows, dp), dp a multiple of
 // 8: fp32 values as three bf16 pieces (each the rounding of what the earlier ones leave),
 // bf16 values as themselves.  Columns d..dp are zero.
+// Two matrices in one launch (rows 0: none).
+struct XentPack { const void* src; int64_t sr, rows; __nv_bfloat16* dst; };
+
 template <typename T>
-__global__ void __launch_bounds__(256) xent_pack_kernel(const T* __restrict__ src, int64_t sr, int64_t rows, int d, int dp,
-                                                        __nv_bfloat16* __restrict__ dst) {
+__global__ void __launch_bounds__(256) xent_pack_kernel(const XentPack x, const XentPack w, int d, int dp) {
     const int per = dp / 8;
-    const int64_t n = rows * per;
+    const int64_t n = (x.rows + w.rows) * per;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t r = i / per;
+        const bool second = i / per >= x.rows;
+        const XentPack& m = second ? w : x;
+        const int64_t r = i / per - (second ? x.rows : 0);
         const int c = (int)(i % per) * 8;
-        const T* s = src + r * sr + c;
+        const T* s = static_cast<const T*>(m.src) + r * m.sr + c;
         float v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = c + j < d ? Elem<T>::to_f(s[j]) : 0.f;
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(256) xent_pack_kernel(const T* __restrict__ sr
                 o[j] = __float2bfloat16_rn(v[j]);
                 v[j] -= __bfloat162float(o[j]);
             }
-            *reinterpret_cast<uint4*>(dst + ((int64_t)pl * rows + r) * dp + c) = *reinterpret_cast<const uint4*>(o);
+            *reinterpret_cast<uint4*>(m.dst + ((int64_t)pl * m.rows + r) * dp + c) = *reinterpret_cast<const uint4*>(o);
         }
     }
 }
@@ -756,20 +760,18 @@ struct Operand {
     bool mn_major(CUtensorMap* m) const { return encode_operand(m, p, inner, rows, planes, row, plane, 64, 64); }
 };
 
-template <typename T>
-static void pack(const void* src, int64_t sr, int64_t rows, int64_t d, int64_t dp, void* dst, cudaStream_t st) {
-    const int64_t n = rows * (dp / 8);
+// x and the weight as the products read them: themselves, or their copies in the workspace.
+static void operands(const swx_xent_args* a, const XentPlan& q, uint8_t* ws, Operand& x, Operand& w, cudaStream_t st) {
+    const int64_t T = a->tokens, V = a->vocab, d = a->dim;
+    x = q.pack_x ? Operand{ws + q.off_x, d, T, q.planes, q.dp, T * q.dp} : Operand{a->x, d, T, 1, a->x_sr, 0};
+    w = q.pack_w ? Operand{ws + q.off_w, d, V, q.planes, q.dp, V * q.dp} : Operand{a->weight, d, V, 1, a->w_sr, 0};
+    const XentPack px{a->x, a->x_sr, q.pack_x ? T : 0, reinterpret_cast<__nv_bfloat16*>(ws + q.off_x)};
+    const XentPack pw{a->weight, a->w_sr, q.pack_w ? V : 0, reinterpret_cast<__nv_bfloat16*>(ws + q.off_w)};
+    const int64_t n = (px.rows + pw.rows) * (q.dp / 8);
+    if (n == 0) return;
     const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 16);
-    xent_pack_kernel<T><<<grid, 256, 0, st>>>(static_cast<const T*>(src), sr, rows, (int)d, (int)dp,
-                                              static_cast<__nv_bfloat16*>(dst));
-}
-
-static Operand operand(const void* src, int64_t sr, int64_t rows, int64_t d, int dtype, bool packed, const XentPlan& q,
-                       uint8_t* ws, int64_t off, cudaStream_t st) {
-    if (!packed) return Operand{src, d, rows, 1, sr, 0};
-    if (dtype == SWX_DTYPE_F32) pack<float>(src, sr, rows, d, q.dp, ws + off, st);
-    else pack<__nv_bfloat16>(src, sr, rows, d, q.dp, ws + off, st);
-    return Operand{ws + off, d, rows, q.planes, q.dp, rows * q.dp};
+    if (a->dtype == SWX_DTYPE_F32) xent_pack_kernel<float><<<grid, 256, 0, st>>>(px, pw, (int)d, (int)q.dp);
+    else xent_pack_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(px, pw, (int)d, (int)q.dp);
 }
 
 template <int EPI, bool A_MN, bool B_MN, bool SUMS = false>
@@ -834,8 +836,8 @@ int swx_xent_fwd(const swx_xent_args* a, void* stream) {
     }
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
-    const Operand x = operand(a->x, a->x_sr, a->tokens, a->dim, a->dtype, q.pack_x, q, ws, q.off_x, st);
-    const Operand w = operand(a->weight, a->w_sr, a->vocab, a->dim, a->dtype, q.pack_w, q, ws, q.off_w, st);
+    Operand x, w;
+    operands(a, q, ws, x, w, st);
     CUtensorMap mx, mw;
     if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
     XentGemm g{};
@@ -875,8 +877,8 @@ int swx_xent_bwd(const swx_xent_args* a, void* stream) {
     if (a->workspace_bytes < q.bwd_total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
-    const Operand x = operand(a->x, a->x_sr, T, d, a->dtype, q.pack_x, q, ws, q.off_x, st);
-    const Operand w = operand(a->weight, a->w_sr, V, d, a->dtype, q.pack_w, q, ws, q.off_w, st);
+    Operand x, w;
+    operands(a, q, ws, x, w, st);
     CUtensorMap x_k, w_k, x_mn, w_mn;
     if (!x.k_major(&x_k) || !w.k_major(&w_k) || !x.mn_major(&x_mn) || !w.mn_major(&w_mn)) return SWX_ERR_CUDA;
     const int npair = q.planes == 3 ? 6 : 1;
