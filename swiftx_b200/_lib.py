@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libswiftx_b200.so")
@@ -256,3 +257,12 @@ def on_device(device):
 
 
 _NOTHING = contextlib.nullcontext()
+
+
+def needs_node(*tensors):
+    """Whether a call on these operands (None: absent) has to go through its autograd function: a gradient is
+    asked of one, or forward-mode differentiation or a trace is under way.  The function refuses a dual
+    number and is a node of a trace; a bare launch would drop the tangent, or leave the trace an empty buffer."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 or torch.jit.is_tracing()

@@ -40,7 +40,7 @@ def _workspace(lib, name, a, like):
 
 def _forward(x, w, targets, ignore_index, reduction):
     """(loss, (row maxima, reciprocal row sums, count) in one buffer) of checked operands."""
-    T = x.shape[0]
+    T = int(x.shape[0])                # (under a trace a size is a tensor)
     with _lib.on_device(x.device):
         lib = _lib.load()
         none = reduction == _lib.XENT_REDUCTIONS["none"]
@@ -97,7 +97,8 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     rounded; under bf16 autocast an fp32 x is cast too.  The gradients are deterministic.
 
     A target outside [0, vocab) other than ignore_index gives a NaN loss (and gradients)
-    instead of a device-side assertion; x has to be finite in ignored rows too.  weight16: a bf16
+    instead of a device-side assertion; x has to be finite in ignored rows too.  Forward-mode dual numbers are
+    refused, and torch.jit.trace records the call as a Python operator.  weight16: a bf16
     copy of an fp32 weight that the caller keeps (used with bf16 x instead of rounding again)."""
     if reduction not in _lib.XENT_REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction {reduction!r}: one of none, mean, sum expected")
@@ -124,7 +125,7 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     t1 = targets if targets.dim() == 1 else targets.reshape(-1)
     opts = (int(ignore_index), _lib.XENT_REDUCTIONS[reduction])
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if _lib.needs_node(x, weight):
         loss = LinearCrossEntropyFn.apply(x2, weight, t1, *opts, weight16)
     else:
         w = weight if weight.dtype == x.dtype else weight.to(x.dtype) if weight16 is None else weight16
