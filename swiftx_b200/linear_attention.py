@@ -9,6 +9,7 @@ Over a sequence it runs chunked, on the tensor cores, with gradients; ``linear_a
 is its form for one token per row, on a state that it updates in place.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -136,8 +137,8 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
     row i has lengths[i] tokens (clamped to 0..L); what lies behind them is not read, gives zeros in
     out and in the gradients, and leaves the state; up to there q, k and v have to be finite (an infinity or
     NaN at one token can reach the outputs of the chunk's earlier tokens).  Returns out (b, L, H, dv), and with return_state the
-    fp32 state after the last token.  Differentiable in q, k, v, log_decay and initial_state;
-    deterministic.  bf16 inputs: the score tiles are rounded to bf16 once, states and log_decay's gradient
+    fp32 state after the last token.  Differentiable in q, k, v, log_decay and initial_state
+    (dual numbers of forward mode are refused, torch.jit.trace records a Python operator); deterministic.  bf16 inputs: the score tiles are rounded to bf16 once, states and log_decay's gradient
     keep fp32 accuracy."""
     _check("linear_attention", q, k, v, log_decay, initial_state, 2)
     if lengths is not None:
@@ -148,8 +149,7 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
     q, k, v = _unit(q), _unit(k), _unit(v)
     if initial_state is not None:
         initial_state = initial_state.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or log_decay.requires_grad
-                                    or (initial_state is not None and initial_state.requires_grad)):
+    if _lib.needs_node(q, k, v, log_decay, initial_state):
         out, state = LinearAttentionFn.apply(q, k, v, log_decay, initial_state, lengths, float(scale), return_state)
     else:
         out, state, _ = _forward(q, k, v, log_decay, initial_state, lengths, float(scale), return_state, False)
@@ -160,12 +160,16 @@ def linear_attention_step(q, k, v, log_decay, state, scale=1.0):
     """One token of ``linear_attention`` for every row: q, k (b, Hk, dk), v (b, H, dv), log_decay
     (b, H) or (H,); ``state``, a dense fp32 (b, H, dk, dv) tensor (as linear_attention returns it), is updated
     in place.  Returns out (b, H, dv) in v's dtype.  Not differentiable: operands that require
-    gradients are refused unless they are disabled."""
+    gradients are refused unless they are disabled, dual numbers and torch.jit.trace always."""
     _check("linear_attention_step", q, k, v, log_decay, state, 1)
     if not state.is_contiguous():
         raise ValueError("linear_attention_step: state must be a dense (b, H, dk, dv) tensor")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state)):
-        raise RuntimeError("linear_attention_step is not differentiable: call it under no_grad, or linear_attention on one token")
+    if _lib.needs_node(q, k, v, log_decay, state):
+        if torch.jit.is_tracing():
+            raise RuntimeError("linear_attention_step cannot be traced: its update of the state would not be recorded")
+        if (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, log_decay, state))) \
+                or any(forward_ad.unpack_dual(t).tangent is not None for t in (q, k, v, log_decay, state)):
+            raise RuntimeError("linear_attention_step is not differentiable: call it under no_grad, or linear_attention on one token")
     q, k, v = _unit(q), _unit(k), _unit(v)
     with _lib.on_device(v.device):
         lib = _lib.load()
