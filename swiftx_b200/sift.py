@@ -525,8 +525,10 @@ class SiftLM(nn.Module):
         w = self.lm_head.weight
         if not (w.is_cuda and self.lm_head.bias is None and w.dtype in (torch.float32, torch.bfloat16)):
             return self(idx, targets)[1]
+        # both flattened, as forward does: the targets may have any shape of as many tokens
         return self._run(idx, lambda h: linear_cross_entropy(
-            h, w, targets, weight16=_W16.get(id(w)) if _W16 is not None and w.dtype == torch.float32 else None))
+            h.reshape(-1, h.shape[-1]), w, targets.reshape(-1),
+            weight16=_W16.get(id(w)) if _W16 is not None and w.dtype == torch.float32 else None))
 
     def _run(self, idx, head):
         """head(the final norm's output), with the bf16 weight copies of forward."""
