@@ -108,8 +108,13 @@ static LaCut la_cut(int nc, int64_t n) {
 // tokens: 128 segments 28.3 us, 64 25.2, 32 29.3; 8 heads x 1024: uncut 22, segments of 4 chunks 27.3, of 2
 // 21.0, of 1 18.0; x 512: uncut 14.3, cut 18.0).
 //
-// The other kernels have three CTAs on an SM (two with dk > 64 or fp32); the backward runs two walks at
-// once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).  Where its
+// The other kernels have three CTAs on an SM (bf16, two with dk > 64; two of the fp32 backward up to dk 64); the backward
+// runs two walks at once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).
+// The fp32 forward, and the fp32 backward above dk 64, fill an SM with one CTA and take two rounds of segments, of a
+// third of the walk or less: with two segments the two rounds would be as long as one of whole walks, and the
+// states come on top (4096 tokens, heads of 64, forward: 148 heads 734 us whole, 873 as two; 100 heads 699 and 793;
+// 74 heads 697 whole, 476 as four, 505 as two in one round; dk 128, 100 heads, forward and backward: 5.78 ms with the backward
+// whole, 6.29 as two; 40 heads 2.09 as seven, 2.40 as three in one round).  Where the backward's
 // last segment would be less than half of the others, all are made shorter by two chunks (forward and
 // backward, 64 heads x 2048 tokens 194 -> 191 us, x 1664 166 -> 153, 80 x 2100 238 -> 218).
 static LaPlan la_plan(const swx_linattn_args* a) {
@@ -118,10 +123,12 @@ static LaPlan la_plan(const swx_linattn_args* a) {
     q.nc = (int)((a->seqlen + LA_C - 1) / LA_C);
     const int64_t heads = a->batch * a->heads * q.nsl, chunks = (q.nc + 1) / 2;
     q.tc = a->dtype == SWX_DTYPE_BF16 && a->dk <= 64 && (heads > 148 ? chunks >= 4 : q.nc >= 2);
-    const int64_t slots = 148 * (a->dk > 64 || a->dtype == SWX_DTYPE_F32 ? 2 : 3);
+    const bool f32 = a->dtype == SWX_DTYPE_F32;
+    const int64_t parts = 148 * (a->dk > 64 || f32 ? 2 : 3) / heads;
+    auto one_to_an_sm = [parts](bool yes) { return yes && parts == 2 ? 1 : parts; };
     const int64_t n = std::max<int64_t>(1, std::min<int64_t>(148 / heads, 64)), segment = (chunks + n - 1) / n;
-    q.fwd = la_cut(q.nc, !q.tc ? slots / heads : 2 * chunks > 3 * segment + 8 ? n : 1);
-    q.bwd = la_cut(q.nc, slots / heads);
+    q.fwd = la_cut(q.nc, !q.tc ? one_to_an_sm(f32) : 2 * chunks > 3 * segment + 8 ? n : 1);
+    q.bwd = la_cut(q.nc, one_to_an_sm(f32 && a->dk > 64));
     if (q.bwd.nseg > 1 && 2 * (q.nc - (q.bwd.nseg - 1) * q.bwd.segc) < q.bwd.segc) {       // a short last segment
         q.bwd.segc -= 2;
         q.bwd.nseg = (q.nc + q.bwd.segc - 1) / q.bwd.segc;
