@@ -480,13 +480,14 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  * gradient keep fp32 accuracy.  fp32 inputs: about 22-bit products.  Deterministic.
  * Backward outputs are dense: dq, dk_out (batch, seqlen, qk_heads, dk) and dv_out in dtype,
  * dlog_decay fp32, (batch, seqlen, heads), or (heads) with decay_per_head, where log_decay is one
- * value per head and the gradient is summed; dinitial_state optional. */
+ * value per head and the gradient is summed; dinitial_state optional.  A wait of a kernel for its own copies or
+ * products that runs out of tries is recorded for swx_device_wait_status; the call's results are incomplete then. */
 typedef struct swx_linattn_args {
     int64_t batch, seqlen, heads, qk_heads, dk, dv;
     int32_t dtype;                    /* SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
     int32_t decay_per_head;
     float scale;
-    int32_t reserved;
+    int32_t wait_polls;               /* tries of each device-side wait: 0 the default (about a second), below 0 none */
     const void* q; int64_t q_sb, q_sl, q_sh;
     const void* k; int64_t k_sb, k_sl, k_sh;
     const void* v; int64_t v_sb, v_sl, v_sh;

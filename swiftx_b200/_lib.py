@@ -138,7 +138,7 @@ class LinattnArgs(ctypes.Structure):
     """Mirror of ``swx_linattn_args``."""
     _fields_ = [
         ("batch", i64), ("seqlen", i64), ("heads", i64), ("qk_heads", i64), ("dk", i64), ("dv", i64),
-        ("dtype", i32), ("decay_per_head", i32), ("scale", ctypes.c_float), ("reserved", i32),
+        ("dtype", i32), ("decay_per_head", i32), ("scale", ctypes.c_float), ("wait_polls", i32),
         ("q", vp), ("q_sb", i64), ("q_sl", i64), ("q_sh", i64),
         ("k", vp), ("k_sb", i64), ("k_sl", i64), ("k_sh", i64),
         ("v", vp), ("v_sb", i64), ("v_sl", i64), ("v_sh", i64),

@@ -19,6 +19,7 @@ namespace swx {
 constexpr int LA_C = 64;                  // tokens per chunk
 constexpr int LA_DV = 64;                 // columns of v per CTA
 constexpr int LA_THREADS = 128;
+constexpr uint32_t LT_POLLS = 1u << 16;   // tries of the pipelined kernels' waits, up to 20 us each
 // How far the loops over a product's contraction are unrolled: whole loops made the two gradient walks larger than
 // the instruction caches (fp32 133 -> 110 us at 2 x 777 x 6 heads; bf16, shorter, the same either way).
 template <typename T> constexpr int LA_UNROLL = sizeof(T) == 4 ? 1 : 2;
@@ -29,6 +30,7 @@ struct LaDev {
     int b, L, H, Hk, dk, dv, nsl;         // nsl: slices of 64 columns of v
     int nc, nseg, segc;                   // chunks; segments; chunks per segment (even)
     bool tc;                              // the pipelined kernels, where the tensors allow it
+    uint32_t polls;                       // tries of each of their waits
     LaTensor q, k, v, dout;
     const float* g; int64_t g_sb, g_sl, g_sh;
     const int64_t* lengths;

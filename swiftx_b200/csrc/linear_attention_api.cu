@@ -185,6 +185,7 @@ static LaDev la_pack(const swx_linattn_args* a, const LaPlan& q, const LaCut& c)
     LaDev p{};
     const int es = a->dtype == SWX_DTYPE_F32 ? 4 : 2;
     p.b = (int)a->batch; p.L = (int)a->seqlen; p.H = (int)a->heads; p.Hk = (int)a->qk_heads; p.dk = (int)a->dk; p.dv = (int)a->dv;
+    p.polls = a->wait_polls == 0 ? LT_POLLS : (uint32_t)std::max(0, a->wait_polls);
     p.nsl = q.nsl; p.tc = q.tc; p.nc = q.nc; p.nseg = c.nseg; p.segc = c.segc;
     p.q = la_tensor(a->q, a->q_sb, a->q_sl, a->q_sh, a->batch, a->seqlen, a->qk_heads, es);
     p.k = la_tensor(a->k, a->k_sb, a->k_sl, a->k_sh, a->batch, a->seqlen, a->qk_heads, es);

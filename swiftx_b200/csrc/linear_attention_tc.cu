@@ -27,7 +27,6 @@ namespace swx {
 constexpr int LT_C = 128;                     // tokens per chunk
 constexpr int LT_BOX = LT_C * 128;            // bytes of 128 rows of 64 bf16 values
 constexpr int LT_RING = 4;                    // gates: one being made, three in use (A is at most two chunks ahead of B)
-constexpr uint32_t LT_POLLS = 1u << 16;
 
 // Decays of a chunk of 128 tokens, as LaGates.
 struct __align__(16) LtGates {
@@ -90,10 +89,16 @@ __device__ __forceinline__ double lt_gates(LtGates& s, LtG r, int lane) {
     return all;
 }
 
-// A bounded wait that every thread makes; after one that ran out the kernel runs on to its end
-// without further waiting (its barriers are all still met) and the status word says so.
-__device__ __forceinline__ void lt_wait(uint64_t* bar, uint32_t parity, bool& ok) {
-    if (ok && !mbar_wait_suspended(bar, parity, LT_POLLS)) ok = false;
+// A bounded wait that every thread makes.  After one that ran out a warp makes no further ones, and the status word
+// says so.  The working warps run on to their end (on whatever is there: all their addresses are in bounds); the loader
+// issues no more copies and the issuer no more products (lt_going), and both see what they have issued end
+// before the CTA goes (lt_landed): its shared and tensor memory may be another CTA's then.
+__device__ __forceinline__ void lt_wait(uint64_t* bar, uint32_t parity, bool& ok, uint32_t polls) {
+    if (ok && !mbar_wait_suspended(bar, parity, polls)) ok = false;
+}
+__device__ __forceinline__ bool lt_going(bool& ok) { return ok = __all_sync(0xffffffffu, ok); }
+__device__ __forceinline__ void lt_landed(uint64_t* bar, uint32_t parity, bool& ok) {
+    if (!mbar_wait_suspended(bar, parity, LT_POLLS)) ok = false;
 }
 
 // 16-byte part j of row r of a swizzled 64-column tile.
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(32 * LS_WARPS, 1)
 lt_state_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y, int* status) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ LtGates gates[LT_RING];
-    __shared__ __align__(8) uint64_t full[LS_RING], ready[2], done[LS_RING];
+    __shared__ __align__(8) uint64_t full[LS_RING], ready[2], done[LS_RING], idle;      // idle: all products have ended
     __shared__ uint32_t tmem_base;
     uint8_t* tiles = smem_raw + (((smem_u32(smem_raw) + 1023) & ~1023u) - smem_u32(smem_raw));
     uint8_t* planes = tiles + LS_RING * 2 * LT_BOX;
@@ -256,6 +261,7 @@ lt_state_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_x, const 
             mbar_init(&done[i], 1);
         }
         for (int i = 0; i < 2; ++i) mbar_init(&ready[i], LT_A);
+        mbar_init(&idle, 1);
         mbar_fence_init();
     }
     __syncwarp();
@@ -268,12 +274,14 @@ lt_state_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_x, const 
     if (warp == LT_A) {                                          // loader
         double total = 0.;
         LtG g = lt_load_g(p, b, h, chunk(0) * LT_C, n > 0 ? len : 0, lane);
+        int i = 0;
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
+        for (; i < n; ++i) {
             const int u = i % LS_RING;
             const LtG now = g;
             if (i + 1 < n) g = lt_load_g(p, b, h, chunk(i + 1) * LT_C, len, lane);
-            if (i >= LS_RING) lt_wait(&done[u], (i / LS_RING - 1) & 1, ok);
+            if (i >= LS_RING) lt_wait(&done[u], (i / LS_RING - 1) & 1, ok, p.polls);
+            if (!lt_going(ok)) break;
             if (lane == 0) {
                 mbar_expect_tx(&full[u], 2 * LT_BOX);
                 tma_load_4d(tiles + 2 * u * LT_BOX, &map_x, 0, chunk(i) * LT_C, hk, b, &full[u]);
@@ -283,16 +291,19 @@ lt_state_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_x, const 
             total += lt_gates(gates[i % LT_RING], now, lane);
             lt_arrive(&full[u], lane);                           // the gates are there
         }
-        for (int i = max(0, n - LS_RING); i < n; ++i) lt_wait(&full[i % LS_RING], (i / LS_RING) & 1, ok);   // all have landed
+        for (int j = max(0, i - LS_RING); j < i; ++j) lt_landed(&full[j % LS_RING], (j / LS_RING) & 1, ok);
         if (lane == 0 && sl == 0) p.dec[((int64_t)b * p.H + h) * p.nseg + seg] = ex2((float)total);
     } else if (warp == LT_A + 1) {                               // issuer
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
-            lt_wait(&ready[i & 1], (i >> 1) & 1, ok);
+            lt_wait(&ready[i & 1], (i >> 1) & 1, ok, p.polls);
+            if (!lt_going(ok)) break;
             tc_fence_after();
             lt_issue_u<0, LT_C / 16>(tmem + 64 * (i & 1), planes + (i & 1) * 3 * LT_BOX, tiles + (2 * (i % LS_RING) + 1) * LT_BOX);
             mma_commit(&done[i % LS_RING]);
         }
+        mma_commit(&idle);
+        lt_landed(&idle, 0, ok);
     } else {
         const int half = warp / 4, row = 32 * (warp & 3) + lane;
         const uint32_t at = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 32 * half;
@@ -301,7 +312,7 @@ lt_state_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_x, const 
         for (int i = 0; i < n; ++i) {
             const int u = i % LS_RING, rows = min(LT_C, len - chunk(i) * LT_C);
             const LtGates& gt = gates[i % LT_RING];
-            lt_wait(&full[u], (i / LS_RING) & 1, ok);
+            lt_wait(&full[u], (i / LS_RING) & 1, ok, p.polls);
             // U of two chunks ago (its weighted tile's buffer) was waited for in the last step
             const float2 G = gt.G[row];
             lt_weigh(tiles + 2 * u * LT_BOX, planes + (i & 1) * 3 * LT_BOX, row, half, REV ? p.scale * ex2(G.x) : la_decay(gt.Gend, G), row < rows);
@@ -310,14 +321,14 @@ lt_state_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_x, const 
             tc_fence_before();
             lt_arrive(&ready[i & 1], lane);
             if (i > 0) {
-                lt_wait(&done[(i - 1) % LS_RING], ((i - 1) / LS_RING) & 1, ok);
+                lt_wait(&done[(i - 1) % LS_RING], ((i - 1) / LS_RING) & 1, ok, p.polls);
                 tc_fence_after();
                 lt_state_add(S, at + 64 * ((i - 1) & 1), all);
             }
             all = gt.all;
         }
         if (n > 0) {
-            lt_wait(&done[(n - 1) % LS_RING], ((n - 1) / LS_RING) & 1, ok);
+            lt_wait(&done[(n - 1) % LS_RING], ((n - 1) / LS_RING) & 1, ok, p.polls);
             tc_fence_after();
             lt_state_add(S, at + 64 * ((n - 1) & 1), all);
         }
@@ -342,9 +353,9 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
     __shared__ LtGates gates[LT_RING];
     // full: a chunk's tiles have landed.  weighed[half], products[half][parity of the chunk]: of the weighted
     // tile.  shared[parity]: S is there.  scored[parity]: the scores.  masked[parity]: P is there.
-    // mixed[place of the ring]: q S and P v, and with them every product of the chunk.  read: both, by B.
+    // mixed[place of the ring]: q S and P v, and with them every product of the chunk.  read: both, by B.  idle: all products have ended.
     //   A barrier has as many places as a fast warp can be phases ahead of the slowest that waits or arrives.
-    __shared__ __align__(8) uint64_t full[LF_RING], weighed[2], products[2][2], shared[2], scored[2], masked[2], mixed[LF_RING], read;
+    __shared__ __align__(8) uint64_t full[LF_RING], weighed[2], products[2][2], shared[2], scored[2], masked[2], mixed[LF_RING], read, idle;
     __shared__ uint32_t tmem_base;
     uint8_t* tiles = smem_raw + (((smem_u32(smem_raw) + 1023) & ~1023u) - smem_u32(smem_raw));
     uint8_t* planes = tiles + LF_RING * LF_TILES;
@@ -373,6 +384,7 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
             mbar_init(&masked[i], LT_B);
         }
         mbar_init(&read, LT_B);
+        mbar_init(&idle, 1);
         mbar_fence_init();
     }
     __syncwarp();
@@ -386,12 +398,14 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
     bool ok = true;
     if (warp == LT_A + LT_B) {                                   // loader
         LtG g = lt_load_g(p, b, h, first * LT_C, n > 0 ? len : 0, lane);
+        int i = 0;
 #pragma unroll 1
-        for (int i = 0; i < n; ++i) {
+        for (; i < n; ++i) {
             const int u = i % LF_RING, t0 = chunk(i) * LT_C;
             const LtG now = g;
             if (i + 1 < n) g = lt_load_g(p, b, h, t0 + LT_C, len, lane);
-            if (i >= LF_RING) lt_wait(&mixed[u], (i / LF_RING - 1) & 1, ok);
+            if (i >= LF_RING) lt_wait(&mixed[u], (i / LF_RING - 1) & 1, ok, p.polls);
+            if (!lt_going(ok)) break;
             if (lane == 0) {
                 mbar_expect_tx(&full[u], LF_TILES);
                 tma_load_4d(tile(i, 1), &map_k, 0, t0, hk, b, &full[u]);
@@ -402,13 +416,14 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
             lt_gates(gates[i % LT_RING], now, lane);
             lt_arrive(&full[u], lane);                           // the gates are there
         }
-        for (int i = max(0, n - LF_RING); i < n; ++i) lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok);   // all have landed
+        for (int j = max(0, i - LF_RING); j < i; ++j) lt_landed(&full[j % LF_RING], (j / LF_RING) & 1, ok);
     } else if (warp == LT_A + LT_B + 1) {                        // issuer
         constexpr uint32_t id_s = mma_bf16_idesc(LT_C, LT_C, false, false), id_o = mma_bf16_idesc(LT_C, 64, false, true);
         auto mix = [&](int i) {                                  // q S and P v
-            lt_wait(&masked[i & 1], (i >> 1) & 1, ok);
-            lt_wait(&shared[i & 1], (i >> 1) & 1, ok);
-            if (i > 0) lt_wait(&read, (i - 1) & 1, ok);
+            lt_wait(&masked[i & 1], (i >> 1) & 1, ok, p.polls);
+            lt_wait(&shared[i & 1], (i >> 1) & 1, ok, p.polls);
+            if (i > 0) lt_wait(&read, (i - 1) & 1, ok, p.polls);
+            if (!lt_going(ok)) return;
             tc_fence_after();
             const uint64_t qd = operand_desc(tile(i, 0), 16), sd = operand_desc(ss + (i & 1) * 64 * 128, 16), vd = operand_desc(tile(i, 2), 16);
 #pragma unroll
@@ -421,24 +436,29 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
             const uint32_t u = t_u + 64 * (i & 1);
-            lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok);
-            if (i >= 2) lt_wait(&mixed[(i - 2) % LF_RING], ((i - 2) / LF_RING) & 1, ok);      // P of two chunks ago has been read
+            lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok, p.polls);
+            if (i >= 2) lt_wait(&mixed[(i - 2) % LF_RING], ((i - 2) / LF_RING) & 1, ok, p.polls);      // P of two chunks ago has been read
+            if (!lt_going(ok)) break;
             tc_fence_after();
             const uint64_t qd = operand_desc(tile(i, 0), 16), kd = operand_desc(tile(i, 1), 16);
 #pragma unroll
             for (int k = 0; k < 4; ++k) mma_bf16_cta(t_sc + 128 * (i & 1), qd + k * 2, kd + k * 2, id_s, k > 0);
             mma_commit(&scored[i & 1]);
             if (i > 0) mix(i - 1);        // (and every warp of A has read U of two chunks ago)
-            lt_wait(&weighed[0], i & 1, ok);
+            lt_wait(&weighed[0], i & 1, ok, p.polls);
+            if (!lt_going(ok)) break;
             tc_fence_after();
             lt_issue_u<0, 4>(u, planes, tile(i, 2));
             mma_commit(&products[0][i & 1]);
-            lt_wait(&weighed[1], i & 1, ok);
+            lt_wait(&weighed[1], i & 1, ok, p.polls);
+            if (!lt_going(ok)) break;
             tc_fence_after();
             lt_issue_u<4, 8>(u, planes, tile(i, 2));
             mma_commit(&products[1][i & 1]);
         }
         if (n > 0) mix(n - 1);
+        mma_commit(&idle);
+        lt_landed(&idle, 0, ok);
     } else if (warp < LT_A) {                                    // A
         const int srow = lt_state_row(warp, lane);
         const uint32_t at = t_u + lanes + 32 * half;
@@ -447,22 +467,22 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
             const int rows = min(LT_C, len - chunk(i) * LT_C);
-            lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok);
+            lt_wait(&full[i % LF_RING], (i / LF_RING) & 1, ok, p.polls);
             // the last chunk's products with this half of the weighted tile
-            if (i > 0) lt_wait(&products[token_half][(i - 1) & 1], ((i - 1) >> 1) & 1, ok);
+            if (i > 0) lt_wait(&products[token_half][(i - 1) & 1], ((i - 1) >> 1) & 1, ok, p.polls);
             const LtGates& gt = gates[i % LT_RING];
             lt_weigh(tile(i, 1), planes, row, half, la_decay(gt.Gend, gt.G[row]), row < rows);
             lt_clear_rows(tile(i, 2), row, half, rows);
             fence_proxy_async_smem();
             lt_arrive(&weighed[token_half], lane);
             if (i > 0) {
-                lt_wait(&products[token_half ^ 1][(i - 1) & 1], ((i - 1) >> 1) & 1, ok);
+                lt_wait(&products[token_half ^ 1][(i - 1) & 1], ((i - 1) >> 1) & 1, ok, p.polls);
                 tc_fence_after();
                 lt_state_add(S, at + 64 * ((i - 1) & 1), all);
             }
             all = gt.all;
             lt_state_save(S, p, bh, 2 * chunk(i), srow, c0, half);
-            if (i >= 2) lt_wait(&mixed[(i - 2) % LF_RING], ((i - 2) / LF_RING) & 1, ok);      // q S of two chunks ago has read this place
+            if (i >= 2) lt_wait(&mixed[(i - 2) % LF_RING], ((i - 2) / LF_RING) & 1, ok, p.polls);      // q S of two chunks ago has read this place
             lt_state_share(S, ss + (i & 1) * 64 * 128, srow, half);
             fence_proxy_async_smem();
             tc_fence_before();
@@ -471,7 +491,7 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
         const bool last = p.s_last && seg == p.nseg - 1;
         if (last || (p.save && live < end)) {
             if (n > 0) {
-                for (int x = 0; x < 2; ++x) lt_wait(&products[x][(n - 1) & 1], ((n - 1) >> 1) & 1, ok);
+                for (int x = 0; x < 2; ++x) lt_wait(&products[x][(n - 1) & 1], ((n - 1) >> 1) & 1, ok, p.polls);
                 tc_fence_after();
                 lt_state_add(S, at + 64 * ((n - 1) & 1), all);
             }
@@ -482,7 +502,7 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
         __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
         auto finish = [&](int i, float Gx) {
             const int t0 = chunk(i) * LT_C;
-            lt_wait(&mixed[i % LF_RING], (i / LF_RING) & 1, ok);
+            lt_wait(&mixed[i % LF_RING], (i / LF_RING) & 1, ok, p.polls);
             tc_fence_after();
             float o[32], pv[32];
             tmem_ld32(t_qs + lanes + 32 * half, o);
@@ -518,7 +538,7 @@ lt_fwd_kernel(const LaDev p, const __grid_constant__ CUtensorMap map_q, const __
 #pragma unroll 1
         for (int i = 0; i < n; ++i) {
             const int rows = min(LT_C, len - chunk(i) * LT_C);
-            lt_wait(&scored[i & 1], (i >> 1) & 1, ok);
+            lt_wait(&scored[i & 1], (i >> 1) & 1, ok, p.polls);
             tc_fence_after();
             const LtGates& gt = gates[i % LT_RING];
             const float2 G = gt.G[row];
