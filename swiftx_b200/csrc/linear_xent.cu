@@ -44,6 +44,11 @@ constexpr int XE_SMEM = 1024 + XE_STAGES * XE_STAGE + XE_EPI_WARPS * XE_OUT;
 // of each addition off (toward zero), an error that grows with the number of additions (dx
 // 4.9e-6 off after 5001 terms in one sum); sums of 256 terms are added up in fp32 instead.
 constexpr int XE_KSUB = 4;
+// The same for the logits, over the width of the operands, 512 terms at a time: up to that nothing is summed outside
+// (3.9e-7 off at operands of one sign, a library's fp32 products 4.8e-7); in one sum 1024 terms were 1.3e-6 off, 4096 8.7e-6
+// and 16384 6.6e-5, 4e-7 each now.  2048 x 8192 x 1024 forward 148 -> 163 us; 256 terms at a time 176, and 384 instead of 326 us
+// at 4096 x 20000 x 512.
+constexpr int XE_KSUB_LOGITS = 8;
 constexpr uint32_t XE_POLLS = 1u << 24;       // about a second
 
 enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW };
@@ -52,7 +57,7 @@ struct XentGemm {
     int M, N;                                 // rows and columns of the result
     int mt, nt, group;                        // tiles; row tiles walked together (XE_LSE, XE_PROB)
     int nk, npair;                            // ring stages of the contraction; pairs of pieces
-    int ksub;                                 // stages summed in tensor memory before the sum moves on (XE_DX, XE_DW)
+    int ksub;                                 // stages summed in tensor memory before the sum moves on
     int ka0, kb0;                             // first contraction index of A and of B
     int a0, b0;                               // first row of A and of B (M / N coordinate)
     int* status;
@@ -210,7 +215,7 @@ __device__ __forceinline__ void xent_emit(const XentGemm& p, float (&v)[32], int
     }
 }
 
-// SUMS: the steps of a tile come in several accumulators (fp32 operands); their sum stays in registers until the tile (or
+// SUMS: the steps of a tile come in several accumulators (fp32 operands: the gradients, and logits of wide operands); their sum stays in registers until the tile (or
 // this pair's part of it) is complete: through memory each time, 1003 tokens x 10007 x 200 took 232 us, 219 with the registers.
 template <int EPI, bool A_MN, bool B_MN, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1)
@@ -349,32 +354,9 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             if (!mbar_wait_cluster(&acc_full[a], aph, XE_POLLS)) { ok = false; break; }
             tc_fence_after();
             const uint32_t at = tmem + ((uint32_t)(sub * 32) << 16) + a * XE_TILE + half * 128;
-            if constexpr (SUMS) {
-#pragma unroll
-                for (int c = 0; c < 8; ++c) {
-                    float v[16];
-                    tmem_ld16(at + c * 16, v);
-                    tmem_ld_wait();
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) tot[c / 2][c % 2 * 16 + j] = r.fresh ? v[j] : tot[c / 2][c % 2 * 16 + j] + v[j];
-                }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[a], 0));
-                if ((a ^= 1) == 0) aph ^= 1;
-                if (live && (r.k1 == p.nk || r.cur >= r.end)) {          // the tile's, or this pair's part of it
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        if (c0 + 32 * c < p.N) xent_emit(p, tot[c], r.part, row, c0 + 32 * c, p.first, last, factor);
-                }
-                continue;
-            }
+            // 32 columns of the row, from 32 c on
             float m = -INFINITY, sum = 0.f;
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                float v[32];
-                tmem_ld32(at + c * 32, v);
-                tmem_ld_wait();
+            auto columns = [&](int c, float (&v)[32]) {
                 const int cc = c0 + c * 32;                 // first of these 32 columns
                 const int64_t yc = y - cc;
                 if (EPI == XE_LSE) {
@@ -445,6 +427,32 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                 } else if (live && cc < p.N) {
                     xent_emit(p, v, r.part, row, cc, p.first, last, factor);
                 }
+            };
+            if constexpr (SUMS) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float v[16];
+                    tmem_ld16(at + c * 16, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) tot[c / 2][c % 2 * 16 + j] = r.fresh ? v[j] : tot[c / 2][c % 2 * 16 + j] + v[j];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[a], 0));
+                if ((a ^= 1) == 0) aph ^= 1;
+                if (r.k1 != p.nk && r.cur < r.end) continue;             // more of the tile (or of this pair's part of it) to come
+#pragma unroll
+                for (int c = 0; c < 4; ++c) columns(c, tot[c]);
+                if (EPI == XE_LSE && live) p.part[(int64_t)(2 * rc.y + half) * p.M + row] = make_float2(m, sum);
+                continue;
+            }
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                float v[32];
+                tmem_ld32(at + c * 32, v);
+                tmem_ld_wait();
+                columns(c, v);
             }
             if (EPI == XE_LSE && live) p.part[(int64_t)(2 * rc.y + half) * p.M + row] = make_float2(m, sum);
             tc_fence_before();
@@ -737,6 +745,9 @@ static XentPlan xent_plan(const swx_xent_args* a) {
     return q;
 }
 
+// Stages of the logits' contraction summed in tensor memory at a time: all of them for bf16 operands.
+static int logits_ksub(const XentPlan& q, int nk) { return q.planes == 3 ? std::min(nk, XE_KSUB_LOGITS) : nk; }
+
 // A (rows, inner) bf16 matrix with `planes` pieces as a 3-D tensor map, 128-byte swizzled.
 static bool encode_operand(CUtensorMap* m, const void* base, int64_t inner, int64_t rows, int64_t planes, int64_t row,
                            int64_t plane, uint32_t box_inner, uint32_t box_rows, bool swizzle = true) {
@@ -842,13 +853,16 @@ int swx_xent_fwd(const swx_xent_args* a, void* stream) {
     if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
     XentGemm g{};
     g.M = (int)a->tokens; g.N = (int)a->vocab; g.mt = (int)q.mt; g.nt = (int)q.nt; g.group = 32;
-    g.nk = g.ksub = (int)((a->dim + XE_K - 1) / XE_K); g.npair = q.planes == 3 ? 6 : 1;
+    g.nk = (int)((a->dim + XE_K - 1) / XE_K); g.npair = q.planes == 3 ? 6 : 1;
+    g.ksub = logits_ksub(q, g.nk);
     g.status = status;
     g.target = a->targets; g.ignore = a->ignore_index;
     g.part = reinterpret_cast<float2*>(ws + q.off_part);
     g.hit = reinterpret_cast<float*>(ws + q.off_hit);
     g.counter = reinterpret_cast<int*>(ws + q.off_cnt);
-    if (launch_gemm<XE_LSE, false, false>(g, mx, mw, mx, XE_PAIRS, st) != cudaSuccess) return SWX_ERR_CUDA;
+    if ((g.ksub < g.nk ? launch_gemm<XE_LSE, false, false, true>(g, mx, mw, mx, XE_PAIRS, st)
+                       : launch_gemm<XE_LSE, false, false>(g, mx, mw, mx, XE_PAIRS, st)) != cudaSuccess)
+        return SWX_ERR_CUDA;
     XentJoin j{};
     j.T = a->tokens; j.V = a->vocab; j.np = (int)(2 * q.nt); j.part = g.part; j.hit = g.hit; j.target = a->targets;
     j.ignore = a->ignore_index; j.row_max = a->row_max; j.row_rsum = a->row_rsum;
@@ -895,10 +909,13 @@ int swx_xent_bwd(const swx_xent_args* a, void* stream) {
         XentGemm g{};
         g.status = status; g.npair = npair; g.planes = q.planes;
         g.M = (int)T; g.N = (int)cw; g.mt = (int)q.mt; g.nt = (int)((cw + XE_TILE - 1) / XE_TILE); g.group = 32;
-        g.nk = g.ksub = (int)((d + XE_K - 1) / XE_K); g.b0 = (int)c0;
+        g.nk = (int)((d + XE_K - 1) / XE_K); g.b0 = (int)c0;
+        g.ksub = logits_ksub(q, g.nk);
         g.target = a->targets; g.ignore = a->ignore_index; g.col0 = (int)c0; g.vocab = V;
         g.row_max = a->row_max; g.row_rsum = a->row_rsum; g.dloss = a->dloss; g.reduction = a->reduction;
-        if (launch_gemm<XE_PROB, false, false>(g, x_k, w_k, p_st, XE_PAIRS, st) != cudaSuccess) return SWX_ERR_CUDA;
+        if ((g.ksub < g.nk ? launch_gemm<XE_PROB, false, false, true>(g, x_k, w_k, p_st, XE_PAIRS, st)
+                           : launch_gemm<XE_PROB, false, false>(g, x_k, w_k, p_st, XE_PAIRS, st)) != cudaSuccess)
+            return SWX_ERR_CUDA;
         if (a->dx) {
             XentGemm h{};
             h.status = status; h.npair = npair;
