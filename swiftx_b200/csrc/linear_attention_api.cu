@@ -100,13 +100,14 @@ static LaCut la_cut(int nc, int64_t n) {
 // starts cost one more reading of k and v, and two launches.
 //
 // The pipelined kernels (linear_attention_tc.cu, one CTA per SM, chunks of 128 tokens) take bf16 heads of up to 64
-// from 65 tokens on, and from 4 chunks on where the heads alone take several rounds.  us, theirs / the other
-// kernels', forward, heads of 64: 8 heads x 64 tokens 8.2 / 6.5, x 100 8.3 / 9.3, x 512 14.3 / 17.0; 128 heads x 256
-// 11.9 / 24.0, x 4096 97 / 176; 512 heads x 128 30 / 21, x 256 40 / 35, x 512 68 / 74, x 4096 373 / 549.
+// from 65 tokens on, and from 129 on where the heads alone take several rounds.  us, theirs / the other
+// kernels', forward, heads of 64: 8 heads x 64 tokens 8.5 / 8.5, x 100 8.6 / 10.6, x 512 14.5 / 18.6; 128 heads x 256
+// 12.7 / 26.8, x 4096 83 / 187; 149 heads x 128 14.8 / 12.8, x 256 18.6 / 31.1, x 384 23.1 / 44.6; 512 heads x 128
+// 30.9 / 22.7, x 256 39.1 / 40.3, x 384 49 / 62, x 4096 310 / 586.
 // An uncut walk takes them 6 us and 2 for each chunk; a cut one 14 and 3 for each chunk of a segment, with the states
 // and their chain; more than 64 segments make the chain longer than what they save (1 head x 16384
-// tokens: 128 segments 28.3 us, 64 25.2, 32 29.3; 8 heads x 1024: uncut 22, segments of 4 chunks 27.3, of 2
-// 21.0, of 1 18.0; x 512: uncut 14.3, cut 18.0).
+// tokens: 128 segments 28.7 us, 64 26.6, 32 30.3; 8 heads x 1024: uncut 24.8, segments of 4 chunks 27.4, of 2
+// 22.5, of 1 18.6; x 512: uncut 16.6, cut 18.6; 64 heads x 2048: uncut 43.8, cut 47.3).
 //
 // The other kernels have three CTAs on an SM (bf16, two with dk > 64; two of the fp32 backward up to dk 64); the backward
 // runs two walks at once, in two rounds rather than one (8 x 2048 x 8 heads of 64: 6 segments 115 us, 3 128, 2 141).
@@ -122,7 +123,7 @@ static LaPlan la_plan(const swx_linattn_args* a) {
     q.nsl = (int)((a->dv + LA_DV - 1) / LA_DV);
     q.nc = (int)((a->seqlen + LA_C - 1) / LA_C);
     const int64_t heads = a->batch * a->heads * q.nsl, chunks = (q.nc + 1) / 2;
-    q.tc = a->dtype == SWX_DTYPE_BF16 && a->dk <= 64 && (heads > 148 ? chunks >= 4 : q.nc >= 2);
+    q.tc = a->dtype == SWX_DTYPE_BF16 && a->dk <= 64 && q.nc >= (heads > 148 ? 3 : 2);
     const bool f32 = a->dtype == SWX_DTYPE_F32;
     const int64_t parts = 148 * (a->dk > 64 || f32 ? 2 : 3) / heads;
     auto one_to_an_sm = [parts](bool yes) { return yes && parts == 2 ? 1 : parts; };

@@ -163,7 +163,8 @@ def test_decay_gradient_differences_across_segments(dtype, decay):
     assert abs(float((got * d).sum()) - want) <= 4 * 2.0 ** -20 * float(bound.norm()) + 2.0 ** -18 * abs(want) + 1e-3
 
 
-@pytest.mark.parametrize("b,L,H,Hk,dk,dv", [(2, 1100, 2, 2, 64, 64), (1, 700, 4, 1, 128, 96), (40, 300, 4, 4, 32, 64)])
+@pytest.mark.parametrize("b,L,H,Hk,dk,dv", [(2, 1100, 2, 2, 64, 64), (1, 700, 4, 1, 128, 96), (40, 300, 4, 4, 32, 64), (38, 129, 4, 2, 64, 40),
+                                             (19, 250, 8, 8, 48, 64)])
 def test_bf16_results_carry_two_roundings(b, L, H, Hk, dk, dv):
     """A result's terms have one factor rounded to bf16 (a score, or the state that is read out), and the result is rounded.
     A rounding of a value of random mantissa is off by 2^-8 / sqrt(3) sqrt(3 / (8 ln 2)) = 1.66e-3 of it in the mean

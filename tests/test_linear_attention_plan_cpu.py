@@ -24,3 +24,9 @@ def test_fp32_walks_are_not_halved(heads):
 def test_fp32_walks_of_other_counts(heads, segments):
     assert _plan(heads, 64, 0) == (segments > 1, segments)
     assert _plan(heads, 128, 0) == (segments > 1, segments)
+
+
+@pytest.mark.parametrize("heads,L", [(149, 129), (149, 256), (200, 384), (222, 500)])
+def test_pipelined_kernels_take_many_heads_uncut(heads, L):
+    """bf16 heads of up to 64 in several rounds: from 129 tokens on the pipelined kernels, which walk them whole."""
+    assert _plan(heads, 64, 1, L)[0] is False
