@@ -420,8 +420,9 @@ int swx_embedding_bwd(const swx_embedding_args* args, void* stream);
  *             ignore_index;  reduced by `reduction` (the mean over the tokens that count)
  * x: (tokens, dim) with row stride x_sr, weight: (vocab, dim) with row stride w_sr, both in
  * dtype (fp32 or bf16), unit element stride; targets: (tokens,) int64.  Products are summed
- * in fp32 (fp32 operands as three bf16 pieces, about 2^-23 relative), the softmax
- * statistics are fp32.  A target outside [0, vocab) that is not ignore_index makes its loss,
+ * in fp32 in the tensor cores, whose additions cut up to 2^-23 of a sum off (fp32 operands: three bf16 pieces, about
+ * 2^-23 relative, and at most 512 terms in one such sum); the softmax statistics are fp32; bf16 operands: the
+ * logits' gradient is rounded to bf16 once for its products.  A target outside [0, vocab) that is not ignore_index makes its loss,
  * and the gradients that it enters, NaN.  Values of x in ignored rows have to be finite
  * (their products with a zero coefficient enter dweight).
  * Forward writes loss (tokens values for SWX_XENT_NONE, else one), count (one value, the
@@ -476,8 +477,11 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  * The sequence is walked in chunks of 64 or 128 tokens on the tensor cores, cut into segments that are
  * walked in parallel where there are few rows and heads.  The forward leaves the states at the start of the
  * backward's swx_linattn_segments(args) segments in seg_states, fp32 (batch, heads, segments, dk,
- * dv), when it is given; the backward needs them where there are 2 segments or more.  bf16 inputs: scores are rounded to bf16 once; states and the decay's
- * gradient keep fp32 accuracy.  fp32 inputs: about 22-bit products.  Deterministic.
+ * dv), when it is given; the backward needs them where there are 2 segments or more.  Carried
+ * states and the decay's gradient keep fp32 accuracy.  bf16 inputs: the scores, and the state where it is read out (its
+ * gradient, for v's), are rounded to bf16 once for their products.  fp32 inputs: about 22-bit products.  Deterministic.
+ * Where heads share q and k, or with dv above 64, the backward's workspace holds two fp32 (batch, seqlen,
+ * heads * ceil(dv / 64), dk) buffers, the heads' parts of dq and dk.
  * Backward outputs are dense: dq, dk_out (batch, seqlen, qk_heads, dk) and dv_out in dtype,
  * dlog_decay fp32, (batch, seqlen, heads), or (heads) with decay_per_head, where log_decay is one
  * value per head and the gradient is summed; dinitial_state optional.  A wait of a kernel for its own copies or

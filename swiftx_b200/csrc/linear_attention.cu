@@ -86,10 +86,12 @@ __global__ void __launch_bounds__(256) la_chain_kernel(const LaDev p, bool rev) 
 
 // ------------------------------------------------------------------ forward
 // Warp = 16 tokens of the chunk (and a quarter of the state).  Per chunk: the state's part of
-// the output, exp(G_t) S^T q; the decayed scores of the 16 tokens with the tokens up to them
-// (rounded to the inputs' type once, as the second product's operand); their product with v; then the
-// state's update.  Tiles arrive by cp.async one chunk ahead.  Bound by the latency of its own steps, three warps to
-// an SM quarter (two at dk 128): 16 x 512 x 16 heads, dk 128, dv 64, bf16 53 us; 2 x 777 x 6 heads, 40 and 56, fp32 47 us.
+// the output, exp(G_t) S^T q; the decayed scores of the 16 tokens with the tokens up to them; their product with v; then the
+// state's update.  The scores, and the state where it is read out, are rounded to the inputs' type once as their products'
+// operands: each term of a bf16 output has one factor rounded, and so a size of error like the output's own
+// rounding (2.35e-3 together, 1.66e-3 by itself), where three pieces would be three products for one.  The state that
+// is carried is fp32.  Tiles arrive by cp.async one chunk ahead.  Bound by the latency of its own steps, three warps to
+// an SM quarter (two at dk 128): 16 x 512 x 16 heads, dk 128, dv 64, bf16 55 us; 2 x 777 x 6 heads, 40 and 56, fp32 47 us.
 template <typename T, int DK> struct LaFwd {
     using Sh = LaShape<T, DK>;
     static constexpr int SMEM = (int)sizeof(T) * (4 * Sh::QK + 2 * Sh::V + Sh::S);

@@ -11,7 +11,8 @@
 // dg_t = dg_{t+1} + q_t . dq_t - k_t . dk_t, from <S, D> at the segment's end.  The dot
 // products are taken from unrounded sums: sum_s A_ts (q_t . k_s) from the two score tiles, and the
 // states' parts with the state kept to 24 bits (three bf16 pieces), so that dg, fp32, has fp32
-// accuracy although dq and dk are rounded to the inputs' type.
+// accuracy although dq and dk are rounded to the inputs' type.  A and P are rounded to the inputs' type once as the
+// operands of their products with k, q and dout, and D for dv: one rounded factor in each term.
 #include "linear_attention.cuh"
 #include "launch_util.cuh"
 

@@ -7,15 +7,18 @@
 //   loader    the tiles of q, k, v by TMA into a ring of three chunks, and the chunk's decays
 //   issuer    all products
 //   8 warps A k weighted by exp(G_end - G_s), as three bf16 pieces (24 bits), in the tile's own
-//             (swizzled) layout; U = weighted k^T v; S = exp(G_end) S + U in fp32 registers, shared in bf16
+//             (swizzled) layout; U = weighted k^T v; S = exp(G_end) S + U in fp32 registers, shared in bf16 for
+//             q S alone (one factor of each term rounded, as with P; shared memory has no room for more pieces)
 //   8 warps B P = masked, decayed scores (bf16), written over the scores in tensor memory, where the
 //             product with v reads them; o = scale exp(G_t) q S + P v, to memory
 // The weighted tile has one buffer in two halves of 64 tokens: one half is made while the other's
 // products run.  The scores and U have two places each in tensor memory.
 // Warp w of a role works on rows 32 (w % 4) .. and, of their columns, on half w / 4.
-// What bounds it now is the chain through a chunk's roles rather than a pipe: 2.1 us a chunk on an idle GPU, 2.8 with
-// 128 CTAs (4 x 8192 x 32 heads of 64: 200 us, products in 29 % of the cycles, a quarter issues in 41 %, shared memory 37 %,
-// DRAM 2.6 TB/s); 4 x 65536 x 32 heads 1.32 to 1.52 ms, 0.66 at the copy rate; 8 x 1000 x 16 heads with dv 128, padded, 41 us.
+// What bounds it now is the chain through a chunk's roles rather than a pipe: 2.2 us a chunk, on an idle GPU and with
+// 128 CTAs (4 x 8192 x 32 heads of 64: 154 us, products in 33 % of the cycles, a quarter issues in 48 %, shared memory 49 %,
+// DRAM 3.5 TB/s); 4 x 65536 x 32 heads 1.15 ms, 0.66 at the copy rate; 8 x 1000 x 16 heads with dv 128, padded, 37 us.
+// The loader's and the issuer's warps vote in each chunk whether to go on, which also keeps them converged: without
+// the vote 200 us, 1.42 ms and 43 us.
 // Separate rings for q, k and v and a second issuing warp were 20 to 30 % slower.
 #include "linear_attention.cuh"
 #include "launch_util.cuh"

@@ -134,12 +134,19 @@ def linear_attention(q, k, v, log_decay, initial_state=None, scale=1.0, lengths=
     and a unit one along the last dimension (a copy otherwise); H a multiple of Hk: head h reads
     q and k of head h // (H // Hk).  log_decay fp32, (b, L, H), or (H,) for fixed decays; 0 keeps
     the state, -inf resets it.  initial_state fp32 (b, H, dk, dv).  lengths, an int64 (b,) tensor:
-    row i has lengths[i] tokens (clamped to 0..L); what lies behind them is not read, gives zeros in
-    out and in the gradients, and leaves the state; up to there q, k and v have to be finite (an infinity or
-    NaN at one token can reach the outputs of the chunk's earlier tokens).  Returns out (b, L, H, dv), and with return_state the
-    fp32 state after the last token.  Differentiable in q, k, v, log_decay and initial_state
-    (dual numbers of forward mode are refused, torch.jit.trace records a Python operator); deterministic.  bf16 inputs: the score tiles are rounded to bf16 once, states and log_decay's gradient
-    keep fp32 accuracy."""
+    row i has lengths[i] tokens (clamped to 0..L); what lies behind them is not used (it may be NaN), gives
+    zeros in out and in the gradients, and leaves the state; up to there q, k and v have to be finite (an
+    infinity or NaN at one token can reach the outputs of the chunk's earlier tokens).  Returns out (b, L, H, dv),
+    and with return_state the fp32 state after the last token.  Differentiable in q, k, v, log_decay and
+    initial_state (dual numbers of forward mode are refused, torch.jit.trace records a Python operator);
+    deterministic.
+
+    Carried states and log_decay's gradient have fp32 accuracy.  bf16 inputs: the score tiles, and the state where
+    it is read out (its gradient, for v's), are rounded to bf16 once for their products, so that a result carries two
+    roundings, a term's and its own (2.35e-3 in the mean square, 1.66e-3 with its own alone).  fp32 inputs: products
+    of two tf32 pieces, about 22 bits (5e-7 off where fp32 products are 2e-7).
+
+    Gradients where heads share q and k, or with dv above 64, take two fp32 buffers of (b, L, H ceil(dv / 64), dk)."""
     _check("linear_attention", q, k, v, log_decay, initial_state, 2)
     if lengths is not None:
         if lengths.dtype != torch.int64 or tuple(lengths.shape) != (v.shape[0],) or lengths.device != v.device:
