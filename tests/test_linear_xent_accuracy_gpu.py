@@ -33,7 +33,8 @@ def test_fp32_logits_of_one_sign(T, V, d):
     assert bool(((got - want).abs() <= bound).all()), float(((got - want).abs() / bound).max())
 
 
-@pytest.mark.parametrize("T,V,d,reduction", [(130, 700, 1030, "mean"), (300, 300, 257, "none"), (70, 2100, 512, "sum"), (257, 90, 2049, "none")])
+@pytest.mark.parametrize("T,V,d,reduction", [(130, 700, 1030, "mean"), (300, 300, 257, "none"), (70, 2100, 512, "sum"), (257, 90, 2049, "none"),
+                                             (17900, 4200, 520, "mean")])        # two pieces of the vocabulary
 def test_fp32_gradients_of_wide_operands(T, V, d, reduction):
     """A dlogit is off by its logit's error, e as above of |x_t| . |W_v|, with the statistics' 2^-20; dx and dW are sums
     of products of those, 256 terms at a time: less than (40 + n / 512) 2^-23 of the sum of magnitudes."""
