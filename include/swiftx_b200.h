@@ -462,6 +462,101 @@ int64_t swx_xent_bwd_workspace_bytes(const swx_xent_args* args);
 int swx_xent_fwd(const swx_xent_args* args, void* stream);
 int swx_xent_bwd(const swx_xent_args* args, void* stream);
 
+/* Log probabilities of given tokens under a linear head, with the entropy and the top
+ * alternatives, without keeping the (tokens, vocab) logits (the head product followed by
+ * log_softmax, gather and topk; models/sift_model.py:107 makes the logits):
+ *   z[t, v] = x[t, :] . weight[v, :],  l = z / temperature - log(sum_v exp(z / temperature))
+ *   log_probs[t] = l[t, targets[t]],  entropy[t] = -sum_v exp(l) l
+ *   top_ids[t, :], top_log_probs[t, :]: the top_k largest z of the row in falling order (the
+ *   lowest word first among equals) and their l; top_k <= SWX_MAX_TOP, 0: none
+ * Operands as for swx_xent_args.  A target equal to ignore_index: zeros, and -1 for each top_ids; one
+ * outside [0, vocab): its log probability, and the gradients that it enters, NaN.  The
+ * statistics are fp32; the alternatives are ordered by products in fp64 of the operands, so that
+ * neither their order nor their ties depend on the rounding of sums.
+ * Forward writes row_max, row_sum (tokens values, both or neither) for the backward.
+ * Backward: d_log_probs, d_entropy (tokens values; either may be NULL: zero), entropy as the forward
+ * wrote it (needed with d_entropy) -> dx and dweight as in swx_xent_args (bf16 operands:
+ * the logits' gradient is rounded to bf16 once for its products).  The alternatives carry no
+ * gradient.  Deterministic.  The workspace starts on 16 bytes. */
+#define SWX_MAX_TOP 128
+typedef struct swx_logprob_args {
+    int64_t tokens, vocab, dim;
+    int32_t dtype;                    /* x, weight, dx: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t dw_dtype;                 /* dweight: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t top_k;
+    float temperature;                /* above 0 */
+    int64_t ignore_index;
+    const void* x; int64_t x_sr;      /* swx_token_logprob: the logits (tokens, vocab) */
+    const void* weight; int64_t w_sr; /* not read by swx_token_logprob */
+    const int64_t* targets;           /* swx_token_logprob: optional */
+    float* log_probs;
+    float* entropy;
+    float* top_log_probs;
+    int64_t* top_ids;
+    float* row_max;
+    float* row_sum;
+    const float* d_log_probs;         /* backward */
+    const float* d_entropy;
+    void* dx;
+    void* dweight;
+    void* workspace; int64_t workspace_bytes;
+} swx_logprob_args;
+
+int64_t swx_logprob_args_size(void);
+/* Scratch bytes of the two calls for these sizes, types, strides and x / weight addresses;
+ * a negated status code for arguments that the calls refuse. */
+int64_t swx_logprob_fwd_workspace_bytes(const swx_logprob_args* args);
+int64_t swx_logprob_bwd_workspace_bytes(const swx_logprob_args* args);
+int swx_logprob_fwd(const swx_logprob_args* args, void* stream);
+int swx_logprob_bwd(const swx_logprob_args* args, void* stream);
+/* The same from logits: x is (tokens, vocab) with any row stride, fp32 or bf16; no workspace, no
+ * gradient.  Logits may be -inf (words that are not allowed): probability 0.  A row with a NaN or
+ * +inf, or with nothing but -inf, has NaN values; its ids are in order all the same (-inf last,
+ * a NaN by its sign first or last). */
+int swx_token_logprob(const swx_logprob_args* args, void* stream);
+
+/* Distillation of a linear head from a teacher's top logits, without keeping the student's (tokens, vocab)
+ * logits.  With l the student's log probabilities at `temperature` (as above) and q a row's
+ * softmax of teacher_logits / temperature over its used entries:
+ *   loss[t] = temperature^2 sum_j q_j (log q_j - l[t, teacher_ids[t, j]])
+ * reduced by `reduction` (the mean over the rows that count).  An entry with an id below 0 or a
+ * logit of -inf is not used; a row without used entries does not count (0, no gradient).  An
+ * id of vocab or more, or a NaN or +inf logit, in a used entry makes its row's loss, and the gradients that it
+ * enters, NaN.  The same id may stand in several entries of a row (their q add up).
+ * teacher_ids (tokens, entries) int64, teacher_logits (tokens, entries) in teacher_dtype (fp32 or
+ * bf16), row strides ids_sr and tl_sr; 1 <= entries <= SWX_MAX_TOP.  Operands, loss, count and gradients as
+ * in swx_xent_args.  Forward writes row_max, row_sum (tokens values; row_sum -1 for a row
+ * that does not count) and entry_logits (tokens, entries; the student's logits of the used entries) for the backward.
+ * Deterministic.  The workspace starts on 16 bytes. */
+typedef struct swx_distill_args {
+    int64_t tokens, vocab, dim, entries;
+    int32_t dtype;                    /* x, weight, dx: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t dw_dtype;                 /* dweight: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
+    int32_t reduction;                /* SWX_XENT_* */
+    int32_t teacher_dtype;
+    float temperature;                /* above 0 */
+    int32_t reserved;
+    const void* x; int64_t x_sr;
+    const void* weight; int64_t w_sr;
+    const int64_t* teacher_ids; int64_t ids_sr;
+    const void* teacher_logits; int64_t tl_sr;
+    float* loss;
+    float* count;
+    float* row_max;
+    float* row_sum;
+    float* entry_logits;
+    const float* dloss;               /* backward */
+    void* dx;
+    void* dweight;
+    void* workspace; int64_t workspace_bytes;
+} swx_distill_args;
+
+int64_t swx_distill_args_size(void);
+int64_t swx_distill_fwd_workspace_bytes(const swx_distill_args* args);
+int64_t swx_distill_bwd_workspace_bytes(const swx_distill_args* args);
+int swx_distill_fwd(const swx_distill_args* args, void* stream);
+int swx_distill_bwd(const swx_distill_args* args, void* stream);
+
 /* Linear attention with a decay for each head: a recurrence with a (dk x dv) state per head,
  * the matrix-state counterpart of the selective scan (models/selective_scan.py:34 keeps a
  * vector of dstate values per channel; it has no reference counterpart of its own):

@@ -134,6 +134,33 @@ class XentArgs(ctypes.Structure):
     ]
 
 
+SWX_MAX_TOP = 128
+
+
+class LogprobArgs(ctypes.Structure):
+    """Mirror of ``swx_logprob_args``."""
+    _fields_ = [
+        ("tokens", i64), ("vocab", i64), ("dim", i64),
+        ("dtype", i32), ("dw_dtype", i32), ("top_k", i32), ("temperature", ctypes.c_float), ("ignore_index", i64),
+        ("x", vp), ("x_sr", i64), ("weight", vp), ("w_sr", i64), ("targets", vp),
+        ("log_probs", vp), ("entropy", vp), ("top_log_probs", vp), ("top_ids", vp), ("row_max", vp), ("row_sum", vp),
+        ("d_log_probs", vp), ("d_entropy", vp), ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
+class DistillArgs(ctypes.Structure):
+    """Mirror of ``swx_distill_args``."""
+    _fields_ = [
+        ("tokens", i64), ("vocab", i64), ("dim", i64), ("entries", i64),
+        ("dtype", i32), ("dw_dtype", i32), ("reduction", i32), ("teacher_dtype", i32),
+        ("temperature", ctypes.c_float), ("reserved", i32),
+        ("x", vp), ("x_sr", i64), ("weight", vp), ("w_sr", i64),
+        ("teacher_ids", vp), ("ids_sr", i64), ("teacher_logits", vp), ("tl_sr", i64),
+        ("loss", vp), ("count", vp), ("row_max", vp), ("row_sum", vp), ("entry_logits", vp),
+        ("dloss", vp), ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 class LinattnArgs(ctypes.Structure):
     """Mirror of ``swx_linattn_args``."""
     _fields_ = [
@@ -169,7 +196,8 @@ def load():
     for fn, st in (("swx_scan_args_size", ScanArgs), ("swx_conv_args_size", ConvArgs),
                    ("swx_decode_args_size", DecodeArgs), ("swx_linear_scan_args_size", LinearScanArgs),
                    ("swx_rmsnorm_args_size", RMSNormArgs), ("swx_embedding_args_size", EmbeddingArgs),
-                   ("swx_xent_args_size", XentArgs),
+                   ("swx_xent_args_size", XentArgs), ("swx_logprob_args_size", LogprobArgs),
+                   ("swx_distill_args_size", DistillArgs),
                    ("swx_linattn_args_size", LinattnArgs)):
         getattr(lib, fn).restype = i64
         if getattr(lib, fn)() != ctypes.sizeof(st):
@@ -187,6 +215,9 @@ def load():
                      ("swx_rmsnorm_fwd", RMSNormArgs), ("swx_rmsnorm_bwd", RMSNormArgs),
                      ("swx_embedding_bwd", EmbeddingArgs),
                      ("swx_xent_fwd", XentArgs), ("swx_xent_bwd", XentArgs),
+                     ("swx_logprob_fwd", LogprobArgs), ("swx_logprob_bwd", LogprobArgs),
+                     ("swx_token_logprob", LogprobArgs),
+                     ("swx_distill_fwd", DistillArgs), ("swx_distill_bwd", DistillArgs),
                      ("swx_linattn_fwd", LinattnArgs), ("swx_linattn_bwd", LinattnArgs),
                      ("swx_linattn_step", LinattnArgs)):
         fn = getattr(lib, name)
@@ -212,9 +243,10 @@ def load():
     lib.swx_rmsnorm_bwd_workspace_bytes.argtypes = [i64]
     lib.swx_embedding_bwd_workspace_bytes.restype = i64
     lib.swx_embedding_bwd_workspace_bytes.argtypes = [i64, i64, i64]
-    for fn in ("swx_xent_fwd_workspace_bytes", "swx_xent_bwd_workspace_bytes"):
-        getattr(lib, fn).restype = i64
-        getattr(lib, fn).argtypes = [ctypes.POINTER(XentArgs)]
+    for op, st in (("xent", XentArgs), ("logprob", LogprobArgs), ("distill", DistillArgs)):
+        for fn in (f"swx_{op}_fwd_workspace_bytes", f"swx_{op}_bwd_workspace_bytes"):
+            getattr(lib, fn).restype = i64
+            getattr(lib, fn).argtypes = [ctypes.POINTER(st)]
     for fn in ("swx_linattn_fwd_workspace_bytes", "swx_linattn_bwd_workspace_bytes"):
         getattr(lib, fn).restype = i64
         getattr(lib, fn).argtypes = [ctypes.POINTER(LinattnArgs)]

@@ -1,0 +1,675 @@
+// The products of a linear head over a large vocabulary, for the operators that never keep its
+// logits (linear_xent.cu, linear_logprob.cu, linear_distill.cu): one matrix product kernel whose
+// epilogue turns a tile of logits into what the operator keeps, and the host side of it.
+//
+// A persistent grid of CTA pairs, 256 x 256 tiles, operands staged by TMA into a ring, tcgen05
+// products issued by one thread per pair into two alternating accumulators in tensor memory, and eight
+// warps per CTA that read an accumulator while the next tile is computed.  linear_xent.cu holds the
+// figures and the kernels that every operator shares (gradient products, operand layout).
+#pragma once
+#include <algorithm>
+
+#include "common.cuh"
+#include "launch_util.cuh"
+#include "tc5.cuh"
+#include "tma_util.cuh"
+
+namespace swx {
+
+constexpr int XE_TILE = 256;                  // rows and columns of a pair's tile
+constexpr int XE_K = 64;                      // contraction steps per ring stage (128 bytes of bf16)
+constexpr int XE_STAGES = 6;
+constexpr int XE_OPERAND = 128 * XE_K * 2;    // bytes of one operand of one CTA in a stage
+constexpr int XE_STAGE = 2 * XE_OPERAND;
+constexpr int XE_EPI_WARPS = 8;
+constexpr int XE_THREADS = 64 + 32 * XE_EPI_WARPS;
+constexpr int XE_OUT = 32 * 128;              // staging bytes of one epilogue warp: 32 rows x 128 bytes
+constexpr int XE_SMEM = 1024 + XE_STAGES * XE_STAGE + XE_EPI_WARPS * XE_OUT;
+// fp32 operands: stages summed in tensor memory at a time.  The tensor core cuts the low bits
+// of each addition off (toward zero), an error that grows with the number of additions (dx
+// 4.9e-6 off after 5001 terms in one sum); sums of 256 terms are added up in fp32 instead.
+constexpr int XE_KSUB = 4;
+// The same for the logits, over the width of the operands, 512 terms at a time: up to that nothing is summed outside
+// (3.9e-7 off at operands of one sign, a library's fp32 products 4.8e-7); in one sum 1024 terms were 1.3e-6 off, 4096 8.7e-6
+// and 16384 6.6e-5, 4e-7 each now.  2048 x 8192 x 1024 forward 148 -> 163 us; 256 terms at a time 176, and 384 instead of 326 us
+// at 4096 x 20000 x 512.
+constexpr int XE_KSUB_LOGITS = 8;
+constexpr uint32_t XE_POLLS = 1u << 24;       // about a second
+
+// Epilogues: XE_LSE (loss) and XE_SCORE* (log probabilities: statistics of scaled logits, with the entropy's sum; for the top
+// alternatives also each 32 columns' two largest logits, or the logits themselves) read logits, XE_PROB and
+// XE_GRAD write the logits' gradient, XE_DX and XE_DW are the gradient products.
+enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW, XE_SCORE, XE_SCORE_TOP, XE_SCORE_ALL, XE_GRAD };
+constexpr bool is_score(int epi) { return epi == XE_SCORE || epi == XE_SCORE_TOP || epi == XE_SCORE_ALL; }
+constexpr bool is_dlogit(int epi) { return epi == XE_PROB || epi == XE_GRAD; }
+constexpr bool is_logits(int epi) { return epi == XE_LSE || is_score(epi) || is_dlogit(epi); }
+constexpr float SCORE_FLOOR = -0x1.fp127f;    // stands for -inf where an infinity's differences would be NaN (its low 5 bits are 0)
+constexpr float SCORE_FAR = -200.f;           // 2^-200 is 0: what lies further below the maximum adds nothing
+
+struct XentGemm {
+    int M, N;                                 // rows and columns of the result
+    int mt, nt, group;                        // tiles; row tiles walked together (logits)
+    int nk, npair;                            // ring stages of the contraction; pairs of pieces
+    int ksub;                                 // stages summed in tensor memory before the sum moves on
+    int ka0, kb0;                             // first contraction index of A and of B
+    int a0, b0;                               // first row of A and of B (M / N coordinate)
+    int* status;
+    // logits
+    const int64_t* target;
+    int64_t ignore;
+    int64_t vocab;
+    int col0;                                 // vocabulary index of column 0
+    float2* part;                             // (2 nt, M): max and sum of a tile half's exponentials
+    float* hit;                               // (M): the target's logit
+    int* counter;                             // zeroed by XE_LSE for the joining kernel
+    const float* row_max; const float* row_rsum;
+    const float* dloss; int reduction;
+    int planes;                               // bf16 pieces of the dlogit
+    // XE_DX / XE_DW
+    // spread: the steps of all tiles are dealt out evenly and a tile's parts are summed in
+    // acc[part][M][N]; else whole tiles go round and the last piece writes the result
+    int spread;
+    float* acc; void* out; int out_bf16; int64_t ld; int first, last;
+    const float* scale_num; const float* scale_den;   // the result's factor: num / den, either may be absent
+    // XE_SCORE*, XE_GRAD: exponents are (logit - maximum) * k2, k2 = log2(e) / temperature
+    float k2, inv_temp;
+    float4* score;                            // (M, 2 nt): a tile half's maximum, sum of exponentials e, sum of e times its exponent
+    float2* rec; int64_t groups;              // XE_SCORE_TOP, (M, groups): the two largest logits of 32 columns, their low 5 bits the column
+    float* all;                               // XE_SCORE_ALL, (M, N)
+    // XE_GRAD: dlogit = 2^u (A + B u) + [column == target] hot, see grad_row
+    const float* row_sum; const float* entropy; const float* d_logp; const float* d_entropy;
+};
+
+// Pieces of A and B multiplied in turn (index: plane of the 3-D tensor map), smallest
+// products first, so that few additions happen at the sum's full magnitude.
+__device__ __forceinline__ int2 piece_pair(int npair, int i) {
+    if (npair == 1) return make_int2(0, 0);
+    constexpr uint32_t A = 2u | 1u << 2 | 0u << 4 | 1u << 6 | 0u << 8 | 0u << 10;
+    constexpr uint32_t B = 0u | 1u << 2 | 2u << 4 | 0u << 6 | 1u << 8 | 0u << 10;
+    return make_int2((A >> (2 * i)) & 3, (B >> (2 * i)) & 3);
+}
+
+// The work of one CTA pair: runs of contraction steps [k0, k1) of a tile, each summed in one
+// accumulator.  Whole tiles go round the pairs; spread, pair c takes the steps
+// [c S / P, (c + 1) S / P) of the S steps of all tiles, so that a tile can have several parts
+// (numbered from the pair that has the tile's first step).
+struct XentRuns {
+    int64_t cur, end, tile;
+    int nk, ksub, P, k0, k1, part;
+    bool spread, fresh;
+    __device__ __forceinline__ XentRuns(const XentGemm& p, int64_t c, int64_t P_) : nk(p.nk), ksub(p.ksub), P((int)P_), part(0), spread(p.spread) {
+        const int64_t tiles = (int64_t)p.mt * p.nt;
+        cur = spread ? c * (tiles * nk) / P : c;
+        end = spread ? (c + 1) * (tiles * nk) / P : tiles;
+        k1 = nk;
+        fresh = true;
+        tile = -1;
+    }
+    __device__ __forceinline__ bool next(const XentGemm& p) {
+        if (cur >= end) return false;
+        if (spread) {
+            const int64_t t = cur / nk;
+            k0 = (int)(cur - t * nk);
+            k1 = (int)min((int64_t)min(nk, k0 + ksub), k0 + (end - cur));
+            fresh = t != tile;
+            if (fresh) {
+                const int64_t total = (int64_t)p.mt * p.nt * nk;
+                const int64_t c = ((cur + 1) * P - 1) / total, lo = ((t * nk + 1) * P - 1) / total;
+                part = (int)(c - lo);
+            }
+            tile = t;
+            cur += k1 - k0;
+        } else {
+            tile = cur;
+            k0 = k1 < nk ? k1 : 0;
+            fresh = k0 == 0;
+            k1 = min(k0 + ksub, nk);
+            if (k1 == nk) cur += P;
+        }
+        return true;
+    }
+};
+
+// Tile t -> (row tile, column tile).  Logits: `group` row tiles of x stay in L2
+// while the weight's column tiles pass by; the gradients: a row tile's column tiles together.
+template <int EPI>
+__device__ __forceinline__ int2 tile_of(const XentGemm& p, int64_t t) {
+    if (is_logits(EPI)) {
+        const int64_t per = (int64_t)p.group * p.nt;
+        const int g = (int)(t / per);
+        const int rows = min(p.group, p.mt - g * p.group);
+        const int64_t r = t - g * per;
+        return make_int2(g * p.group + (int)(r % rows), (int)(r / rows));
+    }
+    return make_int2((int)(t / p.nt), (int)(t % p.nt));
+}
+
+// Factor of a row's dlogit.  A mean's or a sum's upstream gradient is one number for all
+// rows; it multiplies the gradients at the end instead, so that the target's column, near -1,
+// is rounded near a power of two (with the factor inside, every row's -1/n was rounded the
+// same way and the gradients were 3.1e-3 off, 1.9e-3 now, 256 tokens).
+__device__ __forceinline__ float row_scale(const XentGemm& p, int row) {
+    const int64_t y = p.target[row];
+    if (y == p.ignore) return 0.f;
+    if (y < 0 || y >= p.vocab) return __int_as_float(0x7fc00000);
+    return p.reduction == SWX_XENT_NONE ? p.dloss[row] : 1.f;
+}
+
+// A row's coefficients of XE_GRAD.  With u = (z - max) k2, e = 2^u, s the sum of e: p = e / s, the log probability
+// l = u ln2 - ln s, and for upstream gradients g of the target's log probability and h of the entropy H
+//   dz = (g [v == y] - p (g + h (l + H))) / temperature = e (A + B u) + [v == y] hot.
+// Distillation (no targets): dz = p c / temperature with c = temperature^2 times the row's upstream gradient; the
+// teacher's words are set afterwards.
+struct GradRow { float A, B, hot; };
+__device__ __forceinline__ GradRow grad_row(const XentGemm& p, int row) {
+    const float s = p.row_sum[row];
+    if (!p.target) {
+        const float c = p.reduction == SWX_XENT_NONE ? p.dloss[row] : 1.f;
+        return GradRow{s > 0.f ? c / (p.inv_temp * s) : s < 0.f ? 0.f : __int_as_float(0x7fc00000), 0.f, 0.f};     // s < 0: a row that does not count
+    }
+    const int64_t y = p.target[row];
+    if (y == p.ignore) return GradRow{0.f, 0.f, 0.f};
+    if (y < 0 || y >= p.vocab) return GradRow{__int_as_float(0x7fc00000), 0.f, 0.f};
+    const float g = p.d_logp ? p.d_logp[row] : 0.f, h = p.d_entropy ? p.d_entropy[row] : 0.f;
+    const float f = p.inv_temp / s;
+    return GradRow{-f * (g + h * (p.entropy[row] - logf(s))), -f * h * 0.69314718055994531f, p.inv_temp * g};
+}
+
+// 32 columns of a row of a gradient (from cc on), to the running sum in memory or, the last time, to the result.
+__device__ __forceinline__ void xent_emit(const XentGemm& p, float (&v)[32], int part, int row, int cc, bool first, bool last, float factor) {
+    const int n = min(32, p.N - cc);
+    float* acc = p.acc + ((int64_t)part * p.M + row) * p.N + cc;
+    const bool whole = n == 32 && (reinterpret_cast<uintptr_t>(acc) & 15) == 0;
+    if (!first) {
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float4 q = reinterpret_cast<const float4*>(acc)[j];
+                v[4 * j] += q.x; v[4 * j + 1] += q.y; v[4 * j + 2] += q.z; v[4 * j + 3] += q.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) if (j < n) v[j] += acc[j];
+        }
+    }
+    if (last) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] *= factor;
+    }
+    if (!last) {
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                reinterpret_cast<float4*>(acc)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) if (j < n) acc[j] = v[j];
+        }
+    } else if (p.out_bf16) {
+        __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.out) + (int64_t)row * p.ld + cc;
+        if (n == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint32_t w[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[8 * j + 2 * k], v[8 * j + 2 * k + 1]);
+                    w[k] = *reinterpret_cast<const uint32_t*>(&b2);
+                }
+                reinterpret_cast<uint4*>(o)[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) if (j < n) o[j] = __float2bfloat16_rn(v[j]);
+        }
+    } else {
+        float* o = static_cast<float*>(p.out) + (int64_t)row * p.ld + cc;
+        if (n == 32 && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) if (j < n) o[j] = v[j];
+        }
+    }
+}
+
+// SUMS: the steps of a tile come in several accumulators (fp32 operands: the gradients, and logits of wide operands); their sum stays in registers until the tile (or
+// this pair's part of it) is complete: through memory each time, 1003 tokens x 10007 x 200 took 232 us, 219 with the registers.
+template <int EPI, bool A_MN, bool B_MN, bool SUMS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(XE_THREADS, 1)
+xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_p) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t full[XE_STAGES], empty[XE_STAGES], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_base;
+    uint8_t* smem = smem_raw + (((smem_u32(smem_raw) + 1023) & ~1023u) - smem_u32(smem_raw));
+    uint8_t* stage_out = smem + XE_STAGES * XE_STAGE;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t rank = cluster_rank();
+    const int64_t cluster = blockIdx.x / 2, nclusters = gridDim.x / 2;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < XE_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 2 * XE_EPI_WARPS); }
+        mbar_fence_init();
+        if ((EPI == XE_LSE || (EPI == XE_SCORE && p.counter)) && blockIdx.x == 0) *p.counter = 0;
+    }
+    if (warp == 1) tmem_alloc_pair(&tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ---- loads: this CTA's half of the rows of A and B, counted on the leader's barrier
+            int s = 0;
+            uint32_t ph = 0;
+            int64_t issued = 0;
+            bool ok = true;
+            for (XentRuns r(p, cluster, nclusters); ok && r.next(p);) {
+                const int2 rc = tile_of<EPI>(p, r.tile);
+                const int am = p.a0 + rc.x * XE_TILE + (int)rank * 128, bn = p.b0 + rc.y * XE_TILE + (int)rank * 128;
+                for (int i = 0; ok && i < p.npair; ++i) {
+                    const int2 pl = piece_pair(p.npair, i);
+                    for (int k = r.k0; k < r.k1; ++k) {
+                        if (!mbar_wait_cluster(&empty[s], ph ^ 1, XE_POLLS)) { ok = false; break; }
+                        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * XE_STAGE);
+                        const uint32_t bar = map_to_rank(&full[s], 0);
+                        uint8_t* sa = smem + s * XE_STAGE;
+                        uint8_t* sb = sa + XE_OPERAND;
+                        const int ka = p.ka0 + k * XE_K, kb = p.kb0 + k * XE_K;
+                        if (A_MN) {
+                            tma_load_3d_pair(sa, &map_a, am, ka, pl.x, bar);
+                            tma_load_3d_pair(sa + XE_OPERAND / 2, &map_a, am + 64, ka, pl.x, bar);
+                        } else {
+                            tma_load_3d_pair(sa, &map_a, ka, am, pl.x, bar);
+                        }
+                        if (B_MN) {
+                            tma_load_3d_pair(sb, &map_b, bn, kb, pl.y, bar);
+                            tma_load_3d_pair(sb + XE_OPERAND / 2, &map_b, bn + 64, kb, pl.y, bar);
+                        } else {
+                            tma_load_3d_pair(sb, &map_b, kb, bn, pl.y, bar);
+                        }
+                        ++issued;
+                        if (++s == XE_STAGES) { s = 0; ph ^= 1; }
+                    }
+                }
+            }
+            // every stage's copies have landed (both CTAs' bytes count on the leader's barrier)
+            // and every product that reads this CTA's ring has finished before it goes
+            for (int q = 0; q < XE_STAGES; ++q) {
+                const int64_t uses = (issued + XE_STAGES - 1 - q) / XE_STAGES;
+                if (uses == 0) continue;
+                const uint32_t par = (uint32_t)((uses - 1) & 1);
+                if (rank == 0) ok = mbar_wait_cluster(&full[q], par, XE_POLLS) && ok;
+                ok = mbar_wait_cluster(&empty[q], par, XE_POLLS) && ok;
+            }
+            if (!ok && p.status) *p.status = SWX_ERR_TIMEOUT;
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0) {
+            // ---- products, for both CTAs (the whole warp, one lane of it issuing)
+            constexpr uint32_t idesc = mma_bf16_idesc(XE_TILE, XE_TILE, A_MN, B_MN);
+            // 16 contraction steps further: 32 bytes along a K-major row, 16 rows of 128 bytes otherwise
+            constexpr uint64_t da = (A_MN ? 2048 : 32) >> 4, db = (B_MN ? 2048 : 32) >> 4;
+            int s = 0, a = 0;
+            uint32_t ph = 0, aph = 0;
+            bool ok = true;
+            for (XentRuns r(p, cluster, nclusters); ok && r.next(p);) {
+                if (!mbar_wait_cluster(&acc_empty[a], aph ^ 1, XE_POLLS)) { ok = false; break; }
+                tc_fence_after();
+                const int steps = (r.k1 - r.k0) * p.npair;
+                for (int i = 0; i < steps; ++i) {
+                    if (!mbar_wait_cluster(&full[s], ph, XE_POLLS)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint64_t ad = operand_desc(smem + s * XE_STAGE, XE_OPERAND / 2);
+                    const uint64_t bd = operand_desc(smem + s * XE_STAGE + XE_OPERAND, XE_OPERAND / 2);
+#pragma unroll
+                    for (int q = 0; q < XE_K / 16; ++q)
+                        mma_bf16_pair(tmem + a * XE_TILE, ad + q * da, bd + q * db, idesc, i > 0 || q > 0);
+                    mma_commit_pair(&empty[s]);
+                    if (++s == XE_STAGES) { s = 0; ph ^= 1; }
+                }
+                mma_commit_pair(&acc_full[a]);
+                if ((a ^= 1) == 0) aph ^= 1;
+            }
+            if (!ok && p.status) *p.status = SWX_ERR_TIMEOUT;
+        }
+        __syncwarp();
+    } else {
+        // ---- epilogue: this lane's row of the accumulator, one 128-column half per warp
+        const int sub = warp & 3, half = (warp - 2) / 4;
+        uint8_t* so = stage_out + (warp - 2) * XE_OUT;
+        int a = 0;
+        uint32_t aph = 0;
+        bool ok = true;
+        float factor = 1.f;
+        float tot[SUMS ? 4 : 1][32];
+        if (EPI == XE_DX || EPI == XE_DW) {
+            if (p.scale_num) factor = *p.scale_num;
+            if (p.scale_den) factor = *p.scale_den > 0.f ? factor / *p.scale_den : 0.f;   // no token counts: no gradient
+        }
+        for (XentRuns r(p, cluster, nclusters); r.next(p);) {
+            const bool last = p.last && !p.spread;
+            const int2 rc = tile_of<EPI>(p, r.tile);
+            const int row = rc.x * XE_TILE + (int)rank * 128 + sub * 32 + lane;
+            const int c0 = rc.y * XE_TILE + half * 128;
+            const bool live = row < p.M;
+            // the row's target as a column of the result (anything outside it: no match)
+            int64_t y = -1;
+            float scale = 0.f, rmax = 0.f, rsum = 0.f;
+            GradRow gr{0.f, 0.f, 0.f};
+            if (is_logits(EPI) && live) {
+                if (!(is_score(EPI) || EPI == XE_GRAD) || p.target) y = p.target[row] - p.col0;
+                if (EPI == XE_GRAD) {
+                    gr = grad_row(p, row);
+                    rmax = p.row_max[row];
+                }
+                if (EPI == XE_PROB) {
+                    scale = row_scale(p, row);
+                    rmax = p.row_max[row];
+                    rsum = p.row_rsum[row] * scale;
+                }
+            }
+            if (!mbar_wait_cluster(&acc_full[a], aph, XE_POLLS)) { ok = false; break; }
+            tc_fence_after();
+            const uint32_t at = tmem + ((uint32_t)(sub * 32) << 16) + a * XE_TILE + half * 128;
+            // 32 columns of the row, from 32 c on
+            float m = is_score(EPI) ? SCORE_FLOOR : -INFINITY, sum = 0.f, esum = 0.f;
+            auto columns = [&](int c, float (&v)[32]) {
+                const int cc = c0 + c * 32;                 // first of these 32 columns
+                const int64_t yc = y - cc;
+                if (EPI == XE_LSE) {
+                    if (yc >= 0 && yc < 32) {
+                        float h = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) h = yc == j ? v[j] : h;
+                        if (y < p.N) p.hit[row] = h;
+                    }
+                    if (cc + 32 > p.N) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : -INFINITY;
+                    }
+                    float top = v[0];
+#pragma unroll
+                    for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+                    const float nm = fmaxf(m, top);
+                    const float base = nm == -INFINITY ? 0.f : nm;      // nothing but -inf so far: sum stays 0
+                    float add = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) add += ex2((v[j] - base) * LOG2E);
+                    sum = sum * ex2((m - base) * LOG2E) + add;
+                    m = nm;
+                } else if (is_score(EPI)) {
+                    if (yc >= 0 && yc < 32) {
+                        float h = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) h = yc == j ? v[j] : h;
+                        if (y < p.N) p.hit[row] = h;
+                    }
+                    if (EPI == XE_SCORE_ALL && live) {
+                        float* o = p.all + (int64_t)row * p.N + cc;
+                        if (cc + 32 <= p.N && (reinterpret_cast<uintptr_t>(o) & 15) == 0) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) reinterpret_cast<float4*>(o)[j] = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) if (cc + j < p.N) o[j] = v[j];
+                        }
+                    }
+                    if (cc + 32 > p.N) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : -INFINITY;
+                    }
+                    float top = SCORE_FLOOR;
+                    if (EPI == XE_SCORE_TOP) {
+                        // the two largest, each with its column in place of its low bits (a NaN takes neither)
+                        float second = SCORE_FLOOR;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float t = __uint_as_float((__float_as_uint(fmaxf(v[j], SCORE_FLOOR)) & ~31u) | j);
+                            second = fmaxf(second, fminf(top, t));
+                            top = fmaxf(top, t);
+                        }
+                        if (live && cc < p.N) p.rec[(int64_t)row * p.groups + cc / 32] = make_float2(top, second);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
+                    }
+                    // sums relative to the larger maximum: e u becomes c e (u + shift)
+                    const float nm = fmaxf(m, top);
+                    const float shift = fmaxf((m - nm) * p.k2, SCORE_FAR), c2 = ex2(shift);
+                    esum = c2 * (esum + sum * shift);
+                    sum *= c2;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float u = (v[j] - nm) * p.k2, e = ex2(u);
+                        sum += e;
+                        esum += e * fmaxf(u, SCORE_FAR);
+                    }
+                    m = nm;
+                } else if (is_dlogit(EPI)) {
+                    if (EPI == XE_GRAD) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float u = (v[j] - rmax) * p.k2;
+                            v[j] = ex2(u) * fmaf(gr.B, fmaxf(u, SCORE_FAR), gr.A);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - rmax) * LOG2E) * rsum;
+                    }
+                    if (yc >= 0 && yc < 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = yc == j ? v[j] - (EPI == XE_GRAD ? -gr.hot : scale) : v[j];
+                    }
+                    if (EPI == XE_GRAD ? gr.A == 0.f && gr.B == 0.f && gr.hot == 0.f : scale == 0.f) {   // a token that does not count, whatever its logits
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) v[j] = 0.f;
+                    }
+                    // 64 columns of each piece make one 32-row x 128-byte store
+                    for (int pl = 0; pl < p.planes; ++pl) {
+                        if ((c & 1) == 0 || p.planes > 1) {
+                            if (lane == 0) bulk_wait_read();
+                            __syncwarp();
+                        }
+                        uint32_t w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                            w[j] = *reinterpret_cast<const uint32_t*>(&b2);
+                            v[2 * j] -= __low2float(b2);
+                            v[2 * j + 1] -= __high2float(b2);
+                        }
+                        // one piece: 128-byte rows, swizzled (16-byte part j of row r lands at
+                        // j ^ (r % 8)); three: 64-byte rows, plain
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int at_b = p.planes > 1 ? lane * 64 + j * 16
+                                                          : lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4);
+                            *reinterpret_cast<uint4*>(so + at_b) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                        }
+                        if (p.planes > 1 || (c & 1)) {
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            const int x = p.planes > 1 ? cc : cc - 32;
+                            const int y0 = rc.x * XE_TILE + (int)rank * 128 + sub * 32;
+                            if (lane == 0 && x < p.N && y0 < p.M) {
+                                tma_store_3d(&map_p, so, x, y0, pl);
+                                bulk_commit();
+                            }
+                        }
+                    }
+                } else if (live && cc < p.N) {
+                    xent_emit(p, v, r.part, row, cc, p.first, last, factor);
+                }
+            };
+            if constexpr (SUMS) {
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {
+                    float v[16];
+                    tmem_ld16(at + c * 16, v);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) tot[c / 2][c % 2 * 16 + j] = r.fresh ? v[j] : tot[c / 2][c % 2 * 16 + j] + v[j];
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[a], 0));
+                if ((a ^= 1) == 0) aph ^= 1;
+                if (r.k1 != p.nk && r.cur < r.end) continue;             // more of the tile (or of this pair's part of it) to come
+#pragma unroll
+                for (int c = 0; c < 4; ++c) columns(c, tot[c]);
+                if (EPI == XE_LSE && live) p.part[(int64_t)(2 * rc.y + half) * p.M + row] = make_float2(m, sum);
+                if (is_score(EPI) && live) p.score[(int64_t)row * 2 * p.nt + 2 * rc.y + half] = make_float4(m, sum, esum, 0.f);
+                continue;
+            }
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+                float v[32];
+                tmem_ld32(at + c * 32, v);
+                tmem_ld_wait();
+                columns(c, v);
+            }
+            if (EPI == XE_LSE && live) p.part[(int64_t)(2 * rc.y + half) * p.M + row] = make_float2(m, sum);
+            if (is_score(EPI) && live) p.score[(int64_t)row * 2 * p.nt + 2 * rc.y + half] = make_float4(m, sum, esum, 0.f);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[a], 0));
+            if ((a ^= 1) == 0) aph ^= 1;
+        }
+        if (is_dlogit(EPI) && lane == 0) bulk_wait_all();
+        if (!ok && lane == 0 && p.status) *p.status = SWX_ERR_TIMEOUT;
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                       // neither CTA goes while the other may still reach its barriers
+    if (warp == 1) tmem_free_pair(tmem, 512);
+}
+
+// ------------------------------------------------------------------ host side
+// How a gradient product's tiles are dealt out to the CTA pairs (linear_xent.cu `deal`).
+struct XentDeal { int spread, pairs, parts; };
+constexpr int XE_PAIRS = 74, XE_MIN_SHARE = 4;
+
+// A head's operands: x (T, d) and the weight (V, d), row strides in elements.
+struct HeadOps { int64_t T, V, d; int dtype; const void* x; int64_t x_sr; const void* w; int64_t w_sr; };
+
+// Sizes and the workspace: copies of the operands, then (forward) whatever the operator keeps from
+// `base` on, or (backward) a piece of the logits' gradient and the sums of the gradient products.
+struct HeadPlan {
+    int es, planes;                           // bytes of an input value; bf16 pieces
+    int64_t dp;                               // padded contraction length of packed operands
+    bool pack_x, pack_w;
+    int64_t mt, nt, piece;                    // tiles; vocabulary columns per piece of the backward
+    int64_t off_x, off_w, base;
+    int64_t off_p, off_acc, off_acc_w, ldp, bwd_total;
+    XentDeal dx;
+};
+HeadPlan head_plan(const HeadOps& o);
+int head_check(const HeadOps& o);
+
+inline int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// Stages of the logits' contraction summed in tensor memory at a time: all of them for bf16 operands.
+inline int logits_ksub(const HeadPlan& q, int nk) { return q.planes == 3 ? std::min(nk, XE_KSUB_LOGITS) : nk; }
+
+// A (rows, inner) bf16 matrix with `planes` pieces as a 3-D tensor map, 128-byte swizzled.
+inline bool encode_operand(CUtensorMap* m, const void* base, int64_t inner, int64_t rows, int64_t planes, int64_t row,
+                           int64_t plane, uint32_t box_inner, uint32_t box_rows, bool swizzle = true) {
+    const EncodeTiledFn f = encode_tiled();
+    if (!f || !base || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
+    const int64_t rs = row * 2, ps = (planes > 1 ? plane : row * rows) * 2;
+    if (rs % 16 || ps % 16 || rs <= 0 || ps <= 0 || rs >= (int64_t(1) << 40) || ps >= (int64_t(1) << 40)) return false;
+    cuuint64_t dims[3] = {(cuuint64_t)inner, (cuuint64_t)rows, (cuuint64_t)planes};
+    cuuint64_t strides[2] = {(cuuint64_t)rs, (cuuint64_t)ps};
+    cuuint32_t box[3] = {box_inner, box_rows, 1};
+    cuuint32_t unit[3] = {1, 1, 1};
+    return f(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, unit,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Operand {
+    const void* p; int64_t inner, rows, planes, row, plane;
+    // rows of the contraction's other index, 64 contraction steps wide / the transposed use
+    bool k_major(CUtensorMap* m) const { return encode_operand(m, p, inner, rows, planes, row, plane, 64, 128); }
+    bool mn_major(CUtensorMap* m) const { return encode_operand(m, p, inner, rows, planes, row, plane, 64, 64); }
+};
+
+// x and the weight as the products read them: themselves, or their copies in the workspace.
+void head_operands(const HeadOps& o, const HeadPlan& q, uint8_t* ws, Operand& x, Operand& w, cudaStream_t st);
+
+template <int EPI, bool A_MN, bool B_MN, bool SUMS = false>
+static cudaError_t launch_gemm(const XentGemm& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mp,
+                               int64_t pairs, cudaStream_t st) {
+    auto k = xent_gemm_kernel<EPI, A_MN, B_MN, SUMS>;
+    cudaError_t e = allow_smem(k, XE_SMEM);
+    if (e != cudaSuccess) return e;
+    if (!p.spread) pairs = std::min<int64_t>((int64_t)p.mt * p.nt, pairs);
+    k<<<(unsigned)(2 * pairs), XE_THREADS, XE_SMEM, st>>>(p, ma, mb, mp);
+    return cudaGetLastError();
+}
+
+// What a backward pass wants: either gradient may be absent; the results' factor is num / den.
+struct HeadGrads { void* dx; void* dw; int dw_bf16; const float* num; const float* den; };
+
+// dx and dW of the vocabulary's columns [c0, c0 + cw), whose dlogit is in the workspace.
+int head_piece_products(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const Operand& x, const Operand& w, const Operand& pr,
+                        const HeadGrads& gr, int64_t c0, int64_t cw, int* status, cudaStream_t st);
+
+// The logits' product, with the epilogue EPI, over all columns or a piece of them.
+inline XentGemm logits_gemm(const HeadOps& o, const HeadPlan& q, int64_t c0, int64_t cw, int* status) {
+    XentGemm g{};
+    g.status = status; g.npair = q.planes == 3 ? 6 : 1; g.planes = q.planes;
+    g.M = (int)o.T; g.N = (int)cw; g.mt = (int)q.mt; g.nt = (int)((cw + XE_TILE - 1) / XE_TILE); g.group = 32;
+    g.nk = (int)((o.d + XE_K - 1) / XE_K); g.b0 = g.col0 = (int)c0; g.vocab = o.V;
+    g.ksub = logits_ksub(q, g.nk);
+    return g;
+}
+
+template <int EPI>
+static cudaError_t launch_logits(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& store, cudaStream_t st) {
+    return g.ksub < g.nk ? launch_gemm<EPI, false, false, true>(g, x, w, store, XE_PAIRS, st)
+                         : launch_gemm<EPI, false, false>(g, x, w, store, XE_PAIRS, st);
+}
+
+// The scoring and gradient epilogues that more than one operator uses (linear_logprob.cu).
+cudaError_t launch_score(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, cudaStream_t st);
+cudaError_t launch_grad(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& store, cudaStream_t st);
+
+// The gradients, piece by piece of the vocabulary: the logits again and dlogit in the epilogue (`launch`, with the
+// fields that `fill` sets), whatever `patch` does to the piece (its base, first column and columns; a status), and the
+// two products.
+template <class Launch, class Fill, class Patch>
+static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const HeadGrads& gr, cudaStream_t st, Launch launch, Fill fill,
+                         Patch patch) {
+    int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
+    Operand x, w;
+    head_operands(o, q, ws, x, w, st);
+    CUtensorMap x_k, w_k;
+    if (!x.k_major(&x_k) || !w.k_major(&w_k)) return SWX_ERR_CUDA;
+    for (int64_t c0 = 0; c0 < o.V; c0 += q.piece) {
+        const int64_t cw = std::min(q.piece, o.V - c0);
+        const Operand pr{ws + q.off_p, cw, o.T, q.planes, q.ldp, o.T * q.ldp};
+        CUtensorMap p_st;
+        // stores of 32 rows: 64 columns at once for one piece, 32 for each of three
+        if (!encode_operand(&p_st, pr.p, cw, o.T, q.planes, q.ldp, o.T * q.ldp, q.planes == 3 ? 32 : 64, 32, q.planes == 1)) return SWX_ERR_CUDA;
+        XentGemm g = logits_gemm(o, q, c0, cw, status);
+        fill(g);
+        if (launch(g, x_k, w_k, p_st, st) != cudaSuccess) return SWX_ERR_CUDA;
+        int c = patch(reinterpret_cast<__nv_bfloat16*>(ws + q.off_p), c0, cw);
+        if (c == SWX_OK) c = head_piece_products(o, q, ws, x, w, pr, gr, c0, cw, status, st);
+        if (c != SWX_OK) return c;
+    }
+    return SWX_OK;
+}
+
+}  // namespace swx

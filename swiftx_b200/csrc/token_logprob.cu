@@ -1,0 +1,197 @@
+// Log probabilities, entropy and top alternatives of rows of logits (a step of generation):
+// with u = (z - m) log2(e) / tau, s = sum 2^u and w = sum 2^u u over the row,
+//   log_probs = (z_y - m) / tau - ln s,  entropy = ln s - ln2 w / s.
+//
+// One pass over the logits, which bound it.  A row goes to a cluster of 1 to 8 CTAs (so that a few rows
+// reach many SMs, without a second launch); each walks its part in batches of 32 logits a thread with 16-byte loads, keeps
+// running statistics and streams the values past the threshold of the largest so far (topk.cuh).  The first CTA of the cluster
+// joins the parts through distributed shared memory.
+#include "launch_util.cuh"
+#include "tc5.cuh"
+#include "topk.cuh"
+
+namespace swx {
+
+constexpr int TL_THREADS = 256, TL_PER = 32, TL_MAX_PARTS = 8;
+constexpr float TL_FLOOR = -0x1.fp127f, TL_FAR = -200.f, TL_LN2 = 0.69314718055994531f;
+
+struct TokenRows {
+    int64_t V, stride;
+    int parts, top;
+    const void* z; const int64_t* target; int64_t ignore;
+    float k2, inv_temp;
+    float* log_probs; float* entropy; float* top_log_probs; int64_t* top_ids;
+};
+
+__device__ __forceinline__ uint64_t ld_cluster_u64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRows p) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    __shared__ Score part[TL_THREADS / 32];
+    __shared__ Score whole;
+    __shared__ int count, found;
+    constexpr int N = 16 / sizeof(T);          // logits of a 16-byte load
+    const int64_t row = blockIdx.x / p.parts;
+    const int rank = blockIdx.x % p.parts, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const T* z = static_cast<const T*>(p.z) + row * p.stride;
+    uint64_t* buf = reinterpret_cast<uint64_t*>(raw);
+    uint64_t* kept = buf + topk_capacity(p.top, TL_PER);
+    TopK<TL_THREADS, TL_PER> best;
+    if (TOP) best.start(buf, kept, &count, p.top);
+
+    // The row in 16-byte pieces counted from the last boundary at or before its start; the first and the last may be cut
+    const int shift = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+    const int64_t pieces = (p.V + shift + N - 1) / N, per = (pieces + p.parts - 1) / p.parts;
+    const int64_t end = min(pieces, (rank + 1) * per);
+    Score a{TL_FLOOR, 0.f, 0.f};
+    for (int64_t i0 = rank * per; i0 < end; i0 += TL_THREADS * (TL_PER / N)) {
+        float v[TL_PER];
+        uint64_t key[TOP ? TL_PER : 1];
+#pragma unroll
+        for (int j = 0; j < TL_PER / N; ++j) {
+            const int64_t i = i0 + j * TL_THREADS + threadIdx.x, c = i * N - shift;
+            if (i < end && c >= 0 && c + N <= p.V) {
+                const uint4 q = *reinterpret_cast<const uint4*>(z + c);
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    v[j * N + k] = Elem<T>::to_f(reinterpret_cast<const T*>(&q)[k]);
+                    if (TOP) key[j * N + k] = index_key(order_key(v[j * N + k]), (uint32_t)(c + k));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const bool in = i < end && c + k >= 0 && c + k < p.V;
+                    v[j * N + k] = in ? Elem<T>::to_f(z[c + k]) : -INFINITY;
+                    if (TOP) key[j * N + k] = in ? index_key(order_key(v[j * N + k]), (uint32_t)(c + k)) : 0;
+                }
+            }
+        }
+        Score b{TL_FLOOR, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < TL_PER; ++j) b.m = fmaxf(b.m, v[j]);
+        const float nm = fmaxf(a.m, b.m);
+        const float da = fmaxf((a.m - nm) * p.k2, TL_FAR), ca = ex2(da);
+        a.w = ca * (a.w + a.s * da);
+        a.s *= ca;
+        a.m = nm;
+#pragma unroll
+        for (int j = 0; j < TL_PER; ++j) {
+            const float u = (v[j] - nm) * p.k2, e = ex2(u);
+            a.s += e;
+            a.w += e * fmaxf(u, TL_FAR);
+        }
+        if constexpr (TOP) best.push(key);
+    }
+    score_join_warp(a, p.k2, TL_FAR);
+    if (lane == 0) part[warp] = a;
+    if (TOP) best.rank();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a = part[0];
+        for (int i = 1; i < TL_THREADS / 32; ++i) score_join(a, part[i], p.k2, TL_FAR);
+        whole = a;
+        if (TOP) found = best.n;
+    }
+    __syncthreads();
+    if (p.parts > 1) {
+        cluster_sync_all();
+        if (rank == 0) {
+            a = whole;
+            for (int r = 1; r < p.parts; ++r) {
+                const uint32_t o = map_to_rank(&whole, r);
+                score_join(a, Score{ld_cluster_f32(o), ld_cluster_f32(o + 4), ld_cluster_f32(o + 8)}, p.k2, TL_FAR);
+            }
+            if (TOP) {
+                for (int r = 1; r < p.parts; ++r) {
+                    const int n = __float_as_int(ld_cluster_f32(map_to_rank(&found, r)));
+                    const uint32_t from = map_to_rank(buf, r);
+                    for (int i = threadIdx.x; i < n; i += TL_THREADS) buf[best.n + i] = ld_cluster_u64(from + 8 * i);
+                    best.n += n;
+                }
+                __syncthreads();
+                best.rank();
+            }
+        }
+        cluster_sync_all();                    // no CTA goes while the first still reads its shared memory
+        if (rank != 0) return;
+    } else {
+        a = whole;
+    }
+    const float ls = logf(a.s);
+    const int64_t y = p.target ? p.target[row] : 0;
+    const bool live = !p.target || y != p.ignore;
+    if (threadIdx.x == 0) {
+        if (p.target)
+            p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? (Elem<T>::to_f(z[y]) - a.m) * p.inv_temp - ls : __int_as_float(0x7fc00000);
+        p.entropy[row] = live ? ls - TL_LN2 * a.w / a.s : 0.f;
+    }
+    if (TOP) {
+        for (int i = threadIdx.x; i < p.top; i += TL_THREADS) {
+            const uint64_t k = best.buf[i];
+            p.top_log_probs[row * p.top + i] = live ? (order_value((uint32_t)(k >> 32)) - a.m) * p.inv_temp - ls : 0.f;
+            p.top_ids[row * p.top + i] = live ? (int64_t)key_index(k) : -1;
+        }
+    }
+}
+
+// CTAs for each row: enough to reach every SM twice, 4096 logits each or more.
+static int token_parts(int64_t rows, int64_t V) {
+    int parts = 1;
+    while (parts < TL_MAX_PARTS && rows * parts < 296 && V / (2 * parts) >= 4096) parts *= 2;
+    return parts;
+}
+
+template <typename T, bool TOP>
+static cudaError_t launch_token(const TokenRows& p, int64_t rows, cudaStream_t st) {
+    auto k = token_logprob_kernel<T, TOP>;
+    const size_t smem = TOP ? (size_t)(topk_capacity(p.top, TL_PER) + p.top) * 8 : 0;
+    if (TOP) {
+        const cudaError_t e = allow_smem(k, (topk_capacity(SWX_MAX_TOP, TL_PER) + SWX_MAX_TOP) * 8);
+        if (e != cudaSuccess) return e;
+    }
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3((unsigned)(rows * p.parts));
+    c.blockDim = dim3(TL_THREADS);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)p.parts;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, k, p);
+}
+
+}  // namespace swx
+
+using namespace swx;
+
+extern "C" int swx_token_logprob(const swx_logprob_args* a, void* stream) {
+    if (!a || a->tokens < 0 || a->vocab < 1 || a->top_k < 0 || a->top_k > a->vocab) return SWX_ERR_INVALID_ARG;
+    if (!(a->temperature > 0.f) || a->temperature > 1e30f || a->temperature < 1e-30f) return SWX_ERR_INVALID_ARG;
+    if (a->dtype != SWX_DTYPE_F32 && a->dtype != SWX_DTYPE_BF16) return SWX_ERR_UNSUPPORTED;
+    if (a->tokens > (1 << 27) || a->vocab > (1 << 28) || a->top_k > SWX_MAX_TOP) return SWX_ERR_UNSUPPORTED;
+    if (a->tokens == 0) return SWX_OK;
+    if (!a->x || !a->entropy || (a->targets && !a->log_probs) || (a->top_k > 0 && (!a->top_log_probs || !a->top_ids))) return SWX_ERR_INVALID_ARG;
+    TokenRows p{};
+    p.V = a->vocab; p.stride = a->x_sr; p.top = a->top_k; p.z = a->x; p.target = a->targets; p.ignore = a->ignore_index;
+    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E * p.inv_temp;
+    p.log_probs = a->log_probs; p.entropy = a->entropy; p.top_log_probs = a->top_log_probs; p.top_ids = a->top_ids;
+    p.parts = token_parts(a->tokens, a->vocab);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool bf = a->dtype == SWX_DTYPE_BF16;
+    const cudaError_t e = a->top_k > 0 ? (bf ? launch_token<__nv_bfloat16, true>(p, a->tokens, st) : launch_token<float, true>(p, a->tokens, st))
+                                       : (bf ? launch_token<__nv_bfloat16, false>(p, a->tokens, st) : launch_token<float, false>(p, a->tokens, st));
+    return e == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
+}
