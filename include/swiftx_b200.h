@@ -511,8 +511,8 @@ int swx_logprob_fwd(const swx_logprob_args* args, void* stream);
 int swx_logprob_bwd(const swx_logprob_args* args, void* stream);
 /* The same from logits: x is (tokens, vocab) with any row stride, fp32 or bf16; no workspace, no
  * gradient.  Logits may be -inf (words that are not allowed): probability 0.  A row with a NaN or
- * +inf, or with nothing but -inf, has NaN values; its ids are in order all the same (-inf last,
- * a NaN by its sign first or last). */
+ * +inf, or with nothing but -inf, has NaN values; its ids are in order all the same (NaNs
+ * first, -inf last). */
 int swx_token_logprob(const swx_logprob_args* args, void* stream);
 
 /* Distillation of a linear head from a teacher's top logits, without keeping the student's (tokens, vocab)

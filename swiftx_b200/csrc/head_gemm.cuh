@@ -43,7 +43,7 @@ enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW, XE_SCORE, XE_SCORE_TOP, XE_SCORE_A
 constexpr bool is_score(int epi) { return epi == XE_SCORE || epi == XE_SCORE_TOP || epi == XE_SCORE_ALL; }
 constexpr bool is_dlogit(int epi) { return epi == XE_PROB || epi == XE_GRAD; }
 constexpr bool is_logits(int epi) { return epi == XE_LSE || is_score(epi) || is_dlogit(epi); }
-constexpr float SCORE_FLOOR = -0x1.fp127f;    // stands for -inf where an infinity's differences would be NaN (its low 5 bits are 0)
+constexpr float SCORE_FLOOR = -0x1.ffffcp127f;   // below (or at) every logit whose column takes its low 5 bits; its own are 0
 constexpr float SCORE_FAR = -200.f;           // 2^-200 is 0: what lies further below the maximum adds nothing
 
 struct XentGemm {
@@ -380,7 +380,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             tc_fence_after();
             const uint32_t at = tmem + ((uint32_t)(sub * 32) << 16) + a * XE_TILE + half * 128;
             // 32 columns of the row, from 32 c on
-            float m = is_score(EPI) ? SCORE_FLOOR : -INFINITY, sum = 0.f, esum = 0.f;
+            float m = -INFINITY, sum = 0.f, esum = 0.f;
             auto columns = [&](int c, float (&v)[32]) {
                 const int cc = c0 + c * 32;                 // first of these 32 columns
                 const int64_t yc = y - cc;
@@ -426,7 +426,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : -INFINITY;
                     }
-                    float top = SCORE_FLOOR;
+                    float top = EPI == XE_SCORE_TOP ? SCORE_FLOOR : v[0];
                     if (EPI == XE_SCORE_TOP) {
                         // the two largest, each with its column in place of its low bits (a NaN takes neither)
                         float second = SCORE_FLOOR;
@@ -439,16 +439,17 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         if (live && cc < p.N) p.rec[(int64_t)row * p.groups + cc / 32] = make_float2(top, second);
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
+                        for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
                     }
                     // sums relative to the larger maximum: e u becomes c e (u + shift)
                     const float nm = fmaxf(m, top);
-                    const float shift = fmaxf((m - nm) * p.k2, SCORE_FAR), c2 = ex2(shift);
+                    const float base = nm == -INFINITY ? 0.f : nm;      // nothing but -inf so far: the sums stay 0
+                    const float shift = fmaxf((m - base) * p.k2, SCORE_FAR), c2 = ex2(shift);
                     esum = c2 * (esum + sum * shift);
                     sum *= c2;
 #pragma unroll
                     for (int j = 0; j < 32; ++j) {
-                        const float u = (v[j] - nm) * p.k2, e = ex2(u);
+                        const float u = (v[j] - base) * p.k2, e = ex2(u);
                         sum += e;
                         esum += e * fmaxf(u, SCORE_FAR);
                     }

@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillR
     __shared__ double red[DI_WARPS][2];
     const int64_t row = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    Score a{SCORE_FLOOR, 0.f, 0.f};
+    Score a{-INFINITY, 0.f, 0.f};
     for (int i = threadIdx.x; i < p.np; i += DI_THREADS) {
         const float4 s = p.score[row * p.np + i];
         score_join(a, Score{s.x, s.y, s.z}, p.k2, SCORE_FAR);

@@ -51,7 +51,7 @@ __global__ void __launch_bounds__(SC_THREADS) score_rows_kernel(const ScoreRows 
     const int64_t row = (int64_t)blockIdx.x * (SC_THREADS / 32) + threadIdx.x / 32;
     if (row >= p.T) return;
     const int lane = threadIdx.x % 32;
-    Score a{SCORE_FLOOR, 0.f, 0.f};
+    Score a{-INFINITY, 0.f, 0.f};
     for (int i = lane; i < p.np; i += 32) {
         const float4 q = p.score[row * p.np + i];
         score_join(a, Score{q.x, q.y, q.z}, p.k2, SCORE_FAR);
@@ -111,7 +111,7 @@ __global__ void __launch_bounds__(SC_THREADS) score_top_kernel(const ScoreRows p
     uint64_t* val = kept + p.cand;                                   // candidates' products, order-preserving
     int* col = reinterpret_cast<int*>(val + (ALL ? p.cand : 32 * p.cand));
 
-    Score a{SCORE_FLOOR, 0.f, 0.f};
+    Score a{-INFINITY, 0.f, 0.f};
     for (int i = threadIdx.x; i < p.np; i += SC_THREADS) {
         const float4 q = p.score[row * p.np + i];
         score_join(a, Score{q.x, q.y, q.z}, p.k2, SCORE_FAR);
@@ -236,7 +236,7 @@ static int score_check(const swx_logprob_args* a) {
     if (a->x_sr < a->dim || a->w_sr < a->dim) return SWX_ERR_INVALID_ARG;
     if (a->top_k < 0 || a->top_k > a->vocab) return SWX_ERR_INVALID_ARG;
     if (a->top_k > SWX_MAX_TOP) return SWX_ERR_UNSUPPORTED;
-    if (!(a->temperature > 0.f) || a->temperature > 1e30f || a->temperature < 1e-30f) return SWX_ERR_INVALID_ARG;
+    if (!(a->temperature > 0.f) || a->temperature > 1e15f || a->temperature < 1e-15f) return SWX_ERR_INVALID_ARG;
     return SWX_OK;
 }
 

@@ -13,7 +13,7 @@
 namespace swx {
 
 constexpr int TL_THREADS = 256, TL_PER = 32, TL_MAX_PARTS = 8;
-constexpr float TL_FLOOR = -0x1.fp127f, TL_FAR = -200.f, TL_LN2 = 0.69314718055994531f;
+constexpr float TL_FAR = -200.f, TL_LN2 = 0.69314718055994531f;
 
 struct TokenRows {
     int64_t V, stride;
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRo
     const int shift = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
     const int64_t pieces = (p.V + shift + N - 1) / N, per = (pieces + p.parts - 1) / p.parts;
     const int64_t end = min(pieces, (rank + 1) * per);
-    Score a{TL_FLOOR, 0.f, 0.f};
+    Score a{-INFINITY, 0.f, 0.f};
     for (int64_t i0 = rank * per; i0 < end; i0 += TL_THREADS * (TL_PER / N)) {
         float v[TL_PER];
         uint64_t key[TOP ? TL_PER : 1];
@@ -76,17 +76,17 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRo
                 }
             }
         }
-        Score b{TL_FLOOR, 0.f, 0.f};
+        float nm = a.m;
 #pragma unroll
-        for (int j = 0; j < TL_PER; ++j) b.m = fmaxf(b.m, v[j]);
-        const float nm = fmaxf(a.m, b.m);
-        const float da = fmaxf((a.m - nm) * p.k2, TL_FAR), ca = ex2(da);
+        for (int j = 0; j < TL_PER; ++j) nm = fmaxf(nm, v[j]);
+        const float base = nm == -INFINITY ? 0.f : nm;                   // nothing but -inf so far: the sums stay 0
+        const float da = fmaxf((a.m - base) * p.k2, TL_FAR), ca = ex2(da);
         a.w = ca * (a.w + a.s * da);
         a.s *= ca;
         a.m = nm;
 #pragma unroll
         for (int j = 0; j < TL_PER; ++j) {
-            const float u = (v[j] - nm) * p.k2, e = ex2(u);
+            const float u = (v[j] - base) * p.k2, e = ex2(u);
             a.s += e;
             a.w += e * fmaxf(u, TL_FAR);
         }
@@ -179,7 +179,7 @@ using namespace swx;
 
 extern "C" int swx_token_logprob(const swx_logprob_args* a, void* stream) {
     if (!a || a->tokens < 0 || a->vocab < 1 || a->top_k < 0 || a->top_k > a->vocab) return SWX_ERR_INVALID_ARG;
-    if (!(a->temperature > 0.f) || a->temperature > 1e30f || a->temperature < 1e-30f) return SWX_ERR_INVALID_ARG;
+    if (!(a->temperature > 0.f) || a->temperature > 1e15f || a->temperature < 1e-15f) return SWX_ERR_INVALID_ARG;
     if (a->dtype != SWX_DTYPE_F32 && a->dtype != SWX_DTYPE_BF16) return SWX_ERR_UNSUPPORTED;
     if (a->tokens > (1 << 27) || a->vocab > (1 << 28) || a->top_k > SWX_MAX_TOP) return SWX_ERR_UNSUPPORTED;
     if (a->tokens == 0) return SWX_OK;

@@ -6,15 +6,15 @@
 
 namespace swx {
 
-// Bits whose unsigned order is the values' (-0 as 0; a NaN by its sign above or below everything).
+// Bits whose unsigned order is the values' (-0 as 0, a NaN above everything).
 __device__ __forceinline__ uint32_t order_key(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    return v != v ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float order_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ uint64_t order_key(double v) {
     const uint64_t b = (uint64_t)__double_as_longlong(v + 0.);
-    return b >> 63 ? ~b : b | (1ull << 63);
+    return v != v ? ~0ull : b >> 63 ? ~b : b | (1ull << 63);
 }
 __device__ __forceinline__ uint64_t index_key(uint32_t value, uint32_t index) { return (uint64_t)value << 32 | (uint32_t)~index; }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k; }
@@ -85,6 +85,7 @@ struct TopK {
 };
 
 // Statistics of scaled logits in base 2: maximum m of the raw logits, s = sum 2^u and w = sum 2^u u with u = (z - m) k2.
+// (m = -inf with s = w = 0: nothing yet; the differences of infinities, NaN, are dropped by the maximum with `far`.)
 struct Score { float m, s, w; };
 __device__ __forceinline__ void score_join(Score& a, const Score& b, float k2, float far) {
     const float nm = fmaxf(a.m, b.m);

@@ -46,7 +46,7 @@ def _forward(x, w, targets, opts, keep):
         lib = _lib.load()
         a = _args(x, w, targets, *opts)
         out = _outputs(a, x, T, opts[1])
-        stats = out[1].new_empty(2 * T) if keep else None
+        stats = out[1].new_empty(2 * T + 1) if keep else None      # (never empty: it has an address)
         if keep:
             a.row_max = stats.data_ptr()
             a.row_sum = a.row_max + 4 * T
@@ -128,7 +128,7 @@ def token_log_probs(logits, targets=None, top_k=0, temperature=1.0, ignore_index
     Without targets log_probs is None.
 
     Logits of -inf are words that are not allowed (probability 0).  A row with a NaN or +inf, or with nothing but -inf, gives
-    NaN values and ids in order all the same (a NaN first or last).  Not differentiable: logits that require gradients are
+    NaN values and ids in order all the same (NaNs first).  Not differentiable: logits that require gradients are
     refused unless gradients are disabled, dual numbers and torch.jit.trace always."""
     if not logits.is_cuda or (targets is not None and not targets.is_cuda):
         raise RuntimeError("swiftx_b200 token_log_probs runs on CUDA tensors only (no CPU path)")

@@ -36,7 +36,8 @@ from . import embedding as embedding_kernels
 from . import norm as norm_kernels
 from .conv import causal_conv1d_fn, conv1d_backward, conv1d_forward
 from .decode import decode_conv_step, decode_layer_step, decode_ssm_step
-from .loss import linear_cross_entropy
+from .log_probs import LogProbs, linear_log_probs, token_log_probs
+from .loss import linear_cross_entropy, linear_distillation
 from .selective_scan import scan_backward, scan_forward, selective_scan_fn
 
 
@@ -82,6 +83,11 @@ def _linear(x, weight, bias=None):
     if w16 is None or x.dtype != torch.bfloat16:
         return F.linear(x, weight, bias)
     return _Bf16Linear.apply(x, weight, w16)
+
+
+def _head_copy(w):
+    """The running SiftLM forward's bf16 copy of the head's fp32 weight (None without one)."""
+    return _W16.get(id(w)) if _W16 is not None and w.dtype == torch.float32 else None
 
 
 def _bf16_copies(weights, flat=None):
@@ -527,8 +533,26 @@ class SiftLM(nn.Module):
             return self(idx, targets)[1]
         # both flattened, as forward does: the targets may have any shape of as many tokens
         return self._run(idx, lambda h: linear_cross_entropy(
-            h.reshape(-1, h.shape[-1]), w, targets.reshape(-1),
-            weight16=_W16.get(id(w)) if _W16 is not None and w.dtype == torch.float32 else None))
+            h.reshape(-1, h.shape[-1]), w, targets.reshape(-1), weight16=_head_copy(w)))
+
+    def log_probs(self, idx, targets, top_k=0, temperature=1.0, ignore_index=-100):
+        """``linear_log_probs`` of targets (b, L) after idx (b, L): the tokens' log probabilities and the
+        entropy (both differentiable) and the top_k alternatives, without the logits."""
+        w = self._plain_head("log_probs")
+        return self._run(idx, lambda h: linear_log_probs(h, w, targets, top_k=top_k, temperature=temperature,
+                                                         ignore_index=ignore_index, weight16=_head_copy(w)))
+
+    def distillation_loss(self, idx, teacher_ids, teacher_logits, temperature=1.0):
+        """``linear_distillation`` of a teacher's top logits (b, L, K), for instance a larger model's
+        ``log_probs(idx, targets, top_k=K)``: the mean over the tokens that have any."""
+        w = self._plain_head("distillation_loss")
+        return self._run(idx, lambda h: linear_distillation(h, w, teacher_ids, teacher_logits, temperature=temperature,
+                                                            weight16=_head_copy(w)))
+
+    def _plain_head(self, what):
+        if self.lm_head.bias is not None:
+            raise ValueError(f"SiftLM.{what}: the head must not have a bias")
+        return self.lm_head.weight
 
     def _run(self, idx, head):
         """head(the final norm's output), with the bf16 weight copies of forward."""
@@ -570,11 +594,13 @@ class SiftLM(nn.Module):
         return _linear(self.backbone.norm_f(h), self.lm_head.weight, self.lm_head.bias)
 
     @torch.no_grad()
-    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, graphed=False):
+    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, graphed=False, log_probs=None):
         """The prompt ``idx`` (b, T) followed by ``max_new_tokens`` sampled tokens, produced
         through the recurrent step (the prompt is consumed token by token, then each new
         token is sampled from the last logits and fed back).  graphed=True replays each
-        step from one CUDA graph (GraphedStep)."""
+        step from one CUDA graph (GraphedStep).  log_probs=K (0 or more): also returns the
+        ``LogProbs`` of the new tokens (b, max_new_tokens) with their K top alternatives, under
+        the model's own softmax (before temperature and top_k)."""
         if graphed:
             stepper = GraphedStep(self, idx.shape[0], idx.device)
             advance = lambda tok: stepper(tok).clone()  # noqa: E731
@@ -584,13 +610,22 @@ class SiftLM(nn.Module):
         logits = None
         for tok in idx.unbind(1):
             logits = advance(tok)
-        out = [idx]
+        out, scores = [idx], []
         for i in range(max_new_tokens):
             tok = sample(logits, temperature, top_k)
             out.append(tok.unsqueeze(1))
+            if log_probs is not None:
+                scores.append(token_log_probs(logits, tok, top_k=log_probs))
             if i + 1 < max_new_tokens:          # the last token's logits are not needed
                 logits = advance(tok)
-        return torch.cat(out, dim=1)
+        out = torch.cat(out, dim=1)
+        if log_probs is None:
+            return out
+        if not scores:
+            none = out.new_empty((idx.shape[0], 0), dtype=torch.float32)
+            top = (none.new_empty((idx.shape[0], 0, log_probs)), out.new_empty((idx.shape[0], 0, log_probs))) if log_probs else (None, None)
+            return out, LogProbs(none, none.clone(), *top)
+        return out, LogProbs(*(torch.stack(t, 1) if t[0] is not None else None for t in zip(*scores)))
 
 
 class GraphedStep:
