@@ -43,8 +43,14 @@ enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW, XE_SCORE, XE_SCORE_TOP, XE_SCORE_A
 constexpr bool is_score(int epi) { return epi == XE_SCORE || epi == XE_SCORE_TOP || epi == XE_SCORE_ALL; }
 constexpr bool is_dlogit(int epi) { return epi == XE_PROB || epi == XE_GRAD; }
 constexpr bool is_logits(int epi) { return epi == XE_LSE || is_score(epi) || is_dlogit(epi); }
-constexpr float SCORE_FLOOR = -0x1.ffffcp127f;   // below (or at) every logit whose column takes its low 5 bits; its own are 0
+constexpr float SCORE_FLOOR = -0x1p73f;       // logits below it (-9e21; -inf) count as it: times log2(e) / temperature it stays finite
 constexpr float SCORE_FAR = -200.f;           // 2^-200 is 0: what lies further below the maximum adds nothing
+// max(v, SCORE_FLOOR) that keeps a NaN
+__device__ __forceinline__ float above_floor(float v) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(SCORE_FLOOR));
+    return r;
+}
 
 struct XentGemm {
     int M, N;                                 // rows and columns of the result
@@ -74,7 +80,9 @@ struct XentGemm {
     // XE_SCORE*, XE_GRAD: exponents are (logit - maximum) * k2, k2 = log2(e) / temperature
     float k2, inv_temp;
     float4* score;                            // (M, 2 nt): a tile half's maximum, sum of exponentials e, sum of e times its exponent
-    float2* rec; int64_t groups;              // XE_SCORE_TOP, (M, groups): the two largest logits of 32 columns, their low 5 bits the column
+    // XE_SCORE_TOP, (M, groups): the two largest logits of 32 columns, the column in place of their low 5 bits, and the third, the
+    // low 5 bits set or cleared
+    float2* rec; float* third; int64_t groups;
     float* all;                               // XE_SCORE_ALL, (M, N)
     // XE_GRAD: dlogit = 2^u (A + B u) + [column == target] hot, see grad_row
     const float* row_sum; const float* entropy; const float* d_logp; const float* d_entropy;
@@ -424,35 +432,42 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     }
                     if (cc + 32 > p.N) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : -INFINITY;
+                        for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : SCORE_FLOOR;
                     }
-                    float top = EPI == XE_SCORE_TOP ? SCORE_FLOOR : v[0];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = above_floor(v[j]);
+                    float top = SCORE_FLOOR;
                     if (EPI == XE_SCORE_TOP) {
-                        // the two largest, each with its column in place of its low bits (a NaN takes neither)
-                        float second = SCORE_FLOOR;
+                        // the three largest, each with its column in place of its low bits (a NaN takes no part)
+                        float second = SCORE_FLOOR, third = SCORE_FLOOR;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float t = __uint_as_float((__float_as_uint(fmaxf(v[j], SCORE_FLOOR)) & ~31u) | j);
-                            second = fmaxf(second, fminf(top, t));
+                            const float t = __uint_as_float((__float_as_uint(v[j]) & ~31u) | j);
+                            const float lo = fminf(top, t);
                             top = fmaxf(top, t);
+                            third = fmaxf(third, fminf(second, lo));
+                            second = fmaxf(second, lo);
                         }
-                        if (live && cc < p.N) p.rec[(int64_t)row * p.groups + cc / 32] = make_float2(top, second);
+                        if (live && cc < p.N) {
+                            p.rec[(int64_t)row * p.groups + cc / 32] = make_float2(top, second);
+                            p.third[(int64_t)row * p.groups + cc / 32] = third;
+                        }
                     } else {
 #pragma unroll
-                        for (int j = 1; j < 32; ++j) top = fmaxf(top, v[j]);
+                        for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
                     }
                     // sums relative to the larger maximum: e u becomes c e (u + shift)
                     const float nm = fmaxf(m, top);
-                    const float base = nm == -INFINITY ? 0.f : nm;      // nothing but -inf so far: the sums stay 0
-                    const float shift = fmaxf((m - base) * p.k2, SCORE_FAR), c2 = ex2(shift);
-                    esum = c2 * (esum + sum * shift);
-                    sum *= c2;
+                    const float shift = fmaxf((m - nm) * p.k2, SCORE_FAR), c2 = ex2(shift);
+                    float2 s2 = make_float2(sum * c2, 0.f), w2 = make_float2(c2 * (esum + sum * shift), 0.f);
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float u = (v[j] - base) * p.k2, e = ex2(u);
-                        sum += e;
-                        esum += e * fmaxf(u, SCORE_FAR);
+                    for (int j = 0; j < 32; j += 2) {
+                        const float2 u = mul2(add2(f2(v[j], v[j + 1]), bc2(-nm)), bc2(p.k2)), e = ex2x2(u);
+                        s2 = add2(s2, e);
+                        w2 = fma2(e, u, w2);
                     }
+                    sum = s2.x + s2.y;
+                    esum = w2.x + w2.y;
                     m = nm;
                 } else if (is_dlogit(EPI)) {
                     if (EPI == XE_GRAD) {

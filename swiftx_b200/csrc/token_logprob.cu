@@ -3,16 +3,16 @@
 //   log_probs = (z_y - m) / tau - ln s,  entropy = ln s - ln2 w / s.
 //
 // One pass over the logits, which bound it.  A row goes to a cluster of 1 to 8 CTAs (so that a few rows
-// reach many SMs, without a second launch); each walks its part in batches of 32 logits a thread with 16-byte loads, keeps
-// running statistics and streams the values past the threshold of the largest so far (topk.cuh).  The first CTA of the cluster
-// joins the parts through distributed shared memory.
+// reach many SMs, without a second launch); each thread walks its share of the CTA's part with 16-byte loads, four at a
+// time, with running statistics and nothing to wait for; the alternatives come out of the shares whose maxima are
+// large (topk.cuh).  The first CTA of the cluster joins the parts through distributed shared memory.
 #include "launch_util.cuh"
 #include "tc5.cuh"
 #include "topk.cuh"
 
 namespace swx {
 
-constexpr int TL_THREADS = 256, TL_PER = 32, TL_MAX_PARTS = 8;
+constexpr int TL_LOADS = 4, TL_PER = 8, TL_MAX_PARTS = 8;
 constexpr float TL_FAR = -200.f, TL_LN2 = 0.69314718055994531f;
 
 struct TokenRows {
@@ -34,79 +34,115 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
     return v;
 }
 
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRows p) {
+// Piece i of the row, N logits from column i N - shift on: -inf outside it.
+template <typename T, int N = 16 / sizeof(T)>
+__device__ __forceinline__ void load_piece(const T* z, int64_t V, int shift, int64_t i, float (&v)[N]) {
+    const int64_t c = i * N - shift;
+    if (c >= 0 && c + N <= V) {
+        const uint4 q = *reinterpret_cast<const uint4*>(z + c);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = Elem<T>::to_f(reinterpret_cast<const T*>(&q)[k]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = c + k >= 0 && c + k < V ? Elem<T>::to_f(z[c + k]) : -INFINITY;
+    }
+}
+
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS) token_logprob_kernel(const TokenRows p) {
     extern __shared__ __align__(16) uint8_t raw[];
-    __shared__ Score part[TL_THREADS / 32];
+    __shared__ Score part[THREADS / 32];
     __shared__ Score whole;
-    __shared__ int count, found;
+    __shared__ int count, found, owners[THREADS];
+    __shared__ uint32_t scratch[THREADS + 1];
     constexpr int N = 16 / sizeof(T);          // logits of a 16-byte load
     const int64_t row = blockIdx.x / p.parts;
     const int rank = blockIdx.x % p.parts, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const T* z = static_cast<const T*>(p.z) + row * p.stride;
-    uint64_t* buf = reinterpret_cast<uint64_t*>(raw);
-    uint64_t* kept = buf + topk_capacity(p.top, TL_PER);
-    TopK<TL_THREADS, TL_PER> best;
-    if (TOP) best.start(buf, kept, &count, p.top);
 
     // The row in 16-byte pieces counted from the last boundary at or before its start; the first and the last may be cut
     const int shift = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
     const int64_t pieces = (p.V + shift + N - 1) / N, per = (pieces + p.parts - 1) / p.parts;
-    const int64_t end = min(pieces, (rank + 1) * per);
+    const int64_t begin = rank * per, end = min(pieces, begin + per);
     Score a{-INFINITY, 0.f, 0.f};
-    for (int64_t i0 = rank * per; i0 < end; i0 += TL_THREADS * (TL_PER / N)) {
-        float v[TL_PER];
-        uint64_t key[TOP ? TL_PER : 1];
+    uint32_t most = 0;                         // the share's largest value as order_key bits
+    for (int64_t i0 = begin + threadIdx.x; i0 < end; i0 += TL_LOADS * THREADS) {
+        float v[TL_LOADS][N];
 #pragma unroll
-        for (int j = 0; j < TL_PER / N; ++j) {
-            const int64_t i = i0 + j * TL_THREADS + threadIdx.x, c = i * N - shift;
-            if (i < end && c >= 0 && c + N <= p.V) {
-                const uint4 q = *reinterpret_cast<const uint4*>(z + c);
+        for (int j = 0; j < TL_LOADS; ++j) {
+            if (i0 + j * THREADS < end) load_piece<T>(z, p.V, shift, i0 + j * THREADS, v[j]);
+            else {
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    v[j * N + k] = Elem<T>::to_f(reinterpret_cast<const T*>(&q)[k]);
-                    if (TOP) key[j * N + k] = index_key(order_key(v[j * N + k]), (uint32_t)(c + k));
-                }
-            } else {
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const bool in = i < end && c + k >= 0 && c + k < p.V;
-                    v[j * N + k] = in ? Elem<T>::to_f(z[c + k]) : -INFINITY;
-                    if (TOP) key[j * N + k] = in ? index_key(order_key(v[j * N + k]), (uint32_t)(c + k)) : 0;
-                }
+                for (int k = 0; k < N; ++k) v[j][k] = -INFINITY;
             }
         }
         float nm = a.m;
 #pragma unroll
-        for (int j = 0; j < TL_PER; ++j) nm = fmaxf(nm, v[j]);
+        for (int j = 0; j < TL_LOADS; ++j)
+#pragma unroll
+            for (int k = 0; k < N; ++k) nm = fmaxf(nm, v[j][k]);
         const float base = nm == -INFINITY ? 0.f : nm;                   // nothing but -inf so far: the sums stay 0
         const float da = fmaxf((a.m - base) * p.k2, TL_FAR), ca = ex2(da);
-        a.w = ca * (a.w + a.s * da);
-        a.s *= ca;
+        float2 s = make_float2(ca * a.s, 0.f), w = make_float2(ca * (a.w + a.s * da), 0.f);
         a.m = nm;
 #pragma unroll
-        for (int j = 0; j < TL_PER; ++j) {
-            const float u = (v[j] - base) * p.k2, e = ex2(u);
-            a.s += e;
-            a.w += e * fmaxf(u, TL_FAR);
-        }
-        if constexpr (TOP) best.push(key);
+        for (int j = 0; j < TL_LOADS; ++j)
+#pragma unroll
+            for (int k = 0; k < N; k += 2) {
+                const float2 u = mul2(add2(f2(v[j][k], v[j][k + 1]), bc2(-base)), bc2(p.k2)), e = ex2x2(u);
+                s = add2(s, e);
+                w = fma2(e, f2(fmaxf(u.x, TL_FAR), fmaxf(u.y, TL_FAR)), w);
+            }
+        a.s = s.x + s.y;
+        a.w = w.x + w.y;
     }
+    if (TOP) most = begin + threadIdx.x < end ? order_key(a.m) : 0;
+    const bool odd = a.s != a.s;               // a NaN or +inf in the share
     score_join_warp(a, p.k2, TL_FAR);
     if (lane == 0) part[warp] = a;
-    if (TOP) best.rank();
+    uint64_t* buf = reinterpret_cast<uint64_t*>(raw);
+    TopK<THREADS, TL_PER> best{};
+    if constexpr (TOP) {
+        best.start(buf, buf + topk_capacity(p.top, TL_PER), &count, p.top);
+        auto item = [&](int t, int64_t j, auto f) {
+            const int64_t i = begin + t + j * THREADS, c = i * N - shift;
+            if (i >= end) return;
+            float v[N];
+            load_piece<T>(z, p.V, shift, i, v);
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (c + k >= 0 && c + k < p.V) f(v[k], (uint32_t)(c + k));
+        };
+        if (__syncthreads_or(odd) || !best.gather(most, scratch, owners, (per + THREADS - 1) / THREADS, item)) {
+            best.clear();
+            for (int64_t i0 = begin; i0 < end; i0 += THREADS * (TL_PER / N)) {
+                uint64_t key[TL_PER];
+#pragma unroll
+                for (int j = 0; j < TL_PER / N; ++j) {
+                    const int64_t i = i0 + j * THREADS + threadIdx.x, c = i * N - shift;
+                    float v[N];
+                    if (i < end) load_piece<T>(z, p.V, shift, i, v);
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+                        key[j * N + k] = i < end && c + k >= 0 && c + k < p.V ? index_key(order_key(v[k]), (uint32_t)(c + k)) : 0;
+                }
+                best.push(key);
+            }
+        }
+        best.rank();
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
         a = part[0];
-        for (int i = 1; i < TL_THREADS / 32; ++i) score_join(a, part[i], p.k2, TL_FAR);
+        for (int i = 1; i < THREADS / 32; ++i) score_join(a, part[i], p.k2, TL_FAR);
         whole = a;
         if (TOP) found = best.n;
     }
     __syncthreads();
+    a = whole;
     if (p.parts > 1) {
         cluster_sync_all();
         if (rank == 0) {
-            a = whole;
             for (int r = 1; r < p.parts; ++r) {
                 const uint32_t o = map_to_rank(&whole, r);
                 score_join(a, Score{ld_cluster_f32(o), ld_cluster_f32(o + 4), ld_cluster_f32(o + 8)}, p.k2, TL_FAR);
@@ -115,7 +151,7 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRo
                 for (int r = 1; r < p.parts; ++r) {
                     const int n = __float_as_int(ld_cluster_f32(map_to_rank(&found, r)));
                     const uint32_t from = map_to_rank(buf, r);
-                    for (int i = threadIdx.x; i < n; i += TL_THREADS) buf[best.n + i] = ld_cluster_u64(from + 8 * i);
+                    for (int i = threadIdx.x; i < n; i += THREADS) buf[best.n + i] = ld_cluster_u64(from + 8 * i);
                     best.n += n;
                 }
                 __syncthreads();
@@ -124,8 +160,6 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRo
         }
         cluster_sync_all();                    // no CTA goes while the first still reads its shared memory
         if (rank != 0) return;
-    } else {
-        a = whole;
     }
     const float ls = logf(a.s);
     const int64_t y = p.target ? p.target[row] : 0;
@@ -136,7 +170,7 @@ __global__ void __launch_bounds__(TL_THREADS) token_logprob_kernel(const TokenRo
         p.entropy[row] = live ? ls - TL_LN2 * a.w / a.s : 0.f;
     }
     if (TOP) {
-        for (int i = threadIdx.x; i < p.top; i += TL_THREADS) {
+        for (int i = threadIdx.x; i < p.top; i += THREADS) {
             const uint64_t k = best.buf[i];
             p.top_log_probs[row * p.top + i] = live ? (order_value((uint32_t)(k >> 32)) - a.m) * p.inv_temp - ls : 0.f;
             p.top_ids[row * p.top + i] = live ? (int64_t)key_index(k) : -1;
@@ -151,9 +185,9 @@ static int token_parts(int64_t rows, int64_t V) {
     return parts;
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, int THREADS>
 static cudaError_t launch_token(const TokenRows& p, int64_t rows, cudaStream_t st) {
-    auto k = token_logprob_kernel<T, TOP>;
+    auto k = token_logprob_kernel<T, TOP, THREADS>;
     const size_t smem = TOP ? (size_t)(topk_capacity(p.top, TL_PER) + p.top) * 8 : 0;
     if (TOP) {
         const cudaError_t e = allow_smem(k, (topk_capacity(SWX_MAX_TOP, TL_PER) + SWX_MAX_TOP) * 8);
@@ -161,7 +195,7 @@ static cudaError_t launch_token(const TokenRows& p, int64_t rows, cudaStream_t s
     }
     cudaLaunchConfig_t c{};
     c.gridDim = dim3((unsigned)(rows * p.parts));
-    c.blockDim = dim3(TL_THREADS);
+    c.blockDim = dim3(THREADS);
     c.dynamicSmemBytes = smem;
     c.stream = st;
     cudaLaunchAttribute at{};
@@ -171,6 +205,13 @@ static cudaError_t launch_token(const TokenRows& p, int64_t rows, cudaStream_t s
     c.attrs = &at;
     c.numAttrs = 1;
     return cudaLaunchKernelEx(&c, k, p);
+}
+
+// Short rows take small CTAs (more rows at a time; at least as many threads as alternatives).
+template <typename T, bool TOP>
+static cudaError_t launch_token(const TokenRows& p, int64_t rows, cudaStream_t st) {
+    if (p.V * (int64_t)sizeof(T) <= 8192 && p.top <= 64) return launch_token<T, TOP, 64>(p, rows, st);
+    return launch_token<T, TOP, 256>(p, rows, st);
 }
 
 }  // namespace swx

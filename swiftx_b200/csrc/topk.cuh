@@ -1,6 +1,11 @@
-// The K largest of a long row, by one CTA: 64-bit keys (a value's order-preserving bits above the
-// complement of its index, so that no two are equal and ties go to the lowest index) are streamed past a threshold that
-// never exceeds the K-th largest; what passes is gathered in shared memory and ranked at the end.
+// The K largest of a long row, by one CTA.  A key is a value's order-preserving bits above the complement of its
+// index, so that no two are equal and ties go to the lowest index.
+//
+// After a pass in which each thread has kept the largest value of its share, the K-th largest of those maxima is a threshold
+// that at least K values reach, and only the threads whose maximum does have any: their shares (K of them, few
+// hundred values) are read again, and the keys that pass, little more than K as a rule, are gathered in shared memory and ranked.
+// Where too many pass (many equal values, or large ones gathered in few shares) the whole row is streamed past a rising
+// threshold in bounded batches instead (TopK::push), slower and for any order.
 #pragma once
 #include "common.cuh"
 
@@ -22,6 +27,40 @@ __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k;
 // Entries that TopK's buffer holds for `k` and `per` keys a thread: what is kept, and a batch's passers.
 constexpr int topk_capacity(int k, int per) { return k * (per + 1); }
 
+// Finds the k-th largest of the THREADS threads' values, as order_key bits, by one warp: the bits are set from the top while at
+// least k values stay no smaller, over those that differ.  scratch: THREADS + 1 words; all threads call it.
+template <int THREADS>
+__device__ __forceinline__ uint32_t kth_largest(uint32_t mine, int k, uint32_t* scratch) {
+    scratch[threadIdx.x] = mine;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        constexpr int N = THREADS / 32;
+        uint32_t v[N], lo = ~0u, hi = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[j] = scratch[threadIdx.x + 32 * j];
+            lo = min(lo, v[j]);
+            hi = max(hi, v[j]);
+        }
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        const int top = 32 - __clz(lo ^ hi);                   // bits from here up are common
+        uint32_t t = top == 32 ? 0 : hi >> top << top;
+        for (int b = top - 1; b >= 0; --b) {
+            const uint32_t c = t | 1u << b;
+            int n = 0;
+#pragma unroll
+            for (int j = 0; j < N; ++j) n += v[j] >= c;
+            n = __reduce_add_sync(0xffffffffu, n);
+            if (n >= k) t = c;
+            if (n == k) break;
+        }
+        if (threadIdx.x == 0) scratch[THREADS] = t;
+    }
+    __syncthreads();
+    return scratch[THREADS];
+}
+
 // All threads of the CTA (THREADS >= k) call every member together.  A batch is PER keys for each thread, 0 for none.
 template <int THREADS, int PER>
 struct TopK {
@@ -32,9 +71,45 @@ struct TopK {
     uint64_t floor;                           // every key of the k largest so far is at least this
 
     __device__ __forceinline__ void start(uint64_t* buf_, uint64_t* kept_, int* count_, int k_) {
-        buf = buf_; kept = kept_; count = count_; k = k_; n = 0; floor = 1;
+        buf = buf_; kept = kept_; count = count_; k = k_;
+        clear();
+    }
+    __device__ __forceinline__ void clear() {
+        n = 0;
+        floor = 1;
+        __syncthreads();
         if (threadIdx.x == 0) *count = 0;
         __syncthreads();
+    }
+    // One key, by any thread: dropped, but counted, where the buffer is full.
+    __device__ __forceinline__ void add(uint64_t key) {
+        const int at = atomicAdd(count, 1);
+        if (at < topk_capacity(k, PER)) buf[at] = key;
+    }
+    // After the threads' adds: whether all of them found room.
+    __device__ __forceinline__ bool added() {
+        __syncthreads();
+        n = *count;
+        return n <= topk_capacity(k, PER);
+    }
+    // The keys that reach the threshold, from the shares of the threads whose maximum does: item(t, j, f) calls f(value,
+    // index) on entry j < per of thread t's share.  False where they were too many.
+    template <class Item>
+    __device__ __forceinline__ bool gather(uint32_t mine, uint32_t* scratch, int* owners, int64_t per, Item item) {
+        const uint32_t t = kth_largest<THREADS>(mine, k, scratch);
+        if (mine >= t) owners[atomicAdd(count, 1)] = threadIdx.x;
+        __syncthreads();
+        const int m = *count;
+        __syncthreads();
+        if (threadIdx.x == 0) *count = 0;
+        __syncthreads();
+        const uint32_t one = (uint32_t)per;
+        for (uint32_t i = threadIdx.x; i < m * one; i += THREADS)
+            item(owners[i / one], (int64_t)(i % one), [&](float v, uint32_t index) {
+                const uint32_t o = order_key(v);
+                if (o >= t) add(index_key(o, index));
+            });
+        return added();
     }
     // The k-th largest of the threads' largest keys: at least k keys are no smaller.  The bits are found from the top; the keys
     // differ, so the search ends as soon as exactly k threads pass.

@@ -187,6 +187,22 @@ def test_equal_logits_go_to_the_lowest_word(dtype, V):
     assert torch.equal(out.top_ids[7], torch.arange(top, device=DEV))
 
 
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_large_logits_gathered_in_few_groups(dtype):
+    """Groups of 32 words go round 128 threads: the largest logits all in the groups of four of them; rows of a few values."""
+    T, V, d = 4, 100000, 8
+    x, w, y = _inputs(T, V, d, dtype, seed=13, ignored=0)
+    group = torch.arange(V, device=DEV) // 32
+    x[:, 0] = 1.0
+    w[:, 0] = torch.where(group % 128 < 4, 40.0, 0.0)
+    w[:, 1] = 0
+    for top in (1, 3, 60, 128):
+        _check_forward(linear_log_probs(x, w, y, top_k=top), x, w, y, 1.0, top)
+    x[1:] = 0
+    x[1:, 0] = 1.0                                                        # 12512 words alike
+    _check_forward(linear_log_probs(x, w, y, top_k=9), x, w, y, 1.0, 9)
+
+
 def test_close_logits_are_ordered_exactly():
     """Words whose logits differ by a 2^-26th, far below what an fp32 sum tells apart."""
     d, V, top = 64, 4001, 24
@@ -388,11 +404,17 @@ def test_tokens_in_hard_orders():
                         torch.where(torch.arange(V, device=DEV) < V - 50, 0.0, 1.0), -torch.zeros(V, device=DEV)])
     rows[6, ::2] = 0.0                                                    # zeros of either sign are equal
     y = torch.arange(7, device=DEV)
+    # large values in the shares of few threads (16-byte pieces go round 256 threads), in falling and rising order
+    heavy = torch.where(torch.arange(V, device=DEV) // 4 % 256 < 10, 1000 + up, up)
+    rows = torch.cat([rows, heavy[None], (heavy.max() - heavy)[None], torch.where(heavy > 1000, 5.0, up)[None]])
+    y = torch.arange(10, device=DEV)
     for n in (V, V - 1, 9000):
         z = rows[:, :n]
         _check_tokens(z, y, top, 1.0, token_log_probs(z, y, top_k=top))
     many = rows.repeat(60, 1)                                             # one CTA for each row
     _check_tokens(many, y.repeat(60), top, 1.0, token_log_probs(many, y.repeat(60), top_k=top))
+    _check_tokens(rows[:, :2048], y, 64, 1.0, token_log_probs(rows[:, :2048], y, top_k=64))        # the smaller CTAs
+    _check_tokens(rows[:, :2047], y, 2, 1.0, token_log_probs(rows[:, :2047], y, top_k=2))
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
