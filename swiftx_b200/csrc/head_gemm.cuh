@@ -13,6 +13,7 @@
 #include "launch_util.cuh"
 #include "tc5.cuh"
 #include "tma_util.cuh"
+#include "topk.cuh"
 
 namespace swx {
 
@@ -43,12 +44,10 @@ enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW, XE_SCORE, XE_SCORE_TOP, XE_SCORE_A
 constexpr bool is_score(int epi) { return epi == XE_SCORE || epi == XE_SCORE_TOP || epi == XE_SCORE_ALL; }
 constexpr bool is_dlogit(int epi) { return epi == XE_PROB || epi == XE_GRAD; }
 constexpr bool is_logits(int epi) { return epi == XE_LSE || is_score(epi) || is_dlogit(epi); }
-constexpr float SCORE_FLOOR = -0x1p73f;       // logits below it (-9e21; -inf) count as it: times log2(e) / temperature it stays finite
-constexpr float SCORE_FAR = -200.f;           // 2^-200 is 0: what lies further below the maximum adds nothing
-// max(v, SCORE_FLOOR) that keeps a NaN
-__device__ __forceinline__ float above_floor(float v) {
+constexpr float SCORE_FLOOR = -0x1p73f;       // below every logit that counts (-9e21): times log2(e) / temperature it stays finite
+__device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(v), "f"(SCORE_FLOOR));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 
@@ -67,7 +66,7 @@ struct XentGemm {
     int col0;                                 // vocabulary index of column 0
     float2* part;                             // (2 nt, M): max and sum of a tile half's exponentials
     float* hit;                               // (M): the target's logit
-    int* counter;                             // zeroed by XE_LSE for the joining kernel
+    int* counter;                             // zeroed by the forward epilogues (where given) for the kernel after them
     const float* row_max; const float* row_rsum;
     const float* dloss; int reduction;
     int planes;                               // bf16 pieces of the dlogit
@@ -77,12 +76,13 @@ struct XentGemm {
     int spread;
     float* acc; void* out; int out_bf16; int64_t ld; int first, last;
     const float* scale_num; const float* scale_den;   // the result's factor: num / den, either may be absent
-    // XE_SCORE*, XE_GRAD: exponents are (logit - maximum) * k2, k2 = log2(e) / temperature
+    // XE_SCORE*, XE_GRAD: exponents are logit * k2 - m, k2 = log2(e) / temperature, m the largest logit times k2 (rounded once, so
+    // that an exponent is one fused operation, off by its own rounding)
     float k2, inv_temp;
-    float4* score;                            // (M, 2 nt): a tile half's maximum, sum of exponentials e, sum of e times its exponent
-    // XE_SCORE_TOP, (M, groups): the two largest logits of 32 columns, the column in place of their low 5 bits, and the third, the
-    // low 5 bits set or cleared
-    float2* rec; float* third; int64_t groups;
+    float4* score;                            // (M, 2 nt): a tile half's m, sum of exponentials e, sum of e times its exponent
+    // XE_SCORE_TOP, (M, 16 nt): the largest logit of 16 columns, and the second with the largest one's column in place of its
+    // low 4 bits; columns from N on count as SCORE_FLOOR
+    float* largest; float* runner_up;
     float* all;                               // XE_SCORE_ALL, (M, N)
     // XE_GRAD: dlogit = 2^u (A + B u) + [column == target] hot, see grad_row
     const float* row_sum; const float* entropy; const float* d_logp; const float* d_entropy;
@@ -163,7 +163,7 @@ __device__ __forceinline__ float row_scale(const XentGemm& p, int row) {
     return p.reduction == SWX_XENT_NONE ? p.dloss[row] : 1.f;
 }
 
-// A row's coefficients of XE_GRAD.  With u = (z - max) k2, e = 2^u, s the sum of e: p = e / s, the log probability
+// A row's coefficients of XE_GRAD.  With u = z k2 - m, e = 2^u, s the sum of e: p = e / s, the log probability
 // l = u ln2 - ln s, and for upstream gradients g of the target's log probability and h of the entropy H
 //   dz = (g [v == y] - p (g + h (l + H))) / temperature = e (A + B u) + [v == y] hot.
 // Distillation (no targets): dz = p c / temperature with c = temperature^2 times the row's upstream gradient; the
@@ -262,7 +262,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
         for (int s = 0; s < XE_STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(&acc_full[a], 1); mbar_init(&acc_empty[a], 2 * XE_EPI_WARPS); }
         mbar_fence_init();
-        if ((EPI == XE_LSE || (EPI == XE_SCORE && p.counter)) && blockIdx.x == 0) *p.counter = 0;
+        if ((EPI == XE_LSE || (is_score(EPI) && p.counter)) && blockIdx.x == 0) *p.counter = 0;
     }
     if (warp == 1) tmem_alloc_pair(&tmem_base, 512);
     tc_fence_before();
@@ -389,6 +389,21 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             const uint32_t at = tmem + ((uint32_t)(sub * 32) << 16) + a * XE_TILE + half * 128;
             // 32 columns of the row, from 32 c on
             float m = -INFINITY, sum = 0.f, esum = 0.f;
+            float* groups = reinterpret_cast<float*>(so) + lane * 20;   // XE_SCORE_TOP: the 8 groups' largest and second logits
+            // what the scoring keeps of this half of the tile (after the accumulator is given back: the stores need not be
+            // waited for then)
+            auto keep = [&] {
+                if (!is_score(EPI) || !live) return;
+                const int64_t at = (int64_t)row * 2 * p.nt + 2 * rc.y + half;
+                p.score[at] = make_float4(m, sum, esum, 0.f);
+                if (EPI == XE_SCORE_TOP) {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        reinterpret_cast<float4*>(p.largest)[2 * at + i] = reinterpret_cast<const float4*>(groups)[i];
+                        reinterpret_cast<float4*>(p.runner_up)[2 * at + i] = reinterpret_cast<const float4*>(groups)[2 + i];
+                    }
+                }
+            };
             auto columns = [&](int c, float (&v)[32]) {
                 const int cc = c0 + c * 32;                 // first of these 32 columns
                 const int64_t yc = y - cc;
@@ -434,46 +449,57 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : SCORE_FLOOR;
                     }
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = above_floor(v[j]);
                     float top = SCORE_FLOOR;
-                    if (EPI == XE_SCORE_TOP) {
-                        // the three largest, each with its column in place of its low bits (a NaN takes no part)
-                        float second = SCORE_FLOOR, third = SCORE_FLOOR;
+                    if constexpr (EPI == XE_SCORE_TOP) {
+                        // the two largest of either half, with their columns in place of their low bits, and the largest as it
+                        // is (-inf, which the column makes a NaN, and a NaN take no part)
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float t = __uint_as_float((__float_as_uint(v[j]) & ~31u) | j);
-                            const float lo = fminf(top, t);
-                            top = fmaxf(top, t);
-                            third = fmaxf(third, fminf(second, lo));
-                            second = fmaxf(second, lo);
-                        }
-                        if (live && cc < p.N) {
-                            p.rec[(int64_t)row * p.groups + cc / 32] = make_float2(top, second);
-                            p.third[(int64_t)row * p.groups + cc / 32] = third;
+                        for (int g = 0; g < 2; ++g) {
+                            float t1 = SCORE_FLOOR, t2 = SCORE_FLOOR, most = SCORE_FLOOR;
+#pragma unroll
+                            for (int j = 0; j < 16; j += 2) {
+                                const float x0 = v[16 * g + j], x1 = v[16 * g + j + 1];
+                                const float p0 = __uint_as_float((__float_as_uint(x0) & ~15u) | j), p1 = __uint_as_float((__float_as_uint(x1) & ~15u) | (j + 1));
+                                const float hi = fmaxf(p0, p1), lo = fminf(p0, p1);
+                                t2 = max3(t2, fminf(t1, hi), lo);
+                                t1 = fmaxf(t1, hi);
+                                most = max3(most, x0, x1);
+                            }
+                            groups[2 * c + g] = most;
+                            groups[8 + 2 * c + g] = __uint_as_float((__float_as_uint(t2) & ~15u) | (__float_as_uint(t1) & 15u));
+                            top = fmaxf(top, most);
                         }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) top = fmaxf(top, v[j]);
+                        for (int j = 0; j < 32; j += 2) top = max3(top, v[j], v[j + 1]);
                     }
                     // sums relative to the larger maximum: e u becomes c e (u + shift)
-                    const float nm = fmaxf(m, top);
-                    const float shift = fmaxf((m - nm) * p.k2, SCORE_FAR), c2 = ex2(shift);
-                    float2 s2 = make_float2(sum * c2, 0.f), w2 = make_float2(c2 * (esum + sum * shift), 0.f);
+                    const float nm = fmaxf(m, top * p.k2);
+                    const float shift = fmaxf(m - nm, SCORE_FAR), c2 = ex2(shift);
+                    const float s0 = sum * c2, w0 = c2 * (esum + sum * shift);
+                    float2 s2 = make_float2(s0, 0.f), w2 = make_float2(w0, 0.f);
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        const float2 u = mul2(add2(f2(v[j], v[j + 1]), bc2(-nm)), bc2(p.k2)), e = ex2x2(u);
+                        const float2 u = fma2(f2(v[j], v[j + 1]), bc2(p.k2), bc2(-nm)), e = ex2x2(u);
                         s2 = add2(s2, e);
                         w2 = fma2(e, u, w2);
                     }
                     sum = s2.x + s2.y;
                     esum = w2.x + w2.y;
+                    if (esum != esum) {                     // 0 times -inf: those terms are 0
+                        esum = w0;
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float u = fmaf(v[j], p.k2, -nm);
+                            esum += ex2(u) * fmaxf(u, SCORE_FAR);
+                        }
+                    }
                     m = nm;
                 } else if (is_dlogit(EPI)) {
                     if (EPI == XE_GRAD) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float u = (v[j] - rmax) * p.k2;
+                            const float u = fmaf(v[j], p.k2, -rmax);
                             v[j] = ex2(u) * fmaf(gr.B, fmaxf(u, SCORE_FAR), gr.A);
                         }
                     } else {
@@ -542,7 +568,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
 #pragma unroll
                 for (int c = 0; c < 4; ++c) columns(c, tot[c]);
                 if (EPI == XE_LSE && live) p.part[(int64_t)(2 * rc.y + half) * p.M + row] = make_float2(m, sum);
-                if (is_score(EPI) && live) p.score[(int64_t)row * 2 * p.nt + 2 * rc.y + half] = make_float4(m, sum, esum, 0.f);
+                keep();
                 continue;
             }
 #pragma unroll 1
@@ -553,11 +579,11 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                 columns(c, v);
             }
             if (EPI == XE_LSE && live) p.part[(int64_t)(2 * rc.y + half) * p.M + row] = make_float2(m, sum);
-            if (is_score(EPI) && live) p.score[(int64_t)row * 2 * p.nt + 2 * rc.y + half] = make_float4(m, sum, esum, 0.f);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_rank(&acc_empty[a], 0));
             if ((a ^= 1) == 0) aph ^= 1;
+            keep();
         }
         if (is_dlogit(EPI) && lane == 0) bulk_wait_all();
         if (!ok && lane == 0 && p.status) *p.status = SWX_ERR_TIMEOUT;

@@ -9,7 +9,6 @@
 // loss's, with tau p in the epilogue, and the teacher's words set to tau (p_j - q_j) by a small kernel
 // between a piece of the vocabulary's dlogit and its products, each rounded once.
 #include "head_gemm.cuh"
-#include "topk.cuh"
 
 namespace swx {
 
@@ -98,13 +97,7 @@ __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillR
     __shared__ double red[DI_WARPS][2];
     const int64_t row = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    Score a{-INFINITY, 0.f, 0.f};
-    for (int i = threadIdx.x; i < p.np; i += DI_THREADS) {
-        const float4 s = p.score[row * p.np + i];
-        score_join(a, Score{s.x, s.y, s.z}, p.k2, SCORE_FAR);
-    }
-    score_join_warp(a, p.k2, SCORE_FAR);
-    if (lane == 0) part[warp] = a;
+    const Score a = score_join_row<DI_THREADS>(p.score + row * p.np, p.np, part);
     float q[DI_LANE];
     int64_t id[DI_LANE];
     bool live = false, bad = false;
@@ -125,14 +118,11 @@ __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillR
     __syncthreads();
     double sum = 0., n = 0.;
     if (warp == 0) {
-        a = part[0];
-#pragma unroll
-        for (int i = 1; i < DI_WARPS; ++i) score_join(a, part[i], p.k2, SCORE_FAR);
         const float ls = logf(a.s);
         float loss = 0.f;
 #pragma unroll
         for (int i = 0; i < DI_LANE; ++i)
-            if (lane + 32 * i < p.K && id[i] >= 0 && !bad && q[i] != 0.f) loss += q[i] * (logf(q[i]) - ((sz[lane + 32 * i] - a.m) * p.inv_temp - ls));
+            if (lane + 32 * i < p.K && id[i] >= 0 && !bad && q[i] != 0.f) loss += q[i] * (logf(q[i]) - (fmaf(sz[lane + 32 * i], p.k2, -a.m) * 0.69314718055994531f - ls));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
         loss = bad ? __int_as_float(0x7fc00000) : loss / (p.inv_temp * p.inv_temp);
@@ -202,7 +192,7 @@ __global__ void __launch_bounds__(32 * DI_PATCH_WARPS) distill_patch_kernel(cons
     for (int i = 0; i < DI_LANE; ++i) {
         const int j = lane + 32 * i;
         if (j >= p.K || id[i] < p.c0 || id[i] >= p.c0 + p.cw || !first[i]) continue;
-        float v = c * (ex2((p.z[row * p.K + j] - m) * p.k2) / s - all[i]);
+        float v = c * (ex2(fmaf(p.z[row * p.K + j], p.k2, -m)) / s - all[i]);
         __nv_bfloat16* o = p.dz + row * p.ld + (id[i] - p.c0);
         for (int k = 0; k < p.planes; ++k) {
             const __nv_bfloat16 b = __float2bfloat16_rn(v);
@@ -243,7 +233,7 @@ static int distill_check(const swx_distill_args* a) {
 static DistillRows distill_rows(const swx_distill_args* a) {
     DistillRows p{};
     p.T = a->tokens; p.V = a->vocab; p.d = a->dim; p.K = (int)a->entries;
-    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E * p.inv_temp;
+    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E / a->temperature;
     p.ids = a->teacher_ids; p.ids_sr = a->ids_sr; p.logits = a->teacher_logits; p.tl_sr = a->tl_sr;
     p.tl_bf16 = a->teacher_dtype == SWX_DTYPE_BF16;
     p.row_max = a->row_max; p.row_sum = a->row_sum; p.z = a->entry_logits; p.reduction = a->reduction;

@@ -5,21 +5,22 @@
 //   dz_v = (g [v == y] - p_v (g + h (l_v + H))) / tau,  dx = dz W,  dW = dz^T x.
 //
 // Forward: the head's product (head_gemm.cuh) with an epilogue that keeps three floats for each half of a 256-column tile: the
-// maximum m, s = sum e and w = sum e u of e = 2^u, u = (z - m) log2(e) / tau; with alternatives also the three largest logits of every
-// 32 columns (12 bytes), or, for a small vocabulary, the logits.  Then one kernel for the rows: the statistics joined, and
+// maximum m (of z log2(e) / tau), s = sum e and w = sum e u of e = 2^u, u = z log2(e) / tau - m; with alternatives also the two largest logits of every
+// 16 columns (8 bytes), or, for a small vocabulary, the logits.  Then one kernel for the rows: the statistics joined, and
 //   H = ln s - ln2 w / s.
-// Alternatives: the K + 8 groups of 32 columns with the largest maxima hold the K + 8 largest logits; a group whose second value
-// passes too gives two, one whose third does is taken whole.  The tensor core's sums are a few 2^-23 off and the records hold 18
-// bits, enough to turn two close logits round, so the candidates' products are formed again from the operands: in
-// fp32, with a bound of the error, and those that the bound does not tell apart from another exactly.
+// Alternatives: the K + 4 groups of 16 columns with the largest maxima hold the K + 4 largest logits; a group whose second value
+// passes too is taken whole.  The tensor core's sums are a few 2^-23 off, enough to turn two close logits round.  So where two
+// candidates are closer than a bound of that error (from the norms of the row and of the longest word, or unknown where few rows do not
+// pay for reading the words' norms), their products are formed again with a bound of their own, and those that are still
+// too close exactly.
 //
 // Backward: as the loss's, with dz in the epilogue (rounded to bf16 once, the tensor core's operand; fp32 operands: three pieces).
 #include "head_gemm.cuh"
-#include "topk.cuh"
+#include "warp_mma.cuh"
 
 namespace swx {
 
-constexpr int SC_EXTRA = 8;                   // candidates beyond K
+constexpr int SC_EXTRA = 4;                   // candidates beyond K
 constexpr int SC_THREADS = 256, SC_PER = 8;
 constexpr float LN2 = 0.69314718055994531f;
 
@@ -27,12 +28,13 @@ struct ScoreRows {
     int64_t T, V, d;
     int np;                                   // statistics per row
     const float4* score; const float* hit; const int64_t* target; int64_t ignore;
-    float k2, inv_temp;
+    float k2;
     float* row_max; float* row_sum; float* log_probs; float* entropy;
     // alternatives
     int top, cand;                            // K, candidates kept of the records
-    const float2* rec; const float* third; const float* all; int64_t groups;
+    const float* largest; const float* runner_up; const float* all; int64_t groups, stride;
     const void* x; int64_t x_sr; const void* w; int64_t w_sr; int vec;
+    const uint32_t* longest;                  // the largest squared norm of a word, its bits; or none
     float* top_log_probs; int64_t* top_ids;
 };
 
@@ -42,7 +44,7 @@ __device__ __forceinline__ void score_finish(const ScoreRows& p, int64_t row, co
     const float ls = logf(a.s);
     if (p.row_max) { p.row_max[row] = a.m; p.row_sum[row] = a.s; }
     const bool live = y != p.ignore;
-    p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? (p.hit[row] - a.m) * p.inv_temp - ls : __int_as_float(0x7fc00000);
+    p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? fmaf(p.hit[row], p.k2, -a.m) * LN2 - ls : __int_as_float(0x7fc00000);
     p.entropy[row] = live ? ls - LN2 * a.w / a.s : 0.f;
 }
 
@@ -51,12 +53,7 @@ __global__ void __launch_bounds__(SC_THREADS) score_rows_kernel(const ScoreRows 
     const int64_t row = (int64_t)blockIdx.x * (SC_THREADS / 32) + threadIdx.x / 32;
     if (row >= p.T) return;
     const int lane = threadIdx.x % 32;
-    Score a{-INFINITY, 0.f, 0.f};
-    for (int i = lane; i < p.np; i += 32) {
-        const float4 q = p.score[row * p.np + i];
-        score_join(a, Score{q.x, q.y, q.z}, p.k2, SCORE_FAR);
-    }
-    score_join_warp(a, p.k2, SCORE_FAR);
+    const Score a = score_join_parts(p.score + row * p.np, p.np, lane, 32);
     if (lane == 0) score_finish(p, row, a);
 }
 
@@ -71,103 +68,225 @@ __device__ __forceinline__ void unpack(const __nv_bfloat16*, const uint4& q, flo
     v[0] = bf16_pair(q.x); v[1] = bf16_pair(q.y); v[2] = bf16_pair(q.z); v[3] = bf16_pair(q.w);
 }
 
-// Products of a row of x with two rows of the weight over a warp, in fp32: z, and a bound of each one's error.  A lane sums d / 64
+// Products of a row of x with R rows of the weight over a warp, in fp32: z, and a bound of each one's error.  A lane sums d / 64
 // products in each of two chains, which are joined in six steps, 2^-24 of the magnitudes each; |x| |w| bounds those.
-struct Product2 { float z[2], e[2]; };
+constexpr int SC_DOTS = 4;
+struct Products { float z[SC_DOTS], e[SC_DOTS]; };
 template <typename T>
-__device__ __forceinline__ Product2 product2(const T* x, const T* w0, const T* w1, int64_t d, bool vec, int lane) {
+__device__ __forceinline__ Products products(const T* x, const T* const (&w)[SC_DOTS], int64_t d, bool vec, int lane) {
     constexpr int N = 16 / sizeof(T);
-    float2 a[2] = {}, n[3] = {};
+    float2 a[SC_DOTS] = {}, n[SC_DOTS + 1] = {};
     int64_t tail = 0;
     if (vec) {
-#pragma unroll 4
+#pragma unroll 2
         for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
-            float2 xv[N / 2], v0[N / 2], v1[N / 2];
-            unpack(x, *reinterpret_cast<const uint4*>(x + k), xv);
-            unpack(x, *reinterpret_cast<const uint4*>(w0 + k), v0);
-            unpack(x, *reinterpret_cast<const uint4*>(w1 + k), v1);
+            const uint4 qx = *reinterpret_cast<const uint4*>(x + k);
+            uint4 q[SC_DOTS];
 #pragma unroll
-            for (int j = 0; j < N / 2; ++j) {
-                a[0] = fma2(xv[j], v0[j], a[0]);
-                a[1] = fma2(xv[j], v1[j], a[1]);
-                n[0] = fma2(v0[j], v0[j], n[0]);
-                n[1] = fma2(v1[j], v1[j], n[1]);
-                n[2] = fma2(xv[j], xv[j], n[2]);
+            for (int r = 0; r < SC_DOTS; ++r) q[r] = *reinterpret_cast<const uint4*>(w[r] + k);
+            float2 xv[N / 2], v[N / 2];
+            unpack(x, qx, xv);
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) n[SC_DOTS] = fma2(xv[j], xv[j], n[SC_DOTS]);
+#pragma unroll
+            for (int r = 0; r < SC_DOTS; ++r) {
+                unpack(x, q[r], v);
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) {
+                    a[r] = fma2(xv[j], v[j], a[r]);
+                    n[r] = fma2(v[j], v[j], n[r]);
+                }
             }
         }
         tail = d / N * N;
     }
     for (int64_t k = tail + lane; k < d; k += 32) {
-        const float xv = Elem<T>::to_f(x[k]), v0 = Elem<T>::to_f(w0[k]), v1 = Elem<T>::to_f(w1[k]);
-        a[0].x = fmaf(xv, v0, a[0].x);
-        a[1].x = fmaf(xv, v1, a[1].x);
-        n[0].x = fmaf(v0, v0, n[0].x);
-        n[1].x = fmaf(v1, v1, n[1].x);
-        n[2].x = fmaf(xv, xv, n[2].x);
+        const float xv = Elem<T>::to_f(x[k]);
+        n[SC_DOTS].x = fmaf(xv, xv, n[SC_DOTS].x);
+#pragma unroll
+        for (int r = 0; r < SC_DOTS; ++r) {
+            const float v = Elem<T>::to_f(w[r][k]);
+            a[r].x = fmaf(xv, v, a[r].x);
+            n[r].x = fmaf(v, v, n[r].x);
+        }
     }
-    float r[5] = {a[0].x + a[0].y, a[1].x + a[1].y, n[0].x + n[0].y, n[1].x + n[1].y, n[2].x + n[2].y};
+    Products out;
+    float s[2 * SC_DOTS + 1];
+#pragma unroll
+    for (int r = 0; r < SC_DOTS; ++r) { s[r] = a[r].x + a[r].y; s[SC_DOTS + r] = n[r].x + n[r].y; }
+    s[2 * SC_DOTS] = n[SC_DOTS].x + n[SC_DOTS].y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
 #pragma unroll
-        for (int j = 0; j < 5; ++j) r[j] += __shfl_xor_sync(0xffffffffu, r[j], o);
+        for (int j = 0; j < 2 * SC_DOTS + 1; ++j) s[j] += __shfl_xor_sync(0xffffffffu, s[j], o);
     const float f = ((vec ? d * (1.f / 64) : d * (1.f / 32)) + 16.f) * 0x1p-24f * 1.01f;
-    const float xn = f * sqrtf(fmaxf(r[4], 0x1p-100f));       // (smaller squares may have underflowed)
-    return Product2{{r[0], r[1]}, {xn * sqrtf(fmaxf(r[2], 0x1p-100f)), xn * sqrtf(fmaxf(r[3], 0x1p-100f))}};
+    const float xn = f * sqrtf(fmaxf(s[2 * SC_DOTS], 0x1p-100f));       // (smaller squares may have underflowed)
+#pragma unroll
+    for (int r = 0; r < SC_DOTS; ++r) { out.z[r] = s[r]; out.e[r] = xn * sqrtf(fmaxf(s[SC_DOTS + r], 0x1p-100f)); }
+    return out;
 }
 
-// The same product of one row of the weight, exact but for fp64's rounding (2^-53).
+// Products of the candidates list[0 .. n) with the row, z and a bound of the error in out (the order of out is the
+// candidates').  fp32 operands: a warp takes four candidates at a time.
+template <int THREADS>
+__device__ __forceinline__ void candidate_products(const float* x, const float* w, int64_t w_sr, int64_t d, bool vec, const int* col, const int* list,
+                                                   int n, float2* out, float2*) {
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    for (int i = SC_DOTS * warp; i < n; i += SC_DOTS * (THREADS / 32)) {
+        const float* rows[SC_DOTS];
+#pragma unroll
+        for (int r = 0; r < SC_DOTS; ++r) rows[r] = w + col[list[min(i + r, n - 1)]] * w_sr;
+        const Products q = products(x, rows, d, vec, lane);
+        if (lane == 0) {
+#pragma unroll
+            for (int r = 0; r < SC_DOTS; ++r)
+                if (i + r < n) out[list[i + r]] = make_float2(q.z[r], q.e[r]);
+        }
+    }
+}
+
+// bf16 operands: on mma.sync, 16 candidates by 16 steps of the width, straight from memory into the A operand (lane (g, c) takes the 8
+// values from 8 c on of rows g and g + 8 of 32 steps, and the row of x in the same order into column 0 of B; a sum does not see the
+// order).  A second product of the magnitudes into column 1 bounds the error: a warp's sum is cut 2^-22 at most of the magnitudes at
+// each product, the warps' sums are added in fp32.  The warps split the width; 32 candidates at a time.
+constexpr int SC_BLOCK = 32;
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int64_t k, int64_t d) {
+    if (k + 8 <= d) return *reinterpret_cast<const uint4*>(p + k);
+    __align__(16) __nv_bfloat16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < d ? p[k + j] : __nv_bfloat16(0.f);
+    return *reinterpret_cast<const uint4*>(v);
+}
+template <int THREADS>
+__device__ __forceinline__ void candidate_products(const __nv_bfloat16* x, const __nv_bfloat16* w, int64_t w_sr, int64_t d, bool, const int* col,
+                                                   const int* list, int n, float2* out, float2* dots) {
+    constexpr int W = THREADS / 32, G = SC_BLOCK / 16;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
+    const int steps = (int)((d + 31) / 32);
+    const float cut = (2 * ((steps + W - 1) / W) + W + 4) * 0x1p-22f * 1.02f;
+    for (int b = 0; b < n; b += SC_BLOCK) {
+        const __nv_bfloat16* rows[G][2];
+        float acc[G][4] = {};
+        const int groups = (min(SC_BLOCK, n - b) + 15) / 16;
+#pragma unroll
+        for (int r = 0; r < G; ++r)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) rows[r][h] = w + col[list[min(b + 16 * r + 8 * h + g, n - 1)]] * w_sr;
+        for (int s = warp; s < steps; s += W) {
+            const int64_t k = 32 * (int64_t)s + 8 * c;
+            uint4 q[G][2], xq = load8(x, k, d);
+#pragma unroll
+            for (int r = 0; r < G; ++r)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (r < groups) q[r][h] = load8(rows[r][h], k, d);
+            const uint32_t sign = 0x7fff7fffu;
+            const uint32_t bz[2][2] = {{g == 0 ? xq.x : 0, g == 0 ? xq.y : 0}, {g == 0 ? xq.z : 0, g == 0 ? xq.w : 0}};
+            const uint32_t bm[2][2] = {{g == 1 ? xq.x & sign : 0, g == 1 ? xq.y & sign : 0}, {g == 1 ? xq.z & sign : 0, g == 1 ? xq.w & sign : 0}};
+#pragma unroll
+            for (int r = 0; r < G; ++r) {
+                if (r >= groups) continue;
+                const uint32_t a0[4] = {q[r][0].x, q[r][1].x, q[r][0].y, q[r][1].y}, a1[4] = {q[r][0].z, q[r][1].z, q[r][0].w, q[r][1].w};
+                mma_bf16(acc[r], a0, bz[0]);
+                mma_bf16(acc[r], a1, bz[1]);
+                const uint32_t m0[4] = {a0[0] & sign, a0[1] & sign, a0[2] & sign, a0[3] & sign};
+                const uint32_t m1[4] = {a1[0] & sign, a1[1] & sign, a1[2] & sign, a1[3] & sign};
+                mma_bf16(acc[r], m0, bm[0]);
+                mma_bf16(acc[r], m1, bm[1]);
+            }
+        }
+        if (c == 0) {
+#pragma unroll
+            for (int r = 0; r < G; ++r) {
+                dots[warp * SC_BLOCK + 16 * r + g] = make_float2(acc[r][0], acc[r][1]);
+                dots[warp * SC_BLOCK + 16 * r + 8 + g] = make_float2(acc[r][2], acc[r][3]);
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < min(SC_BLOCK, n - b); i += THREADS) {
+            float2 t = dots[i];
+#pragma unroll
+            for (int j = 1; j < W; ++j) {
+                const float2 u = dots[j * SC_BLOCK + i];
+                t.x += u.x;
+                t.y += u.y;
+            }
+            out[list[b + i]] = make_float2(t.x, t.y * cut);
+        }
+        __syncthreads();
+    }
+}
+
+// The same product of one row of the weight, exact but for fp64's rounding (2^-53 of the magnitudes).
 template <typename T>
-__device__ __forceinline__ double product_exact(const T* x, const T* w, int64_t d, int lane) {
+__device__ __forceinline__ double product_exact(const T* x, const T* w, int64_t d, bool vec, int lane) {
+    constexpr int N = 16 / sizeof(T);
     double a = 0.;
-    for (int64_t k = lane; k < d; k += 32) a = fma((double)Elem<T>::to_f(x[k]), (double)Elem<T>::to_f(w[k]), a);
+    int64_t tail = 0;
+    if (vec) {
+#pragma unroll 2
+        for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
+            const uint4 qx = *reinterpret_cast<const uint4*>(x + k), qw = *reinterpret_cast<const uint4*>(w + k);
+            float2 xv[N / 2], v[N / 2];
+            unpack(x, qx, xv);
+            unpack(x, qw, v);
+#pragma unroll
+            for (int j = 0; j < N / 2; ++j) a = fma((double)xv[j].x, (double)v[j].x, fma((double)xv[j].y, (double)v[j].y, a));
+        }
+        tail = d / N * N;
+    }
+    for (int64_t k = tail + lane; k < d; k += 32) a = fma((double)Elem<T>::to_f(x[k]), (double)Elem<T>::to_f(w[k]), a);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     return a;
 }
 
-static int score_candidates(bool all, int cand) { return all ? cand : 32 * cand; }
+// Columns that the candidates can come to: cand + cand / 2 values, or groups taken whole.
+static __host__ __device__ int score_candidates(bool all, int cand) { return (all ? 1 : 16) * (cand + cand / 2); }
 
 static size_t score_top_smem(bool all, int cand) {
-    return (size_t)topk_capacity(cand, SC_PER) * 8 + cand * 8 + (size_t)score_candidates(all, cand) * 12;
+    return (size_t)topk_capacity(cand, SC_PER) * 8 + cand * 8 + (size_t)score_candidates(all, cand) * 16;
 }
 
-__device__ __forceinline__ float drop_column(float v) { return __uint_as_float(__float_as_uint(v) & ~31u); }
+__device__ __forceinline__ float drop_column(float v) { return __uint_as_float(__float_as_uint(v) & ~15u); }
 
-// CTA = one row: its statistics, the candidates from the records (ALL: from the logits), their products, their ranks.
+// CTA = one row: its statistics, the candidates from the records (ALL: from the logits), their order.
 // THREADS is at least the number of candidates.
 template <typename T, bool ALL, int THREADS>
 __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     extern __shared__ __align__(16) uint8_t raw[];
-    __shared__ int count, ncand, owners[THREADS];
-    __shared__ uint32_t scratch[THREADS + 1], error;                 // error: the largest of the candidates' bounds, its bits
+    __shared__ int count, ncand, nlist, owners[THREADS];
+    __shared__ uint32_t scratch[THREADS + 1];
     __shared__ Score part[THREADS / 32];
+    __shared__ float norms[THREADS / 32];
+    __shared__ float2 dots[sizeof(T) == 2 ? THREADS / 32 * SC_BLOCK : 1];
     const int64_t row = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint64_t* buf = reinterpret_cast<uint64_t*>(raw);
     uint64_t* kept = buf + topk_capacity(p.cand, SC_PER);
-    double* val = reinterpret_cast<double*>(kept + p.cand);          // candidates' products
-    int* col = reinterpret_cast<int*>(val + (ALL ? p.cand : 32 * p.cand));
+    uint64_t* val = kept + p.cand;                                   // candidates' logits: value and error, then order_key bits of fp64
+    float2* ze = reinterpret_cast<float2*>(val);
+    int* col = reinterpret_cast<int*>(val + score_candidates(ALL, p.cand));
+    int* list = col + score_candidates(ALL, p.cand);
+    const T* x = static_cast<const T*>(p.x) + row * p.x_sr;
+    const T* w = static_cast<const T*>(p.w);
 
-    // the largest of this thread's share of the values: logits (a NaN as -inf), or the records' first ones without their columns
+    // the largest of this thread's share of the values: logits (a NaN as -inf), or the records' largest ones
     const int64_t n = ALL ? p.V : p.groups;
-    const float2* rec = p.rec + row * p.groups;
-    const float* all = p.all + row * p.V;
-    auto value = [&](int64_t i) { const float z = ALL ? all[i] : drop_column(rec[i].x); return ALL && z != z ? -INFINITY : z; };
+    const float* from = ALL ? p.all + row * p.V : p.largest + row * p.stride;
+    auto value = [&](int64_t i) { const float z = from[i]; return ALL && z != z ? -INFINITY : z; };
     float most = -INFINITY;
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t i = threadIdx.x; i < n; i += THREADS) most = fmaxf(most, value(i));
-    Score a{-INFINITY, 0.f, 0.f};
-    for (int i = threadIdx.x; i < p.np; i += THREADS) {
-        const float4 q = p.score[row * p.np + i];
-        score_join(a, Score{q.x, q.y, q.z}, p.k2, SCORE_FAR);
-    }
-    score_join_warp(a, p.k2, SCORE_FAR);
-    if (lane == 0) part[warp] = a;
-    if (threadIdx.x == 0) { ncand = 0; error = 0; }
-    __syncthreads();
-    a = part[0];
+    if (threadIdx.x == 0) { ncand = 0; nlist = 0; }
+    if (p.longest) {
+        float xx = 0.f;
+        for (int64_t k = threadIdx.x; k < p.d; k += THREADS) { const float v = Elem<T>::to_f(x[k]); xx = fmaf(v, v, xx); }
 #pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) score_join(a, part[i], p.k2, SCORE_FAR);
+        for (int o = 16; o > 0; o >>= 1) xx += __shfl_xor_sync(0xffffffffu, xx, o);
+        if (lane == 0) norms[warp] = xx;
+    }
+    const Score a = score_join_row<THREADS>(p.score + row * p.np, p.np, part);
     if (threadIdx.x == 0) score_finish(p, row, a);
     if (p.target[row] == p.ignore) {                                 // a token that does not count
         for (int i = threadIdx.x; i < p.top; i += THREADS) {
@@ -179,11 +298,14 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
 
     TopK<THREADS, SC_PER> best{};
     best.start(buf, kept, &count, p.cand);
-    auto item = [&](int t, int64_t j, auto f) {
+    struct Entry { float v; uint32_t i; };
+    auto load = [&](int t, int64_t j, Entry& e) {
         const int64_t i = t + j * THREADS;
-        if (i < n) f(value(i), (uint32_t)i);
+        e.i = (uint32_t)i;
+        e.v = i < n ? value(i) : __int_as_float(0x7fc00000);
     };
-    if (!best.gather(threadIdx.x < n ? order_key(most) : 0, scratch, owners, (n + THREADS - 1) / THREADS, item)) {
+    auto emit = [&](const Entry& e, auto f) { if (e.v == e.v) f(e.v, e.i); };
+    if (!best.template gather<Entry>(threadIdx.x < n ? order_key(most) : 0, scratch, owners, (n + THREADS - 1) / THREADS, load, emit)) {
         best.clear();
         for (int64_t i0 = 0; i0 < n; i0 += THREADS * SC_PER) {
             uint64_t key[SC_PER];
@@ -195,72 +317,128 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
             best.push(key);
         }
     }
-    best.rank();
-    // the columns of the candidates
+    // candidates: what passed the threshold, cut to the largest where that is far more than asked for; ze.y < 0: not known yet
+    if (best.n > p.cand + p.cand / 2) best.rank();
     const int m = best.n;
-    if (ALL) {
-        for (int i = threadIdx.x; i < m; i += THREADS) col[i] = (int)key_index(buf[i]);
-        if (threadIdx.x == 0) ncand = m;
-    } else {
-        const float least = order_value((uint32_t)(buf[m - 1] >> 32));
-        for (int i = threadIdx.x; i < m; i += THREADS) {
-            const int g = (int)key_index(buf[i]);
-            const float2 r = rec[g];
-            const bool two = drop_column(r.y) >= least;
-            if (two && drop_column(p.third[row * p.groups + g]) >= least) {
-                const int c = (int)min((int64_t)32, p.V - (int64_t)g * 32), at = atomicAdd(&ncand, c);
-                for (int j = 0; j < c; ++j) col[at + j] = g * 32 + j;
-            } else {
-                const int at = atomicAdd(&ncand, two ? 2 : 1);
-                col[at] = g * 32 + (int)(__float_as_uint(r.x) & 31u);
-                if (two) col[at + 1] = g * 32 + (int)(__float_as_uint(r.y) & 31u);
+    float off = INFINITY;                                            // bound of the error of the product's logits
+    if (p.longest) {
+        float xx = norms[0];
+#pragma unroll
+        for (int i = 1; i < THREADS / 32; ++i) xx += norms[i];
+        // (d / 16 + 8) products' cuts of 2^-23 of the magnitudes, as much again for three pieces; norms of squares that underflowed
+        off = (p.d * (1.f / 16) + 8.f) * (sizeof(T) == 4 ? 0x1p-22f : 0x1p-23f) * 1.01f * sqrtf(fmaxf(xx, 0x1p-100f)) *
+              sqrtf(fmaxf(__uint_as_float(*p.longest), 0x1p-100f));
+    }
+    const float least = ALL ? 0.f : order_value((uint32_t)(best.floor >> 32));
+    for (int i = threadIdx.x; i < m; i += THREADS) {
+        const uint32_t g = key_index(buf[i]);
+        const float z = order_value((uint32_t)(buf[i] >> 32));
+        const float second = ALL ? 0.f : p.runner_up[row * p.stride + g];
+        if (ALL) {
+            const int at = atomicAdd(&ncand, 1);
+            col[at] = (int)g;
+            ze[at] = make_float2(z, off);
+        } else if (drop_column(second) >= drop_column(least)) {
+            const int c = (int)min((int64_t)16, p.V - (int64_t)g * 16), at = atomicAdd(&ncand, c);
+            for (int j = 0; j < c; ++j) {
+                col[at + j] = (int)g * 16 + j;
+                ze[at + j] = make_float2(0.f, -1.f);
             }
+        } else {
+            const int at = atomicAdd(&ncand, 1);
+            col[at] = (int)(g * 16 + (__float_as_uint(second) & 15u));
+            ze[at] = make_float2(z, off);
         }
     }
     __syncthreads();
     const int nc = ncand;
-    const T* x = static_cast<const T*>(p.x) + row * p.x_sr;
-    const T* w = static_cast<const T*>(p.w);
-    for (int i = 2 * warp; i < nc; i += 2 * (THREADS / 32)) {
-        const int i1 = min(i + 1, nc - 1);
-        const Product2 z = product2<T>(x, w + col[i] * p.w_sr, w + col[i1] * p.w_sr, p.d, p.vec, lane);
-        if (lane == 0) {
-            val[i] = z.z[0];
-            if (i1 > i) val[i1] = z.z[1];
-            const float e = fmaxf(z.e[0], z.e[1]);
-            atomicMax(&error, e == e && z.e[0] + z.e[1] == z.e[0] + z.e[1] ? __float_as_uint(e) : 0x7f800000u);
+    // those not known, or not told apart from a known one: their products again
+    for (int i = threadIdx.x; i < nc; i += THREADS) {
+        const float2 z = ze[i];
+        bool close = z.y < 0.f;
+#pragma unroll 4
+        for (int j = 0; j < nc; ++j) {
+            const float2 o = ze[j];
+            close |= (j != i) & (o.y >= 0.f) & !(fabsf(o.x - z.x) > 2.0001f * off);
         }
+        if (close) list[atomicAdd(&nlist, 1)] = i;
     }
     __syncthreads();
-    // candidates that the bound does not tell apart from another, marked by the sign of their column
-    const double apart = 2. * __uint_as_float(error);
+    candidate_products<THREADS>(x, w, p.w_sr, p.d, p.vec, col, list, nlist, ze, dots);
+    __syncthreads();
+    // those still not told apart from another (the bounds' sum, and the difference's own rounding): exactly, marked by the sign of their column
     for (int i = threadIdx.x; i < nc; i += THREADS) {
+        const float2 z = ze[i];
         bool close = false;
-        for (int j = 0; j < nc; ++j) close |= j != i && !(fabs(val[j] - val[i]) > apart);
+#pragma unroll 4
+        for (int j = 0; j < nc; ++j) {
+            const float2 o = ze[j];
+            close |= (j != i) & !(fabsf(o.x - z.x) > (o.y + z.y) * 1.0001f);
+        }
         if (close) col[i] = ~col[i];
     }
     __syncthreads();
     for (int i = warp; i < nc; i += THREADS / 32) {
         const int c = col[i];
-        if (c >= 0) continue;
-        const double z = product_exact<T>(x, w + (int64_t)~c * p.w_sr, p.d, lane);
-        if (lane == 0) { val[i] = z; col[i] = ~c; }
+        const double z = c >= 0 ? ze[i].x : product_exact<T>(x, w + (int64_t)~c * p.w_sr, p.d, p.vec, lane);
+        __syncwarp();
+        if (lane == 0) {
+            val[i] = order_key(z);
+            if (c < 0) col[i] = ~c;
+        }
     }
     __syncthreads();
-    const double lse = (double)a.m * p.inv_temp + log((double)a.s);
+    const float ls = logf(a.s);
     for (int i = threadIdx.x; i < nc; i += THREADS) {
-        const double z = val[i];
-        const uint64_t v = order_key(z);
+        const uint64_t v = val[i];
         const int c = col[i];
         int r = 0;
+#pragma unroll 4
         for (int j = 0; j < nc; ++j) {
-            const uint64_t o = order_key(val[j]);
-            r += o > v || (o == v && col[j] < c);
+            const uint64_t o = val[j];
+            r += (int)(o > v) + (int)((o == v) & (col[j] < c));
         }
         if (r < p.top) {
-            p.top_log_probs[row * p.top + r] = (float)(z * p.inv_temp - lse);
+            const double z = __longlong_as_double((long long)(v >> 63 ? v & ~(1ull << 63) : ~v));
+            p.top_log_probs[row * p.top + r] = (float)(z * p.k2 - (double)a.m) * LN2 - ls;
             p.top_ids[row * p.top + r] = c;
         }
+    }
+}
+
+// The largest squared norm of a word, a warp for each (fp32 sums of squares: 2^-24 for each of d / 32 additions, far inside the
+// bound's slack).  One read of the weight: 50001 x 1024 bf16 about 20 us.
+template <typename T>
+__global__ void __launch_bounds__(256) longest_word_kernel(const T* w, int64_t w_sr, int64_t V, int64_t d, bool vec, uint32_t* longest) {
+    __shared__ float most[8];
+    constexpr int N = 16 / sizeof(T);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    float top = 0.f;
+    for (int64_t v = (int64_t)blockIdx.x * 8 + warp; v < V; v += (int64_t)gridDim.x * 8) {
+        const T* r = w + v * w_sr;
+        float2 s = {0.f, 0.f};
+        int64_t tail = 0;
+        if (vec) {
+#pragma unroll 4
+            for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
+                float2 q[N / 2];
+                unpack(r, *reinterpret_cast<const uint4*>(r + k), q);
+#pragma unroll
+                for (int j = 0; j < N / 2; ++j) s = fma2(q[j], q[j], s);
+            }
+            tail = d / N * N;
+        }
+        for (int64_t k = tail + lane; k < d; k += 32) { const float q = Elem<T>::to_f(r[k]); s.x = fmaf(q, q, s.x); }
+        float t = s.x + s.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        top = t == t ? fmaxf(top, t) : INFINITY;
+    }
+    if (lane == 0) most[warp] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 8; ++i) top = fmaxf(top, most[i]);
+        atomicMax(longest, __float_as_uint(top));
     }
 }
 
@@ -273,8 +451,9 @@ cudaError_t launch_grad(const XentGemm& g, const CUtensorMap& x, const CUtensorM
 }
 
 struct ScorePlan {
-    int cand; bool all; int64_t groups;
-    int64_t off_score, off_hit, off_rec, off_third, total;
+    int cand; bool all; int64_t groups, stride;
+    int64_t off_score, off_hit, off_rec, off_second, off_longest, total;
+    bool longest;
 };
 
 static ScorePlan score_plan(const HeadPlan& q, int64_t T, int64_t V, int top) {
@@ -285,11 +464,15 @@ static ScorePlan score_plan(const HeadPlan& q, int64_t T, int64_t V, int top) {
     f.total = f.off_rec;
     if (top > 0) {
         f.cand = (int)std::min<int64_t>(V, top + SC_EXTRA);
-        f.groups = (V + 31) / 32;
+        f.groups = (V + 15) / 16;
+        f.stride = 16 * q.nt;
         // few groups for each candidate: most would be taken whole, or there are not enough of them
-        f.all = V <= 2048 || f.groups < 2 * f.cand;
-        f.off_third = f.off_rec + up256(f.all ? T * V * 4 : T * f.groups * 8);
-        f.total = f.off_third + (f.all ? 0 : up256(T * f.groups * 4));
+        f.all = V <= 2048 || V < 32 * f.cand;
+        f.off_second = f.off_rec + up256(f.all ? T * V * 4 : T * f.stride * 4);
+        f.off_longest = f.off_second + (f.all ? 0 : up256(T * f.stride * 4));
+        f.total = f.off_longest + 256;
+        // the words' norms are one read of the weight, and without them every candidate's word is read
+        f.longest = T * f.cand > V;
     }
     return f;
 }
@@ -320,7 +503,8 @@ static cudaError_t launch_top(const ScoreRows& p, cudaStream_t st) {
 
 template <typename T>
 static cudaError_t launch_top(const ScoreRows& p, bool all, cudaStream_t st) {
-    if (p.cand <= 128) return all ? launch_top<T, true, 128>(p, st) : launch_top<T, false, 128>(p, st);
+    // few rows: more warps for each one's candidates
+    if (p.cand <= 128 && p.T > 148) return all ? launch_top<T, true, 128>(p, st) : launch_top<T, false, 128>(p, st);
     return all ? launch_top<T, true, 256>(p, st) : launch_top<T, false, 256>(p, st);
 }
 
@@ -362,11 +546,12 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
     if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
     XentGemm g = logits_gemm(o, q, 0, o.V, status);
     g.target = a->targets; g.ignore = a->ignore_index;
-    g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E * g.inv_temp;
+    g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
     g.score = reinterpret_cast<float4*>(ws + f.off_score);
     g.hit = reinterpret_cast<float*>(ws + f.off_hit);
-    g.rec = reinterpret_cast<float2*>(ws + f.off_rec); g.third = reinterpret_cast<float*>(ws + f.off_third); g.groups = f.groups;
+    g.largest = reinterpret_cast<float*>(ws + f.off_rec); g.runner_up = reinterpret_cast<float*>(ws + f.off_second);
     g.all = reinterpret_cast<float*>(ws + f.off_rec);
+    g.counter = f.longest ? reinterpret_cast<int*>(ws + f.off_longest) : nullptr;
     const cudaError_t e = a->top_k == 0 ? launch_score(g, mx, mw, st)
                           : f.all       ? launch_logits<XE_SCORE_ALL>(g, mx, mw, mx, st)
                                         : launch_logits<XE_SCORE_TOP>(g, mx, mw, mx, st);
@@ -374,19 +559,27 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
     ScoreRows p{};
     p.T = o.T; p.V = o.V; p.d = o.d; p.np = (int)(2 * q.nt);
     p.score = g.score; p.hit = g.hit; p.target = a->targets; p.ignore = a->ignore_index;
-    p.k2 = g.k2; p.inv_temp = g.inv_temp;
+    p.k2 = g.k2;
     p.row_max = a->row_max; p.row_sum = a->row_sum; p.log_probs = a->log_probs; p.entropy = a->entropy;
     if (a->top_k == 0) {
         score_rows_kernel<<<(unsigned)((o.T + SC_THREADS / 32 - 1) / (SC_THREADS / 32)), SC_THREADS, 0, st>>>(p);
         return cudaGetLastError() == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
     }
-    p.top = a->top_k; p.cand = f.cand; p.rec = g.rec; p.third = g.third; p.all = g.all; p.groups = f.groups;
+    p.top = a->top_k; p.cand = f.cand; p.largest = g.largest; p.runner_up = g.runner_up; p.stride = f.stride; p.all = g.all; p.groups = f.groups;
     p.top_log_probs = a->top_log_probs; p.top_ids = a->top_ids;
     // the operands in their own type: bf16 ones from their copies where those were made (their rows start on 16 bytes)
     const bool bf = o.dtype == SWX_DTYPE_BF16;
     p.x = bf ? x.p : o.x; p.x_sr = bf ? x.row : o.x_sr;
     p.w = bf ? w.p : o.w; p.w_sr = bf ? w.row : o.w_sr;
     p.vec = bf || (aligned16(o.x) && aligned16(o.w) && o.x_sr % 4 == 0 && o.w_sr % 4 == 0);
+    if (f.longest) {
+        uint32_t* longest = reinterpret_cast<uint32_t*>(g.counter);
+        const unsigned grid = (unsigned)std::min<int64_t>((o.V + 7) / 8, 148 * 8);
+        if (bf) longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p.w), p.w_sr, p.V, p.d, true, longest);
+        else longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p.w), p.w_sr, p.V, p.d, p.vec != 0, longest);
+        if (cudaGetLastError() != cudaSuccess) return SWX_ERR_CUDA;
+        p.longest = longest;
+    }
     const cudaError_t r = bf ? launch_top<__nv_bfloat16>(p, f.all, st) : launch_top<float>(p, f.all, st);
     return r == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
 }
@@ -410,7 +603,7 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, nullptr, nullptr};
     return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_grad, [a](XentGemm& g) {
         g.target = a->targets; g.ignore = a->ignore_index;
-        g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E * g.inv_temp;
+        g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
         g.row_max = a->row_max; g.row_sum = a->row_sum; g.entropy = a->entropy;
         g.d_logp = a->d_log_probs; g.d_entropy = a->d_entropy;
     }, [](__nv_bfloat16*, int64_t, int64_t) { return (int)SWX_OK; });

@@ -1,6 +1,6 @@
 // Log probabilities, entropy and top alternatives of rows of logits (a step of generation):
-// with u = (z - m) log2(e) / tau, s = sum 2^u and w = sum 2^u u over the row,
-//   log_probs = (z_y - m) / tau - ln s,  entropy = ln s - ln2 w / s.
+// with m the largest z, u = (z - m) log2(e) / tau, s = sum 2^u and w = sum 2^u u over the row,
+//   log_probs = ln2 u_y - ln s,  entropy = ln s - ln2 w / s.
 //
 // One pass over the logits, which bound it.  A row goes to a cluster of 1 to 8 CTAs (so that a few rows
 // reach many SMs, without a second launch); each thread walks its share of the CTA's part with 16-byte loads, four at a
@@ -13,7 +13,7 @@
 namespace swx {
 
 constexpr int TL_LOADS = 4, TL_PER = 8, TL_MAX_PARTS = 8;
-constexpr float TL_FAR = -200.f, TL_LN2 = 0.69314718055994531f;
+constexpr float TL_LN2 = 0.69314718055994531f;
 
 struct TokenRows {
     int64_t V, stride;
@@ -65,7 +65,6 @@ __global__ void __launch_bounds__(THREADS) token_logprob_kernel(const TokenRows 
     const int64_t pieces = (p.V + shift + N - 1) / N, per = (pieces + p.parts - 1) / p.parts;
     const int64_t begin = rank * per, end = min(pieces, begin + per);
     Score a{-INFINITY, 0.f, 0.f};
-    uint32_t most = 0;                         // the share's largest value as order_key bits
     for (int64_t i0 = begin + threadIdx.x; i0 < end; i0 += TL_LOADS * THREADS) {
         float v[TL_LOADS][N];
 #pragma unroll
@@ -82,7 +81,7 @@ __global__ void __launch_bounds__(THREADS) token_logprob_kernel(const TokenRows 
 #pragma unroll
             for (int k = 0; k < N; ++k) nm = fmaxf(nm, v[j][k]);
         const float base = nm == -INFINITY ? 0.f : nm;                   // nothing but -inf so far: the sums stay 0
-        const float da = fmaxf((a.m - base) * p.k2, TL_FAR), ca = ex2(da);
+        const float da = fmaxf((a.m - base) * p.k2, SCORE_FAR), ca = ex2(da);
         float2 s = make_float2(ca * a.s, 0.f), w = make_float2(ca * (a.w + a.s * da), 0.f);
         a.m = nm;
 #pragma unroll
@@ -91,29 +90,31 @@ __global__ void __launch_bounds__(THREADS) token_logprob_kernel(const TokenRows 
             for (int k = 0; k < N; k += 2) {
                 const float2 u = mul2(add2(f2(v[j][k], v[j][k + 1]), bc2(-base)), bc2(p.k2)), e = ex2x2(u);
                 s = add2(s, e);
-                w = fma2(e, f2(fmaxf(u.x, TL_FAR), fmaxf(u.y, TL_FAR)), w);
+                w = fma2(e, f2(fmaxf(u.x, SCORE_FAR), fmaxf(u.y, SCORE_FAR)), w);
             }
         a.s = s.x + s.y;
         a.w = w.x + w.y;
     }
-    if (TOP) most = begin + threadIdx.x < end ? order_key(a.m) : 0;
     const bool odd = a.s != a.s;               // a NaN or +inf in the share
-    score_join_warp(a, p.k2, TL_FAR);
+    const float most = a.m;                    // the share's largest
+    score_join_warp(a, p.k2);
     if (lane == 0) part[warp] = a;
     uint64_t* buf = reinterpret_cast<uint64_t*>(raw);
     TopK<THREADS, TL_PER> best{};
     if constexpr (TOP) {
         best.start(buf, buf + topk_capacity(p.top, TL_PER), &count, p.top);
-        auto item = [&](int t, int64_t j, auto f) {
-            const int64_t i = begin + t + j * THREADS, c = i * N - shift;
-            if (i >= end) return;
-            float v[N];
-            load_piece<T>(z, p.V, shift, i, v);
+        struct Piece { float v[N]; int64_t c; };
+        auto load = [&](int t, int64_t j, Piece& e) {
+            const int64_t i = begin + t + j * THREADS;
+            e.c = i < end ? i * N - shift : p.V;
+            if (i < end) load_piece<T>(z, p.V, shift, i, e.v);
+        };
+        auto emit = [&](const Piece& e, auto f) {
 #pragma unroll
             for (int k = 0; k < N; ++k)
-                if (c + k >= 0 && c + k < p.V) f(v[k], (uint32_t)(c + k));
+                if (e.c + k >= 0 && e.c + k < p.V) f(e.v[k], (uint32_t)(e.c + k));
         };
-        if (__syncthreads_or(odd) || !best.gather(most, scratch, owners, (per + THREADS - 1) / THREADS, item)) {
+        if (__syncthreads_or(odd) || !best.template gather<Piece>(begin + threadIdx.x < end ? order_key(most) : 0, scratch, owners, (per + THREADS - 1) / THREADS, load, emit)) {
             best.clear();
             for (int64_t i0 = begin; i0 < end; i0 += THREADS * (TL_PER / N)) {
                 uint64_t key[TL_PER];
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(THREADS) token_logprob_kernel(const TokenRows 
     __syncthreads();
     if (threadIdx.x == 0) {
         a = part[0];
-        for (int i = 1; i < THREADS / 32; ++i) score_join(a, part[i], p.k2, TL_FAR);
+        for (int i = 1; i < THREADS / 32; ++i) score_join(a, part[i], p.k2);
         whole = a;
         if (TOP) found = best.n;
     }
@@ -145,7 +146,7 @@ __global__ void __launch_bounds__(THREADS) token_logprob_kernel(const TokenRows 
         if (rank == 0) {
             for (int r = 1; r < p.parts; ++r) {
                 const uint32_t o = map_to_rank(&whole, r);
-                score_join(a, Score{ld_cluster_f32(o), ld_cluster_f32(o + 4), ld_cluster_f32(o + 8)}, p.k2, TL_FAR);
+                score_join(a, Score{ld_cluster_f32(o), ld_cluster_f32(o + 4), ld_cluster_f32(o + 8)}, p.k2);
             }
             if (TOP) {
                 for (int r = 1; r < p.parts; ++r) {
@@ -227,7 +228,7 @@ extern "C" int swx_token_logprob(const swx_logprob_args* a, void* stream) {
     if (!a->x || !a->entropy || (a->targets && !a->log_probs) || (a->top_k > 0 && (!a->top_log_probs || !a->top_ids))) return SWX_ERR_INVALID_ARG;
     TokenRows p{};
     p.V = a->vocab; p.stride = a->x_sr; p.top = a->top_k; p.z = a->x; p.target = a->targets; p.ignore = a->ignore_index;
-    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E * p.inv_temp;
+    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E / a->temperature;
     p.log_probs = a->log_probs; p.entropy = a->entropy; p.top_log_probs = a->top_log_probs; p.top_ids = a->top_ids;
     p.parts = token_parts(a->tokens, a->vocab);
     cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -1,8 +1,8 @@
 // The K largest of a long row, by one CTA.  A key is a value's order-preserving bits above the complement of its
 // index, so that no two are equal and ties go to the lowest index.
 //
-// After a pass in which each thread has kept the largest value of its share, the K-th largest of those maxima is a threshold
-// that at least K values reach, and only the threads whose maximum does have any: their shares (K of them, few
+// After a pass in which each thread has kept the largest value of its share, about the K-th largest of those maxima is a threshold
+// that at least K values reach, and only the threads whose maximum does have any: their shares (some K of them, few
 // hundred values) are read again, and the keys that pass, little more than K as a rule, are gathered in shared memory and ranked.
 // Where too many pass (many equal values, or large ones gathered in few shares) the whole row is streamed past a rising
 // threshold in bounded batches instead (TopK::push), slower and for any order.
@@ -27,10 +27,11 @@ __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k;
 // Entries that TopK's buffer holds for `k` and `per` keys a thread: what is kept, and a batch's passers.
 constexpr int topk_capacity(int k, int per) { return k * (per + 1); }
 
-// Finds the k-th largest of the THREADS threads' values, as order_key bits, by one warp: the bits are set from the top while at
-// least k values stay no smaller, over those that differ.  scratch: THREADS + 1 words; all threads call it.
+// A threshold that at least k of the THREADS threads' values (order_key bits) reach, and at most k + k / 4 where the values differ,
+// by one warp: the bits of the k-th largest are set from the top, over those that differ, until it is that close.
+// scratch: THREADS + 1 words; all threads call it.
 template <int THREADS>
-__device__ __forceinline__ uint32_t kth_largest(uint32_t mine, int k, uint32_t* scratch) {
+__device__ __forceinline__ uint32_t about_kth(uint32_t mine, int k, uint32_t* scratch) {
     scratch[threadIdx.x] = mine;
     __syncthreads();
     if (threadIdx.x < 32) {
@@ -53,7 +54,7 @@ __device__ __forceinline__ uint32_t kth_largest(uint32_t mine, int k, uint32_t* 
             for (int j = 0; j < N; ++j) n += v[j] >= c;
             n = __reduce_add_sync(0xffffffffu, n);
             if (n >= k) t = c;
-            if (n == k) break;
+            if (n >= k && n <= k + k / 4) break;
         }
         if (threadIdx.x == 0) scratch[THREADS] = t;
     }
@@ -92,23 +93,33 @@ struct TopK {
         n = *count;
         return n <= topk_capacity(k, PER);
     }
-    // The keys that reach the threshold, from the shares of the threads whose maximum does: item(t, j, f) calls f(value,
-    // index) on entry j < per of thread t's share.  False where they were too many.
-    template <class Item>
-    __device__ __forceinline__ bool gather(uint32_t mine, uint32_t* scratch, int* owners, int64_t per, Item item) {
-        const uint32_t t = kth_largest<THREADS>(mine, k, scratch);
+    // The keys that reach the threshold, from the shares of the threads whose maximum does: load(t, j, e) reads entry j < per of
+    // thread t's share into e, and emit(e, f) calls f(value, index) on what it holds.  A warp takes a share, four of them
+    // at a time so that their loads overlap.  False where they were too many.
+    template <class Entry, class Load, class Emit>
+    __device__ __forceinline__ bool gather(uint32_t mine, uint32_t* scratch, int* owners, int64_t per, Load load, Emit emit) {
+        const uint32_t t = about_kth<THREADS>(mine, k, scratch);
         if (mine >= t) owners[atomicAdd(count, 1)] = threadIdx.x;
         __syncthreads();
         const int m = *count;
         __syncthreads();
         if (threadIdx.x == 0) *count = 0;
         __syncthreads();
-        const uint32_t one = (uint32_t)per;
-        for (uint32_t i = threadIdx.x; i < m * one; i += THREADS)
-            item(owners[i / one], (int64_t)(i % one), [&](float v, uint32_t index) {
-                const uint32_t o = order_key(v);
-                if (o >= t) add(index_key(o, index));
-            });
+        for (int i0 = threadIdx.x / 32; i0 < m; i0 += 4 * (THREADS / 32))
+            for (int64_t j = threadIdx.x % 32; j < per; j += 32) {
+                Entry e[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i0 + u * (THREADS / 32) < m) load(owners[i0 + u * (THREADS / 32)], j, e[u]);
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (i0 + u * (THREADS / 32) < m)
+                        emit(e[u], [&](float v, uint32_t index) {
+                            const uint32_t o = order_key(v);
+                            if (o >= t) add(index_key(o, index));
+                        });
+            }
+        floor = (uint64_t)t << 32;
         return added();
     }
     // The k-th largest of the threads' largest keys: at least k keys are no smaller.  The bits are found from the top; the keys
@@ -159,23 +170,77 @@ struct TopK {
     }
 };
 
-// Statistics of scaled logits in base 2: maximum m of the raw logits, s = sum 2^u and w = sum 2^u u with u = (z - m) k2.
-// (m = -inf with s = w = 0: nothing yet; the differences of infinities, NaN, are dropped by the maximum with `far`.)
+// Statistics of scaled logits in base 2: m the largest (times k2), s = sum 2^u and w = sum 2^u u with u = z k2 - m; or, with k =
+// k2 handed to the joins, m the largest itself and u = (z - m) k2 (logits at the lowest end of their type would overflow in z k2).
+// (m = -inf with s = w = 0: nothing yet; the differences of infinities, NaN, are dropped by the maximum with SCORE_FAR.)
+constexpr float SCORE_FAR = -200.f;           // 2^-200 is 0: what lies further below the maximum adds nothing
 struct Score { float m, s, w; };
-__device__ __forceinline__ void score_join(Score& a, const Score& b, float k2, float far) {
-    const float nm = fmaxf(a.m, b.m);
-    const float da = fmaxf((a.m - nm) * k2, far), db = fmaxf((b.m - nm) * k2, far);
-    const float ca = ex2(da), cb = ex2(db);
-    a.w = ca * (a.w + a.s * da) + cb * (b.w + b.s * db);
-    a.s = ca * a.s + cb * b.s;
-    a.m = nm;
+// The same relative to a larger m.
+__device__ __forceinline__ void score_move(Score& a, float m, float k = 1.f) {
+    const float d = fmaxf((a.m - m) * k, SCORE_FAR), c = ex2(d);
+    a.w = c * (a.w + a.s * d);
+    a.s *= c;
+    a.m = m;
 }
-__device__ __forceinline__ void score_join_warp(Score& a, float k2, float far) {
+__device__ __forceinline__ void score_join(Score& a, Score b, float k = 1.f) {
+    const float m = fmaxf(a.m, b.m);
+    score_move(a, m, k);
+    score_move(b, m, k);
+    a.s += b.s;
+    a.w += b.w;
+}
+__device__ __forceinline__ void score_join_warp(Score& a, float k = 1.f) {
+    float m = a.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    score_move(a, m, k);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        const Score b{__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.w, o)};
-        score_join(a, b, k2, far);
+        a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+        a.w += __shfl_xor_sync(0xffffffffu, a.w, o);
     }
+}
+// The statistics of a whole row by `threads` threads (of which this is number t), from its np parts, before they are joined.
+__device__ __forceinline__ Score score_join_parts(const float4* q, int np, int t, int threads) {
+    Score a{-INFINITY, 0.f, 0.f};
+    for (int i0 = t; i0 < np; i0 += 4 * threads) {
+        float4 v[4];
+        float m = a.m;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            v[u] = i0 + u * threads < np ? q[i0 + u * threads] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+            m = fmaxf(m, v[u].x);
+        }
+        score_move(a, m);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            Score b{v[u].x, v[u].y, v[u].z};
+            score_move(b, m);
+            a.s += b.s;
+            a.w += b.w;
+        }
+    }
+    score_join_warp(a);
+    return a;
+}
+// The same by a CTA, joined; parts: shared memory for one Score a warp.
+template <int THREADS>
+__device__ __forceinline__ Score score_join_row(const float4* q, int np, Score* parts) {
+    Score a = score_join_parts(q, np, threadIdx.x, THREADS);
+    if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = a;
+    __syncthreads();
+    float m = parts[0].m;
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, parts[i].m);
+    a = Score{m, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < THREADS / 32; ++i) {
+        Score b = parts[i];
+        score_move(b, m);
+        a.s += b.s;
+        a.w += b.w;
+    }
+    return a;
 }
 
 }  // namespace swx
