@@ -595,6 +595,15 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
     if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
+// Eight values of a row from k on (a multiple of 8; rows start on 16 bytes), zeros from d on.
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int64_t k, int64_t d) {
+    if (k + 8 <= d) return *reinterpret_cast<const uint4*>(p + k);
+    __align__(16) __nv_bfloat16 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = k + j < d ? p[k + j] : __nv_bfloat16(0.f);
+    return *reinterpret_cast<const uint4*>(v);
+}
+
 // ------------------------------------------------------------------ host side
 // How a gradient product's tiles are dealt out to the CTA pairs (linear_xent.cu `deal`).
 struct XentDeal { int spread, pairs, parts; };
@@ -686,6 +695,10 @@ static cudaError_t launch_logits(const XentGemm& g, const CUtensorMap& x, const 
 // The scoring and gradient epilogues that more than one operator uses (linear_logprob.cu).
 cudaError_t launch_score(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, cudaStream_t st);
 cudaError_t launch_grad(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& store, cudaStream_t st);
+
+// The scoring of a few rows without tiles (linear_logprob_few.cu): its CTAs, 0 where it does not take them, and the launch.
+int score_few_ctas(const HeadOps& o);
+cudaError_t launch_score_few(const XentGemm& g, const HeadOps& o, const Operand& x, const Operand& w, bool top, int ctas, cudaStream_t st);
 
 // The gradients, piece by piece of the vocabulary: the logits again and dlogit in the epilogue (`launch`, with the
 // fields that `fill` sets), whatever `patch` does to the piece (its base, first column and columns; a status), and the

@@ -55,4 +55,22 @@ inline cudaError_t sm_fit(K kernel, int threads, int smem, int* sms, int* per_sm
     return e;
 }
 
+// A launch whose blocks may be set up while the stream's previous kernel still runs; the kernel has to call
+// wait_for_previous() before anything else.
+template <typename... Params, typename... Args>
+inline cudaError_t launch_after(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(threads);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    return cudaLaunchKernelEx(&c, kernel, args...);
+}
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace swx

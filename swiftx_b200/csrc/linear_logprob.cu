@@ -50,6 +50,7 @@ __device__ __forceinline__ void score_finish(const ScoreRows& p, int64_t row, co
 
 // Warp = one row.
 __global__ void __launch_bounds__(SC_THREADS) score_rows_kernel(const ScoreRows p) {
+    wait_for_previous();
     const int64_t row = (int64_t)blockIdx.x * (SC_THREADS / 32) + threadIdx.x / 32;
     if (row >= p.T) return;
     const int lane = threadIdx.x % 32;
@@ -148,66 +149,73 @@ __device__ __forceinline__ void candidate_products(const float* x, const float* 
 // bf16 operands: on mma.sync, 16 candidates by 16 steps of the width, straight from memory into the A operand (lane (g, c) takes the 8
 // values from 8 c on of rows g and g + 8 of 32 steps, and the row of x in the same order into column 0 of B; a sum does not see the
 // order).  A second product of the magnitudes into column 1 bounds the error: a warp's sum is cut 2^-22 at most of the magnitudes at
-// each product, the warps' sums are added in fp32.  The warps split the width; 32 candidates at a time.
-constexpr int SC_BLOCK = 32;
-__device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int64_t k, int64_t d) {
-    if (k + 8 <= d) return *reinterpret_cast<const uint4*>(p + k);
-    __align__(16) __nv_bfloat16 v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = k + j < d ? p[k + j] : __nv_bfloat16(0.f);
-    return *reinterpret_cast<const uint4*>(v);
-}
+// each product, the warps' sums are added in fp32.  The warps split the width.  Two steps' loads at a time: for 16 candidates in the small
+// CTAs that many rows take (their registers decide how many run), for 32 in the large ones.
+constexpr int score_block(int threads) { return threads == 128 ? 16 : 32; }
 template <int THREADS>
 __device__ __forceinline__ void candidate_products(const __nv_bfloat16* x, const __nv_bfloat16* w, int64_t w_sr, int64_t d, bool, const int* col,
                                                    const int* list, int n, float2* out, float2* dots) {
-    constexpr int W = THREADS / 32, G = SC_BLOCK / 16;
+    constexpr int W = THREADS / 32, B = score_block(THREADS), G = B / 16;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, c = lane % 4;
     const int steps = (int)((d + 31) / 32);
     const float cut = (2 * ((steps + W - 1) / W) + W + 4) * 0x1p-22f * 1.02f;
-    for (int b = 0; b < n; b += SC_BLOCK) {
+    for (int b = 0; b < n; b += B) {
         const __nv_bfloat16* rows[G][2];
         float acc[G][4] = {};
-        const int groups = (min(SC_BLOCK, n - b) + 15) / 16;
+        const int groups = (min(B, n - b) + 15) / 16;
 #pragma unroll
         for (int r = 0; r < G; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) rows[r][h] = w + col[list[min(b + 16 * r + 8 * h + g, n - 1)]] * w_sr;
-        for (int s = warp; s < steps; s += W) {
-            const int64_t k = 32 * (int64_t)s + 8 * c;
-            uint4 q[G][2], xq = load8(x, k, d);
+        constexpr int D = 2;                   // steps whose loads are issued together
+        for (int s0 = warp; s0 < steps; s0 += D * W) {
+            uint4 q[D][G][2], xq[D];
 #pragma unroll
-            for (int r = 0; r < G; ++r)
+            for (int i = 0; i < D; ++i) {
+                const int s = s0 + i * W;
+                const int64_t k = 32 * (int64_t)s + 8 * c;
+                if (s >= steps) continue;
+                xq[i] = load8(x, k, d);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (r < groups) q[r][h] = load8(rows[r][h], k, d);
+                for (int r = 0; r < G; ++r)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (r < groups) q[i][r][h] = load8(rows[r][h], k, d);
+            }
             const uint32_t sign = 0x7fff7fffu;
-            const uint32_t bz[2][2] = {{g == 0 ? xq.x : 0, g == 0 ? xq.y : 0}, {g == 0 ? xq.z : 0, g == 0 ? xq.w : 0}};
-            const uint32_t bm[2][2] = {{g == 1 ? xq.x & sign : 0, g == 1 ? xq.y & sign : 0}, {g == 1 ? xq.z & sign : 0, g == 1 ? xq.w & sign : 0}};
 #pragma unroll
-            for (int r = 0; r < G; ++r) {
-                if (r >= groups) continue;
-                const uint32_t a0[4] = {q[r][0].x, q[r][1].x, q[r][0].y, q[r][1].y}, a1[4] = {q[r][0].z, q[r][1].z, q[r][0].w, q[r][1].w};
-                mma_bf16(acc[r], a0, bz[0]);
-                mma_bf16(acc[r], a1, bz[1]);
-                const uint32_t m0[4] = {a0[0] & sign, a0[1] & sign, a0[2] & sign, a0[3] & sign};
-                const uint32_t m1[4] = {a1[0] & sign, a1[1] & sign, a1[2] & sign, a1[3] & sign};
-                mma_bf16(acc[r], m0, bm[0]);
-                mma_bf16(acc[r], m1, bm[1]);
+            for (int i = 0; i < D; ++i) {
+                if (s0 + i * W >= steps) continue;
+                const uint4 v = xq[i];
+                const uint32_t bz[2][2] = {{g == 0 ? v.x : 0, g == 0 ? v.y : 0}, {g == 0 ? v.z : 0, g == 0 ? v.w : 0}};
+                const uint32_t bm[2][2] = {{g == 1 ? v.x & sign : 0, g == 1 ? v.y & sign : 0}, {g == 1 ? v.z & sign : 0, g == 1 ? v.w & sign : 0}};
+#pragma unroll
+                for (int r = 0; r < G; ++r) {
+                    if (r >= groups) continue;
+                    const uint4 *u = q[i][r];
+                    const uint32_t a0[4] = {u[0].x, u[1].x, u[0].y, u[1].y}, a1[4] = {u[0].z, u[1].z, u[0].w, u[1].w};
+                    mma_bf16(acc[r], a0, bz[0]);
+                    mma_bf16(acc[r], a1, bz[1]);
+                    const uint32_t m0[4] = {a0[0] & sign, a0[1] & sign, a0[2] & sign, a0[3] & sign};
+                    const uint32_t m1[4] = {a1[0] & sign, a1[1] & sign, a1[2] & sign, a1[3] & sign};
+                    mma_bf16(acc[r], m0, bm[0]);
+                    mma_bf16(acc[r], m1, bm[1]);
+                }
             }
         }
         if (c == 0) {
 #pragma unroll
             for (int r = 0; r < G; ++r) {
-                dots[warp * SC_BLOCK + 16 * r + g] = make_float2(acc[r][0], acc[r][1]);
-                dots[warp * SC_BLOCK + 16 * r + 8 + g] = make_float2(acc[r][2], acc[r][3]);
+                dots[warp * B + 16 * r + g] = make_float2(acc[r][0], acc[r][1]);
+                dots[warp * B + 16 * r + 8 + g] = make_float2(acc[r][2], acc[r][3]);
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < min(SC_BLOCK, n - b); i += THREADS) {
+        for (int i = threadIdx.x; i < min(B, n - b); i += THREADS) {
             float2 t = dots[i];
 #pragma unroll
             for (int j = 1; j < W; ++j) {
-                const float2 u = dots[j * SC_BLOCK + i];
+                const float2 u = dots[j * B + i];
                 t.x += u.x;
                 t.y += u.y;
             }
@@ -259,7 +267,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     __shared__ uint32_t scratch[THREADS + 1];
     __shared__ Score part[THREADS / 32];
     __shared__ float norms[THREADS / 32];
-    __shared__ float2 dots[sizeof(T) == 2 ? THREADS / 32 * SC_BLOCK : 1];
+    __shared__ float2 dots[sizeof(T) == 2 ? THREADS / 32 * score_block(THREADS) : 1];
     const int64_t row = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     uint64_t* buf = reinterpret_cast<uint64_t*>(raw);
@@ -270,6 +278,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     int* list = col + score_candidates(ALL, p.cand);
     const T* x = static_cast<const T*>(p.x) + row * p.x_sr;
     const T* w = static_cast<const T*>(p.w);
+    wait_for_previous();
 
     // the largest of this thread's share of the values: logits (a NaN as -inf), or the records' largest ones
     const int64_t n = ALL ? p.V : p.groups;
@@ -451,15 +460,19 @@ cudaError_t launch_grad(const XentGemm& g, const CUtensorMap& x, const CUtensorM
 }
 
 struct ScorePlan {
+    int few, np;                              // CTAs of the few rows' kernel or 0; statistics of a row
     int cand; bool all; int64_t groups, stride;
     int64_t off_score, off_hit, off_rec, off_second, off_longest, total;
     bool longest;
 };
 
-static ScorePlan score_plan(const HeadPlan& q, int64_t T, int64_t V, int top) {
+static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
+    const int64_t T = o.T, V = o.V;
     ScorePlan f{};
+    f.few = score_few_ctas(o);
+    f.np = f.few ? f.few : (int)(2 * q.nt);
     f.off_score = q.base;
-    f.off_hit = f.off_score + up256(2 * q.nt * T * 16);
+    f.off_hit = f.off_score + up256(f.np * T * 16);
     f.off_rec = f.off_hit + up256(T * 4);
     f.total = f.off_rec;
     if (top > 0) {
@@ -468,6 +481,8 @@ static ScorePlan score_plan(const HeadPlan& q, int64_t T, int64_t V, int top) {
         f.stride = 16 * q.nt;
         // few groups for each candidate: most would be taken whole, or there are not enough of them
         f.all = V <= 2048 || V < 32 * f.cand;
+        if (f.all) f.few = 0;
+        f.np = f.few ? f.few : (int)(2 * q.nt);
         f.off_second = f.off_rec + up256(f.all ? T * V * 4 : T * f.stride * 4);
         f.off_longest = f.off_second + (f.all ? 0 : up256(T * f.stride * 4));
         f.total = f.off_longest + 256;
@@ -497,8 +512,7 @@ static cudaError_t launch_top(const ScoreRows& p, cudaStream_t st) {
     const int smem = (int)score_top_smem(ALL, p.cand);
     const cudaError_t e = allow_smem(score_top_kernel<T, ALL, THREADS>, (int)score_top_smem(ALL, std::min(THREADS, SWX_MAX_TOP + SC_EXTRA)));
     if (e != cudaSuccess) return e;
-    score_top_kernel<T, ALL, THREADS><<<(unsigned)p.T, THREADS, smem, st>>>(p);
-    return cudaGetLastError();
+    return launch_after(score_top_kernel<T, ALL, THREADS>, (unsigned)p.T, THREADS, smem, st, p);
 }
 
 template <typename T>
@@ -518,7 +532,7 @@ int64_t swx_logprob_args_size(void) { return (int64_t)sizeof(swx_logprob_args); 
 
 int64_t swx_logprob_fwd_workspace_bytes(const swx_logprob_args* a) {
     const int c = score_check(a);
-    return c != SWX_OK ? -c : score_plan(head_plan(ops_of(a)), a->tokens, a->vocab, a->top_k).total;
+    return c != SWX_OK ? -c : score_plan(ops_of(a), head_plan(ops_of(a)), a->top_k).total;
 }
 
 int64_t swx_logprob_bwd_workspace_bytes(const swx_logprob_args* a) {
@@ -536,7 +550,7 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         return SWX_ERR_INVALID_ARG;
     const HeadOps o = ops_of(a);
     const HeadPlan q = head_plan(o);
-    const ScorePlan f = score_plan(q, o.T, o.V, a->top_k);
+    const ScorePlan f = score_plan(o, q, a->top_k);
     if (a->workspace_bytes < f.total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
@@ -552,18 +566,19 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
     g.largest = reinterpret_cast<float*>(ws + f.off_rec); g.runner_up = reinterpret_cast<float*>(ws + f.off_second);
     g.all = reinterpret_cast<float*>(ws + f.off_rec);
     g.counter = f.longest ? reinterpret_cast<int*>(ws + f.off_longest) : nullptr;
-    const cudaError_t e = a->top_k == 0 ? launch_score(g, mx, mw, st)
+    const cudaError_t e = f.few ? launch_score_few(g, o, x, w, a->top_k > 0, f.few, st)
+                          : a->top_k == 0 ? launch_score(g, mx, mw, st)
                           : f.all       ? launch_logits<XE_SCORE_ALL>(g, mx, mw, mx, st)
                                         : launch_logits<XE_SCORE_TOP>(g, mx, mw, mx, st);
     if (e != cudaSuccess) return SWX_ERR_CUDA;
     ScoreRows p{};
-    p.T = o.T; p.V = o.V; p.d = o.d; p.np = (int)(2 * q.nt);
+    p.T = o.T; p.V = o.V; p.d = o.d; p.np = f.np;
     p.score = g.score; p.hit = g.hit; p.target = a->targets; p.ignore = a->ignore_index;
     p.k2 = g.k2;
     p.row_max = a->row_max; p.row_sum = a->row_sum; p.log_probs = a->log_probs; p.entropy = a->entropy;
     if (a->top_k == 0) {
-        score_rows_kernel<<<(unsigned)((o.T + SC_THREADS / 32 - 1) / (SC_THREADS / 32)), SC_THREADS, 0, st>>>(p);
-        return cudaGetLastError() == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
+        const unsigned grid = (unsigned)((o.T + SC_THREADS / 32 - 1) / (SC_THREADS / 32));
+        return launch_after(score_rows_kernel, grid, SC_THREADS, 0, st, p) == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
     }
     p.top = a->top_k; p.cand = f.cand; p.largest = g.largest; p.runner_up = g.runner_up; p.stride = f.stride; p.all = g.all; p.groups = f.groups;
     p.top_log_probs = a->top_log_probs; p.top_ids = a->top_ids;

@@ -108,6 +108,8 @@ def _run(x, w, y, g, h, **kw):
     (1, 1, 1, BF, 1, 1.0), (1, 65, 17, BF, 65, 1.0), (5, 300, 8, FP, 20, 0.7), (256, 256, 64, BF, 0, 1.0), (257, 257, 65, BF, 7, 1.5),
     (300, 513, 200, FP, 0, 2.0), (70, 2049, 40, BF, 5, 1.0), (130, 3001, 72, FP, 128, 1.0), (33, 5001, 40, FP, 3, 0.5),
     (520, 9001, 264, BF, 31, 1.0), (64, 300, 1030, FP, 64, 1.0), (40, 20011, 128, BF, 128, 1.0), (3, 50001, 64, BF, 1, 3.0),
+    (16, 9001, 1030, BF, 20, 1.0), (9, 4001, 33, BF, 0, 0.7), (1, 12345, 1024, BF, 128, 1.0), (8, 2049, 8, BF, 2, 1.0), (17, 2100, 64, BF, 4, 1.0),
+    (15, 3001, 4104, BF, 11, 2.0), (2, 2500, 2304, BF, 5, 1.0), (7, 3001, 40, FP, 9, 1.0),
 ])
 def test_values_alternatives_and_gradients(T, V, d, dtype, top, temp):
     x, w, y = _inputs(T, V, d, dtype, seed=T + V)
@@ -237,11 +239,13 @@ def test_ignored_and_bad_targets():
         assert torch.equal(out.log_probs[5:], base.log_probs[5:]) and torch.equal(dx[5:], bdx[5:])
 
 
-def test_words_that_weights_of_infinity_mask():
-    x, w, y = _inputs(40, 300, 32, BF, ignored=0.0)
+@pytest.mark.parametrize("T,V", [(40, 300), (40, 3000), (11, 3000)])
+def test_words_that_weights_of_infinity_mask(T, V):
+    x, w, y = _inputs(T, V, 32, BF, ignored=0.0)
     x = x.abs() + 0.125
-    keep = torch.ones(300, dtype=torch.bool, device=DEV)
-    keep[[5, 40, 41, 299]] = False
+    keep = torch.ones(V, dtype=torch.bool, device=DEV)
+    keep[[5, 40, 41, V - 1]] = False
+    keep[96:160] = False                                                  # whole groups
     w[~keep] = -math.inf
     y[~keep[y]] = 6
     out = linear_log_probs(x, w, y, top_k=20)
@@ -257,7 +261,7 @@ def test_words_that_weights_of_infinity_mask():
     x[3, 2] = math.nan
     out = linear_log_probs(x, w, y, top_k=20)
     assert torch.isnan(out.log_probs[3]) and torch.isnan(out.entropy[3])
-    assert bool((out.top_ids >= 0).all() & (out.top_ids < 300).all()) and out.top_ids[3].unique().numel() == 20
+    assert bool((out.top_ids >= 0).all() & (out.top_ids < V).all()) and out.top_ids[3].unique().numel() == 20
 
 
 def test_layouts():
