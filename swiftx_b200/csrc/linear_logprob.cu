@@ -225,25 +225,47 @@ __device__ __forceinline__ void candidate_products(const __nv_bfloat16* x, const
     }
 }
 
-// The same product of one row of the weight, exact but for fp64's rounding (2^-53 of the magnitudes).
-template <typename T>
-__device__ __forceinline__ double product_exact(const T* x, const T* w, int64_t d, bool vec, int lane) {
-    constexpr int N = 16 / sizeof(T);
+// The same product of one row of the weight, exact but for a last rounding.  fp32 operands: in fp64 (2^-53 of the magnitudes).
+__device__ __forceinline__ double product_exact(const float* x, const float* w, int64_t d, bool vec, int lane) {
     double a = 0.;
     int64_t tail = 0;
     if (vec) {
-#pragma unroll 2
-        for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
-            const uint4 qx = *reinterpret_cast<const uint4*>(x + k), qw = *reinterpret_cast<const uint4*>(w + k);
-            float2 xv[N / 2], v[N / 2];
-            unpack(x, qx, xv);
-            unpack(x, qw, v);
-#pragma unroll
-            for (int j = 0; j < N / 2; ++j) a = fma((double)xv[j].x, (double)v[j].x, fma((double)xv[j].y, (double)v[j].y, a));
+#pragma unroll 4
+        for (int64_t k = lane * 4; k + 4 <= d; k += 128) {
+            const float4 xv = *reinterpret_cast<const float4*>(x + k), v = *reinterpret_cast<const float4*>(w + k);
+            a = fma((double)xv.x, (double)v.x, fma((double)xv.y, (double)v.y, fma((double)xv.z, (double)v.z, fma((double)xv.w, (double)v.w, a))));
         }
-        tail = d / N * N;
+        tail = d / 4 * 4;
     }
-    for (int64_t k = tail + lane; k < d; k += 32) a = fma((double)Elem<T>::to_f(x[k]), (double)Elem<T>::to_f(w[k]), a);
+    for (int64_t k = tail + lane; k < d; k += 32) a = fma((double)x[k], (double)w[k], a);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    return a;
+}
+// bf16 operands: the products (16 bits) are exact in fp32; a lane sums its own with what each addition rounds off kept in a second
+// sum (Knuth's two-sum; hi + lo is good to about 2^-46 of the magnitudes), the lanes' sums are added in fp64.
+struct TwoSum {
+    float2 hi = {0.f, 0.f}, lo = {0.f, 0.f};
+    __device__ __forceinline__ void add(float2 p) {
+        const float2 s = add2(hi, p), b = add2(s, f2(-hi.x, -hi.y));
+        const float2 r = add2(hi, f2(b.x - s.x, b.y - s.y)), q = add2(p, f2(-b.x, -b.y));
+        lo = add2(lo, add2(r, q));
+        hi = s;
+    }
+    static __device__ __forceinline__ double one(float h, float l) { return isinf(h) ? (double)h : (double)h + (double)l; }
+    __device__ __forceinline__ double value() const { return one(hi.x, lo.x) + one(hi.y, lo.y); }
+};
+__device__ __forceinline__ double product_exact(const __nv_bfloat16* x, const __nv_bfloat16* w, int64_t d, bool, int lane) {
+    TwoSum s[2];
+#pragma unroll 1
+    for (int64_t k = lane * 8; k < d; k += 256) {
+        float2 xv[4], v[4];
+        unpack(x, load8(x, k, d), xv);
+        unpack(x, load8(w, k, d), v);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j & 1].add(mul2(xv[j], v[j]));
+    }
+    double a = s[0].value() + s[1].value();
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     return a;
@@ -389,7 +411,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     __syncthreads();
     for (int i = warp; i < nc; i += THREADS / 32) {
         const int c = col[i];
-        const double z = c >= 0 ? ze[i].x : product_exact<T>(x, w + (int64_t)~c * p.w_sr, p.d, p.vec, lane);
+        const double z = c >= 0 ? ze[i].x : product_exact(x, w + (int64_t)~c * p.w_sr, p.d, p.vec, lane);
         __syncwarp();
         if (lane == 0) {
             val[i] = order_key(z);
@@ -423,25 +445,34 @@ __global__ void __launch_bounds__(256) longest_word_kernel(const T* w, int64_t w
     constexpr int N = 16 / sizeof(T);
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     float top = 0.f;
-    for (int64_t v = (int64_t)blockIdx.x * 8 + warp; v < V; v += (int64_t)gridDim.x * 8) {
-        const T* r = w + v * w_sr;
-        float2 s = {0.f, 0.f};
+    const int64_t step = (int64_t)gridDim.x * 8;
+    for (int64_t v = (int64_t)blockIdx.x * 8 + warp; v < V; v += 2 * step) {
+        const T* r[2] = {w + v * w_sr, w + min(v + step, V - 1) * w_sr};
+        float2 s[2] = {};
         int64_t tail = 0;
         if (vec) {
 #pragma unroll 4
             for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
-                float2 q[N / 2];
-                unpack(r, *reinterpret_cast<const uint4*>(r + k), q);
+                float2 q[2][N / 2];
 #pragma unroll
-                for (int j = 0; j < N / 2; ++j) s = fma2(q[j], q[j], s);
+                for (int i = 0; i < 2; ++i) unpack(r[i], *reinterpret_cast<const uint4*>(r[i] + k), q[i]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < N / 2; ++j) s[i] = fma2(q[i][j], q[i][j], s[i]);
             }
             tail = d / N * N;
         }
-        for (int64_t k = tail + lane; k < d; k += 32) { const float q = Elem<T>::to_f(r[k]); s.x = fmaf(q, q, s.x); }
-        float t = s.x + s.y;
+        for (int64_t k = tail + lane; k < d; k += 32)
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-        top = t == t ? fmaxf(top, t) : INFINITY;
+            for (int i = 0; i < 2; ++i) { const float q = Elem<T>::to_f(r[i][k]); s[i].x = fmaf(q, q, s[i].x); }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            float t = s[i].x + s[i].y;
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+            top = t == t ? fmaxf(top, t) : INFINITY;
+        }
     }
     if (lane == 0) most[warp] = top;
     __syncthreads();
@@ -486,8 +517,9 @@ static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
         f.off_second = f.off_rec + up256(f.all ? T * V * 4 : T * f.stride * 4);
         f.off_longest = f.off_second + (f.all ? 0 : up256(T * f.stride * 4));
         f.total = f.off_longest + 256;
-        // the words' norms are one read of the weight, and without them every candidate's word is read
-        f.longest = T * f.cand > V;
+        // the words' norms are one read of the weight, and without them every candidate's word is read (64 MB of them, which
+        // come from the L2 as a rule, take less time than a launch and its read)
+        f.longest = T * f.cand > V && T * f.cand * o.d * q.es > (int64_t(64) << 20);
     }
     return f;
 }
@@ -517,8 +549,8 @@ static cudaError_t launch_top(const ScoreRows& p, cudaStream_t st) {
 
 template <typename T>
 static cudaError_t launch_top(const ScoreRows& p, bool all, cudaStream_t st) {
-    // few rows: more warps for each one's candidates
-    if (p.cand <= 128 && p.T > 148) return all ? launch_top<T, true, 128>(p, st) : launch_top<T, false, 128>(p, st);
+    // many candidates (a threshold needs many more shares than those), or few rows (more warps for each): larger CTAs
+    if (p.cand <= 64 && p.T > 148) return all ? launch_top<T, true, 128>(p, st) : launch_top<T, false, 128>(p, st);
     return all ? launch_top<T, true, 256>(p, st) : launch_top<T, false, 256>(p, st);
 }
 

@@ -190,9 +190,10 @@ template <typename T, bool TOP, int THREADS>
 static cudaError_t launch_token(const TokenRows& p, int64_t rows, cudaStream_t st) {
     auto k = token_logprob_kernel<T, TOP, THREADS>;
     const size_t smem = TOP ? (size_t)(topk_capacity(p.top, TL_PER) + p.top) * 8 : 0;
-    if (TOP) {
-        const cudaError_t e = allow_smem(k, (topk_capacity(SWX_MAX_TOP, TL_PER) + SWX_MAX_TOP) * 8);
-        if (e != cudaSuccess) return e;
+    static_assert((topk_capacity(SWX_MAX_TOP, TL_PER) + SWX_MAX_TOP) * 8 <= 40 * 1024, "more shared memory than a launch has by itself");
+    if (p.parts == 1) {
+        k<<<(unsigned)rows, THREADS, smem, st>>>(p);
+        return cudaGetLastError();
     }
     cudaLaunchConfig_t c{};
     c.gridDim = dim3((unsigned)(rows * p.parts));

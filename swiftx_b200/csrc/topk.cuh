@@ -27,7 +27,8 @@ __device__ __forceinline__ uint32_t key_index(uint64_t k) { return ~(uint32_t)k;
 // Entries that TopK's buffer holds for `k` and `per` keys a thread: what is kept, and a batch's passers.
 constexpr int topk_capacity(int k, int per) { return k * (per + 1); }
 
-// A threshold that at least k of the THREADS threads' values (order_key bits) reach, and at most k + k / 4 where the values differ,
+// A threshold that at least k of the THREADS threads' values (order_key bits) reach, and few more where the values differ (a quarter
+// of k, and of the threads that are not among the k: close to all of them the values say little about the whole),
 // by one warp: the bits of the k-th largest are set from the top, over those that differ, until it is that close.
 // scratch: THREADS + 1 words; all threads call it.
 template <int THREADS>
@@ -54,7 +55,7 @@ __device__ __forceinline__ uint32_t about_kth(uint32_t mine, int k, uint32_t* sc
             for (int j = 0; j < N; ++j) n += v[j] >= c;
             n = __reduce_add_sync(0xffffffffu, n);
             if (n >= k) t = c;
-            if (n >= k && n <= k + k / 4) break;
+            if (n >= k && n <= k + min(k, THREADS - k) / 4) break;
         }
         if (threadIdx.x == 0) scratch[THREADS] = t;
     }
@@ -158,6 +159,7 @@ struct TopK {
         for (int i = threadIdx.x; i < n; i += THREADS) {
             const uint64_t mine = buf[i];
             int r = 0;
+#pragma unroll 4
             for (int j = 0; j < n; ++j) r += buf[j] > mine;
             if (r < k) kept[r] = mine;
         }

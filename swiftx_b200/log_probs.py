@@ -24,11 +24,15 @@ class LogProbs(NamedTuple):
 
 def _outputs(a, like, T, top_k, with_log_probs=True):
     """(log_probs, entropy, top_log_probs, top_ids), set in the argument struct."""
-    lp = like.new_empty(T, dtype=torch.float32) if with_log_probs else None
     ent = like.new_empty(T, dtype=torch.float32)
-    vals = like.new_empty((T, top_k), dtype=torch.float32) if top_k else None
-    ids = like.new_empty((T, top_k), dtype=torch.int64) if top_k else None
-    a.log_probs, a.entropy, a.top_log_probs, a.top_ids = (t.data_ptr() if t is not None else None for t in (lp, ent, vals, ids))
+    a.entropy = ent.data_ptr()
+    lp = vals = ids = None
+    if with_log_probs:
+        lp = torch.empty_like(ent)
+        a.log_probs = lp.data_ptr()
+    if top_k:
+        vals, ids = ent.new_empty((T, top_k)), ent.new_empty((T, top_k), dtype=torch.int64)
+        a.top_log_probs, a.top_ids = vals.data_ptr(), ids.data_ptr()
     return lp, ent, vals, ids
 
 
@@ -153,7 +157,7 @@ def token_log_probs(logits, targets=None, top_k=0, temperature=1.0, ignore_index
         a.top_k, a.temperature, a.ignore_index = top_k, temperature, ignore_index
         t1 = None
         if targets is not None:
-            t1 = targets.reshape(-1).contiguous()
+            t1 = (targets if targets.dim() == 1 else targets.reshape(-1)).contiguous()
             a.targets = t1.data_ptr()
         out = _outputs(a, z, z.shape[0], top_k, targets is not None)
         _lib.check(lib.swx_token_logprob(a, _lib.stream_ptr(z.device)), "swx_token_logprob")
