@@ -526,9 +526,9 @@ int swx_token_logprob(const swx_logprob_args* args, void* stream);
  * enters, NaN.  The same id may stand in several entries of a row (their q add up).
  * teacher_ids (tokens, entries) int64, teacher_logits (tokens, entries) in teacher_dtype (fp32 or
  * bf16), row strides ids_sr and tl_sr; 1 <= entries <= SWX_MAX_TOP.  Operands, loss, count and gradients as
- * in swx_xent_args.  Forward writes row_max, row_sum (tokens values; row_sum -1 for a row
- * that does not count) and entry_logits (tokens, entries; the student's logits of the used entries) for the backward.
- * Deterministic.  The workspace starts on 16 bytes. */
+ * in swx_xent_args.  Forward leaves in `saved` (swx_distill_saved_bytes) what the backward reads of it: the rows' statistics, and
+ * the teacher's words with their shares and the student's logits; the backward does not read the teacher's tensors.
+ * Deterministic.  Workspace and saved start on 16 bytes. */
 typedef struct swx_distill_args {
     int64_t tokens, vocab, dim, entries;
     int32_t dtype;                    /* x, weight, dx: SWX_DTYPE_F32 or SWX_DTYPE_BF16 */
@@ -543,9 +543,7 @@ typedef struct swx_distill_args {
     const void* teacher_logits; int64_t tl_sr;
     float* loss;
     float* count;
-    float* row_max;
-    float* row_sum;
-    float* entry_logits;
+    void* saved; int64_t saved_bytes;
     const float* dloss;               /* backward */
     void* dx;
     void* dweight;
@@ -553,6 +551,7 @@ typedef struct swx_distill_args {
 } swx_distill_args;
 
 int64_t swx_distill_args_size(void);
+int64_t swx_distill_saved_bytes(const swx_distill_args* args);
 int64_t swx_distill_fwd_workspace_bytes(const swx_distill_args* args);
 int64_t swx_distill_bwd_workspace_bytes(const swx_distill_args* args);
 int swx_distill_fwd(const swx_distill_args* args, void* stream);

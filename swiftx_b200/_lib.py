@@ -156,7 +156,7 @@ class DistillArgs(ctypes.Structure):
         ("temperature", ctypes.c_float), ("reserved", i32),
         ("x", vp), ("x_sr", i64), ("weight", vp), ("w_sr", i64),
         ("teacher_ids", vp), ("ids_sr", i64), ("teacher_logits", vp), ("tl_sr", i64),
-        ("loss", vp), ("count", vp), ("row_max", vp), ("row_sum", vp), ("entry_logits", vp),
+        ("loss", vp), ("count", vp), ("saved", vp), ("saved_bytes", i64),
         ("dloss", vp), ("dx", vp), ("dweight", vp), ("workspace", vp), ("workspace_bytes", i64),
     ]
 
@@ -247,6 +247,8 @@ def load():
         for fn in (f"swx_{op}_fwd_workspace_bytes", f"swx_{op}_bwd_workspace_bytes"):
             getattr(lib, fn).restype = i64
             getattr(lib, fn).argtypes = [ctypes.POINTER(st)]
+    lib.swx_distill_saved_bytes.restype = i64
+    lib.swx_distill_saved_bytes.argtypes = [ctypes.POINTER(DistillArgs)]
     for fn in ("swx_linattn_fwd_workspace_bytes", "swx_linattn_bwd_workspace_bytes"):
         getattr(lib, fn).restype = i64
         getattr(lib, fn).argtypes = [ctypes.POINTER(LinattnArgs)]

@@ -38,11 +38,14 @@ constexpr int XE_KSUB_LOGITS = 8;
 constexpr uint32_t XE_POLLS = 1u << 24;       // about a second
 
 // Epilogues: XE_LSE (loss) and XE_SCORE* (log probabilities: statistics of scaled logits, with the entropy's sum; for the top
-// alternatives also each 32 columns' two largest logits, or the logits themselves) read logits, XE_PROB and
-// XE_GRAD write the logits' gradient, XE_DX and XE_DW are the gradient products.
-enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW, XE_SCORE, XE_SCORE_TOP, XE_SCORE_ALL, XE_GRAD };
-constexpr bool is_score(int epi) { return epi == XE_SCORE || epi == XE_SCORE_TOP || epi == XE_SCORE_ALL; }
-constexpr bool is_dlogit(int epi) { return epi == XE_PROB || epi == XE_GRAD; }
+// alternatives also the two largest logits of 16 columns, or the logits themselves; for distillation the logits at each row's
+// words) read logits, XE_PROB and XE_GRAD* write the logits' gradient (XE_GRAD_IDS: with a row's words apart), XE_DX and XE_DW are
+// the gradient products.
+enum XentEpi { XE_LSE, XE_PROB, XE_DX, XE_DW, XE_SCORE, XE_SCORE_TOP, XE_SCORE_ALL, XE_SCORE_IDS, XE_GRAD, XE_GRAD_IDS };
+constexpr bool is_score(int epi) { return epi == XE_SCORE || epi == XE_SCORE_TOP || epi == XE_SCORE_ALL || epi == XE_SCORE_IDS; }
+constexpr bool is_grad(int epi) { return epi == XE_GRAD || epi == XE_GRAD_IDS; }
+constexpr bool is_dlogit(int epi) { return epi == XE_PROB || is_grad(epi); }
+constexpr bool has_ids(int epi) { return epi == XE_SCORE_IDS || epi == XE_GRAD_IDS; }
 constexpr bool is_logits(int epi) { return epi == XE_LSE || is_score(epi) || is_dlogit(epi); }
 constexpr float SCORE_FLOOR = -0x1p73f;       // below every logit that counts (-9e21): times log2(e) / temperature it stays finite
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -84,6 +87,9 @@ struct XentGemm {
     // low 4 bits; columns from N on count as SCORE_FLOOR
     float* largest; float* runner_up;
     float* all;                               // XE_SCORE_ALL, (M, N)
+    // XE_SCORE_IDS, XE_GRAD_IDS: each row's words in rising order, their logits and shares, (M, nids), and how many of them lie before
+    // each 128 columns of the vocabulary, (M, stride)
+    const int* ids; float* id_logit; const float* id_share; const uint8_t* before; int nids, before_stride;
     // XE_GRAD: dlogit = 2^u (A + B u) + [column == target] hot, see grad_row
     const float* row_sum; const float* entropy; const float* d_logp; const float* d_entropy;
 };
@@ -166,12 +172,12 @@ __device__ __forceinline__ float row_scale(const XentGemm& p, int row) {
 // A row's coefficients of XE_GRAD.  With u = z k2 - m, e = 2^u, s the sum of e: p = e / s, the log probability
 // l = u ln2 - ln s, and for upstream gradients g of the target's log probability and h of the entropy H
 //   dz = (g [v == y] - p (g + h (l + H))) / temperature = e (A + B u) + [v == y] hot.
-// Distillation (no targets): dz = p c / temperature with c = temperature^2 times the row's upstream gradient; the
-// teacher's words are set afterwards.
+// Distillation (no targets): dz = (p - Q) c / temperature with c = temperature^2 times the row's upstream gradient and Q the
+// word's share, if it is one of the teacher's.
 struct GradRow { float A, B, hot; };
 __device__ __forceinline__ GradRow grad_row(const XentGemm& p, int row) {
     const float s = p.row_sum[row];
-    if (!p.target) {
+    if (!p.target) {                          // (XE_GRAD_IDS: at a row's words, less their share of c temperature)
         const float c = p.reduction == SWX_XENT_NONE ? p.dloss[row] : 1.f;
         return GradRow{s > 0.f ? c / (p.inv_temp * s) : s < 0.f ? 0.f : __int_as_float(0x7fc00000), 0.f, 0.f};     // s < 0: a row that does not count
     }
@@ -373,16 +379,37 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
             float scale = 0.f, rmax = 0.f, rsum = 0.f;
             GradRow gr{0.f, 0.f, 0.f};
             if (is_logits(EPI) && live) {
-                if (!(is_score(EPI) || EPI == XE_GRAD) || p.target) y = p.target[row] - p.col0;
-                if (EPI == XE_GRAD) {
+                if (!(is_score(EPI) || is_grad(EPI)) || (!has_ids(EPI) && p.target)) y = p.target[row] - p.col0;
+                if (is_grad(EPI)) {
                     gr = grad_row(p, row);
                     rmax = p.row_max[row];
+                    if (EPI == XE_GRAD_IDS) rsum = p.row_sum[row];
                 }
                 if (EPI == XE_PROB) {
                     scale = row_scale(p, row);
                     rmax = p.row_max[row];
                     rsum = p.row_rsum[row] * scale;
                 }
+            }
+            // the row's next word in this half of the tile: its entry, its column, its logit and share (while the products run; a search
+            // among the words here instead of two counts made by then took 5 to 15 % of the product's time)
+            int id = 0, id_end = 0, word = INT32_MAX;
+            float word_z = 0.f, word_share = 0.f;
+            const int64_t words = (int64_t)row * p.nids;
+            auto fetch_word = [&] {
+                word = INT32_MAX;
+                if (id >= id_end) return;
+                word = p.ids[words + id] - p.col0;
+                if (is_grad(EPI)) {
+                    word_z = p.id_logit[words + id];
+                    word_share = p.id_share[words + id];
+                }
+            };
+            if (has_ids(EPI) && live && c0 < p.N) {
+                const uint8_t* b = p.before + (int64_t)row * p.before_stride + (p.col0 + c0) / 128;       // (a piece starts at a whole tile)
+                id = b[0];
+                id_end = b[1];
+                fetch_word();
             }
             if (!mbar_wait_cluster(&acc_full[a], aph, XE_POLLS)) { ok = false; break; }
             tc_fence_after();
@@ -434,6 +461,19 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
 #pragma unroll
                         for (int j = 0; j < 32; ++j) h = yc == j ? v[j] : h;
                         if (y < p.N) p.hit[row] = h;
+                    }
+                    if (EPI == XE_SCORE_IDS && __any_sync(0xffffffffu, word < cc + 32)) {
+                        // the columns through shared memory (16-byte parts of a lane's row swapped about, against bank conflicts)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<float4*>(so + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                        while (word < cc + 32) {
+                            const int j = word - cc;
+                            p.id_logit[words + id] = *reinterpret_cast<const float*>(so + lane * 128 + (((j >> 2) ^ (lane & 7)) << 4) + (j & 3) * 4);
+                            ++id;
+                            fetch_word();
+                        }
+                        __syncwarp();
                     }
                     if (EPI == XE_SCORE_ALL && live) {
                         float* o = p.all + (int64_t)row * p.N + cc;
@@ -496,7 +536,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     }
                     m = nm;
                 } else if (is_dlogit(EPI)) {
-                    if (EPI == XE_GRAD) {
+                    if (is_grad(EPI)) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
                             const float u = fmaf(v[j], p.k2, -rmax);
@@ -508,9 +548,9 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     }
                     if (yc >= 0 && yc < 32) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = yc == j ? v[j] - (EPI == XE_GRAD ? -gr.hot : scale) : v[j];
+                        for (int j = 0; j < 32; ++j) v[j] = yc == j ? v[j] - (is_grad(EPI) ? -gr.hot : scale) : v[j];
                     }
-                    if (EPI == XE_GRAD ? gr.A == 0.f && gr.B == 0.f && gr.hot == 0.f : scale == 0.f) {   // a token that does not count, whatever its logits
+                    if (is_grad(EPI) ? gr.A == 0.f && gr.B == 0.f && gr.hot == 0.f : scale == 0.f) {   // a token that does not count, whatever its logits
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = 0.f;
                     }
@@ -535,6 +575,20 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                             const int at_b = p.planes > 1 ? lane * 64 + j * 16
                                                           : lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4);
                             *reinterpret_cast<uint4*>(so + at_b) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                        }
+                        if (EPI == XE_GRAD_IDS) {
+                            // the row's words among these columns: their own values, in place of what was just written
+                            const int id0 = id;
+                            while (word < cc + 32) {
+                                float r = gr.A * (ex2(fmaf(word_z, p.k2, -rmax)) - rsum * word_share);
+                                for (int q = 0; q < pl; ++q) r -= __bfloat162float(__float2bfloat16_rn(r));
+                                const int j = word - cc;
+                                const int at_b = p.planes > 1 ? lane * 64 + j * 2 : lane * 128 + ((((c & 1) * 4 + (j >> 3)) ^ (lane & 7)) << 4) + (j & 7) * 2;
+                                *reinterpret_cast<__nv_bfloat16*>(so + at_b) = __float2bfloat16_rn(r);
+                                ++id;
+                                fetch_word();
+                            }
+                            if (pl + 1 < p.planes && id != id0) { id = id0; fetch_word(); }
                         }
                         if (p.planes > 1 || (c & 1)) {
                             fence_proxy_async_smem();
@@ -692,20 +746,14 @@ static cudaError_t launch_logits(const XentGemm& g, const CUtensorMap& x, const 
                          : launch_gemm<EPI, false, false>(g, x, w, store, XE_PAIRS, st);
 }
 
-// The scoring and gradient epilogues that more than one operator uses (linear_logprob.cu).
-cudaError_t launch_score(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, cudaStream_t st);
-cudaError_t launch_grad(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& store, cudaStream_t st);
-
 // The scoring of a few rows without tiles (linear_logprob_few.cu): its CTAs, 0 where it does not take them, and the launch.
 int score_few_ctas(const HeadOps& o);
 cudaError_t launch_score_few(const XentGemm& g, const HeadOps& o, const Operand& x, const Operand& w, bool top, int ctas, cudaStream_t st);
 
 // The gradients, piece by piece of the vocabulary: the logits again and dlogit in the epilogue (`launch`, with the
-// fields that `fill` sets), whatever `patch` does to the piece (its base, first column and columns; a status), and the
-// two products.
-template <class Launch, class Fill, class Patch>
-static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const HeadGrads& gr, cudaStream_t st, Launch launch, Fill fill,
-                         Patch patch) {
+// fields that `fill` sets), and the two products.
+template <class Launch, class Fill>
+static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const HeadGrads& gr, cudaStream_t st, Launch launch, Fill fill) {
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
     Operand x, w;
     head_operands(o, q, ws, x, w, st);
@@ -720,8 +768,7 @@ static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const
         XentGemm g = logits_gemm(o, q, c0, cw, status);
         fill(g);
         if (launch(g, x_k, w_k, p_st, st) != cudaSuccess) return SWX_ERR_CUDA;
-        int c = patch(reinterpret_cast<__nv_bfloat16*>(ws + q.off_p), c0, cw);
-        if (c == SWX_OK) c = head_piece_products(o, q, ws, x, w, pr, gr, c0, cw, status, st);
+        const int c = head_piece_products(o, q, ws, x, w, pr, gr, c0, cw, status, st);
         if (c != SWX_OK) return c;
     }
     return SWX_OK;

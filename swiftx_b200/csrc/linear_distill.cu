@@ -1,143 +1,184 @@
 // Distillation of a linear head from a teacher's top logits, without keeping the student's logits:
 //   q = softmax over a row's used entries of t / tau,  l_v = z_v / tau - log sum exp(z / tau),  z = x W^T,
-//   loss = tau^2 sum_j q_j (log q_j - l_{id_j}),  dz_v = tau c (p_v - sum_j q_j [v == id_j]),
-// with p = e^l and c the row's upstream gradient (over the number of rows that count for the mean).
+//   loss = tau^2 sum_j q_j (log q_j - l_{id_j}),  dz_v = tau c (p_v - Q_v),
+// with p = e^l, Q_v the sum of the q of the entries of word v and c the row's upstream gradient (over the number of rows
+// that count for the mean).
 //
-// Forward: the head's product with the statistics of head_gemm.cuh's scoring epilogue, then one CTA for each row: the
-// student's logits at the teacher's words as dot products of their own (the entries are spread over the vocabulary, at most a few
-// to a tile), the softmax of the entries and the row's loss; the last CTA adds the rows up.  Backward: as the
-// loss's, with tau p in the epilogue, and the teacher's words set to tau (p_j - q_j) by a small kernel
-// between a piece of the vocabulary's dlogit and its products, each rounded once.
+// Forward: a kernel sorts each row's words (and counts those before each half tile) and takes the softmax of its entries;
+// the head's product with the scoring epilogue of head_gemm.cuh, which also picks the logits at the words; a kernel joins
+// the rows' statistics and losses.  Backward: as the loss's, with tau c p in the epilogue, and tau c (p - Q) in its place at the
+// words before the tile leaves shared memory, each rounded once.
+// (With the words' logits as dot products of their own, 32 rows of the weight for each token, and dlogit set at the words by a
+// launch after each piece, 8192 x 50001 x 1024 took 104 and 52 us more.)
 #include "head_gemm.cuh"
 
 namespace swx {
 
-constexpr int DI_THREADS = 128, DI_WARPS = DI_THREADS / 32, DI_PATCH_WARPS = 4;
-constexpr int DI_LANE = SWX_MAX_TOP / 32;     // entries of a lane
+constexpr int DI_WARPS = 4, DI_THREADS = 32 * DI_WARPS;
+constexpr float DI_LN2 = 0.69314718055994531f;
+
+// What the forward leaves for the backward: rows' statistics, and their words.
+struct DistillSaved {
+    float* row_max; float* row_sum; float* teacher;    // (T): the teacher's sum q log q
+    int* ids; float* share; float* logit;              // (T, K), ids in rising order and INT32_MAX behind them
+    uint8_t* before; int stride;                       // (T, stride): how many ids lie before each 128 columns
+};
 
 struct DistillRows {
-    int64_t T, V, d;
+    int64_t T, V;
     int K, np;
     const float4* score;
     float k2, inv_temp;
     const int64_t* ids; int64_t ids_sr; const void* logits; int64_t tl_sr; int tl_bf16;
-    const void* x; int64_t x_sr; const void* w; int64_t w_sr; int vec;
-    float* row_max; float* row_sum; float* z;
+    DistillSaved s;
     float* rows; double2* sums; float* loss; float* count; int reduction; int* counter;
-    // backward
-    const float* dloss; __nv_bfloat16* dz; int64_t ld, plane; int planes; int64_t c0, cw;
 };
 
-// A warp's softmax over the entries of a row: q (0 where not used), ids, whether an entry is used, whether one is outside the vocabulary.
-__device__ __forceinline__ void teacher_row(const DistillRows& p, int64_t row, int lane, float (&q)[DI_LANE], int64_t (&id)[DI_LANE], bool& live, bool& bad) {
+// Warp = one row, NL entries a lane: the softmax of its used entries, and its different words in rising order with their shares.
+// row_sum: 1 for a row that counts, -1 for one that does not, NaN for one with a bad entry (no words then).
+template <int NL>
+__global__ void __launch_bounds__(DI_THREADS) distill_prepare_kernel(const DistillRows p) {
+    __shared__ int sorted[DI_WARPS][32 * NL + 1];
+    const int64_t row = (int64_t)blockIdx.x * DI_WARPS + threadIdx.x / 32;
+    if (row >= p.T) return;
+    const int lane = threadIdx.x % 32;
+    int* mine = sorted[threadIdx.x / 32];
+    float q[NL], all[NL];
+    int id[NL];
+    bool first[NL], odd = false;
     float top = -INFINITY;
-    bad = false;
-    bool nan = false;
 #pragma unroll
-    for (int i = 0; i < DI_LANE; ++i) {
+    for (int i = 0; i < NL; ++i) {
         const int j = lane + 32 * i;
         id[i] = -1;
         q[i] = -INFINITY;
         if (j < p.K) {
-            id[i] = p.ids[row * p.ids_sr + j];
+            const int64_t v = p.ids[row * p.ids_sr + j];
             const float t = p.tl_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[row * p.tl_sr + j])
                                       : static_cast<const float*>(p.logits)[row * p.tl_sr + j];
-            if (id[i] >= 0) q[i] = t * p.inv_temp;
+            if (v >= 0 && t != -INFINITY) {
+                odd |= v >= p.V || t != t || t == INFINITY;
+                id[i] = v < p.V ? (int)v : 0;
+                q[i] = t * p.inv_temp;
+            }
         }
-        if (q[i] == -INFINITY) id[i] = -1;
-        bad |= id[i] >= p.V;
-        nan |= q[i] != q[i];
         top = fmaxf(top, q[i]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    bad = __any_sync(0xffffffffu, bad || nan || top == INFINITY);
-    live = bad || top > -INFINITY;
+    const bool bad = __any_sync(0xffffffffu, odd);
+    bool some = false;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < DI_LANE; ++i) {
-        q[i] = id[i] < 0 ? 0.f : ex2((q[i] - top) * LOG2E);
+    for (int i = 0; i < NL; ++i) {
+        some |= id[i] >= 0;
+        q[i] = id[i] < 0 ? 0.f : ex2((q[i] - (top == -INFINITY ? 0.f : top)) * LOG2E);
         sum += q[i];
     }
+    const bool live = __any_sync(0xffffffffu, some);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const float r = live ? 1.f / sum : 0.f;
+    float self = 0.f;
 #pragma unroll
-    for (int i = 0; i < DI_LANE; ++i) q[i] *= r;
-}
-
-template <typename T>
-__device__ __forceinline__ float dot(const T* x, const T* w, int64_t d, bool vec, int lane) {
-    constexpr int N = 16 / sizeof(T);
-    float a[2] = {0.f, 0.f};
-    int64_t tail = 0;
-    if (vec) {
-#pragma unroll 2
-        for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
-            const uint4 qx = *reinterpret_cast<const uint4*>(x + k), qw = *reinterpret_cast<const uint4*>(w + k);
-#pragma unroll
-            for (int j = 0; j < N; ++j) a[j & 1] = fmaf(Elem<T>::to_f(reinterpret_cast<const T*>(&qx)[j]), Elem<T>::to_f(reinterpret_cast<const T*>(&qw)[j]), a[j & 1]);
-        }
-        tail = d / N * N;
+    for (int i = 0; i < NL; ++i) {
+        q[i] = live && !bad ? q[i] / sum : 0.f;
+        if (q[i] != 0.f) self += q[i] * logf(q[i]);
+        if (bad) id[i] = -1;
+        all[i] = 0.f;
+        first[i] = id[i] >= 0;
     }
-    for (int64_t k = tail + lane; k < d; k += 32) a[0] = fmaf(Elem<T>::to_f(x[k]), Elem<T>::to_f(w[k]), a[0]);
-    float s = a[0] + a[1];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    return s;
+    for (int o = 16; o > 0; o >>= 1) self += __shfl_xor_sync(0xffffffffu, self, o);
+    // a word's place is the number of smaller ones; the shares of one that stands in several entries go to the first of them, and the
+    // others count it once
+    int rank[NL] = {}, n = 0;
+#pragma unroll
+    for (int h = 0; h < NL; ++h)
+        for (int j = 0; j < min(32, p.K - 32 * h); ++j) {
+            const float qj = __shfl_sync(0xffffffffu, q[h], j);
+            const int idj = __shfl_sync(0xffffffffu, id[h], j);
+            bool again = false;               // an earlier entry is of the same word
+#pragma unroll
+            for (int i = 0; i < NL; ++i) {
+                const bool same = id[i] == idj;
+                const int apart = lane + 32 * i - (j + 32 * h);
+                all[i] += same ? qj : 0.f;
+                first[i] = first[i] && !(same && apart > 0);
+                again |= __any_sync(0xffffffffu, same && apart < 0);
+            }
+            if (idj < 0 || again) continue;
+            ++n;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) rank[i] += idj < id[i];
+        }
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const int j = lane + 32 * i;
+        if (first[i]) {
+            mine[rank[i]] = p.s.ids[row * p.K + rank[i]] = id[i];
+            p.s.share[row * p.K + rank[i]] = all[i];
+        }
+        if (j >= n && j < p.K) p.s.ids[row * p.K + j] = INT32_MAX;
+    }
+    if (lane == 0) mine[n] = INT32_MAX;
+    __syncwarp();
+    // 16 counts a lane: a search, then along the words
+    for (int h = 16 * lane; h < p.s.stride; h += 512) {
+        int at = 0;
+        for (int hi = n; at < hi;) {
+            const int mid = (at + hi) / 2;
+            if (mine[mid] < 128 * (int64_t)h) at = mid + 1;
+            else hi = mid;
+        }
+        uint32_t w[4] = {};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            while (mine[at] < 128 * ((int64_t)h + i) && at < n) ++at;
+            w[i / 4] |= (uint32_t)at << (8 * (i % 4));
+        }
+        *reinterpret_cast<uint4*>(p.s.before + row * p.s.stride + h) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (lane == 0) {
+        p.s.row_sum[row] = bad ? __int_as_float(0x7fc00000) : live ? 1.f : -1.f;
+        p.s.teacher[row] = self;
+    }
 }
 
-// CTA = one row.
-template <typename T>
+// Warp = one row: its statistics and loss.  Each CTA leaves the sum of its rows' losses and the count of its rows; the last CTA to
+// finish adds those up (fp64, a fixed order whichever CTA it is).
 __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillRows p) {
-    __shared__ int64_t sid[SWX_MAX_TOP];
-    __shared__ float sz[SWX_MAX_TOP];
-    __shared__ Score part[DI_WARPS];
     __shared__ int is_last;
     __shared__ double red[DI_WARPS][2];
-    const int64_t row = blockIdx.x;
+    wait_for_previous();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const Score a = score_join_row<DI_THREADS>(p.score + row * p.np, p.np, part);
-    float q[DI_LANE];
-    int64_t id[DI_LANE];
-    bool live = false, bad = false;
-    if (warp == 0) {
-        teacher_row(p, row, lane, q, id, live, bad);
-#pragma unroll
-        for (int i = 0; i < DI_LANE; ++i)
-            if (lane + 32 * i < p.K) sid[lane + 32 * i] = bad ? -1 : id[i];
-    }
-    __syncthreads();
-    const T* x = static_cast<const T*>(p.x) + row * p.x_sr;
-    for (int j = warp; j < p.K; j += DI_WARPS) {
-        const int64_t v = sid[j];
-        if (v < 0) continue;
-        const float z = dot<T>(x, static_cast<const T*>(p.w) + v * p.w_sr, p.d, p.vec, lane);
-        if (lane == 0) { sz[j] = z; p.z[row * p.K + j] = z; }
-    }
-    __syncthreads();
+    const int64_t row = (int64_t)blockIdx.x * DI_WARPS + warp;
     double sum = 0., n = 0.;
-    if (warp == 0) {
-        const float ls = logf(a.s);
+    if (row < p.T) {
+        const Score a = score_join_parts(p.score + row * p.np, p.np, lane, 32);
+        const float ls = logf(a.s), mark = p.s.row_sum[row];
         float loss = 0.f;
-#pragma unroll
-        for (int i = 0; i < DI_LANE; ++i)
-            if (lane + 32 * i < p.K && id[i] >= 0 && !bad && q[i] != 0.f) loss += q[i] * (logf(q[i]) - (fmaf(sz[lane + 32 * i], p.k2, -a.m) * 0.69314718055994531f - ls));
+        for (int j = lane; j < p.K; j += 32) {
+            const float share = mark > 0.f && p.s.ids[row * p.K + j] != INT32_MAX ? p.s.share[row * p.K + j] : 0.f;
+            if (share != 0.f) loss += share * (fmaf(p.s.logit[row * p.K + j], p.k2, -a.m) * DI_LN2 - ls);
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);
-        loss = bad ? __int_as_float(0x7fc00000) : loss / (p.inv_temp * p.inv_temp);
-        if (!live) loss = 0.f;
+        loss = mark < 0.f ? 0.f : mark > 0.f ? (p.s.teacher[row] - loss) / (p.inv_temp * p.inv_temp) : mark;
+        __syncwarp();
         if (lane == 0) {
-            p.row_max[row] = a.m;
-            p.row_sum[row] = !live ? -1.f : bad ? __int_as_float(0x7fc00000) : a.s;
+            p.s.row_max[row] = a.m;
+            if (mark > 0.f) p.s.row_sum[row] = a.s;
             if (p.rows) p.rows[row] = loss;
         }
         sum = loss;
-        n = live ? 1. : 0.;
+        n = mark < 0.f ? 0. : 1.;
     }
     if (p.reduction == SWX_XENT_NONE) return;
+    if (lane == 0) { red[warp][0] = sum; red[warp][1] = n; }
+    __syncthreads();
     if (threadIdx.x == 0) {
-        p.sums[row] = make_double2(sum, n);
+        for (int i = 1; i < DI_WARPS; ++i) { sum += red[i][0]; n += red[i][1]; }
+        p.sums[blockIdx.x] = make_double2(sum, n);
         __threadfence();
         is_last = atomicAdd(p.counter, 1) == (int)gridDim.x - 1;
     }
@@ -164,44 +205,6 @@ __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillR
     }
 }
 
-// Warp = one row: dlogit at the teacher's words inside the piece, tau c (p_j - q_j) in place of tau c p_j.
-__global__ void __launch_bounds__(32 * DI_PATCH_WARPS) distill_patch_kernel(const DistillRows p) {
-    const int64_t row = (int64_t)blockIdx.x * DI_PATCH_WARPS + threadIdx.x / 32;
-    if (row >= p.T) return;
-    const int lane = threadIdx.x % 32;
-    const float s = p.row_sum[row], m = p.row_max[row];
-    if (!(s > 0.f)) return;                   // a row that does not count is zero, one with a bad entry NaN throughout
-    float q[DI_LANE], all[DI_LANE];
-    int64_t id[DI_LANE];
-    bool live, bad, first[DI_LANE];
-    teacher_row(p, row, lane, q, id, live, bad);
-#pragma unroll
-    for (int i = 0; i < DI_LANE; ++i) { all[i] = 0.f; first[i] = true; }
-    for (int j = 0; j < p.K; ++j) {           // the same word may stand in several entries; its first one writes
-        float qj = 0.f;
-        int64_t idj = -1;
-#pragma unroll
-        for (int i = 0; i < DI_LANE; ++i)
-            if (j / 32 == i) { qj = __shfl_sync(0xffffffffu, q[i], j % 32); idj = __shfl_sync(0xffffffffu, id[i], j % 32); }
-#pragma unroll
-        for (int i = 0; i < DI_LANE; ++i)
-            if (id[i] == idj) { all[i] += qj; first[i] = first[i] && j >= lane + 32 * i; }
-    }
-    const float c = (p.reduction == SWX_XENT_NONE ? p.dloss[row] : 1.f) / p.inv_temp;
-#pragma unroll
-    for (int i = 0; i < DI_LANE; ++i) {
-        const int j = lane + 32 * i;
-        if (j >= p.K || id[i] < p.c0 || id[i] >= p.c0 + p.cw || !first[i]) continue;
-        float v = c * (ex2(fmaf(p.z[row * p.K + j], p.k2, -m)) / s - all[i]);
-        __nv_bfloat16* o = p.dz + row * p.ld + (id[i] - p.c0);
-        for (int k = 0; k < p.planes; ++k) {
-            const __nv_bfloat16 b = __float2bfloat16_rn(v);
-            o[k * p.plane] = b;
-            v -= __bfloat162float(b);
-        }
-    }
-}
-
 // ------------------------------------------------------------------ host side
 struct DistillPlan { int64_t off_score, off_sums, off_cnt, total; };
 
@@ -209,9 +212,26 @@ static DistillPlan distill_plan(const HeadPlan& q, int64_t T) {
     DistillPlan f{};
     f.off_score = q.base;
     f.off_sums = f.off_score + up256(2 * q.nt * T * 16);
-    f.off_cnt = f.off_sums + up256(T * 16);
+    f.off_cnt = f.off_sums + up256((T + DI_WARPS - 1) / DI_WARPS * 16);
     f.total = f.off_cnt + 256;
     return f;
+}
+
+// Counts for each half of the vocabulary's tiles and their end, whole 16-byte pieces.
+static int64_t before_stride(int64_t V) { return ((V + XE_TILE - 1) / XE_TILE * 2 + 1 + 15) / 16 * 16; }
+static int64_t saved_bytes(int64_t T, int64_t V, int64_t K) { return 3 * up256(T * 4) + 3 * up256(T * K * 4) + T * before_stride(V); }
+
+static DistillSaved saved_of(uint8_t* b, int64_t T, int64_t V, int64_t K) {
+    DistillSaved s{};
+    s.row_max = reinterpret_cast<float*>(b); b += up256(T * 4);
+    s.row_sum = reinterpret_cast<float*>(b); b += up256(T * 4);
+    s.teacher = reinterpret_cast<float*>(b); b += up256(T * 4);
+    s.ids = reinterpret_cast<int*>(b); b += up256(T * K * 4);
+    s.share = reinterpret_cast<float*>(b); b += up256(T * K * 4);
+    s.logit = reinterpret_cast<float*>(b); b += up256(T * K * 4);
+    s.before = b;
+    s.stride = (int)before_stride(V);
+    return s;
 }
 
 static HeadOps ops_of(const swx_distill_args* a) {
@@ -230,14 +250,10 @@ static int distill_check(const swx_distill_args* a) {
     return SWX_OK;
 }
 
-static DistillRows distill_rows(const swx_distill_args* a) {
-    DistillRows p{};
-    p.T = a->tokens; p.V = a->vocab; p.d = a->dim; p.K = (int)a->entries;
-    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E / a->temperature;
-    p.ids = a->teacher_ids; p.ids_sr = a->ids_sr; p.logits = a->teacher_logits; p.tl_sr = a->tl_sr;
-    p.tl_bf16 = a->teacher_dtype == SWX_DTYPE_BF16;
-    p.row_max = a->row_max; p.row_sum = a->row_sum; p.z = a->entry_logits; p.reduction = a->reduction;
-    return p;
+static void fill_words(XentGemm& g, const DistillSaved& s, const swx_distill_args* a) {
+    g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
+    g.ids = s.ids; g.id_logit = s.logit; g.id_share = s.share; g.nids = (int)a->entries;
+    g.before = s.before; g.before_stride = s.stride;
 }
 
 }  // namespace swx
@@ -247,6 +263,11 @@ using namespace swx;
 extern "C" {
 
 int64_t swx_distill_args_size(void) { return (int64_t)sizeof(swx_distill_args); }
+
+int64_t swx_distill_saved_bytes(const swx_distill_args* a) {
+    const int c = distill_check(a);
+    return c != SWX_OK ? -c : saved_bytes(a->tokens, a->vocab, a->entries);
+}
 
 int64_t swx_distill_fwd_workspace_bytes(const swx_distill_args* a) {
     const int c = distill_check(a);
@@ -270,36 +291,38 @@ int swx_distill_fwd(const swx_distill_args* a, void* stream) {
         if (cudaMemsetAsync(a->count, 0, 4, st) != cudaSuccess) return SWX_ERR_CUDA;
         return cudaMemsetAsync(a->loss, a->reduction == SWX_XENT_MEAN ? 0xff : 0, 4, st) == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
     }
-    if (!a->x || !a->weight || !a->teacher_ids || !a->teacher_logits || !a->row_max || !a->row_sum || !a->entry_logits || !a->workspace ||
-        (none && !a->loss))
-        return SWX_ERR_INVALID_ARG;
+    if (!a->x || !a->weight || !a->teacher_ids || !a->teacher_logits || !a->saved || !a->workspace || (none && !a->loss)) return SWX_ERR_INVALID_ARG;
     const HeadOps o = ops_of(a);
     const HeadPlan q = head_plan(o);
     const DistillPlan f = distill_plan(q, o.T);
     if (a->workspace_bytes < f.total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
+    if (a->saved_bytes < saved_bytes(o.T, o.V, a->entries) || !aligned16(a->saved)) return SWX_ERR_INVALID_ARG;
     uint8_t* ws = static_cast<uint8_t*>(a->workspace);
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
+    DistillRows p{};
+    p.T = o.T; p.V = o.V; p.K = (int)a->entries; p.np = (int)(2 * q.nt);
+    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E / a->temperature;
+    p.ids = a->teacher_ids; p.ids_sr = a->ids_sr; p.logits = a->teacher_logits; p.tl_sr = a->tl_sr;
+    p.tl_bf16 = a->teacher_dtype == SWX_DTYPE_BF16;
+    p.s = saved_of(static_cast<uint8_t*>(a->saved), o.T, o.V, p.K);
+    const unsigned rows = (unsigned)((o.T + DI_WARPS - 1) / DI_WARPS);
+    if (p.K <= 32) distill_prepare_kernel<1><<<rows, DI_THREADS, 0, st>>>(p);
+    else if (p.K <= 64) distill_prepare_kernel<2><<<rows, DI_THREADS, 0, st>>>(p);
+    else distill_prepare_kernel<4><<<rows, DI_THREADS, 0, st>>>(p);
+    if (cudaGetLastError() != cudaSuccess) return SWX_ERR_CUDA;
     Operand x, w;
     head_operands(o, q, ws, x, w, st);
     CUtensorMap mx, mw;
     if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
-    DistillRows p = distill_rows(a);
     XentGemm g = logits_gemm(o, q, 0, o.V, status);
-    g.inv_temp = p.inv_temp; g.k2 = p.k2;
+    fill_words(g, p.s, a);
     g.score = reinterpret_cast<float4*>(ws + f.off_score);
     g.counter = reinterpret_cast<int*>(ws + f.off_cnt);
-    if (launch_score(g, mx, mw, st) != cudaSuccess) return SWX_ERR_CUDA;
-    p.np = (int)(2 * q.nt); p.score = g.score;
-    // the operands in their own type: bf16 ones from their copies where those were made (their rows start on 16 bytes)
-    const bool bf = o.dtype == SWX_DTYPE_BF16;
-    p.x = bf ? x.p : o.x; p.x_sr = bf ? x.row : o.x_sr;
-    p.w = bf ? w.p : o.w; p.w_sr = bf ? w.row : o.w_sr;
-    p.vec = bf || (aligned16(o.x) && aligned16(o.w) && o.x_sr % 4 == 0 && o.w_sr % 4 == 0);
+    if (launch_logits<XE_SCORE_IDS>(g, mx, mw, mx, st) != cudaSuccess) return SWX_ERR_CUDA;
+    p.score = g.score;
     p.rows = none ? a->loss : nullptr; p.sums = reinterpret_cast<double2*>(ws + f.off_sums);
-    p.loss = a->loss; p.count = a->count; p.counter = g.counter;
-    if (bf) distill_rows_kernel<__nv_bfloat16><<<(unsigned)o.T, DI_THREADS, 0, st>>>(p);
-    else distill_rows_kernel<float><<<(unsigned)o.T, DI_THREADS, 0, st>>>(p);
-    return cudaGetLastError() == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
+    p.loss = a->loss; p.count = a->count; p.counter = g.counter; p.reduction = a->reduction;
+    return launch_after(distill_rows_kernel, rows, DI_THREADS, 0, st, p) == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
 }
 
 int swx_distill_bwd(const swx_distill_args* a, void* stream) {
@@ -313,23 +336,17 @@ int swx_distill_bwd(const swx_distill_args* a, void* stream) {
         return cudaMemsetAsync(a->dweight, 0, (size_t)(a->vocab * a->dim) * (a->dw_dtype == SWX_DTYPE_F32 ? 4 : 2), st) == cudaSuccess
                    ? SWX_OK : SWX_ERR_CUDA;
     }
-    if (!a->x || !a->weight || !a->teacher_ids || !a->teacher_logits || !a->row_max || !a->row_sum || !a->entry_logits || !a->dloss ||
-        !a->workspace || (a->reduction == SWX_XENT_MEAN && !a->count))
-        return SWX_ERR_INVALID_ARG;
+    if (!a->x || !a->weight || !a->saved || !a->dloss || !a->workspace || (a->reduction == SWX_XENT_MEAN && !a->count)) return SWX_ERR_INVALID_ARG;
     const HeadOps o = ops_of(a);
     const HeadPlan q = head_plan(o);
     if (a->workspace_bytes < q.bwd_total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
-    DistillRows p = distill_rows(a);
-    p.dloss = a->dloss; p.ld = q.ldp; p.plane = o.T * q.ldp; p.planes = q.planes;
+    if (a->saved_bytes < saved_bytes(o.T, o.V, a->entries) || !aligned16(a->saved)) return SWX_ERR_INVALID_ARG;
+    const DistillSaved s = saved_of(static_cast<uint8_t*>(a->saved), o.T, o.V, a->entries);
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, a->reduction == SWX_XENT_NONE ? nullptr : a->dloss,
                        a->reduction == SWX_XENT_MEAN ? a->count : nullptr};
-    return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_grad, [&p, a](XentGemm& g) {
-        g.inv_temp = p.inv_temp; g.k2 = p.k2;
-        g.row_max = a->row_max; g.row_sum = a->row_sum; g.dloss = a->dloss; g.reduction = a->reduction;
-    }, [&p, st](__nv_bfloat16* dz, int64_t c0, int64_t cw) {
-        p.dz = dz; p.c0 = c0; p.cw = cw;
-        distill_patch_kernel<<<(unsigned)((p.T + DI_PATCH_WARPS - 1) / DI_PATCH_WARPS), 32 * DI_PATCH_WARPS, 0, st>>>(p);
-        return (int)(cudaGetLastError() == cudaSuccess ? SWX_OK : SWX_ERR_CUDA);
+    return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_logits<XE_GRAD_IDS>, [&s, a](XentGemm& g) {
+        fill_words(g, s, a);
+        g.row_max = s.row_max; g.row_sum = s.row_sum; g.dloss = a->dloss; g.reduction = a->reduction;
     });
 }
 

@@ -483,13 +483,6 @@ __global__ void __launch_bounds__(256) longest_word_kernel(const T* w, int64_t w
 }
 
 // ------------------------------------------------------------------ host side
-cudaError_t launch_score(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, cudaStream_t st) {
-    return launch_logits<XE_SCORE>(g, x, w, x, st);
-}
-cudaError_t launch_grad(const XentGemm& g, const CUtensorMap& x, const CUtensorMap& w, const CUtensorMap& store, cudaStream_t st) {
-    return launch_logits<XE_GRAD>(g, x, w, store, st);
-}
-
 struct ScorePlan {
     int few, np;                              // CTAs of the few rows' kernel or 0; statistics of a row
     int cand; bool all; int64_t groups, stride;
@@ -497,8 +490,12 @@ struct ScorePlan {
     bool longest;
 };
 
+// Rows of one product: what it keeps for the rows' kernel is bounded (8192 rows x 50001: 51 MB of statistics, 205 MB of records),
+// and 32 row tiles keep a tile of the weight in use as long as more would.
+constexpr int64_t SC_ROWS = 32 * XE_TILE;
+
 static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
-    const int64_t T = o.T, V = o.V;
+    const int64_t T = std::min(o.T, SC_ROWS), V = o.V;
     ScorePlan f{};
     f.few = score_few_ctas(o);
     f.np = f.few ? f.few : (int)(2 * q.nt);
@@ -519,7 +516,7 @@ static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
         f.total = f.off_longest + 256;
         // the words' norms are one read of the weight, and without them every candidate's word is read (64 MB of them, which
         // come from the L2 as a rule, take less time than a launch and its read)
-        f.longest = T * f.cand > V && T * f.cand * o.d * q.es > (int64_t(64) << 20);
+        f.longest = o.T * f.cand > V && o.T * f.cand * o.d * q.es > (int64_t(64) << 20);
     }
     return f;
 }
@@ -588,47 +585,61 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
     Operand x, w;
     head_operands(o, q, ws, x, w, st);
-    CUtensorMap mx, mw;
-    if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
-    XentGemm g = logits_gemm(o, q, 0, o.V, status);
-    g.target = a->targets; g.ignore = a->ignore_index;
-    g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
-    g.score = reinterpret_cast<float4*>(ws + f.off_score);
-    g.hit = reinterpret_cast<float*>(ws + f.off_hit);
-    g.largest = reinterpret_cast<float*>(ws + f.off_rec); g.runner_up = reinterpret_cast<float*>(ws + f.off_second);
-    g.all = reinterpret_cast<float*>(ws + f.off_rec);
-    g.counter = f.longest ? reinterpret_cast<int*>(ws + f.off_longest) : nullptr;
-    const cudaError_t e = f.few ? launch_score_few(g, o, x, w, a->top_k > 0, f.few, st)
-                          : a->top_k == 0 ? launch_score(g, mx, mw, st)
-                          : f.all       ? launch_logits<XE_SCORE_ALL>(g, mx, mw, mx, st)
-                                        : launch_logits<XE_SCORE_TOP>(g, mx, mw, mx, st);
-    if (e != cudaSuccess) return SWX_ERR_CUDA;
-    ScoreRows p{};
-    p.T = o.T; p.V = o.V; p.d = o.d; p.np = f.np;
-    p.score = g.score; p.hit = g.hit; p.target = a->targets; p.ignore = a->ignore_index;
-    p.k2 = g.k2;
-    p.row_max = a->row_max; p.row_sum = a->row_sum; p.log_probs = a->log_probs; p.entropy = a->entropy;
-    if (a->top_k == 0) {
-        const unsigned grid = (unsigned)((o.T + SC_THREADS / 32 - 1) / (SC_THREADS / 32));
-        return launch_after(score_rows_kernel, grid, SC_THREADS, 0, st, p) == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
-    }
-    p.top = a->top_k; p.cand = f.cand; p.largest = g.largest; p.runner_up = g.runner_up; p.stride = f.stride; p.all = g.all; p.groups = f.groups;
-    p.top_log_probs = a->top_log_probs; p.top_ids = a->top_ids;
-    // the operands in their own type: bf16 ones from their copies where those were made (their rows start on 16 bytes)
     const bool bf = o.dtype == SWX_DTYPE_BF16;
-    p.x = bf ? x.p : o.x; p.x_sr = bf ? x.row : o.x_sr;
-    p.w = bf ? w.p : o.w; p.w_sr = bf ? w.row : o.w_sr;
-    p.vec = bf || (aligned16(o.x) && aligned16(o.w) && o.x_sr % 4 == 0 && o.w_sr % 4 == 0);
-    if (f.longest) {
-        uint32_t* longest = reinterpret_cast<uint32_t*>(g.counter);
-        const unsigned grid = (unsigned)std::min<int64_t>((o.V + 7) / 8, 148 * 8);
-        if (bf) longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p.w), p.w_sr, p.V, p.d, true, longest);
-        else longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p.w), p.w_sr, p.V, p.d, p.vec != 0, longest);
-        if (cudaGetLastError() != cudaSuccess) return SWX_ERR_CUDA;
-        p.longest = longest;
+    bool longest = f.longest;                 // the words' norms are still to be read
+    for (int64_t r0 = 0; r0 < o.T; r0 += SC_ROWS) {
+        HeadOps oc = o;
+        oc.T = std::min(SC_ROWS, o.T - r0);
+        oc.x = static_cast<const uint8_t*>(o.x) + r0 * o.x_sr * q.es;
+        HeadPlan qc = q;
+        qc.mt = (oc.T + XE_TILE - 1) / XE_TILE;
+        Operand xc = x;                       // (pieces of fp32 operands keep their distance)
+        xc.rows = oc.T;
+        xc.p = static_cast<const uint8_t*>(x.p) + r0 * x.row * 2;
+        CUtensorMap mx, mw;
+        if (!xc.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
+        XentGemm g = logits_gemm(oc, qc, 0, o.V, status);
+        g.target = a->targets + r0; g.ignore = a->ignore_index;
+        g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
+        g.score = reinterpret_cast<float4*>(ws + f.off_score);
+        g.hit = reinterpret_cast<float*>(ws + f.off_hit);
+        g.largest = reinterpret_cast<float*>(ws + f.off_rec); g.runner_up = reinterpret_cast<float*>(ws + f.off_second);
+        g.all = reinterpret_cast<float*>(ws + f.off_rec);
+        g.counter = longest ? reinterpret_cast<int*>(ws + f.off_longest) : nullptr;
+        const cudaError_t e = f.few ? launch_score_few(g, oc, xc, w, a->top_k > 0, f.few, st)
+                              : a->top_k == 0 ? launch_logits<XE_SCORE>(g, mx, mw, mx, st)
+                              : f.all       ? launch_logits<XE_SCORE_ALL>(g, mx, mw, mx, st)
+                                            : launch_logits<XE_SCORE_TOP>(g, mx, mw, mx, st);
+        if (e != cudaSuccess) return SWX_ERR_CUDA;
+        ScoreRows p{};
+        p.T = oc.T; p.V = o.V; p.d = o.d; p.np = f.np;
+        p.score = g.score; p.hit = g.hit; p.target = g.target; p.ignore = a->ignore_index;
+        p.k2 = g.k2;
+        p.row_max = a->row_max ? a->row_max + r0 : nullptr; p.row_sum = a->row_sum ? a->row_sum + r0 : nullptr;
+        p.log_probs = a->log_probs + r0; p.entropy = a->entropy + r0;
+        if (a->top_k == 0) {
+            const unsigned grid = (unsigned)((oc.T + SC_THREADS / 32 - 1) / (SC_THREADS / 32));
+            if (launch_after(score_rows_kernel, grid, SC_THREADS, 0, st, p) != cudaSuccess) return SWX_ERR_CUDA;
+            continue;
+        }
+        p.top = a->top_k; p.cand = f.cand; p.largest = g.largest; p.runner_up = g.runner_up; p.stride = f.stride; p.all = g.all; p.groups = f.groups;
+        p.top_log_probs = a->top_log_probs + r0 * a->top_k; p.top_ids = a->top_ids + r0 * a->top_k;
+        // the operands in their own type: bf16 ones from their copies where those were made (their rows start on 16 bytes)
+        p.x = bf ? xc.p : oc.x; p.x_sr = bf ? x.row : o.x_sr;
+        p.w = bf ? w.p : o.w; p.w_sr = bf ? w.row : o.w_sr;
+        p.vec = bf || (aligned16(o.x) && aligned16(o.w) && o.x_sr % 4 == 0 && o.w_sr % 4 == 0);
+        if (f.longest) p.longest = reinterpret_cast<const uint32_t*>(ws + f.off_longest);
+        if (longest) {
+            uint32_t* out = reinterpret_cast<uint32_t*>(g.counter);
+            const unsigned grid = (unsigned)std::min<int64_t>((o.V + 7) / 8, 148 * 8);
+            if (bf) longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p.w), p.w_sr, p.V, p.d, true, out);
+            else longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p.w), p.w_sr, p.V, p.d, p.vec != 0, out);
+            if (cudaGetLastError() != cudaSuccess) return SWX_ERR_CUDA;
+            longest = false;
+        }
+        if ((bf ? launch_top<__nv_bfloat16>(p, f.all, st) : launch_top<float>(p, f.all, st)) != cudaSuccess) return SWX_ERR_CUDA;
     }
-    const cudaError_t r = bf ? launch_top<__nv_bfloat16>(p, f.all, st) : launch_top<float>(p, f.all, st);
-    return r == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
+    return SWX_OK;
 }
 
 int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
@@ -648,12 +659,12 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
     const HeadPlan q = head_plan(o);
     if (a->workspace_bytes < q.bwd_total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, nullptr, nullptr};
-    return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_grad, [a](XentGemm& g) {
+    return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_logits<XE_GRAD>, [a](XentGemm& g) {
         g.target = a->targets; g.ignore = a->ignore_index;
         g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
         g.row_max = a->row_max; g.row_sum = a->row_sum; g.entropy = a->entropy;
         g.d_logp = a->d_log_probs; g.d_entropy = a->d_entropy;
-    }, [](__nv_bfloat16*, int64_t, int64_t) { return (int)SWX_OK; });
+    });
 }
 
 }  // extern "C"

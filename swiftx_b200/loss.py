@@ -164,61 +164,59 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     return loss.view(targets.shape) if reduction == "none" and targets.dim() != 1 else loss
 
 
-def _distill_args(x, w, ids, logits, temperature, reduction):
+def _distill_args(x, w, entries, temperature, reduction):
     a = _lib.DistillArgs()
     set_operands(a, x, w)
-    a.entries, a.reduction, a.temperature, a.teacher_dtype = ids.shape[1], reduction, temperature, _DT[logits.dtype]
-    a.teacher_ids, a.ids_sr = ids.data_ptr(), ids.stride(0)
-    a.teacher_logits, a.tl_sr = logits.data_ptr(), logits.stride(0)
+    a.entries, a.reduction, a.temperature = entries, reduction, temperature
     return a
 
 
-def _set_stats(a, stats):
-    """row_max, row_sum, entry_logits and count in one buffer."""
-    a.row_max = stats.data_ptr()
-    a.row_sum, a.entry_logits = a.row_max + 4 * a.tokens, a.row_max + 8 * a.tokens
-    a.count = a.entry_logits + 4 * a.tokens * a.entries
-
-
 def _distill_forward(x, w, ids, logits, temperature, reduction):
+    """The loss, what the backward needs of it, and the count."""
     T = int(x.shape[0])                # (under a trace a size is a tensor)
     with _lib.on_device(x.device):
         lib = _lib.load()
         loss = x.new_empty((T,) if reduction == _lib.XENT_REDUCTIONS["none"] else (), dtype=torch.float32)
-        stats = loss.new_empty(T * (2 + int(ids.shape[1])) + 1)
-        a = _distill_args(x, w, ids, logits, temperature, reduction)
-        a.loss = loss.data_ptr()
-        _set_stats(a, stats)
+        count = torch.empty_like(loss) if loss.dim() == 0 else loss
+        a = _distill_args(x, w, ids.shape[1], temperature, reduction)
+        a.teacher_dtype = _DT[logits.dtype]
+        a.teacher_ids, a.ids_sr = ids.data_ptr(), ids.stride(0)
+        a.teacher_logits, a.tl_sr = logits.data_ptr(), logits.stride(0)
+        a.loss, a.count = loss.data_ptr(), count.data_ptr()
+        a.saved_bytes = lib.swx_distill_saved_bytes(a)
+        saved = x.new_empty(a.saved_bytes, dtype=torch.uint8)
+        a.saved = saved.data_ptr()
         ws = _workspace(lib, "swx_distill_fwd_workspace_bytes", a, loss)  # noqa: F841
         _lib.check(lib.swx_distill_fwd(a, _lib.stream_ptr(x.device)), "swx_distill_fwd")
-    return loss, stats
+    return loss, saved, count
 
 
 class LinearDistillationFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, ids, logits, temperature, reduction, weight16=None):
         x, w = _rows(x), _rows(product_weight(x, weight, weight16))
-        loss, stats = _distill_forward(x, w, ids, logits, temperature, reduction)
-        ctx.save_for_backward(x, w, ids, logits, stats)
-        ctx.opts = (temperature, reduction, weight.dtype)
+        loss, saved, count = _distill_forward(x, w, ids, logits, temperature, reduction)
+        ctx.save_for_backward(x, w, saved, count if count is not loss else None)
+        ctx.opts = (ids.shape[1], temperature, reduction, weight.dtype)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, w, ids, logits, stats = ctx.saved_tensors
-        temperature, reduction, w_dtype = ctx.opts
+        x, w, saved, count = ctx.saved_tensors
+        *opts, w_dtype = ctx.opts
         dloss = dloss.float().contiguous()
         with _lib.on_device(x.device):
             lib = _lib.load()
             dx = torch.empty_like(x, memory_format=torch.contiguous_format) if ctx.needs_input_grad[0] else None
             dw = w.new_empty(w.shape, dtype=w_dtype) if ctx.needs_input_grad[1] else None
-            a = _distill_args(x, w, ids, logits, temperature, reduction)
-            _set_stats(a, stats)
+            a = _distill_args(x, w, *opts)
+            a.saved, a.saved_bytes = saved.data_ptr(), saved.numel()
+            a.count = count.data_ptr() if count is not None else None
             a.dw_dtype, a.dloss = _DT[w_dtype], dloss.data_ptr()
             a.dx = dx.data_ptr() if dx is not None else None
             a.dweight = dw.data_ptr() if dw is not None else None
-            ws = _workspace(lib, "swx_distill_bwd_workspace_bytes", a, stats)  # noqa: F841
+            ws = _workspace(lib, "swx_distill_bwd_workspace_bytes", a, dloss)  # noqa: F841
             _lib.check(lib.swx_distill_bwd(a, _lib.stream_ptr(x.device)), "swx_distill_bwd")
         return dx, dw, None, None, None, None, None
 

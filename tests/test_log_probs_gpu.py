@@ -323,6 +323,17 @@ def test_several_pieces_of_the_vocabulary():
     _check_gradients(x, w, y, 1.0, g, h, dx, dw)
 
 
+@pytest.mark.parametrize("T,V,d,dtype,top", [(8700, 3001, 40, BF, 6), (8193, 300, 24, FP, 3), (16400, 2500, 32, FP, 9), (9000, 700, 33, BF, 0)])
+def test_more_rows_than_one_product_takes(T, V, d, dtype, top):
+    x, w, y = _inputs(T, V, d, dtype, seed=14)
+    out = linear_log_probs(x, w, y, top_k=top)
+    _check_forward(out, x, w, y, 1.0, top)
+    xo = torch.zeros(T, d + 3, device=DEV, dtype=dtype)[:, 3:]            # rows off 16 bytes
+    xo.copy_(x)
+    for a, b in zip(linear_log_probs(xo, w, y, top_k=top), out):
+        assert (a is None and b is None) or torch.equal(a, b) or (a.is_floating_point() and float((a - b).abs().max()) <= E)
+
+
 def test_deterministic_streams_and_graphs():
     x, w, y = _inputs(603, 5001, 72, BF, seed=6)
     g, h = _upstream(603)

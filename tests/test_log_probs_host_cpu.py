@@ -56,7 +56,7 @@ def test_distillation_arguments(change, status):
     lib = _lib.load()
     a = _distill(**change)
     assert lib.swx_distill_fwd(a, None) == status and lib.swx_distill_bwd(a, None) == status
-    assert lib.swx_distill_fwd_workspace_bytes(a) == lib.swx_distill_bwd_workspace_bytes(a) == -status
+    assert lib.swx_distill_fwd_workspace_bytes(a) == lib.swx_distill_bwd_workspace_bytes(a) == lib.swx_distill_saved_bytes(a) == -status
     assert lib.swx_distill_fwd(None, None) == lib.swx_distill_bwd(None, None) == INVALID
 
 
@@ -93,13 +93,19 @@ def test_distillation_buffers():
     lib = _lib.load()
     a = _distill()
     assert lib.swx_distill_fwd(a, None) == INVALID
-    a.loss = a.count = a.teacher_ids = a.teacher_logits = a.row_max = a.row_sum = a.entry_logits = a.workspace = 4096
+    a.loss = a.count = a.teacher_ids = a.teacher_logits = a.saved = a.workspace = 4096
+    a.saved_bytes = lib.swx_distill_saved_bytes(a)
     a.workspace_bytes = lib.swx_distill_fwd_workspace_bytes(a) - 1
-    assert lib.swx_distill_fwd(a, None) == INVALID
+    assert lib.swx_distill_fwd(a, None) == INVALID                               # a short workspace
     a.workspace_bytes, a.workspace = 1 << 30, 4096 + 8
+    assert lib.swx_distill_fwd(a, None) == INVALID                               # off 16 bytes
+    a.workspace, a.saved_bytes = 4096, a.saved_bytes - 1
+    assert lib.swx_distill_fwd(a, None) == INVALID                               # too little to keep for the backward
+    a.saved_bytes, a.saved = 1 << 30, 4096 + 8
     assert lib.swx_distill_fwd(a, None) == INVALID
+    a.saved = 4096
     assert lib.swx_distill_bwd(a, None) == _lib.SWX_OK                           # no gradient asked for
-    a.dx, a.workspace = 4096, 4096
+    a.dx = 4096
     assert lib.swx_distill_bwd(a, None) == INVALID                               # no dloss
     a.dloss, a.workspace_bytes = 4096, lib.swx_distill_bwd_workspace_bytes(a) - 1
     assert lib.swx_distill_bwd(a, None) == INVALID
@@ -109,15 +115,19 @@ def test_distillation_buffers():
 
 
 def test_workspaces_do_not_hold_the_logits():
+    """Scoring takes 8192 rows at a time: statistics of 16 bytes for 128 logits of them, 8 bytes for 16 with alternatives, and the
+    targets' logits; distillation keeps 16 bytes for 128 logits of each row, and 12 bytes and a count for 128 words beside each entry."""
     lib = _lib.load()
     T, V, d = 65536, 131072, 64
     logits = 2 * T * V
     a = _score(T, V, d)
-    plain = lib.swx_logprob_fwd_workspace_bytes(a)
+    rows = 8192 * V
+    assert lib.swx_logprob_fwd_workspace_bytes(a) <= rows / 8 + 4 * 8192 + 4096
     a.top_k = 20
-    assert plain < logits / 8 and lib.swx_logprob_fwd_workspace_bytes(a) < logits / 4
+    assert lib.swx_logprob_fwd_workspace_bytes(a) <= rows / 8 + rows / 2 + 4 * 8192 + 4096
     assert lib.swx_logprob_bwd_workspace_bytes(a) < logits / 16 + 4 * T * d
     b = _distill(T, V, d)
+    assert lib.swx_distill_saved_bytes(b) <= T * (12 + 12 * 4 + V / 128 + 17) + 4096
     assert lib.swx_distill_fwd_workspace_bytes(b) < logits / 8 and lib.swx_distill_bwd_workspace_bytes(b) < logits / 16 + 4 * T * d
 
 
