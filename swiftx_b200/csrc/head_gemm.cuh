@@ -649,6 +649,13 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
     if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
+// What the tensor core takes off a sum of n additions of bf16 products on average, relative: it cuts each addition's low bits
+// off (toward zero).  Sums of terms of either sign came out 0.21 to 0.26 2^-24 n too small at n = 4 to 512 (of one sign 0.25 to 0.5 up to
+// n = 64, more beyond).  All logits together too small act like a higher temperature, which the entropy shows first (8192 rows x
+// 50001 x 1024: 8e-7 off); the scale of the exponents makes up for the mean.  fp32 operands are summed otherwise.
+inline float mean_cut(int dtype, int64_t additions) { return dtype == SWX_DTYPE_BF16 ? 0.23f * 0x1p-24f * (float)additions : 0.f; }
+inline float exponent_scale(float temperature, float cut) { return (float)(1.4426950408889634 / temperature * (1. + cut)); }
+
 // Eight values of a row from k on (a multiple of 8; rows start on 16 bytes), zeros from d on.
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int64_t k, int64_t d) {
     if (k + 8 <= d) return *reinterpret_cast<const uint4*>(p + k);

@@ -251,7 +251,7 @@ static int distill_check(const swx_distill_args* a) {
 }
 
 static void fill_words(XentGemm& g, const DistillSaved& s, const swx_distill_args* a) {
-    g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
+    g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut(a->dtype, (a->dim + 15) / 16));
     g.ids = s.ids; g.id_logit = s.logit; g.id_share = s.share; g.nids = (int)a->entries;
     g.before = s.before; g.before_stride = s.stride;
 }
@@ -301,7 +301,7 @@ int swx_distill_fwd(const swx_distill_args* a, void* stream) {
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
     DistillRows p{};
     p.T = o.T; p.V = o.V; p.K = (int)a->entries; p.np = (int)(2 * q.nt);
-    p.inv_temp = 1.f / a->temperature; p.k2 = LOG2E / a->temperature;
+    p.inv_temp = 1.f / a->temperature;
     p.ids = a->teacher_ids; p.ids_sr = a->ids_sr; p.logits = a->teacher_logits; p.tl_sr = a->tl_sr;
     p.tl_bf16 = a->teacher_dtype == SWX_DTYPE_BF16;
     p.s = saved_of(static_cast<uint8_t*>(a->saved), o.T, o.V, p.K);
@@ -316,6 +316,7 @@ int swx_distill_fwd(const swx_distill_args* a, void* stream) {
     if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
     XentGemm g = logits_gemm(o, q, 0, o.V, status);
     fill_words(g, p.s, a);
+    p.k2 = g.k2;
     g.score = reinterpret_cast<float4*>(ws + f.off_score);
     g.counter = reinterpret_cast<int*>(ws + f.off_cnt);
     if (launch_logits<XE_SCORE_IDS>(g, mx, mw, mx, st) != cudaSuccess) return SWX_ERR_CUDA;

@@ -28,7 +28,7 @@ struct ScoreRows {
     int64_t T, V, d;
     int np;                                   // statistics per row
     const float4* score; const float* hit; const int64_t* target; int64_t ignore;
-    float k2;
+    float k2, cut;                            // log2(e) / temperature; the products' mean cut (they are to be taken 1 + cut times)
     float* row_max; float* row_sum; float* log_probs; float* entropy;
     // alternatives
     int top, cand;                            // K, candidates kept of the records
@@ -44,7 +44,7 @@ __device__ __forceinline__ void score_finish(const ScoreRows& p, int64_t row, co
     const float ls = logf(a.s);
     if (p.row_max) { p.row_max[row] = a.m; p.row_sum[row] = a.s; }
     const bool live = y != p.ignore;
-    p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? fmaf(p.hit[row], p.k2, -a.m) * LN2 - ls : __int_as_float(0x7fc00000);
+    p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? fmaf(fmaf(p.hit[row], p.cut, p.hit[row]), p.k2, -a.m) * LN2 - ls : __int_as_float(0x7fc00000);
     p.entropy[row] = live ? ls - LN2 * a.w / a.s : 0.f;
 }
 
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
         if (ALL) {
             const int at = atomicAdd(&ncand, 1);
             col[at] = (int)g;
-            ze[at] = make_float2(z, off);
+            ze[at] = make_float2(fmaf(z, p.cut, z), off);
         } else if (drop_column(second) >= drop_column(least)) {
             const int c = (int)min((int64_t)16, p.V - (int64_t)g * 16), at = atomicAdd(&ncand, c);
             for (int j = 0; j < c; ++j) {
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
         } else {
             const int at = atomicAdd(&ncand, 1);
             col[at] = (int)(g * 16 + (__float_as_uint(second) & 15u));
-            ze[at] = make_float2(z, off);
+            ze[at] = make_float2(fmaf(z, p.cut, z), off);
         }
     }
     __syncthreads();
@@ -600,7 +600,8 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         if (!xc.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
         XentGemm g = logits_gemm(oc, qc, 0, o.V, status);
         g.target = a->targets + r0; g.ignore = a->ignore_index;
-        g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
+        const float cut = mean_cut(o.dtype, f.few ? (o.d + 63) / 64 : (o.d + 15) / 16);
+        g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, cut);
         g.score = reinterpret_cast<float4*>(ws + f.off_score);
         g.hit = reinterpret_cast<float*>(ws + f.off_hit);
         g.largest = reinterpret_cast<float*>(ws + f.off_rec); g.runner_up = reinterpret_cast<float*>(ws + f.off_second);
@@ -614,7 +615,7 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         ScoreRows p{};
         p.T = oc.T; p.V = o.V; p.d = o.d; p.np = f.np;
         p.score = g.score; p.hit = g.hit; p.target = g.target; p.ignore = a->ignore_index;
-        p.k2 = g.k2;
+        p.k2 = exponent_scale(a->temperature, 0.f); p.cut = cut;
         p.row_max = a->row_max ? a->row_max + r0 : nullptr; p.row_sum = a->row_sum ? a->row_sum + r0 : nullptr;
         p.log_probs = a->log_probs + r0; p.entropy = a->entropy + r0;
         if (a->top_k == 0) {
@@ -661,7 +662,7 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, nullptr, nullptr};
     return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_logits<XE_GRAD>, [a](XentGemm& g) {
         g.target = a->targets; g.ignore = a->ignore_index;
-        g.inv_temp = 1.f / a->temperature; g.k2 = LOG2E / a->temperature;
+        g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut(a->dtype, (a->dim + 15) / 16));
         g.row_max = a->row_max; g.row_sum = a->row_sum; g.entropy = a->entropy;
         g.d_logp = a->d_log_probs; g.d_entropy = a->d_entropy;
     });
