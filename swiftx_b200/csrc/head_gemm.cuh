@@ -649,13 +649,6 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
     if (warp == 1) tmem_free_pair(tmem, 512);
 }
 
-// What the tensor core takes off a sum of n additions of bf16 products on average, relative: it cuts each addition's low bits
-// off (toward zero).  Sums of terms of either sign came out 0.21 to 0.26 2^-24 n too small at n = 4 to 512 (of one sign 0.25 to 0.5 up to
-// n = 64, more beyond).  All logits together too small act like a higher temperature, which the entropy shows first (8192 rows x
-// 50001 x 1024: 8e-7 off); the scale of the exponents makes up for the mean.  fp32 operands are summed otherwise.
-inline float mean_cut(int dtype, int64_t additions) { return dtype == SWX_DTYPE_BF16 ? 0.23f * 0x1p-24f * (float)additions : 0.f; }
-inline float exponent_scale(float temperature, float cut) { return (float)(1.4426950408889634 / temperature * (1. + cut)); }
-
 // Eight values of a row from k on (a multiple of 8; rows start on 16 bytes), zeros from d on.
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* p, int64_t k, int64_t d) {
     if (k + 8 <= d) return *reinterpret_cast<const uint4*>(p + k);
@@ -672,6 +665,17 @@ constexpr int XE_PAIRS = 74, XE_MIN_SHARE = 4;
 
 // A head's operands: x (T, d) and the weight (V, d), row strides in elements.
 struct HeadOps { int64_t T, V, d; int dtype; const void* x; int64_t x_sr; const void* w; int64_t w_sr; };
+
+// What the tensor core takes off a sum of n additions of bf16 products on average, relative: it cuts each addition's low bits
+// off (toward zero).  Sums of terms of either sign came out 0.21 to 0.26 2^-24 n too small at n = 4 to 512 (of one sign 0.25 to 0.5 up to
+// n = 64, more beyond).  All logits together too small act like a higher temperature, which the entropy shows first (8192 rows x
+// 50001 x 1024: 8e-7 off); the scale of the exponents makes up for the mean.
+inline float mean_cut(int64_t additions) { return 0.23f * 0x1p-24f * (float)additions; }
+// Additions of a logit's sum at its full size: fp32 operands' largest pieces come last, 512 terms at a time.
+inline int64_t logit_additions(const HeadOps& o) {
+    return std::min((o.d + 15) / 16, o.dtype == SWX_DTYPE_BF16 ? INT64_MAX : (int64_t)(XE_KSUB_LOGITS * XE_K / 16));
+}
+inline float exponent_scale(float temperature, float cut) { return (float)(1.4426950408889634 / temperature * (1. + cut)); }
 
 // Sizes and the workspace: copies of the operands, then (forward) whatever the operator keeps from
 // `base` on, or (backward) a piece of the logits' gradient and the sums of the gradient products.

@@ -600,7 +600,7 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         if (!xc.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
         XentGemm g = logits_gemm(oc, qc, 0, o.V, status);
         g.target = a->targets + r0; g.ignore = a->ignore_index;
-        const float cut = mean_cut(o.dtype, f.few ? (o.d + 63) / 64 : (o.d + 15) / 16);
+        const float cut = mean_cut(f.few ? (o.d + 63) / 64 : logit_additions(o));
         g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, cut);
         g.score = reinterpret_cast<float4*>(ws + f.off_score);
         g.hit = reinterpret_cast<float*>(ws + f.off_hit);
@@ -662,7 +662,7 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, nullptr, nullptr};
     return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_logits<XE_GRAD>, [a](XentGemm& g) {
         g.target = a->targets; g.ignore = a->ignore_index;
-        g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut(a->dtype, (a->dim + 15) / 16));
+        g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut(logit_additions(ops_of(a))));
         g.row_max = a->row_max; g.row_sum = a->row_sum; g.entropy = a->entropy;
         g.d_logp = a->d_log_probs; g.d_entropy = a->d_entropy;
     });
