@@ -285,7 +285,7 @@ __device__ __forceinline__ float drop_column(float v) { return __uint_as_float(_
 template <typename T, bool ALL, int THREADS>
 __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     extern __shared__ __align__(16) uint8_t raw[];
-    __shared__ int count, ncand, nlist, owners[THREADS];
+    __shared__ int count[2], ncand, nlist, owners[THREADS];
     __shared__ uint32_t scratch[THREADS + 1];
     __shared__ Score part[THREADS / 32];
     __shared__ float norms[THREADS / 32];
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     float most = -INFINITY;
 #pragma unroll 8
     for (int64_t i = threadIdx.x; i < n; i += THREADS) most = fmaxf(most, value(i));
-    if (threadIdx.x == 0) { ncand = 0; nlist = 0; }
+    if (threadIdx.x == 0) count[0] = count[1] = ncand = nlist = 0;
     if (p.longest) {
         float xx = 0.f;
         for (int64_t k = threadIdx.x; k < p.d; k += THREADS) { const float v = Elem<T>::to_f(x[k]); xx = fmaf(v, v, xx); }
@@ -327,8 +327,7 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
         return;
     }
 
-    TopK<THREADS, SC_PER> best{};
-    best.start(buf, kept, &count, p.cand);
+    TopK<THREADS, SC_PER> best(buf, kept, count, p.cand);
     struct Entry { float v; uint32_t i; };
     auto load = [&](int t, int64_t j, Entry& e) {
         const int64_t i = t + j * THREADS;

@@ -29,8 +29,8 @@ constexpr int topk_capacity(int k, int per) { return k * (per + 1); }
 
 // A threshold that at least k of the THREADS threads' values (order_key bits) reach, and few more where the values differ (a quarter
 // of k, and of the threads that are not among the k: close to all of them the values say little about the whole),
-// by one warp: the bits of the k-th largest are set from the top, over those that differ, until it is that close.
-// scratch: THREADS + 1 words; all threads call it.
+// by one warp: the bits of the k-th largest are set from the top, over those that differ, until it is that close.  A value with all
+// bits set asks for no threshold, and is returned.  scratch: THREADS + 1 words; all threads call it.
 template <int THREADS>
 __device__ __forceinline__ uint32_t about_kth(uint32_t mine, int k, uint32_t* scratch) {
     scratch[threadIdx.x] = mine;
@@ -48,7 +48,8 @@ __device__ __forceinline__ uint32_t about_kth(uint32_t mine, int k, uint32_t* sc
         hi = __reduce_max_sync(0xffffffffu, hi);
         const int top = 32 - __clz(lo ^ hi);                   // bits from here up are common
         uint32_t t = top == 32 ? 0 : hi >> top << top;
-        for (int b = top - 1; b >= 0; --b) {
+        if (hi == ~0u) t = hi;
+        for (int b = top - 1; b >= 0 && hi != ~0u; --b) {
             const uint32_t c = t | 1u << b;
             int n = 0;
 #pragma unroll
@@ -68,14 +69,11 @@ template <int THREADS, int PER>
 struct TopK {
     uint64_t* buf;                            // topk_capacity(k, PER)
     uint64_t* kept;                           // k
-    int* count;                               // one int of shared memory
+    int* count;                               // two ints of shared memory, 0 before the first barrier
     int k, n;
     uint64_t floor;                           // every key of the k largest so far is at least this
 
-    __device__ __forceinline__ void start(uint64_t* buf_, uint64_t* kept_, int* count_, int k_) {
-        buf = buf_; kept = kept_; count = count_; k = k_;
-        clear();
-    }
+    __device__ __forceinline__ TopK(uint64_t* buf_, uint64_t* kept_, int* count_, int k_) : buf(buf_), kept(kept_), count(count_), k(k_), n(0), floor(1) {}
     __device__ __forceinline__ void clear() {
         n = 0;
         floor = 1;
@@ -84,9 +82,11 @@ struct TopK {
         __syncthreads();
     }
     // One key, by any thread: dropped, but counted, where the buffer is full.
-    __device__ __forceinline__ void add(uint64_t key) {
+    __device__ __forceinline__ void add(float v, uint32_t index, uint32_t least) {
+        const uint32_t o = order_key(v);
+        if (o < least) return;
         const int at = atomicAdd(count, 1);
-        if (at < topk_capacity(k, PER)) buf[at] = key;
+        if (at < topk_capacity(k, PER)) buf[at] = index_key(o, index);
     }
     // After the threads' adds: whether all of them found room.
     __device__ __forceinline__ bool added() {
@@ -96,16 +96,14 @@ struct TopK {
     }
     // The keys that reach the threshold, from the shares of the threads whose maximum does: load(t, j, e) reads entry j < per of
     // thread t's share into e, and emit(e, f) calls f(value, index) on what it holds.  A warp takes a share, four of them
-    // at a time so that their loads overlap.  False where they were too many.
+    // at a time so that their loads overlap.  False where they were too many, or a maximum asks for no threshold.
     template <class Entry, class Load, class Emit>
     __device__ __forceinline__ bool gather(uint32_t mine, uint32_t* scratch, int* owners, int64_t per, Load load, Emit emit) {
         const uint32_t t = about_kth<THREADS>(mine, k, scratch);
-        if (mine >= t) owners[atomicAdd(count, 1)] = threadIdx.x;
+        if (t == ~0u) return false;
+        if (mine >= t) owners[atomicAdd(count + 1, 1)] = threadIdx.x;
         __syncthreads();
-        const int m = *count;
-        __syncthreads();
-        if (threadIdx.x == 0) *count = 0;
-        __syncthreads();
+        const int m = count[1];
         for (int i0 = threadIdx.x / 32; i0 < m; i0 += 4 * (THREADS / 32))
             for (int64_t j = threadIdx.x % 32; j < per; j += 32) {
                 Entry e[4];
@@ -114,12 +112,17 @@ struct TopK {
                     if (i0 + u * (THREADS / 32) < m) load(owners[i0 + u * (THREADS / 32)], j, e[u]);
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
-                    if (i0 + u * (THREADS / 32) < m)
-                        emit(e[u], [&](float v, uint32_t index) {
-                            const uint32_t o = order_key(v);
-                            if (o >= t) add(index_key(o, index));
-                        });
+                    if (i0 + u * (THREADS / 32) < m) emit(e[u], [&](float v, uint32_t index) { add(v, index, t); });
             }
+        floor = (uint64_t)t << 32;
+        return added();
+    }
+    // The same of shares that the threads still hold: each(f) calls f(value, index) on this thread's values.
+    template <class Each>
+    __device__ __forceinline__ bool gather_held(uint32_t mine, uint32_t* scratch, Each each) {
+        const uint32_t t = about_kth<THREADS>(mine, k, scratch);
+        if (t == ~0u) return false;
+        if (mine >= t) each([&](float v, uint32_t index) { add(v, index, t); });
         floor = (uint64_t)t << 32;
         return added();
     }
@@ -153,9 +156,8 @@ struct TopK {
         n = *count;
         __syncthreads();
     }
-    // The buffer cut to its k largest, in falling order (at the start of it and in `kept`).  A key's rank is the
-    // number of larger ones.
-    __device__ __forceinline__ void rank() {
+    // The buffer's k largest, in falling order, into `kept`: a key's rank is the number of larger ones.
+    __device__ __forceinline__ void order() {
         for (int i = threadIdx.x; i < n; i += THREADS) {
             const uint64_t mine = buf[i];
             int r = 0;
@@ -165,6 +167,10 @@ struct TopK {
         }
         __syncthreads();
         n = n < k ? n : k;
+    }
+    // The buffer cut to them.
+    __device__ __forceinline__ void rank() {
+        order();
         for (int i = threadIdx.x; i < n; i += THREADS) buf[i] = kept[i];
         if (threadIdx.x == 0) *count = n;
         __syncthreads();
