@@ -536,12 +536,32 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     }
                     m = nm;
                 } else if (is_dlogit(EPI)) {
-                    if (is_grad(EPI)) {
+                    if (is_grad(EPI) && (SUMS || has_ids(EPI))) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float u = fmaf(v[j], p.k2, -rmax);
-                            v[j] = ex2(u) * fmaf(gr.B, fmaxf(u, SCORE_FAR), gr.A);
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 u = fma2(f2(v[j], v[j + 1]), bc2(p.k2), bc2(-rmax)), e = ex2x2(u);
+                            const float2 x = mul2(e, has_ids(EPI) ? bc2(gr.A) : fma2(f2(fmaxf(u.x, SCORE_FAR), fmaxf(u.y, SCORE_FAR)), bc2(gr.B), bc2(gr.A)));
+                            v[j] = x.x;
+                            v[j + 1] = x.y;
                         }
+                    } else if (is_grad(EPI)) {
+                        float2 any = make_float2(0.f, 0.f);
+                        float2 x[16];
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float2 u = fma2(f2(v[2 * j], v[2 * j + 1]), bc2(p.k2), bc2(-rmax));
+                            x[j] = mul2(ex2x2(u), fma2(u, bc2(gr.B), bc2(gr.A)));
+                            any = add2(any, x[j]);
+                        }
+                        if (any.x + any.y != any.x + any.y) {                       // 0 times -inf: those are 0
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) {
+                                const float u0 = fmaf(v[2 * j], p.k2, -rmax), u1 = fmaf(v[2 * j + 1], p.k2, -rmax);
+                                x[j] = f2(ex2(u0) * fmaf(fmaxf(u0, SCORE_FAR), gr.B, gr.A), ex2(u1) * fmaf(fmaxf(u1, SCORE_FAR), gr.B, gr.A));
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) { v[2 * j] = x[j].x; v[2 * j + 1] = x[j].y; }
                     } else {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = ex2((v[j] - rmax) * LOG2E) * rsum;
@@ -565,8 +585,10 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         for (int j = 0; j < 16; ++j) {
                             const __nv_bfloat162 b2 = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
                             w[j] = *reinterpret_cast<const uint32_t*>(&b2);
-                            v[2 * j] -= __low2float(b2);
-                            v[2 * j + 1] -= __high2float(b2);
+                            if (p.planes > 1) {
+                                v[2 * j] -= __low2float(b2);
+                                v[2 * j + 1] -= __high2float(b2);
+                            }
                         }
                         // one piece: 128-byte rows, swizzled (16-byte part j of row r lands at
                         // j ^ (r % 8)); three: 64-byte rows, plain

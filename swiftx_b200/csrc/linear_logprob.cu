@@ -515,7 +515,7 @@ static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
         f.total = f.off_longest + 256;
         // the words' norms are one read of the weight, and without them every candidate's word is read (64 MB of them, which
         // come from the L2 as a rule, take less time than a launch and its read)
-        f.longest = o.T * f.cand > V && o.T * f.cand * o.d * q.es > (int64_t(64) << 20);
+        f.longest = !f.few && o.T * f.cand > V && o.T * f.cand * o.d * q.es > (int64_t(64) << 20);
     }
     return f;
 }

@@ -109,7 +109,8 @@ def _run(x, w, y, g, h, **kw):
     (300, 513, 200, FP, 0, 2.0), (70, 2049, 40, BF, 5, 1.0), (130, 3001, 72, FP, 128, 1.0), (33, 5001, 40, FP, 3, 0.5),
     (520, 9001, 264, BF, 31, 1.0), (64, 300, 1030, FP, 64, 1.0), (40, 20011, 128, BF, 128, 1.0), (3, 50001, 64, BF, 1, 3.0),
     (16, 9001, 1030, BF, 20, 1.0), (9, 4001, 33, BF, 0, 0.7), (1, 12345, 1024, BF, 128, 1.0), (8, 2049, 8, BF, 2, 1.0), (17, 2100, 64, BF, 4, 1.0),
-    (15, 3001, 4104, BF, 11, 2.0), (2, 2500, 2304, BF, 5, 1.0), (7, 3001, 40, FP, 9, 1.0),
+    (15, 3001, 4104, BF, 11, 2.0), (2, 2500, 2304, BF, 5, 1.0), (7, 3001, 40, FP, 9, 1.0), (60, 4001, 1030, FP, 9, 1.0),
+    (300, 9001, 520, BF, 100, 1.0), (2100, 5000, 2048, BF, 12, 1.0),
 ])
 def test_values_alternatives_and_gradients(T, V, d, dtype, top, temp):
     x, w, y = _inputs(T, V, d, dtype, seed=T + V)
