@@ -285,7 +285,7 @@ __device__ __forceinline__ float drop_column(float v) { return __uint_as_float(_
 template <typename T, bool ALL, int THREADS>
 __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     extern __shared__ __align__(16) uint8_t raw[];
-    __shared__ int count[2], ncand, nlist, owners[THREADS];
+    __shared__ int count[2], ncand, nlist, nexact, owners[THREADS];
     __shared__ uint32_t scratch[THREADS + 1];
     __shared__ Score part[THREADS / 32];
     __shared__ float norms[THREADS / 32];
@@ -385,54 +385,63 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
     // those not known, or not told apart from a known one: their products again
     for (int i = threadIdx.x; i < nc; i += THREADS) {
         const float2 z = ze[i];
-        bool close = z.y < 0.f;
+        bool close = z.y < 0.f || off == INFINITY;
+        if (off < INFINITY) {
 #pragma unroll 4
-        for (int j = 0; j < nc; ++j) {
-            const float2 o = ze[j];
-            close |= (j != i) & (o.y >= 0.f) & !(fabsf(o.x - z.x) > 2.0001f * off);
+            for (int j = 0; j < nc; ++j) {
+                const float2 o = ze[j];
+                close |= (j != i) & (o.y >= 0.f) & !(fabsf(o.x - z.x) > 2.0001f * off);
+            }
         }
         if (close) list[atomicAdd(&nlist, 1)] = i;
     }
     __syncthreads();
     candidate_products<THREADS>(x, w, p.w_sr, p.d, p.vec, col, list, nlist, ze, dots);
+    if (threadIdx.x == 0) nexact = 0;
     __syncthreads();
-    // those still not told apart from another (the bounds' sum, and the difference's own rounding): exactly, marked by the sign of their column
+    // their ranks (equal ones by their columns), and those still not told apart from another (the bounds' sum, and the difference's own rounding)
+    const float ls = logf(a.s);
+    auto put = [&](int rank, double z, int c) {
+        if (rank >= p.top) return;
+        p.top_log_probs[row * p.top + rank] = (float)(z * p.k2 - (double)a.m) * LN2 - ls;
+        p.top_ids[row * p.top + rank] = c;
+    };
     for (int i = threadIdx.x; i < nc; i += THREADS) {
         const float2 z = ze[i];
+        const int c = col[i];
+        int r = 0;
         bool close = false;
 #pragma unroll 4
         for (int j = 0; j < nc; ++j) {
             const float2 o = ze[j];
+            r += (int)(o.x > z.x) + (int)((o.x == z.x) & (col[j] < c));
             close |= (j != i) & !(fabsf(o.x - z.x) > (o.y + z.y) * 1.0001f);
         }
-        if (close) col[i] = ~col[i];
+        if (close) list[atomicAdd(&nexact, 1)] = i;
+        else put(r, z.x, c);
     }
     __syncthreads();
-    for (int i = warp; i < nc; i += THREADS / 32) {
-        const int c = col[i];
-        const double z = c >= 0 ? ze[i].x : product_exact(x, w + (int64_t)~c * p.w_sr, p.d, p.vec, lane);
-        __syncwarp();
-        if (lane == 0) {
-            val[i] = order_key(z);
-            if (c < 0) col[i] = ~c;
-        }
+    const int ne = nexact;
+    if (ne == 0) return;
+    // exactly: a candidate that is told apart from all others keeps its rank, so the close ones are ranked anew
+    for (int i = threadIdx.x; i < nc; i += THREADS) val[i] = order_key((double)ze[i].x);
+    __syncthreads();
+    for (int k = warp; k < ne; k += THREADS / 32) {
+        const int i = list[k];
+        const double z = product_exact(x, w + (int64_t)col[i] * p.w_sr, p.d, p.vec, lane);
+        if (lane == 0) val[i] = order_key(z);
     }
     __syncthreads();
-    const float ls = logf(a.s);
-    for (int i = threadIdx.x; i < nc; i += THREADS) {
+    for (int k = threadIdx.x; k < ne; k += THREADS) {
+        const int i = list[k], c = col[i];
         const uint64_t v = val[i];
-        const int c = col[i];
         int r = 0;
 #pragma unroll 4
         for (int j = 0; j < nc; ++j) {
             const uint64_t o = val[j];
             r += (int)(o > v) + (int)((o == v) & (col[j] < c));
         }
-        if (r < p.top) {
-            const double z = __longlong_as_double((long long)(v >> 63 ? v & ~(1ull << 63) : ~v));
-            p.top_log_probs[row * p.top + r] = (float)(z * p.k2 - (double)a.m) * LN2 - ls;
-            p.top_ids[row * p.top + r] = c;
-        }
+        put(r, __longlong_as_double((long long)(v >> 63 ? v & ~(1ull << 63) : ~v)), c);
     }
 }
 
