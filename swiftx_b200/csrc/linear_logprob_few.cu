@@ -33,14 +33,14 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
     }
     const int64_t groups = ((int64_t)p.N + 15) / 16;
     int buf = 0;
-    // steps s0, s0 + 4, ... of a group's words; the next group's are on their way while this one's sums are joined
+    // steps s0, s0 + 1, ... of a group's words (512 bytes of a row together); the next group's are on their way while this one's sums are joined
     uint4 v0[SF_DEPTH], v1[SF_DEPTH];
     auto fetch = [&](int64_t q, int s0) {
         const __nv_bfloat16* w0 = w + min(16 * q + g, (int64_t)p.N - 1) * w_sr;
         const __nv_bfloat16* w1 = w + min(16 * q + 8 + g, (int64_t)p.N - 1) * w_sr;
 #pragma unroll
         for (int i = 0; i < SF_DEPTH; ++i) {
-            const int s = s0 + i * SF_WARPS;
+            const int s = s0 + i;
             const int64_t k = 32 * (int64_t)s + 8 * c;
             if (s < steps) {
                 v0[i] = load8(w0, k, d);
@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
             }
         }
     };
-    fetch(blockIdx.x, warp);
+    fetch(blockIdx.x, SF_DEPTH * warp);
     // the tokens' values, rows of 64 bytes a step and 64 more, so that the 8 rows of a load lie in different banks
     uint4* sx = reinterpret_cast<uint4*>(raw);
     const int stride = 4 * steps + 4;
@@ -59,10 +59,10 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
     __syncthreads();
     for (int64_t q = blockIdx.x; q < groups; q += gridDim.x, buf ^= 1) {
         float acc[NT][4] = {};
-        for (int s0 = warp;;) {
+        for (int s0 = SF_DEPTH * warp;;) {
 #pragma unroll
             for (int i = 0; i < SF_DEPTH; ++i) {
-                const int s = s0 + i * SF_WARPS;
+                const int s = s0 + i;
                 if (s >= steps) continue;
                 const uint32_t a0[4] = {v0[i].x, v1[i].x, v0[i].y, v1[i].y}, a1[4] = {v0[i].z, v1[i].z, v0[i].w, v1[i].w};
 #pragma unroll
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
             if (s0 >= steps) break;
             fetch(q, s0);
         }
-        if (q + gridDim.x < groups) fetch(q + gridDim.x, warp);
+        if (q + gridDim.x < groups) fetch(q + gridDim.x, SF_DEPTH * warp);
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             sums[buf][warp][8 * n + 2 * c][g] = acc[n][0];
