@@ -362,6 +362,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
         int a = 0;
         uint32_t aph = 0;
         bool ok = true;
+        int flip = 0;                         // which half of the staging memory the next store of three pieces takes
         float factor = 1.f;
         float tot[SUMS ? 4 : 1][32];
         if (EPI == XE_DX || EPI == XE_DW) {
@@ -574,10 +575,15 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j] = 0.f;
                     }
-                    // 64 columns of each piece make one 32-row x 128-byte store
+                    // one piece: 64 columns make one store of 32 rows x 128 bytes; three: 32 columns of each one of 64 bytes, two of which
+                    // have room, so that a store need not have been read before the next is made
                     for (int pl = 0; pl < p.planes; ++pl) {
+                        uint8_t* to = so + (p.planes > 1 ? flip * (XE_OUT / 2) : 0);
                         if ((c & 1) == 0 || p.planes > 1) {
-                            if (lane == 0) bulk_wait_read();
+                            if (lane == 0) {
+                                if (p.planes > 1) bulk_wait_read_but_one();
+                                else bulk_wait_read();
+                            }
                             __syncwarp();
                         }
                         uint32_t w[16];
@@ -590,13 +596,11 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                                 v[2 * j + 1] -= __high2float(b2);
                             }
                         }
-                        // one piece: 128-byte rows, swizzled (16-byte part j of row r lands at
-                        // j ^ (r % 8)); three: 64-byte rows, plain
+                        // rows swizzled: 16-byte part j of row r of 128 bytes lands at j ^ (r % 8), of 64 bytes at j ^ (r / 2 % 4)
+                        auto part = [&](int j) { return p.planes > 1 ? lane * 64 + ((j ^ (lane >> 1 & 3)) << 4) : lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4); };
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            const int at_b = p.planes > 1 ? lane * 64 + j * 16
-                                                          : lane * 128 + ((((c & 1) * 4 + j) ^ (lane & 7)) << 4);
-                            *reinterpret_cast<uint4*>(so + at_b) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+                            *reinterpret_cast<uint4*>(to + part(j)) = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                         }
                         if (EPI == XE_GRAD_IDS) {
                             // the row's words among these columns: their own values, in place of what was just written
@@ -605,8 +609,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                                 float r = gr.A * (ex2(fmaf(word_z, p.k2, -rmax)) - rsum * word_share);
                                 for (int q = 0; q < pl; ++q) r -= __bfloat162float(__float2bfloat16_rn(r));
                                 const int j = word - cc;
-                                const int at_b = p.planes > 1 ? lane * 64 + j * 2 : lane * 128 + ((((c & 1) * 4 + (j >> 3)) ^ (lane & 7)) << 4) + (j & 7) * 2;
-                                *reinterpret_cast<__nv_bfloat16*>(so + at_b) = __float2bfloat16_rn(r);
+                                *reinterpret_cast<__nv_bfloat16*>(to + part(j >> 3) + (j & 7) * 2) = __float2bfloat16_rn(r);
                                 ++id;
                                 fetch_word();
                             }
@@ -617,9 +620,12 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                             __syncwarp();
                             const int x = p.planes > 1 ? cc : cc - 32;
                             const int y0 = rc.x * XE_TILE + (int)rank * 128 + sub * 32;
-                            if (lane == 0 && x < p.N && y0 < p.M) {
-                                tma_store_3d(&map_p, so, x, y0, pl);
-                                bulk_commit();
+                            if (x < p.N && y0 < p.M) {
+                                if (lane == 0) {
+                                    tma_store_3d(&map_p, to, x, y0, pl);
+                                    bulk_commit();
+                                }
+                                flip ^= 1;
                             }
                         }
                     }
@@ -719,9 +725,9 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Stages of the logits' contraction summed in tensor memory at a time: all of them for bf16 operands.
 inline int logits_ksub(const HeadPlan& q, int nk) { return q.planes == 3 ? std::min(nk, XE_KSUB_LOGITS) : nk; }
 
-// A (rows, inner) bf16 matrix with `planes` pieces as a 3-D tensor map, 128-byte swizzled.
+// A (rows, inner) bf16 matrix with `planes` pieces as a 3-D tensor map, swizzled within the box's rows of 128 or 64 bytes.
 inline bool encode_operand(CUtensorMap* m, const void* base, int64_t inner, int64_t rows, int64_t planes, int64_t row,
-                           int64_t plane, uint32_t box_inner, uint32_t box_rows, bool swizzle = true) {
+                           int64_t plane, uint32_t box_inner, uint32_t box_rows, int swizzle = 128) {
     const EncodeTiledFn f = encode_tiled();
     if (!f || !base || (reinterpret_cast<uintptr_t>(base) & 15)) return false;
     const int64_t rs = row * 2, ps = (planes > 1 ? plane : row * rows) * 2;
@@ -731,7 +737,7 @@ inline bool encode_operand(CUtensorMap* m, const void* base, int64_t inner, int6
     cuuint32_t box[3] = {box_inner, box_rows, 1};
     cuuint32_t unit[3] = {1, 1, 1};
     return f(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, unit,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -797,7 +803,7 @@ static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const
         const Operand pr{ws + q.off_p, cw, o.T, q.planes, q.ldp, o.T * q.ldp};
         CUtensorMap p_st;
         // stores of 32 rows: 64 columns at once for one piece, 32 for each of three
-        if (!encode_operand(&p_st, pr.p, cw, o.T, q.planes, q.ldp, o.T * q.ldp, q.planes == 3 ? 32 : 64, 32, q.planes == 1)) return SWX_ERR_CUDA;
+        if (!encode_operand(&p_st, pr.p, cw, o.T, q.planes, q.ldp, o.T * q.ldp, q.planes == 3 ? 32 : 64, 32, q.planes == 3 ? 64 : 128)) return SWX_ERR_CUDA;
         XentGemm g = logits_gemm(o, q, c0, cw, status);
         fill(g);
         if (launch(g, x_k, w_k, p_st, st) != cudaSuccess) return SWX_ERR_CUDA;
