@@ -14,7 +14,7 @@
 // operands staged by TMA into a ring, tcgen05 products issued by one thread per pair into
 // two alternating accumulators in tensor memory, and eight warps per CTA that read an
 // accumulator while the next tile is computed.  The tensor pipe bounds it: 4096 tokens x 32768 x 1024 bf16, cold,
-// forward 178 us (88 % of the SM's active cycles on products, 1547 TFLOP/s), dlogit 199 us (79 %; it writes 268 MB), dx 190
+// forward 178 us (88 % of the SM's active cycles on products, 1547 TFLOP/s), dlogit 184 us (it writes 268 MB), dx 190
 // (93 %, on 64 of 74 pairs); 8192 x 50001 x 1024 0.51, 0.57, 0.58 and 0.60 ms, where a library
 // product of the same size alone takes 0.56 to 0.61.  The logits' epilogue (an exponential for each) fits behind a
 // tile's products from about 512 values of the contraction on; below that it bounds the forward.

@@ -107,7 +107,8 @@ def linear_log_probs(x, weight, targets, top_k=0, temperature=1.0, ignore_index=
     128.  log_probs and entropy are differentiable in x and weight (a gradient of one alone may be asked for);
     the alternatives are not.  Ignored tokens: zeros, ids of -1 and no gradient, whatever x holds there as long as it is
     finite.  Alternatives are in falling order, the lowest word first among equals; they are ordered by fp64
-    products of the operands, so that rounding changes neither their order nor their ties.
+    products of the operands, so that rounding changes neither their order nor their ties (among the top_k + 4 or more words
+    with the largest fp32 products: where more words than that differ by a rounding of those, others of them may be missing).
 
     bf16 operands: products summed in fp32 in the tensor cores, the logits' gradient rounded to bf16 once
     for its products; fp32 operands keep fp32 accuracy and have to be finite.  A target outside [0, vocab) other than
