@@ -87,6 +87,7 @@ struct XentGemm {
     // low 4 bits; columns from N on count as SCORE_FLOOR
     float* largest; float* runner_up;
     float* all;                               // XE_SCORE_ALL, (M, N)
+    int beside;                               // the next kernel (the words' norms) may start beside this one
     // XE_SCORE_IDS, XE_GRAD_IDS: each row's words in rising order, their logits and shares, (M, nids), and how many of them lie before
     // each 128 columns of the vocabulary, (M, stride)
     const int* ids; float* id_logit; const float* id_share; const uint8_t* before; int nids, before_stride;
@@ -276,6 +277,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
     cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
+    if ((EPI == XE_SCORE_TOP || EPI == XE_SCORE_ALL) && p.beside) let_next_start();
 
     if (warp == 0) {
         if (lane == 0) {

@@ -15,11 +15,11 @@ namespace swx {
 int device_symbol_address(const void* sym, void** out);
 int* wait_status_address();
 
-// Opt a kernel into more than 48 KB of dynamic shared memory.  Done once per kernel
+// Opt a kernel into more than 48 KB of dynamic shared memory (or set another of its attributes).  Done once per kernel
 // and device (cached), so later launches -- e.g. inside CUDA-graph capture -- make no
 // runtime configuration calls.
 template <typename K>
-inline cudaError_t allow_smem(K kernel, int bytes) {
+inline cudaError_t allow_smem(K kernel, int bytes, cudaFuncAttribute attribute = cudaFuncAttributeMaxDynamicSharedMemorySize) {
     struct Entry { int dev; const void* fn; };
     static std::mutex mu;
     static std::vector<Entry> done;
@@ -30,7 +30,7 @@ inline cudaError_t allow_smem(K kernel, int bytes) {
     std::lock_guard<std::mutex> lock(mu);
     for (const Entry& x : done)
         if (x.dev == dev && x.fn == fn) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    e = cudaFuncSetAttribute(kernel, attribute, bytes);
     if (e == cudaSuccess) done.push_back({dev, fn});
     return e;
 }
@@ -56,7 +56,7 @@ inline cudaError_t sm_fit(K kernel, int threads, int smem, int* sms, int* per_sm
 }
 
 // A launch whose blocks may be set up while the stream's previous kernel still runs; the kernel has to call
-// wait_for_previous() before anything else.
+// wait_for_previous() before anything else, or, where it needs nothing of that kernel, before it ends.
 template <typename... Params, typename... Args>
 inline cudaError_t launch_after(void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t st, Args... args) {
     cudaLaunchConfig_t c{};
@@ -71,6 +71,8 @@ inline cudaError_t launch_after(void (*kernel)(Params...), unsigned grid, unsign
     c.numAttrs = 1;
     return cudaLaunchKernelEx(&c, kernel, args...);
 }
+// Once every block of the kernel has called it (or ended), a launch_after of the stream's next kernel may start beside this one.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 }  // namespace swx

@@ -22,6 +22,7 @@ namespace swx {
 
 constexpr int SC_EXTRA = 4;                   // candidates beyond K
 constexpr int SC_THREADS = 256, SC_PER = 8;
+constexpr int SC_NORM_THREADS = 128;
 constexpr float LN2 = 0.69314718055994531f;
 
 struct ScoreRows {
@@ -446,48 +447,36 @@ __global__ void __launch_bounds__(THREADS) score_top_kernel(const ScoreRows p) {
 }
 
 // The largest squared norm of a word, a warp for each (fp32 sums of squares: 2^-24 for each of d / 32 additions, far inside the
-// bound's slack).  One read of the weight: 50001 x 1024 bf16 about 20 us.
+// bound's slack).  One read of the weight, beside the logits' product: that kernel's 10 warps of up to 160 registers leave
+// each quarter of an SM one warp of 32 (4096 rows of 50001 x 1024 with 32 alternatives 431 us with this kernel behind the
+// product, 410 so).  Where the product takes more registers (fp32 operands) this one fills the SMs after it.
 template <typename T>
-__global__ void __launch_bounds__(256) longest_word_kernel(const T* w, int64_t w_sr, int64_t V, int64_t d, bool vec, uint32_t* longest) {
-    __shared__ float most[8];
-    constexpr int N = 16 / sizeof(T);
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+__global__ void __launch_bounds__(SC_NORM_THREADS, 2048 / SC_NORM_THREADS) longest_word_kernel(const T* w, int64_t w_sr, int64_t V, int64_t d, bool vec, uint32_t* longest) {
+    constexpr int N = 16 / sizeof(T), W = SC_NORM_THREADS / 32;
+    const int lane = threadIdx.x % 32;
     float top = 0.f;
-    const int64_t step = (int64_t)gridDim.x * 8;
-    for (int64_t v = (int64_t)blockIdx.x * 8 + warp; v < V; v += 2 * step) {
-        const T* r[2] = {w + v * w_sr, w + min(v + step, V - 1) * w_sr};
-        float2 s[2] = {};
+    for (int64_t v = (int64_t)blockIdx.x * W + threadIdx.x / 32; v < V; v += (int64_t)gridDim.x * W) {
+        const T* r = w + v * w_sr;
+        float2 s = make_float2(0.f, 0.f);
         int64_t tail = 0;
         if (vec) {
 #pragma unroll 4
             for (int64_t k = lane * N; k + N <= d; k += 32 * N) {
-                float2 q[2][N / 2];
+                float2 q[N / 2];
+                unpack(r, *reinterpret_cast<const uint4*>(r + k), q);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) unpack(r[i], *reinterpret_cast<const uint4*>(r[i] + k), q[i]);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < N / 2; ++j) s[i] = fma2(q[i][j], q[i][j], s[i]);
+                for (int j = 0; j < N / 2; ++j) s = fma2(q[j], q[j], s);
             }
             tail = d / N * N;
         }
-        for (int64_t k = tail + lane; k < d; k += 32)
+        for (int64_t k = tail + lane; k < d; k += 32) { const float q = Elem<T>::to_f(r[k]); s.x = fmaf(q, q, s.x); }
+        float t = s.x + s.y;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) { const float q = Elem<T>::to_f(r[i][k]); s[i].x = fmaf(q, q, s[i].x); }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            float t = s[i].x + s[i].y;
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
-            top = t == t ? fmaxf(top, t) : INFINITY;
-        }
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        top = t == t ? fmaxf(top, t) : INFINITY;
     }
-    if (lane == 0) most[warp] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int i = 1; i < 8; ++i) top = fmaxf(top, most[i]);
-        atomicMax(longest, __float_as_uint(top));
-    }
+    if (lane == 0) atomicMax(longest, __float_as_uint(top));
+    if (blockIdx.x == 0) wait_for_previous(); // so that this kernel ends after the product's
 }
 
 // ------------------------------------------------------------------ host side
@@ -522,7 +511,7 @@ static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
         f.off_second = f.off_rec + up256(f.all ? T * V * 4 : T * f.stride * 4);
         f.off_longest = f.off_second + (f.all ? 0 : up256(T * f.stride * 4));
         f.total = f.off_longest + 256;
-        // the words' norms are one read of the weight, and without them every candidate's word is read (64 MB of them, which
+        // the words' norms are one read of the weight beside the product, and without them every candidate's word is read (64 MB of them, which
         // come from the L2 as a rule, take less time than a launch and its read)
         f.longest = !f.few && o.T * f.cand > V && o.T * f.cand * o.d * q.es > (int64_t(64) << 20);
     }
@@ -550,6 +539,16 @@ static cudaError_t launch_top(const ScoreRows& p, cudaStream_t st) {
     const cudaError_t e = allow_smem(score_top_kernel<T, ALL, THREADS>, (int)score_top_smem(ALL, std::min(THREADS, SWX_MAX_TOP + SC_EXTRA)));
     if (e != cudaSuccess) return e;
     return launch_after(score_top_kernel<T, ALL, THREADS>, (unsigned)p.T, THREADS, smem, st, p);
+}
+
+// One CTA an SM, with the shared memory's split that the product needs (a kernel that wants another one has to wait for the SM).
+template <typename T>
+static cudaError_t launch_longest(const HeadOps& o, const void* w, int64_t w_sr, bool vec, uint32_t* out, cudaStream_t st) {
+    auto k = longest_word_kernel<T>;
+    cudaError_t e;
+    if ((e = allow_smem(k, cudaSharedmemCarveoutMaxShared, cudaFuncAttributePreferredSharedMemoryCarveout)) != cudaSuccess) return e;
+    const unsigned grid = (unsigned)std::min<int64_t>((o.V + SC_NORM_THREADS / 32 - 1) / (SC_NORM_THREADS / 32), 148 * (2048 / SC_NORM_THREADS));
+    return launch_after(k, grid, SC_NORM_THREADS, 0, st, static_cast<const T*>(w), w_sr, o.V, o.d, vec, out);
 }
 
 template <typename T>
@@ -594,6 +593,11 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
     Operand x, w;
     head_operands(o, q, ws, x, w, st);
     const bool bf = o.dtype == SWX_DTYPE_BF16;
+    // the rows' operands in their own type: bf16 ones from their copies where those were made (their rows start on 16 bytes)
+    const void* sw = bf ? w.p : o.w;
+    const int64_t w_sr = bf ? w.row : o.w_sr;
+    const bool vec = bf || (aligned16(o.x) && aligned16(o.w) && o.x_sr % 4 == 0 && o.w_sr % 4 == 0);
+    uint32_t* norm = reinterpret_cast<uint32_t*>(ws + f.off_longest);
     bool longest = f.longest;                 // the words' norms are still to be read
     for (int64_t r0 = 0; r0 < o.T; r0 += SC_ROWS) {
         HeadOps oc = o;
@@ -614,12 +618,16 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         g.hit = reinterpret_cast<float*>(ws + f.off_hit);
         g.largest = reinterpret_cast<float*>(ws + f.off_rec); g.runner_up = reinterpret_cast<float*>(ws + f.off_second);
         g.all = reinterpret_cast<float*>(ws + f.off_rec);
-        g.counter = longest ? reinterpret_cast<int*>(ws + f.off_longest) : nullptr;
+        if (longest && cudaMemsetAsync(norm, 0, 4, st) != cudaSuccess) return SWX_ERR_CUDA;
+        g.beside = longest;
         const cudaError_t e = f.few ? launch_score_few(g, oc, xc, w, a->top_k > 0, f.few, st)
                               : a->top_k == 0 ? launch_logits<XE_SCORE>(g, mx, mw, mx, st)
                               : f.all       ? launch_logits<XE_SCORE_ALL>(g, mx, mw, mx, st)
                                             : launch_logits<XE_SCORE_TOP>(g, mx, mw, mx, st);
         if (e != cudaSuccess) return SWX_ERR_CUDA;
+        if (longest && (bf ? launch_longest<__nv_bfloat16>(o, sw, w_sr, vec, norm, st) : launch_longest<float>(o, sw, w_sr, vec, norm, st)) != cudaSuccess)
+            return SWX_ERR_CUDA;
+        longest = false;
         ScoreRows p{};
         p.T = oc.T; p.V = o.V; p.d = o.d; p.np = f.np;
         p.score = g.score; p.hit = g.hit; p.target = g.target; p.ignore = a->ignore_index;
@@ -633,19 +641,9 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         }
         p.top = a->top_k; p.cand = f.cand; p.largest = g.largest; p.runner_up = g.runner_up; p.stride = f.stride; p.all = g.all; p.groups = f.groups;
         p.top_log_probs = a->top_log_probs + r0 * a->top_k; p.top_ids = a->top_ids + r0 * a->top_k;
-        // the operands in their own type: bf16 ones from their copies where those were made (their rows start on 16 bytes)
         p.x = bf ? xc.p : oc.x; p.x_sr = bf ? x.row : o.x_sr;
-        p.w = bf ? w.p : o.w; p.w_sr = bf ? w.row : o.w_sr;
-        p.vec = bf || (aligned16(o.x) && aligned16(o.w) && o.x_sr % 4 == 0 && o.w_sr % 4 == 0);
-        if (f.longest) p.longest = reinterpret_cast<const uint32_t*>(ws + f.off_longest);
-        if (longest) {
-            uint32_t* out = reinterpret_cast<uint32_t*>(g.counter);
-            const unsigned grid = (unsigned)std::min<int64_t>((o.V + 7) / 8, 148 * 8);
-            if (bf) longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(p.w), p.w_sr, p.V, p.d, true, out);
-            else longest_word_kernel<<<grid, 256, 0, st>>>(static_cast<const float*>(p.w), p.w_sr, p.V, p.d, p.vec != 0, out);
-            if (cudaGetLastError() != cudaSuccess) return SWX_ERR_CUDA;
-            longest = false;
-        }
+        p.w = sw; p.w_sr = w_sr; p.vec = vec;
+        if (f.longest) p.longest = norm;
         if ((bf ? launch_top<__nv_bfloat16>(p, f.all, st) : launch_top<float>(p, f.all, st)) != cudaSuccess) return SWX_ERR_CUDA;
     }
     return SWX_OK;
