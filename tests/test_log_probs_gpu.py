@@ -335,6 +335,25 @@ def test_more_rows_than_one_product_takes(T, V, d, dtype, top):
         assert (a is None and b is None) or torch.equal(a, b) or (a.is_floating_point() and float((a - b).abs().max()) <= E)
 
 
+@pytest.mark.parametrize("T,V,d,dtype,top", [(4001, 10007, 201, FP, 20), (2600, 6001, 521, BF, 40), (2200, 1024, 1024, BF, 12)])
+def test_norms_of_the_words(T, V, d, dtype, top):
+    """Sizes whose candidates' bound comes from the longest word, here the last one: eager, and replayed with other operands."""
+    assert T * (top + 4) > V and T * (top + 4) * d * (4 if dtype == FP else 2) > 64 << 20 and V * d < 32 << 20
+    x, w, y = _inputs(T, V, d, dtype, seed=T)
+    w[-1] *= 2
+    with torch.no_grad():
+        _check_forward(linear_log_probs(x, w, y, top_k=top), x, w, y, 1.0, top)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = linear_log_probs(x, w, y, top_k=top)
+        w.mul_(-2), x.mul_(0.5)
+        graph.replay()
+        _check_forward(out, x, w, y, 1.0, top)
+        for a, b in zip(out, linear_log_probs(x, w, y, top_k=top)):
+            assert torch.equal(a, b)
+    assert _lib.load().swx_device_wait_status() == _lib.SWX_OK
+
+
 def test_deterministic_streams_and_graphs():
     x, w, y = _inputs(603, 5001, 72, BF, seed=6)
     g, h = _upstream(603)
