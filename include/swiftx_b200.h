@@ -473,7 +473,7 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  * outside [0, vocab): its log probability, and the gradients that it enters, NaN.  The
  * statistics are fp32; the alternatives are ordered by products in fp64 of the operands, so that
  * neither their order nor their ties depend on the rounding of sums.
- * Forward writes row_max (the largest z times log2(e) / temperature) and row_sum (tokens values, both or
+ * Forward writes row_max (the largest z) and row_sum (the sum of exp((z - row_max) / temperature); tokens values, both or
  * neither) for the backward.
  * Backward: d_log_probs, d_entropy (tokens values; either may be NULL: zero), entropy as the forward
  * wrote it (needed with d_entropy) -> dx and dweight as in swx_xent_args (bf16 operands:

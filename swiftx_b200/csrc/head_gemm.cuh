@@ -79,8 +79,9 @@ struct XentGemm {
     int spread;
     float* acc; void* out; int out_bf16; int64_t ld; int first, last;
     const float* scale_num; const float* scale_den;   // the result's factor: num / den, either may be absent
-    // XE_SCORE*, XE_GRAD: exponents are logit * k2 - m, k2 = log2(e) / temperature, m the largest logit times k2 (rounded once, so
-    // that an exponent is one fused operation, off by its own rounding)
+    // XE_SCORE*, XE_GRAD: exponents are (logit - m) * k2, k2 = log2(e) / temperature, m the largest logit.  The difference comes first,
+    // so that the largest term is 1 at any temperature (with m k2 rounded and one fused operation for each exponent, its residual, a 2^-24th of
+    // |m| k2, went into the sums: 2^500 at a temperature of 1e-8)
     float k2, inv_temp;
     float4* score;                            // (M, 2 nt): a tile half's m, sum of exponentials e, sum of e times its exponent
     // XE_SCORE_TOP, (M, 16 nt): the largest logit of 16 columns, and the second with the largest one's column in place of its
@@ -170,7 +171,7 @@ __device__ __forceinline__ float row_scale(const XentGemm& p, int row) {
     return p.reduction == SWX_XENT_NONE ? p.dloss[row] : 1.f;
 }
 
-// A row's coefficients of XE_GRAD.  With u = z k2 - m, e = 2^u, s the sum of e: p = e / s, the log probability
+// A row's coefficients of XE_GRAD.  With u = (z - m) k2, e = 2^u, s the sum of e: p = e / s, the log probability
 // l = u ln2 - ln s, and for upstream gradients g of the target's log probability and h of the entropy H
 //   dz = (g [v == y] - p (g + h (l + H))) / temperature = e (A + B u) + [v == y] hot.
 // Distillation (no targets): dz = (p - Q) c / temperature with c = temperature^2 times the row's upstream gradient and Q the
@@ -517,13 +518,13 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         for (int j = 0; j < 32; j += 2) top = max3(top, v[j], v[j + 1]);
                     }
                     // sums relative to the larger maximum: e u becomes c e (u + shift)
-                    const float nm = fmaxf(m, top * p.k2);
-                    const float shift = fmaxf(m - nm, SCORE_FAR), c2 = ex2(shift);
+                    const float nm = fmaxf(m, top);
+                    const float shift = fmaxf((m - nm) * p.k2, SCORE_FAR), c2 = ex2(shift);
                     const float s0 = sum * c2, w0 = c2 * (esum + sum * shift);
                     float2 s2 = make_float2(s0, 0.f), w2 = make_float2(w0, 0.f);
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        const float2 u = fma2(f2(v[j], v[j + 1]), bc2(p.k2), bc2(-nm)), e = ex2x2(u);
+                        const float2 u = mul2(add2(f2(v[j], v[j + 1]), bc2(-nm)), bc2(p.k2)), e = ex2x2(u);
                         s2 = add2(s2, e);
                         w2 = fma2(e, u, w2);
                     }
@@ -533,7 +534,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         esum = w0;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float u = fmaf(v[j], p.k2, -nm);
+                            const float u = (v[j] - nm) * p.k2;
                             esum += ex2(u) * fmaxf(u, SCORE_FAR);
                         }
                     }
@@ -542,7 +543,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     if (is_grad(EPI) && (SUMS || has_ids(EPI))) {
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
-                            const float2 u = fma2(f2(v[j], v[j + 1]), bc2(p.k2), bc2(-rmax)), e = ex2x2(u);
+                            const float2 u = mul2(add2(f2(v[j], v[j + 1]), bc2(-rmax)), bc2(p.k2)), e = ex2x2(u);
                             const float2 x = mul2(e, has_ids(EPI) ? bc2(gr.A) : fma2(f2(fmaxf(u.x, SCORE_FAR), fmaxf(u.y, SCORE_FAR)), bc2(gr.B), bc2(gr.A)));
                             v[j] = x.x;
                             v[j + 1] = x.y;
@@ -552,14 +553,14 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         float2 x[16];
 #pragma unroll
                         for (int j = 0; j < 16; ++j) {
-                            const float2 u = fma2(f2(v[2 * j], v[2 * j + 1]), bc2(p.k2), bc2(-rmax));
+                            const float2 u = mul2(add2(f2(v[2 * j], v[2 * j + 1]), bc2(-rmax)), bc2(p.k2));
                             x[j] = mul2(ex2x2(u), fma2(u, bc2(gr.B), bc2(gr.A)));
                             any = add2(any, x[j]);
                         }
                         if (any.x + any.y != any.x + any.y) {                       // 0 times -inf: those are 0
 #pragma unroll
                             for (int j = 0; j < 16; ++j) {
-                                const float u0 = fmaf(v[2 * j], p.k2, -rmax), u1 = fmaf(v[2 * j + 1], p.k2, -rmax);
+                                const float u0 = (v[2 * j] - rmax) * p.k2, u1 = (v[2 * j + 1] - rmax) * p.k2;
                                 x[j] = f2(ex2(u0) * fmaf(fmaxf(u0, SCORE_FAR), gr.B, gr.A), ex2(u1) * fmaf(fmaxf(u1, SCORE_FAR), gr.B, gr.A));
                             }
                         }
@@ -608,7 +609,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                             // the row's words among these columns: their own values, in place of what was just written
                             const int id0 = id;
                             while (word < cc + 32) {
-                                float r = gr.A * (ex2(fmaf(word_z, p.k2, -rmax)) - rsum * word_share);
+                                float r = gr.A * (ex2((word_z - rmax) * p.k2) - rsum * word_share);
                                 for (int q = 0; q < pl; ++q) r -= __bfloat162float(__float2bfloat16_rn(r));
                                 const int j = word - cc;
                                 *reinterpret_cast<__nv_bfloat16*>(to + part(j >> 3) + (j & 7) * 2) = __float2bfloat16_rn(r);

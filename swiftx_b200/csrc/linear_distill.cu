@@ -154,12 +154,12 @@ __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillR
     const int64_t row = (int64_t)blockIdx.x * DI_WARPS + warp;
     double sum = 0., n = 0.;
     if (row < p.T) {
-        const Score a = score_join_parts(p.score + row * p.np, p.np, lane, 32);
+        const Score a = score_join_parts(p.score + row * p.np, p.np, p.k2, lane, 32);
         const float ls = logf(a.s), mark = p.s.row_sum[row];
         float loss = 0.f;
         for (int j = lane; j < p.K; j += 32) {
             const float share = mark > 0.f && p.s.ids[row * p.K + j] != INT32_MAX ? p.s.share[row * p.K + j] : 0.f;
-            if (share != 0.f) loss += share * (fmaf(p.s.logit[row * p.K + j], p.k2, -a.m) * DI_LN2 - ls);
+            if (share != 0.f) loss += share * ((p.s.logit[row * p.K + j] - a.m) * p.k2 * DI_LN2 - ls);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, o);

@@ -5,7 +5,7 @@
 //   dz_v = (g [v == y] - p_v (g + h (l_v + H))) / tau,  dx = dz W,  dW = dz^T x.
 //
 // Forward: the head's product (head_gemm.cuh) with an epilogue that keeps three floats for each half of a 256-column tile: the
-// maximum m (of z log2(e) / tau), s = sum e and w = sum e u of e = 2^u, u = z log2(e) / tau - m; with alternatives also the two largest logits of every
+// maximum m, s = sum e and w = sum e u of e = 2^u, u = (z - m) log2(e) / tau; with alternatives also the two largest logits of every
 // 16 columns (8 bytes), or, for a small vocabulary, the logits.  Then one kernel for the rows: the statistics joined, and
 //   H = ln s - ln2 w / s.
 // Alternatives: the K + 4 groups of 16 columns with the largest maxima hold the K + 4 largest logits; a group whose second value
@@ -29,7 +29,9 @@ struct ScoreRows {
     int64_t T, V, d;
     int np;                                   // statistics per row
     const float4* score; const float* hit; const int64_t* target; int64_t ignore;
-    float k2, cut;                            // log2(e) / temperature; the products' mean cut (they are to be taken 1 + cut times)
+    // the statistics' exponents' scale (the products': (1 + cut) log2(e) / temperature); the products' mean cut, and log2(e) /
+    // temperature for logits that carry it or do without
+    float k2, cut, exact_k2;
     float* row_max; float* row_sum; float* log_probs; float* entropy;
     // alternatives
     int top, cand;                            // K, candidates kept of the records
@@ -39,13 +41,13 @@ struct ScoreRows {
     float* top_log_probs; int64_t* top_ids;
 };
 
-// A row's results from its statistics.
+// A row's results from its statistics: the target's logit as the sums saw it, so that no value is above 0.
 __device__ __forceinline__ void score_finish(const ScoreRows& p, int64_t row, const Score& a) {
     const int64_t y = p.target[row];
     const float ls = logf(a.s);
     if (p.row_max) { p.row_max[row] = a.m; p.row_sum[row] = a.s; }
     const bool live = y != p.ignore;
-    p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? fmaf(fmaf(p.hit[row], p.cut, p.hit[row]), p.k2, -a.m) * LN2 - ls : __int_as_float(0x7fc00000);
+    p.log_probs[row] = !live ? 0.f : y >= 0 && y < p.V ? (p.hit[row] - a.m) * p.k2 * LN2 - ls : __int_as_float(0x7fc00000);
     p.entropy[row] = live ? ls - LN2 * a.w / a.s : 0.f;
 }
 
@@ -55,7 +57,7 @@ __global__ void __launch_bounds__(SC_THREADS) score_rows_kernel(const ScoreRows 
     const int64_t row = (int64_t)blockIdx.x * (SC_THREADS / 32) + threadIdx.x / 32;
     if (row >= p.T) return;
     const int lane = threadIdx.x % 32;
-    const Score a = score_join_parts(p.score + row * p.np, p.np, lane, 32);
+    const Score a = score_join_parts(p.score + row * p.np, p.np, p.k2, lane, 32);
     if (lane == 0) score_finish(p, row, a);
 }
 
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
         for (int o = 16; o > 0; o >>= 1) xx += __shfl_xor_sync(0xffffffffu, xx, o);
         if (lane == 0) norms[warp] = xx;
     }
-    const Score a = score_join_row<THREADS>(p.score + row * p.np, p.np, part);
+    const Score a = score_join_row<THREADS>(p.score + row * p.np, p.np, p.k2, part);
     if (threadIdx.x == 0) score_finish(p, row, a);
     if (p.target[row] == p.ignore) {                                 // a token that does not count
         for (int i = threadIdx.x; i < p.top; i += THREADS) {
@@ -362,6 +364,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
               sqrtf(fmaxf(__uint_as_float(*p.longest), 0x1p-100f));
     }
     const float least = ALL ? 0.f : order_value((uint32_t)(best.floor >> 32));
+    for (int i = threadIdx.x; i < p.cand; i += THREADS) kept[i] = 0;  // from here on: the candidates by rank
     for (int i = threadIdx.x; i < m; i += THREADS) {
         const uint32_t g = key_index(buf[i]);
         const float z = order_value((uint32_t)(buf[i] >> 32));
@@ -402,12 +405,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
     if (threadIdx.x == 0) nexact = 0;
     __syncthreads();
     // their ranks (equal ones by their columns), and those still not told apart from another (the bounds' sum, and the difference's own rounding)
-    const float ls = logf(a.s);
-    auto put = [&](int rank, double z, int c) {
-        if (rank >= p.top) return;
-        p.top_log_probs[row * p.top + rank] = (float)(z * p.k2 - (double)a.m) * LN2 - ls;
-        p.top_ids[row * p.top + rank] = c;
-    };
+    auto put = [&](int rank, int i) { if (rank < p.top) kept[rank] = i; };
     for (int i = threadIdx.x; i < nc; i += THREADS) {
         const float2 z = ze[i];
         const int c = col[i];
@@ -420,11 +418,23 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
             close |= (j != i) & !(fabsf(o.x - z.x) > (o.y + z.y) * 1.0001f);
         }
         if (close) list[atomicAdd(&nexact, 1)] = i;
-        else put(r, z.x, c);
+        else put(r, i);
     }
     __syncthreads();
     const int ne = nexact;
-    if (ne == 0) return;
+    // the first alternative has the statistics' maximum (its own sum, with other roundings, would put its probability above 1, by a part of
+    // |z| / temperature), and the others their distance from the first
+    const float ls = logf(a.s);
+    auto write = [&](auto z) {
+        for (int i = threadIdx.x; i < p.top; i += THREADS) {
+            p.top_log_probs[row * p.top + i] = (float)((z(kept[i]) - z(kept[0])) * p.exact_k2) * LN2 - ls;
+            p.top_ids[row * p.top + i] = col[kept[i]];
+        }
+    };
+    if (ne == 0) {
+        write([&](uint64_t i) { return (double)ze[i].x; });
+        return;
+    }
     // exactly: a candidate that is told apart from all others keeps its rank, so the close ones are ranked anew
     for (int i = threadIdx.x; i < nc; i += THREADS) val[i] = order_key((double)ze[i].x);
     __syncthreads();
@@ -443,8 +453,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
             const uint64_t o = val[j];
             r += (int)(o > v) + (int)((o == v) & (col[j] < c));
         }
-        put(r, __longlong_as_double((long long)(v >> 63 ? v & ~(1ull << 63) : ~v)), c);
+        put(r, i);
     }
+    __syncthreads();
+    write([&](uint64_t i) { const uint64_t v = val[i]; return __longlong_as_double((long long)(v >> 63 ? v & ~(1ull << 63) : ~v)); });
 }
 
 // The largest squared norm of a word, a warp for each (fp32 sums of squares: 2^-24 for each of d / 32 additions, far inside the
@@ -632,7 +644,7 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         ScoreRows p{};
         p.T = oc.T; p.V = o.V; p.d = o.d; p.np = f.np;
         p.score = g.score; p.hit = g.hit; p.target = g.target; p.ignore = a->ignore_index;
-        p.k2 = exponent_scale(a->temperature, 0.f); p.cut = cut;
+        p.k2 = g.k2; p.cut = cut; p.exact_k2 = exponent_scale(a->temperature, 0.f);
         p.row_max = a->row_max ? a->row_max + r0 : nullptr; p.row_sum = a->row_sum ? a->row_sum + r0 : nullptr;
         p.log_probs = a->log_probs + r0; p.entropy = a->entropy + r0;
         if (a->top_k == 0) {

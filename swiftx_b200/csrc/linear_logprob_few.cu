@@ -80,9 +80,9 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
         const bool in = v < p.N;
         if (in && t < p.M && v == y) p.hit[t] = z;
         if (in) {
-            const float m = fmaxf(a.m, z * p.k2), base = m == -INFINITY ? 0.f : m;
-            score_move(a, base);
-            const float u = fmaf(z, p.k2, -base), e = ex2(u);
+            const float m = fmaxf(a.m, z), base = m == -INFINITY ? 0.f : m;
+            score_move(a, base, p.k2);
+            const float u = (z - base) * p.k2, e = ex2(u);
             a.m = m;
             a.s += e;
             a.w += e * fmaxf(u, SCORE_FAR);
@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
     float m = a.m;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    score_move(a, m);
+    score_move(a, m, p.k2);
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
         a.s += __shfl_xor_sync(0xffffffffu, a.s, o);

@@ -178,26 +178,26 @@ struct TopK {
     }
 };
 
-// Statistics of scaled logits in base 2: m the largest (times k2), s = sum 2^u and w = sum 2^u u with u = z k2 - m; or, with k =
-// k2 handed to the joins, m the largest itself and u = (z - m) k2 (logits at the lowest end of their type would overflow in z k2).
+// Statistics of scaled logits in base 2: m the largest logit, s = sum 2^u and w = sum 2^u u with u = (z - m) k, k = log2(e) /
+// temperature.  m stays unscaled: the largest term is 1 whatever the temperature, so s is at least 1 and w at most 0.
 // (m = -inf with s = w = 0: nothing yet; the differences of infinities, NaN, are dropped by the maximum with SCORE_FAR.)
 constexpr float SCORE_FAR = -200.f;           // 2^-200 is 0: what lies further below the maximum adds nothing
 struct Score { float m, s, w; };
 // The same relative to a larger m.
-__device__ __forceinline__ void score_move(Score& a, float m, float k = 1.f) {
+__device__ __forceinline__ void score_move(Score& a, float m, float k) {
     const float d = fmaxf((a.m - m) * k, SCORE_FAR), c = ex2(d);
     a.w = c * (a.w + a.s * d);
     a.s *= c;
     a.m = m;
 }
-__device__ __forceinline__ void score_join(Score& a, Score b, float k = 1.f) {
+__device__ __forceinline__ void score_join(Score& a, Score b, float k) {
     const float m = fmaxf(a.m, b.m);
     score_move(a, m, k);
     score_move(b, m, k);
     a.s += b.s;
     a.w += b.w;
 }
-__device__ __forceinline__ void score_join_warp(Score& a, float k = 1.f) {
+__device__ __forceinline__ void score_join_warp(Score& a, float k) {
     float m = a.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
@@ -209,7 +209,7 @@ __device__ __forceinline__ void score_join_warp(Score& a, float k = 1.f) {
     }
 }
 // The statistics of a whole row by `threads` threads (of which this is number t), from its np parts, before they are joined.
-__device__ __forceinline__ Score score_join_parts(const float4* q, int np, int t, int threads) {
+__device__ __forceinline__ Score score_join_parts(const float4* q, int np, float k, int t, int threads) {
     Score a{-INFINITY, 0.f, 0.f};
     for (int i0 = t; i0 < np; i0 += 4 * threads) {
         float4 v[4];
@@ -219,22 +219,22 @@ __device__ __forceinline__ Score score_join_parts(const float4* q, int np, int t
             v[u] = i0 + u * threads < np ? q[i0 + u * threads] : make_float4(-INFINITY, 0.f, 0.f, 0.f);
             m = fmaxf(m, v[u].x);
         }
-        score_move(a, m);
+        score_move(a, m, k);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
             Score b{v[u].x, v[u].y, v[u].z};
-            score_move(b, m);
+            score_move(b, m, k);
             a.s += b.s;
             a.w += b.w;
         }
     }
-    score_join_warp(a);
+    score_join_warp(a, k);
     return a;
 }
 // The same by a CTA, joined; parts: shared memory for one Score a warp.
 template <int THREADS>
-__device__ __forceinline__ Score score_join_row(const float4* q, int np, Score* parts) {
-    Score a = score_join_parts(q, np, threadIdx.x, THREADS);
+__device__ __forceinline__ Score score_join_row(const float4* q, int np, float k, Score* parts) {
+    Score a = score_join_parts(q, np, k, threadIdx.x, THREADS);
     if (threadIdx.x % 32 == 0) parts[threadIdx.x / 32] = a;
     __syncthreads();
     float m = parts[0].m;
@@ -244,7 +244,7 @@ __device__ __forceinline__ Score score_join_row(const float4* q, int np, Score* 
 #pragma unroll
     for (int i = 0; i < THREADS / 32; ++i) {
         Score b = parts[i];
-        score_move(b, m);
+        score_move(b, m, k);
         a.s += b.s;
         a.w += b.w;
     }

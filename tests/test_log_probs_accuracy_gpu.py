@@ -1,0 +1,105 @@
+"""linear_log_probs and linear_distillation where a value is known far closer than the tolerances of a whole row: certain
+words, small temperatures, logits that are exact.
+
+Tolerances.  Exponents are (z - m) log2(e) / tau of logits z and their maximum m, so a row's largest term is 1 whatever the
+temperature: the logarithm of the sum and the values are off by R = 2^-20 of 1 and the sizes of what is added (2^-21 for
+exponentials, 2^-23 twice for an exponent, 2^-24 for each of the few terms that count), of the logits as they were summed.
+"""
+import math
+
+import pytest
+import torch
+
+from swiftx_b200.log_probs import linear_log_probs
+from swiftx_b200.loss import linear_distillation
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, FP = torch.bfloat16, torch.float32
+R = 2.0 ** -20
+TEMPS = (1.0, 0.7, 1e-2, 1e-3, 1e-6, 1e-8, 1e-15)
+
+
+def _certain(T, V, d, dtype, word, seed=0):
+    """Rows whose softmax is all on one word.  A row's values add up to 5 to 60, its word's weights are 0.5 to 1.5 and all others' -90 to
+    -30: with the operands' roundings (2^-8 each) the word's logit is at least 2.48 and the others' at most -148.8."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.rand(T, d, generator=g, device=DEV) + 0.5
+    x *= torch.linspace(5, 60, T, device=DEV)[:, None] / x.sum(1, keepdim=True)
+    w = -60 * (torch.rand(V, d, generator=g, device=DEV) + 0.5)
+    w[word] = torch.rand(d, generator=g, device=DEV) + 0.5
+    return x.to(dtype), w.to(dtype)
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(40, 300, 64, BF), (300, 3001, 1024, BF), (8, 3001, 1024, BF), (3, 2500, 40, BF), (90, 700, 200, FP), (70, 2600, 1030, FP)])
+@pytest.mark.parametrize("temp", TEMPS)
+def test_a_certain_word(T, V, d, dtype, temp):
+    """The others lie 151 / temperature or more below the word: 3001 e^-151 is below 2^-200, the log probability and the entropy are 0."""
+    for word in (0, V // 2, V - 1):
+        x, w = _certain(T, V, d, dtype, word, seed=V + word)
+        y = torch.full((T,), word, device=DEV)
+        out = linear_log_probs(x, w, y, top_k=min(5, V), temperature=temp)
+        assert bool((out.top_ids[:, 0] == word).all())
+        for t in (out.log_probs, -out.entropy, out.top_log_probs[:, 0]):
+            assert bool((t <= 0).all()) and bool((t >= -R).all()), (float(t.max()), float(t.min()))
+        assert bool((out.top_log_probs[:, 1:] <= -150).all())
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(40, 300, 64, BF), (70, 3001, 256, BF), (3, 3001, 256, BF), (40, 300, 64, FP), (70, 3001, 1030, FP)])
+@pytest.mark.parametrize("temp", [1e-3, 1e-4, 2.0 ** -16])
+def test_small_differences_of_large_logits(T, V, d, dtype, temp):
+    """Logits 32 + k 2^-16, exact in every sum, of a few words, all others far below: the distribution at a small temperature
+    is that of the differences k 2^-16 / tau.  (The products' mean cut moves a difference by 2^-18 of itself at most.)"""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    n = 24
+    at = torch.randperm(V, generator=g, device=DEV)[:n]
+    k = torch.arange(n, device=DEV) * max(1, int(temp * 2.0 ** 16 / 4))
+    assert int(k[-1]) < 2 ** 12
+    x = torch.zeros(T, d, device=DEV)
+    x[:, 0], x[:, 1], x[:, 2] = 1, 1, 1
+    w = torch.zeros(V, d, device=DEV)
+    w[:, 0] = -64.0
+    w[at, 0] = 32.0
+    w[at, 1] = (k // 16).float() * 2.0 ** -12
+    w[at, 2] = (k % 16).float() * 2.0 ** -16
+    x, w = x.to(dtype), w.to(dtype)
+    y = at[torch.arange(T, device=DEV) % n]
+    l = torch.log_softmax((x.double() @ w.double().t()) / temp, 1)
+    H = -(l.exp() * l).sum(1)
+    out = linear_log_probs(x, w, y, top_k=n, temperature=temp)
+    lp = l.gather(1, y[:, None])[:, 0]
+    far = (R + 2.0 ** -18) * (l[:, at].abs().amax(1) + 1)
+    for got, want in ((out.log_probs, lp), (out.entropy, H)):
+        assert bool(((got.double() - want).abs() <= far).all()), float(((got.double() - want).abs() / far).max())
+    assert torch.equal(out.top_ids[0], at.flip(0)) if int(k[1]) else True
+    err = (out.top_log_probs.double() - l.gather(1, out.top_ids)).abs()
+    assert bool((err <= far[:, None]).all()), float((err / far[:, None]).max())
+    assert bool((out.log_probs <= 0).all()) and bool((out.top_log_probs <= 0).all()) and bool((out.entropy >= 0).all())
+
+
+@pytest.mark.parametrize("dtype,T,V,d", [(BF, 600, 5001, 1024), (BF, 7, 5001, 1024), (FP, 200, 300, 256), (BF, 200, 900, 512)])
+@pytest.mark.parametrize("temp", [1.0, 0.05])
+def test_no_probability_is_above_one(dtype, T, V, d, temp):
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.randn(T, d, generator=g, device=DEV).to(dtype)
+    w = (torch.randn(V, d, generator=g, device=DEV) * 12 / d ** 0.5).to(dtype)
+    y = (x.double() @ w.double().t()).argmax(1)
+    out = linear_log_probs(x, w, y, top_k=9, temperature=temp)
+    assert bool((out.log_probs <= 0).all()) and bool((out.top_log_probs <= 0).all()) and bool((out.entropy >= 0).all())
+    assert bool((out.top_log_probs[:, 1:] <= out.top_log_probs[:, :-1]).all())
+    assert bool(torch.isfinite(torch.log1p(-torch.exp(out.top_log_probs[:, 5:].double()))).all())
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(40, 300, 64, BF), (300, 3001, 1024, BF), (8, 3001, 1024, BF), (90, 700, 200, FP), (70, 2600, 1030, FP)])
+@pytest.mark.parametrize("temp", (1.0, 1e-3, 1e-6, 1e-8, 1e-15))
+def test_distillation_of_a_certain_word(T, V, d, dtype, temp):
+    """Teacher and student are both certain of one word: no loss (R temperature^2), no gradient (temperature R of it)."""
+    word = V - 2
+    x, w = _certain(T, V, d, dtype, word, seed=V)
+    x.requires_grad_(), w.requires_grad_()
+    ids = torch.tensor([word, 5], device=DEV).expand(T, 2)
+    logits = torch.tensor([0.0, -math.inf], device=DEV).expand(T, 2)
+    loss = linear_distillation(x, w, ids, logits, temperature=temp)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    assert 0 <= float(loss.detach()) <= R * temp * temp
+    assert float(dx.abs().max()) <= temp * R * float(w.detach().abs().max()) and float(dw.abs().max()) <= temp * R * float(x.detach().abs().max())
