@@ -470,7 +470,8 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  *   top_ids[t, :], top_log_probs[t, :]: the top_k largest z of the row in falling order (the
  *   lowest word first among equals) and their l; top_k <= SWX_MAX_TOP, 0: none
  * Operands as for swx_xent_args.  A target equal to ignore_index: zeros, and -1 for each top_ids; one
- * outside [0, vocab): its log probability, and the gradients that it enters, NaN.  The
+ * outside [0, vocab): its log probability, and the gradients that it enters, NaN.  A row with a NaN or +inf
+ * logit, or with nothing but -inf, has NaN values and gradients.  The
  * statistics are fp32; the alternatives are ordered by products in fp64 of the operands, so that
  * neither their order nor their ties depend on the rounding of sums.
  * Forward writes row_max (the largest z) and row_sum (the sum of exp((z - row_max) / temperature); tokens values, both or

@@ -47,7 +47,7 @@ constexpr bool is_grad(int epi) { return epi == XE_GRAD || epi == XE_GRAD_IDS; }
 constexpr bool is_dlogit(int epi) { return epi == XE_PROB || is_grad(epi); }
 constexpr bool has_ids(int epi) { return epi == XE_SCORE_IDS || epi == XE_GRAD_IDS; }
 constexpr bool is_logits(int epi) { return epi == XE_LSE || is_score(epi) || is_dlogit(epi); }
-constexpr float SCORE_FLOOR = -0x1p73f;       // below every logit that counts (-9e21): times log2(e) / temperature it stays finite
+constexpr float SCORE_FLOOR = -0x1.ffffep127f;   // the records' lowest value: finite with any column in its low 4 bits
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -85,7 +85,7 @@ struct XentGemm {
     float k2, inv_temp;
     float4* score;                            // (M, 2 nt): a tile half's m, sum of exponentials e, sum of e times its exponent
     // XE_SCORE_TOP, (M, 16 nt): the largest logit of 16 columns, and the second with the largest one's column in place of its
-    // low 4 bits; columns from N on count as SCORE_FLOOR
+    // low 4 bits; SCORE_FLOOR stands for -inf, NaN and columns from N on
     float* largest; float* runner_up;
     float* all;                               // XE_SCORE_ALL, (M, N)
     int beside;                               // the next kernel (the words' norms) may start beside this one
@@ -460,6 +460,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     sum = sum * ex2((m - base) * LOG2E) + add;
                     m = nm;
                 } else if (is_score(EPI)) {
+                    if (cc >= p.N) return;
                     if (yc >= 0 && yc < 32) {
                         float h = 0.f;
 #pragma unroll
@@ -491,15 +492,16 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                     }
                     if (cc + 32 > p.N) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : SCORE_FLOOR;
+                        for (int j = 0; j < 32; ++j) v[j] = cc + j < p.N ? v[j] : -INFINITY;
                     }
-                    float top = SCORE_FLOOR;
+                    float top = -INFINITY;
                     if constexpr (EPI == XE_SCORE_TOP) {
                         // the two largest of either half, with their columns in place of their low bits, and the largest as it
-                        // is (-inf, which the column makes a NaN, and a NaN take no part)
+                        // is (-inf, which the column makes a NaN, and a NaN are no value's column; beside one the second may be as large as the
+                        // largest, and the group is taken whole)
 #pragma unroll
                         for (int g = 0; g < 2; ++g) {
-                            float t1 = SCORE_FLOOR, t2 = SCORE_FLOOR, most = SCORE_FLOOR;
+                            float t1 = SCORE_FLOOR, t2 = SCORE_FLOOR, most = -INFINITY;
 #pragma unroll
                             for (int j = 0; j < 16; j += 2) {
                                 const float x0 = v[16 * g + j], x1 = v[16 * g + j + 1];
@@ -509,7 +511,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                                 t1 = fmaxf(t1, hi);
                                 most = max3(most, x0, x1);
                             }
-                            groups[2 * c + g] = most;
+                            groups[2 * c + g] = fmaxf(most, SCORE_FLOOR);
                             groups[8 + 2 * c + g] = __uint_as_float((__float_as_uint(t2) & ~15u) | (__float_as_uint(t1) & 15u));
                             top = fmaxf(top, most);
                         }
@@ -518,13 +520,13 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         for (int j = 0; j < 32; j += 2) top = max3(top, v[j], v[j + 1]);
                     }
                     // sums relative to the larger maximum: e u becomes c e (u + shift)
-                    const float nm = fmaxf(m, top);
-                    const float shift = fmaxf((m - nm) * p.k2, SCORE_FAR), c2 = ex2(shift);
+                    const float nm = fmaxf(m, top), base = nm == -INFINITY ? 0.f : nm;      // nothing but -inf so far: the sums stay 0
+                    const float shift = fmaxf((m - base) * p.k2, SCORE_FAR), c2 = ex2(shift);
                     const float s0 = sum * c2, w0 = c2 * (esum + sum * shift);
                     float2 s2 = make_float2(s0, 0.f), w2 = make_float2(w0, 0.f);
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        const float2 u = mul2(add2(f2(v[j], v[j + 1]), bc2(-nm)), bc2(p.k2)), e = ex2x2(u);
+                        const float2 u = mul2(add2(f2(v[j], v[j + 1]), bc2(-base)), bc2(p.k2)), e = ex2x2(u);
                         s2 = add2(s2, e);
                         w2 = fma2(e, u, w2);
                     }
@@ -534,7 +536,7 @@ xent_gemm_kernel(const XentGemm p, const __grid_constant__ CUtensorMap map_a, co
                         esum = w0;
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float u = (v[j] - nm) * p.k2;
+                            const float u = (v[j] - base) * p.k2;
                             esum += ex2(u) * fmaxf(u, SCORE_FAR);
                         }
                     }

@@ -112,7 +112,7 @@ def linear_log_probs(x, weight, targets, top_k=0, temperature=1.0, ignore_index=
 
     bf16 operands: products summed in fp32 in the tensor cores, the logits' gradient rounded to bf16 once
     for its products; fp32 operands keep fp32 accuracy and have to be finite.  A target outside [0, vocab) other than
-    ignore_index gives NaN.  Dual numbers are refused, torch.jit.trace records a Python operator.  Deterministic."""
+    ignore_index gives NaN, and so does a row with a NaN or +inf logit, or with nothing but -inf.  Dual numbers are refused, torch.jit.trace records a Python operator.  Deterministic."""
     x = check_head("linear_log_probs", x, weight, targets, weight16)
     _check_top("linear_log_probs", top_k, weight.shape[0])
     check_temperature("linear_log_probs", temperature)

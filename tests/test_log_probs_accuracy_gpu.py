@@ -103,3 +103,55 @@ def test_distillation_of_a_certain_word(T, V, d, dtype, temp):
     dx, dw = torch.autograd.grad(loss, (x, w))
     assert 0 <= float(loss.detach()) <= R * temp * temp
     assert float(dx.abs().max()) <= temp * R * float(w.detach().abs().max()) and float(dw.abs().max()) <= temp * R * float(x.detach().abs().max())
+
+
+@pytest.mark.parametrize("T,V,top", [(20, 256, 6), (20, 300, 6), (5, 300, 0), (20, 3001, 6), (20, 3001, 0), (5, 3001, 6), (5, 3001, 0), (20, 3100, 40), (400, 2306, 100)])
+def test_rows_without_a_word(T, V, top):
+    """A row whose logits are all -inf gives NaN (as token_log_probs does) on any number of words and rows, its alternatives in order; the
+    rows beside it stay as they were."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, 40, generator=g, device=DEV).to(BF)
+    w = torch.randn(V, 40, generator=g, device=DEV).to(BF)
+    y = torch.randint(0, V, (T,), generator=g, device=DEV)
+    x[:, 0] = 0
+    w[:, 0] = -3e38
+    base = linear_log_probs(x, w, y, top_k=top)
+    x[3, 0] = 3e38
+    x.requires_grad_()
+    out = linear_log_probs(x, w, y, top_k=top)
+    rest = torch.arange(T, device=DEV) != 3
+    for a, b in zip(out, base):
+        if a is None:
+            continue
+        assert torch.equal(a[rest], b[rest])
+        if a.is_floating_point():
+            assert bool(torch.isnan(a[3]).all())
+        else:
+            assert torch.equal(a[3], torch.arange(top, device=DEV))
+    dx, = torch.autograd.grad((out.log_probs + out.entropy).sum(), x)
+    # (column 0 is a sum of -3e38 times the logits' gradients, whose magnitudes add up to as much as 2: over the largest fp32)
+    assert bool(torch.isnan(dx[3]).all()) and bool(torch.isfinite(dx[rest][:, 1:]).all())
+    loss = linear_distillation(x, w, y[:, None], torch.zeros(T, 1, device=DEV), reduction="none").detach()
+    assert bool(torch.isnan(loss[3])) and bool(torch.isfinite(loss[rest]).all())
+
+
+@pytest.mark.parametrize("T,V", [(20, 256), (20, 300), (20, 3001), (5, 3001)])
+def test_logits_far_below_zero(T, V):
+    """Logits of -1e24 and less, finite: the largest is certain, the others lie their distance below (each product rounded
+    to 2^-22 of itself)."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.zeros(T, 16, device=DEV, dtype=BF)
+    w = torch.zeros(V, 16, device=DEV, dtype=BF)
+    x[:, 3] = 1e20
+    w[:, 3] = -(torch.rand(V, generator=g, device=DEV) + 0.125) * 1e6
+    z = x.double() @ w.double().t()
+    y = z.argmax(1)
+    out = linear_log_probs(x, w, y, top_k=8)
+    ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :8]
+    best = z.amax(1, keepdim=True)
+    ties = (z == best).sum(1)
+    assert torch.equal(out.top_ids, ids)
+    for got in (out.log_probs + ties.log(), out.entropy - ties.log(), out.top_log_probs[:, 0] + ties.log()):
+        assert bool((got.abs() <= R).all())
+    far = z.gather(1, ids) - best
+    assert bool(((out.top_log_probs - far).abs() <= 2.0 ** -20 * z.abs().amax() + R * far.abs() + 8).all())
