@@ -795,14 +795,17 @@ int score_few_ctas(const HeadOps& o);
 cudaError_t launch_score_few(const XentGemm& g, const HeadOps& o, const Operand& x, const Operand& w, bool top, int ctas, cudaStream_t st);
 
 // The gradients, piece by piece of the vocabulary: the logits again and dlogit in the epilogue (`launch`, with the
-// fields that `fill` sets), and the two products.
-template <class Launch, class Fill>
-static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const HeadGrads& gr, cudaStream_t st, Launch launch, Fill fill) {
+// fields that `fill` sets), and the two products.  `before` may use the operands' maps for a step ahead of them.
+struct NoStep { int operator()(const CUtensorMap&, const CUtensorMap&, int*) const { return SWX_OK; } };
+template <class Launch, class Fill, class Before = NoStep>
+static int head_backward(const HeadOps& o, const HeadPlan& q, uint8_t* ws, const HeadGrads& gr, cudaStream_t st, Launch launch, Fill fill, Before before = {}) {
     int* status = wait_status_address();      // also makes a context current on this thread, which the tensor maps need
     Operand x, w;
     head_operands(o, q, ws, x, w, st);
     CUtensorMap x_k, w_k;
     if (!x.k_major(&x_k) || !w.k_major(&w_k)) return SWX_ERR_CUDA;
+    const int ready = before(x_k, w_k, status);
+    if (ready != SWX_OK) return ready;
     for (int64_t c0 = 0; c0 < o.V; c0 += q.piece) {
         const int64_t cw = std::min(q.piece, o.V - c0);
         const Operand pr{ws + q.off_p, cw, o.T, q.planes, q.ldp, o.T * q.ldp};

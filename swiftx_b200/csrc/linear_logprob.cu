@@ -531,6 +531,20 @@ static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
     return f;
 }
 
+// The backward's workspace.  Few rows' statistics come from other products than the backward's (mma.sync's sums differ from the tiles' by
+// their roundings, which a small temperature makes large: a certain word's dlogit was 0.87 instead of 0 at 1e-3): it
+// takes them again from its own (forward and backward of 1 and 8 tokens x 50001 x 1024: 175 -> 199 us, 167 -> 187).
+struct ScoreBwd { bool again; int64_t off_score, off_hit, off_stats, total; };
+static ScoreBwd score_bwd_plan(const HeadOps& o, const HeadPlan& q) {
+    ScoreBwd f{};
+    f.again = score_few_ctas(o) > 0;
+    f.off_score = up256(q.bwd_total);
+    f.off_hit = f.off_score + up256(2 * q.nt * o.T * 16);
+    f.off_stats = f.off_hit + up256(o.T * 4);
+    f.total = f.again ? f.off_stats + up256(4 * o.T * 4) : q.bwd_total;
+    return f;
+}
+
 static HeadOps ops_of(const swx_logprob_args* a) {
     return HeadOps{a->tokens, a->vocab, a->dim, a->dtype, a->x, a->x_sr, a->weight, a->w_sr};
 }
@@ -586,7 +600,7 @@ int64_t swx_logprob_fwd_workspace_bytes(const swx_logprob_args* a) {
 
 int64_t swx_logprob_bwd_workspace_bytes(const swx_logprob_args* a) {
     const int c = score_check(a);
-    return c != SWX_OK ? -c : head_plan(ops_of(a)).bwd_total;
+    return c != SWX_OK ? -c : score_bwd_plan(ops_of(a), head_plan(ops_of(a))).total;
 }
 
 int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
@@ -677,14 +691,36 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
         return SWX_ERR_INVALID_ARG;
     const HeadOps o = ops_of(a);
     const HeadPlan q = head_plan(o);
-    if (a->workspace_bytes < q.bwd_total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
+    const ScoreBwd f = score_bwd_plan(o, q);
+    if (a->workspace_bytes < f.total || !aligned16(a->workspace)) return SWX_ERR_INVALID_ARG;
+    uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+    float* stats = reinterpret_cast<float*>(ws + f.off_stats);
+    const float* row_max = f.again ? stats : a->row_max;
+    const float* row_sum = f.again ? stats + o.T : a->row_sum;
+    const float* entropy = f.again ? stats + 2 * o.T : a->entropy;
+    const float k2 = exponent_scale(a->temperature, mean_cut(logit_additions(o)));
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, nullptr, nullptr};
-    return head_backward(o, q, static_cast<uint8_t*>(a->workspace), gr, st, launch_logits<XE_GRAD>, [a](XentGemm& g) {
+    auto fill = [=](XentGemm& g) {
         g.target = a->targets; g.ignore = a->ignore_index;
-        g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut(logit_additions(ops_of(a))));
-        g.row_max = a->row_max; g.row_sum = a->row_sum; g.entropy = a->entropy;
+        g.inv_temp = 1.f / a->temperature; g.k2 = k2;
+        g.row_max = row_max; g.row_sum = row_sum; g.entropy = entropy;
         g.d_logp = a->d_log_probs; g.d_entropy = a->d_entropy;
-    });
+    };
+    auto statistics = [=](const CUtensorMap& x, const CUtensorMap& w, int* status) -> int {
+        if (!f.again) return SWX_OK;
+        XentGemm g = logits_gemm(o, q, 0, o.V, status);
+        g.target = a->targets; g.ignore = a->ignore_index; g.k2 = k2;
+        g.score = reinterpret_cast<float4*>(ws + f.off_score);
+        g.hit = reinterpret_cast<float*>(ws + f.off_hit);
+        if (launch_logits<XE_SCORE>(g, x, w, x, st) != cudaSuccess) return SWX_ERR_CUDA;
+        ScoreRows p{};
+        p.T = o.T; p.V = o.V; p.np = (int)(2 * q.nt);
+        p.score = g.score; p.hit = g.hit; p.target = g.target; p.ignore = g.ignore; p.k2 = k2;
+        p.row_max = stats; p.row_sum = stats + o.T; p.entropy = stats + 2 * o.T; p.log_probs = stats + 3 * o.T;
+        return launch_after(score_rows_kernel, (unsigned)((o.T + SC_THREADS / 32 - 1) / (SC_THREADS / 32)), SC_THREADS, 0, st, p) == cudaSuccess
+                   ? SWX_OK : SWX_ERR_CUDA;
+    };
+    return head_backward(o, q, ws, gr, st, launch_logits<XE_GRAD>, fill, statistics);
 }
 
 }  // extern "C"

@@ -155,3 +155,35 @@ def test_logits_far_below_zero(T, V):
         assert bool((got.abs() <= R).all())
     far = z.gather(1, ids) - best
     assert bool(((out.top_log_probs - far).abs() <= 2.0 ** -20 * z.abs().amax() + R * far.abs() + 8).all())
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(8, 3001, 1024, BF), (1, 5000, 2056, BF), (3, 2500, 40, BF), (9, 3001, 1024, BF), (300, 3001, 1024, BF), (8, 3001, 1024, FP)])
+@pytest.mark.parametrize("temp", (1.0, 1e-2, 1e-3, 1e-6))
+def test_gradients_of_a_certain_word(T, V, d, dtype, temp):
+    """They vanish: dz is R / temperature of the upstream gradients at most."""
+    x, w = _certain(T, V, d, dtype, 7, seed=T)
+    x.requires_grad_(), w.requires_grad_()
+    for top in (0, 4):
+        out = linear_log_probs(x, w, torch.full((T,), 7, device=DEV), top_k=top, temperature=temp)
+        for which in ((1.0, 0.0), (0.0, 1.0)):
+            dx, dw = torch.autograd.grad(out[:2], (x, w), [torch.full((T,), c, device=DEV) for c in which], retain_graph=True)
+            assert float(dx.abs().max()) <= R / temp * float(w.detach().abs().max()), (top, which, float(dx.abs().max()))
+            assert float(dw.abs().max()) <= R / temp * float(x.detach().abs().sum(0).max()), (top, which, float(dw.abs().max()))
+
+
+@pytest.mark.parametrize("T", [1, 5, 8])
+@pytest.mark.parametrize("temp", [1.0, 0.02])
+def test_few_rows_have_the_gradients_of_many(T, temp):
+    """The first rows of a larger batch: the same logits, statistics and products with the weight, so the same gradient of x bit by bit."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    V, d = 3001, 520
+    x = torch.randn(64, d, generator=g, device=DEV).to(BF)
+    w = (torch.randn(V, d, generator=g, device=DEV) * 3 / d ** 0.5).to(BF)
+    y = torch.randint(0, V, (64,), generator=g, device=DEV)
+    a, b = torch.randn(64, generator=g, device=DEV), torch.randn(64, generator=g, device=DEV)
+    got = []
+    for n in (T, 64):
+        xs = x[:n].clone().requires_grad_()
+        out = linear_log_probs(xs, w, y[:n], temperature=temp)
+        got.append(torch.autograd.grad(out[:2], xs, (a[:n], b[:n]))[0])
+    assert torch.equal(got[0], got[1][:T])
