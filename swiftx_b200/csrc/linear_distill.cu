@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(DI_THREADS) distill_prepare_kernel(const Disti
             if (v >= 0 && t != -INFINITY) {
                 odd |= v >= p.V || t != t || t == INFINITY;
                 id[i] = v < p.V ? (int)v : 0;
-                q[i] = t * p.inv_temp;
+                q[i] = t;
             }
         }
         top = fmaxf(top, q[i]);
@@ -72,7 +72,8 @@ __global__ void __launch_bounds__(DI_THREADS) distill_prepare_kernel(const Disti
 #pragma unroll
     for (int i = 0; i < NL; ++i) {
         some |= id[i] >= 0;
-        q[i] = id[i] < 0 ? 0.f : ex2((q[i] - (top == -INFINITY ? 0.f : top)) * LOG2E);
+        // (the difference first: a type's lowest value over a small temperature would be -inf)
+        q[i] = id[i] < 0 ? 0.f : ex2((q[i] - top) * (LOG2E * p.inv_temp));
         sum += q[i];
     }
     const bool live = __any_sync(0xffffffffu, some);

@@ -187,3 +187,32 @@ def test_few_rows_have_the_gradients_of_many(T, temp):
         out = linear_log_probs(xs, w, y[:n], temperature=temp)
         got.append(torch.autograd.grad(out[:2], xs, (a[:n], b[:n]))[0])
     assert torch.equal(got[0], got[1][:T])
+
+
+@pytest.mark.parametrize("teacher", [FP, BF])
+@pytest.mark.parametrize("temp", [1e-3, 0.5, 1.0, 3.0])
+def test_teacher_logits_of_the_lowest_value(teacher, temp):
+    """A teacher's softmax sees differences alone: entries that all stand at the type's lowest value (or at any other) are equal, and beside
+    others they have no share."""
+    g = torch.Generator(device=DEV).manual_seed(0)
+    T, V, K = 30, 400, 5
+    x, w = torch.randn(T, 24, generator=g, device=DEV), torch.randn(V, 24, generator=g, device=DEV)
+    ids = torch.rand(T, V, generator=g, device=DEV).topk(K, 1).indices
+    low = torch.finfo(teacher).min
+
+    def run(logits):
+        xs, ws = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = linear_distillation(xs, ws, ids, logits.to(teacher), temperature=temp, reduction="none")
+        return loss.detach(), *torch.autograd.grad(loss, (xs, ws), torch.ones_like(loss))
+    zero = torch.zeros(T, K, device=DEV)
+    equal = run(zero)
+    assert all(bool(torch.isfinite(t).all()) for t in equal)
+    for value in (low, -1e30, 3e38, -7.5):
+        for a, b in zip(run(zero + value), equal):
+            assert torch.equal(a, b)
+    some = torch.arange(K, device=DEV) % 2 == 0
+    # (unused words stand behind the others: a row's three terms are added in another order, 2^-23 of them, which are the loss and
+    # the teacher's share of it, temperature^2 log 3)
+    a, b = run(torch.where(some, zero, low)), run(torch.where(some, zero, -math.inf))
+    assert bool(((a[0] - b[0]).abs() <= 2.0 ** -21 * (b[0].abs() + 2 * temp ** 2)).all())
+    assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
