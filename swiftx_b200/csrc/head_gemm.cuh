@@ -700,15 +700,20 @@ constexpr int XE_PAIRS = 74, XE_MIN_SHARE = 4;
 struct HeadOps { int64_t T, V, d; int dtype; const void* x; int64_t x_sr; const void* w; int64_t w_sr; };
 
 // What the tensor core takes off a sum of n additions of bf16 products on average, relative: it cuts each addition's low bits
-// off (toward zero).  Sums of terms of either sign came out 0.21 to 0.26 2^-24 n too small at n = 4 to 512 (of one sign 0.25 to 0.5 up to
-// n = 64, more beyond).  All logits together too small act like a higher temperature, which the entropy shows first (8192 rows x
-// 50001 x 1024: 8e-7 off); the scale of the exponents makes up for the mean.
-inline float mean_cut(int64_t additions) { return 0.23f * 0x1p-24f * (float)additions; }
-// Additions of a logit's sum at its full size: fp32 operands' largest pieces come last, 512 terms at a time.
-inline int64_t logit_additions(const HeadOps& o) {
-    return std::min((o.d + 15) / 16, o.dtype == SWX_DTYPE_BF16 ? INT64_MAX : (int64_t)(XE_KSUB_LOGITS * XE_K / 16));
-}
-inline float exponent_scale(float temperature, float cut) { return (float)(1.4426950408889634 / temperature * (1. + cut)); }
+// off (toward zero).  Sums of terms of either sign came out 0.20 2^-24 n too small at n = 4, 0.225 at 64 and 0.26 at 512; of one sign 0.14,
+// 0.45 and 1.07.  All logits together too small act like a higher temperature, which the entropy shows first (8192 rows x
+// 50001 x 1024: 8e-7 off); the scale of the exponents makes up for the mean of either sign.  Sums that are exact (rows of a few values, small
+// integers) lose nothing: their differences come out 0.23 2^-24 n too large instead (9e-7 of them at a width of 1024).
+constexpr int64_t XE_CUT_ADDITIONS = 512;
+inline double mean_cut(double additions) { return 0.23 * 0x1p-24 * additions; }
+// Scoring and distillation sum the logits of bf16 operands 8192 terms at a time in tensor memory, in fp32 beyond, so that no more
+// additions come together than were measured (65536 terms: 6.6e-5 too small in one sum, 7.9e-6 so and 9e-7 with the mean made up for).
+constexpr int XE_KSUB_SCORES = XE_CUT_ADDITIONS * 16 / XE_K;
+inline int score_ksub(const HeadOps& o) { return o.dtype == SWX_DTYPE_BF16 ? XE_KSUB_SCORES : XE_KSUB_LOGITS; }
+inline void set_score_sums(XentGemm& g, const HeadOps& o) { g.ksub = std::min(g.nk, score_ksub(o)); }
+// Additions of a logit's sum at its full size (fp32 operands' largest pieces come last).
+inline int64_t logit_additions(const HeadOps& o) { return std::min<int64_t>((o.d + 15) / 16, score_ksub(o) * XE_K / 16); }
+inline float exponent_scale(float temperature, double cut) { return (float)(1.4426950408889634 / temperature * (1. + cut)); }
 
 // Sizes and the workspace: copies of the operands, then (forward) whatever the operator keeps from
 // `base` on, or (backward) a piece of the logits' gradient and the sums of the gradient products.
@@ -792,6 +797,7 @@ static cudaError_t launch_logits(const XentGemm& g, const CUtensorMap& x, const 
 
 // The scoring of a few rows without tiles (linear_logprob_few.cu): its CTAs, 0 where it does not take them, and the launch.
 int score_few_ctas(const HeadOps& o);
+double few_additions(int64_t d);              // of a logit there
 cudaError_t launch_score_few(const XentGemm& g, const HeadOps& o, const Operand& x, const Operand& w, bool top, int ctas, cudaStream_t st);
 
 // The gradients, piece by piece of the vocabulary: the logits again and dlogit in the epilogue (`launch`, with the

@@ -252,7 +252,8 @@ static int distill_check(const swx_distill_args* a) {
 }
 
 static void fill_words(XentGemm& g, const DistillSaved& s, const swx_distill_args* a) {
-    g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut(logit_additions(ops_of(a))));
+    set_score_sums(g, ops_of(a));
+    g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, mean_cut((double)logit_additions(ops_of(a))));
     g.ids = s.ids; g.id_logit = s.logit; g.id_share = s.share; g.nids = (int)a->entries;
     g.before = s.before; g.before_stride = s.stride;
 }

@@ -638,8 +638,9 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         CUtensorMap mx, mw;
         if (!xc.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
         XentGemm g = logits_gemm(oc, qc, 0, o.V, status);
+        set_score_sums(g, o);
         g.target = a->targets + r0; g.ignore = a->ignore_index;
-        const float cut = mean_cut(f.few ? (o.d + 63) / 64 : logit_additions(o));
+        const double cut = mean_cut(f.few ? few_additions(o.d) : (double)logit_additions(o));
         g.inv_temp = 1.f / a->temperature; g.k2 = exponent_scale(a->temperature, cut);
         g.score = reinterpret_cast<float4*>(ws + f.off_score);
         g.hit = reinterpret_cast<float*>(ws + f.off_hit);
@@ -658,7 +659,7 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         ScoreRows p{};
         p.T = oc.T; p.V = o.V; p.d = o.d; p.np = f.np;
         p.score = g.score; p.hit = g.hit; p.target = g.target; p.ignore = a->ignore_index;
-        p.k2 = g.k2; p.cut = cut; p.exact_k2 = exponent_scale(a->temperature, 0.f);
+        p.k2 = g.k2; p.cut = (float)cut; p.exact_k2 = exponent_scale(a->temperature, 0.);
         p.row_max = a->row_max ? a->row_max + r0 : nullptr; p.row_sum = a->row_sum ? a->row_sum + r0 : nullptr;
         p.log_probs = a->log_probs + r0; p.entropy = a->entropy + r0;
         if (a->top_k == 0) {
@@ -698,9 +699,10 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
     const float* row_max = f.again ? stats : a->row_max;
     const float* row_sum = f.again ? stats + o.T : a->row_sum;
     const float* entropy = f.again ? stats + 2 * o.T : a->entropy;
-    const float k2 = exponent_scale(a->temperature, mean_cut(logit_additions(o)));
+    const float k2 = exponent_scale(a->temperature, mean_cut((double)logit_additions(o)));
     const HeadGrads gr{a->dx, a->dweight, a->dw_dtype == SWX_DTYPE_BF16, nullptr, nullptr};
     auto fill = [=](XentGemm& g) {
+        set_score_sums(g, o);                 // the same sums as the forward's
         g.target = a->targets; g.ignore = a->ignore_index;
         g.inv_temp = 1.f / a->temperature; g.k2 = k2;
         g.row_max = row_max; g.row_sum = row_sum; g.entropy = entropy;
@@ -709,6 +711,7 @@ int swx_logprob_bwd(const swx_logprob_args* a, void* stream) {
     auto statistics = [=](const CUtensorMap& x, const CUtensorMap& w, int* status) -> int {
         if (!f.again) return SWX_OK;
         XentGemm g = logits_gemm(o, q, 0, o.V, status);
+        set_score_sums(g, o);
         g.target = a->targets; g.ignore = a->ignore_index; g.k2 = k2;
         g.score = reinterpret_cast<float4*>(ws + f.off_score);
         g.hit = reinterpret_cast<float*>(ws + f.off_hit);

@@ -117,6 +117,18 @@ __global__ void __launch_bounds__(SF_THREADS, SF_PER_SM) score_few_kernel(const 
     if (word == 0 && t < p.M) p.score[(int64_t)t * gridDim.x + blockIdx.x] = make_float4(m, a.s, a.w, 0.f);
 }
 
+// A warp's sums are of 8 steps (two products each) of every 32: their numbers of additions, weighed by the terms that they hold.
+double few_additions(int64_t d) {
+    const int64_t steps = (d + 31) / 32;
+    double n = 0.;
+    for (int w = 0; w < SF_WARPS; ++w) {
+        const int64_t rest = steps % (SF_DEPTH * SF_WARPS) - SF_DEPTH * w;
+        const double s = (double)(steps / (SF_DEPTH * SF_WARPS) * SF_DEPTH + std::max<int64_t>(0, std::min<int64_t>(rest, SF_DEPTH)));
+        n += 2. * s * s / (double)steps;
+    }
+    return n;
+}
+
 static int few_smem(int64_t d) { return 8 * (int)(4 * ((d + 31) / 32) + 4) * 16; }
 
 // CTAs of the kernel for these sizes (each leaves one statistic of a token); 0: not taken.

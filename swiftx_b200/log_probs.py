@@ -110,8 +110,9 @@ def linear_log_probs(x, weight, targets, top_k=0, temperature=1.0, ignore_index=
     products of the operands, so that rounding changes neither their order nor their ties (among the top_k + 4 or more words
     with the largest fp32 products: where more words than that differ by a rounding of those, others of them may be missing).
 
-    bf16 operands: products summed in fp32 in the tensor cores, the logits' gradient rounded to bf16 once
-    for its products; fp32 operands keep fp32 accuracy and have to be finite.  A target outside [0, vocab) other than
+    bf16 operands: products summed in fp32 in the tensor cores (8192 terms at a time), the logits' gradient rounded to bf16 once
+    for its products.  The tensor cores' additions cut off; the exponents' scale makes up for the mean of that, 2^-26 of the logits for
+    each 16 terms, which the loss does not (sums that lose nothing, as of one-hot rows, are too large by as much, 9e-7 at a width of 1024).  fp32 operands keep fp32 accuracy and have to be finite.  A target outside [0, vocab) other than
     ignore_index gives NaN, and so does a row with a NaN or +inf logit, or with nothing but -inf.  Dual numbers are refused, torch.jit.trace records a Python operator.  Deterministic."""
     x = check_head("linear_log_probs", x, weight, targets, weight16)
     _check_top("linear_log_probs", top_k, weight.shape[0])

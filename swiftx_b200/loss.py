@@ -233,8 +233,8 @@ def linear_distillation(x, weight, teacher_ids, teacher_logits, temperature=1.0,
     Returns the fp32 loss: its mean over the rows that count, their sum, or (reduction "none") one
     value for each row, 0 where nothing counts.
 
-    Accuracy, the types of the gradients, weight16, autocast, dual numbers and traces: as for
-    ``linear_cross_entropy``.  An id of vocab or more, or a teacher logit of NaN or +inf, in a used entry gives a NaN loss
+    The types of the gradients, weight16, autocast, dual numbers and traces: as for ``linear_cross_entropy``; the student's logits and
+    their accuracy: as for ``linear_log_probs``.  An id of vocab or more, or a teacher logit of NaN or +inf, in a used entry gives a NaN loss
     (and gradients).  The teacher is a constant: a teacher_logits that requires gradients is refused.
     Deterministic."""
     if reduction not in _lib.XENT_REDUCTIONS:

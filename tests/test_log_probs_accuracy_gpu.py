@@ -216,3 +216,86 @@ def test_teacher_logits_of_the_lowest_value(teacher, temp):
     a, b = run(torch.where(some, zero, low)), run(torch.where(some, zero, -math.inf))
     assert bool(((a[0] - b[0]).abs() <= 2.0 ** -21 * (b[0].abs() + 2 * temp ** 2)).all())
     assert torch.equal(a[1], b[1]) and torch.equal(a[2], b[2])
+
+
+def _cut(d, dtype):
+    """The share of a logit that the products' mean cut changes it by at most where its sum is exact: 0.25 2^-24 for each 16 of the terms that are
+    summed in the tensor core at a time (8192; 512 of fp32 operands)."""
+    return 0.25 * 2.0 ** -24 * min((d + 15) // 16, 512 if dtype == BF else 32)
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(40, 300, 64, BF), (300, 3001, 1024, BF), (6, 3001, 1024, BF), (20, 400, 8192, BF), (20, 300, 16400, BF), (20, 300, 65536, BF),
+                                         (60, 3001, 256, FP), (40, 300, 16384, FP)])
+@pytest.mark.parametrize("kind", ["one word a row", "small integers"])
+def test_exact_logits(T, V, d, dtype, kind):
+    """Sums that no addition rounds: values are off by the mean cut of the logits' distances, and R."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    if kind == "one word a row":
+        x = torch.zeros(T, d, device=DEV)
+        at = torch.randint(0, d, (T,), generator=g, device=DEV)
+        x[torch.arange(T, device=DEV), at] = 1.0
+        w = torch.randn(V, d, generator=g, device=DEV).to(dtype) * 6
+    else:
+        x = torch.randint(-2, 3, (T, d), generator=g, device=DEV).float()
+        w = torch.randint(-2, 3, (V, d), generator=g, device=DEV).to(dtype) * 2.0 ** -math.ceil(math.log2(d) / 2)
+    x = x.to(dtype)
+    y = torch.randint(0, V, (T,), generator=g, device=DEV)
+    z = x.double() @ w.double().t()
+    l = torch.log_softmax(z, 1)
+    p = l.exp()
+    H = -(p * l).sum(1)
+    mean = (p * z).sum(1)
+    out = linear_log_probs(x, w, y)
+    lp, zy = l.gather(1, y[:, None])[:, 0], z.gather(1, y[:, None])[:, 0]
+    for got, want, moved in ((out.log_probs, lp, (zy - mean).abs()), (out.entropy, H, (p * (z - mean[:, None]) ** 2).sum(1))):
+        bound = _cut(d, dtype) * moved + R * (1 + lp.abs() + H)
+        assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() / bound).max())
+    loss = linear_distillation(x, w, y[:, None], torch.zeros(T, 1, device=DEV), reduction="none").double()
+    bound = _cut(d, dtype) * (zy - mean).abs() + R * (1 + lp.abs() + H)
+    assert bool(((loss + lp).abs() <= bound).all()), float(((loss + lp).abs() / bound).max())
+
+
+@pytest.mark.parametrize("T,V,d,dtype", [(300, 2000, 1024, BF), (300, 2000, 4096, BF), (200, 600, 16384, BF), (200, 600, 65536, BF), (200, 600, 8200, BF),
+                                         (300, 2000, 1024, FP), (100, 600, 16384, FP)])
+def test_mean_error_of_dense_rows(T, V, d, dtype):
+    """Terms of either sign are cut 0.20 to 0.27 2^-24 for each 16 of the n that come together, of which 0.23 are made up for: the entropy is off
+    by 0.06 2^-24 n / 16 of the logits' variance on average over the rows (the roundings of each logit average out), and by 2^-22 of 1 and
+    itself; distillation's loss by as much of its logits' distances.  Without the mean made up for they would be 4 times as far off."""
+    g = torch.Generator(device=DEV).manual_seed(d)
+    x = torch.randn(T, d, generator=g, device=DEV).to(dtype)
+    w = (torch.randn(V, d, generator=g, device=DEV) * 2 / d ** 0.5).to(dtype)
+    y = torch.randint(0, V, (T,), generator=g, device=DEV)
+    z = x.double() @ w.double().t()
+    l = torch.log_softmax(z, 1)
+    p = l.exp()
+    H = -(p * l).sum(1)
+    mean = (p * z).sum(1)
+    var = (p * (z - mean[:, None]) ** 2).sum(1)
+    share = 0.06 / 0.25 * _cut(d, dtype)
+    out = linear_log_probs(x, w, y)
+    off = float((out.entropy.double() - H).mean().abs())
+    assert off <= share * float(var.mean()) + 2.0 ** -22 * float(1 + H.mean()), (off, share * float(var.mean()))
+    loss = linear_distillation(x, w, y[:, None], torch.zeros(T, 1, device=DEV))
+    lp, zy = l.gather(1, y[:, None])[:, 0], z.gather(1, y[:, None])[:, 0]
+    off = abs(float(loss) + float(lp.mean()))
+    assert off <= share * float((zy - mean).mean().abs()) + 2.0 ** -22 * float(1 + lp.abs().mean()), (off, share)
+
+
+def test_gradients_of_wide_bf16_rows():
+    """9000 terms are summed in two pieces, forward and backward alike: a certain word's gradient vanishes, others are a logit's rounding
+    (2^-8 of it) and the result's from float64 in the mean square."""
+    T, V, d = 40, 300, 9000
+    x, w = _certain(T, V, d, BF, 7)
+    x.requires_grad_(), w.requires_grad_()
+    out = linear_log_probs(x, w, torch.full((T,), 7, device=DEV), temperature=1e-3)
+    for t, o in zip(torch.autograd.grad(out[:2], (x, w), [torch.ones(T, device=DEV)] * 2), (w, x)):
+        assert float(t.abs().max()) <= 1e3 * R * T * float(o.detach().abs().max())
+    g = torch.Generator(device=DEV).manual_seed(1)
+    x = torch.randn(T, d, generator=g, device=DEV).to(BF).requires_grad_()
+    w = (torch.randn(V, d, generator=g, device=DEV) * 2 / d ** 0.5).to(BF).requires_grad_()
+    y = torch.randint(0, V, (T,), generator=g, device=DEV)
+    got = torch.autograd.grad(linear_log_probs(x, w, y).log_probs.sum(), (x, w))
+    xd, wd = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    want = torch.autograd.grad(torch.log_softmax(xd @ wd.t(), 1).gather(1, y[:, None]).sum(), (xd, wd))
+    for a, b in zip(got, want):
+        assert float((a.double() - b).norm()) <= 2.0 ** -7 * float(b.norm())
