@@ -751,11 +751,17 @@ inline bool encode_operand(CUtensorMap* m, const void* base, int64_t inner, int6
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows of one product of scoring and distillation: what it keeps for the rows' kernel is bounded (8192 rows x 50001: 51 MB of statistics,
+// 205 MB of records), and 32 row tiles keep a tile of the weight in use as long as more would.
+constexpr int64_t SC_ROWS = 32 * XE_TILE;
+
 struct Operand {
     const void* p; int64_t inner, rows, planes, row, plane;
     // rows of the contraction's other index, 64 contraction steps wide / the transposed use
     bool k_major(CUtensorMap* m) const { return encode_operand(m, p, inner, rows, planes, row, plane, 64, 128); }
     bool mn_major(CUtensorMap* m) const { return encode_operand(m, p, inner, rows, planes, row, plane, 64, 64); }
+    // n rows from r0 on (pieces keep their distance)
+    Operand part(int64_t r0, int64_t n) const { return Operand{static_cast<const uint8_t*>(p) + r0 * row * 2, inner, n, planes, row, plane}; }
 };
 
 // x and the weight as the products read them: themselves, or their copies in the workspace.

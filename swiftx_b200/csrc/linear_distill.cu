@@ -26,6 +26,7 @@ struct DistillSaved {
 
 struct DistillRows {
     int64_t T, V;
+    int64_t r0, rows_all;                              // the rows of one product, r0 to T, of all
     int K, np;
     const float4* score;
     float k2, inv_temp;
@@ -145,17 +146,17 @@ __global__ void __launch_bounds__(DI_THREADS) distill_prepare_kernel(const Disti
     }
 }
 
-// Warp = one row: its statistics and loss.  Each CTA leaves the sum of its rows' losses and the count of its rows; the last CTA to
-// finish adds those up (fp64, a fixed order whichever CTA it is).
+// Warp = one row: its statistics and loss.  Each CTA leaves the sum of its rows' losses and the count of its rows; the last CTA of the
+// last product's rows to finish adds those of all up (fp64, a fixed order whichever CTA it is).
 __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillRows p) {
     __shared__ int is_last;
     __shared__ double red[DI_WARPS][2];
     wait_for_previous();
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int64_t row = (int64_t)blockIdx.x * DI_WARPS + warp;
+    const int64_t row = p.r0 + (int64_t)blockIdx.x * DI_WARPS + warp;
     double sum = 0., n = 0.;
     if (row < p.T) {
-        const Score a = score_join_parts(p.score + row * p.np, p.np, p.k2, lane, 32);
+        const Score a = score_join_parts(p.score + (row - p.r0) * p.np, p.np, p.k2, lane, 32);
         const float ls = logf(a.s), mark = p.s.row_sum[row];
         float loss = 0.f;
         for (int j = lane; j < p.K; j += 32) {
@@ -179,16 +180,16 @@ __global__ void __launch_bounds__(DI_THREADS) distill_rows_kernel(const DistillR
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 1; i < DI_WARPS; ++i) { sum += red[i][0]; n += red[i][1]; }
-        p.sums[blockIdx.x] = make_double2(sum, n);
+        p.sums[p.r0 / DI_WARPS + blockIdx.x] = make_double2(sum, n);
         __threadfence();
-        is_last = atomicAdd(p.counter, 1) == (int)gridDim.x - 1;
+        is_last = p.T == p.rows_all && atomicAdd(p.counter, 1) == (int)gridDim.x - 1;
     }
     __syncthreads();
     if (!is_last) return;
     __threadfence();
     sum = n = 0.;
 #pragma unroll 4
-    for (int i = threadIdx.x; i < (int)gridDim.x; i += DI_THREADS) {
+    for (int i = threadIdx.x; i < (int)(p.r0 / DI_WARPS + gridDim.x); i += DI_THREADS) {
         const double2 s = __ldcg(p.sums + i);
         sum += s.x;
         n += s.y;
@@ -212,7 +213,7 @@ struct DistillPlan { int64_t off_score, off_sums, off_cnt, total; };
 static DistillPlan distill_plan(const HeadPlan& q, int64_t T) {
     DistillPlan f{};
     f.off_score = q.base;
-    f.off_sums = f.off_score + up256(2 * q.nt * T * 16);
+    f.off_sums = f.off_score + up256(2 * q.nt * std::min(T, SC_ROWS) * 16);
     f.off_cnt = f.off_sums + up256((T + DI_WARPS - 1) / DI_WARPS * 16);
     f.total = f.off_cnt + 256;
     return f;
@@ -314,18 +315,29 @@ int swx_distill_fwd(const swx_distill_args* a, void* stream) {
     if (cudaGetLastError() != cudaSuccess) return SWX_ERR_CUDA;
     Operand x, w;
     head_operands(o, q, ws, x, w, st);
-    CUtensorMap mx, mw;
-    if (!x.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
-    XentGemm g = logits_gemm(o, q, 0, o.V, status);
-    fill_words(g, p.s, a);
-    p.k2 = g.k2;
-    g.score = reinterpret_cast<float4*>(ws + f.off_score);
-    g.counter = reinterpret_cast<int*>(ws + f.off_cnt);
-    if (launch_logits<XE_SCORE_IDS>(g, mx, mw, mx, st) != cudaSuccess) return SWX_ERR_CUDA;
-    p.score = g.score;
+    CUtensorMap mw;
+    if (!w.k_major(&mw)) return SWX_ERR_CUDA;
     p.rows = none ? a->loss : nullptr; p.sums = reinterpret_cast<double2*>(ws + f.off_sums);
-    p.loss = a->loss; p.count = a->count; p.counter = g.counter; p.reduction = a->reduction;
-    return launch_after(distill_rows_kernel, rows, DI_THREADS, 0, st, p) == cudaSuccess ? SWX_OK : SWX_ERR_CUDA;
+    p.loss = a->loss; p.count = a->count; p.reduction = a->reduction; p.rows_all = o.T;
+    for (int64_t r0 = 0; r0 < o.T; r0 += SC_ROWS) {
+        HeadOps oc = o;
+        oc.T = std::min(SC_ROWS, o.T - r0);
+        HeadPlan qc = q;
+        qc.mt = (oc.T + XE_TILE - 1) / XE_TILE;
+        CUtensorMap mx;
+        if (!x.part(r0, oc.T).k_major(&mx)) return SWX_ERR_CUDA;
+        XentGemm g = logits_gemm(oc, qc, 0, o.V, status);
+        DistillSaved s = p.s;                  // these rows' words
+        s.ids += r0 * p.K; s.share += r0 * p.K; s.logit += r0 * p.K; s.before += r0 * s.stride;
+        fill_words(g, s, a);
+        g.score = reinterpret_cast<float4*>(ws + f.off_score);
+        g.counter = reinterpret_cast<int*>(ws + f.off_cnt);
+        if (launch_logits<XE_SCORE_IDS>(g, mx, mw, mx, st) != cudaSuccess) return SWX_ERR_CUDA;
+        p.T = r0 + oc.T; p.r0 = r0; p.k2 = g.k2; p.score = g.score; p.counter = g.counter;
+        const unsigned ctas = (unsigned)((oc.T + DI_WARPS - 1) / DI_WARPS);
+        if (launch_after(distill_rows_kernel, ctas, DI_THREADS, 0, st, p) != cudaSuccess) return SWX_ERR_CUDA;
+    }
+    return SWX_OK;
 }
 
 int swx_distill_bwd(const swx_distill_args* a, void* stream) {

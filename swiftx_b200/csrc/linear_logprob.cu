@@ -500,10 +500,6 @@ struct ScorePlan {
     bool longest;
 };
 
-// Rows of one product: what it keeps for the rows' kernel is bounded (8192 rows x 50001: 51 MB of statistics, 205 MB of records),
-// and 32 row tiles keep a tile of the weight in use as long as more would.
-constexpr int64_t SC_ROWS = 32 * XE_TILE;
-
 static ScorePlan score_plan(const HeadOps& o, const HeadPlan& q, int top) {
     const int64_t T = std::min(o.T, SC_ROWS), V = o.V;
     ScorePlan f{};
@@ -632,9 +628,7 @@ int swx_logprob_fwd(const swx_logprob_args* a, void* stream) {
         oc.x = static_cast<const uint8_t*>(o.x) + r0 * o.x_sr * q.es;
         HeadPlan qc = q;
         qc.mt = (oc.T + XE_TILE - 1) / XE_TILE;
-        Operand xc = x;                       // (pieces of fp32 operands keep their distance)
-        xc.rows = oc.T;
-        xc.p = static_cast<const uint8_t*>(x.p) + r0 * x.row * 2;
+        const Operand xc = x.part(r0, oc.T);
         CUtensorMap mx, mw;
         if (!xc.k_major(&mx) || !w.k_major(&mw)) return SWX_ERR_CUDA;
         XentGemm g = logits_gemm(oc, qc, 0, o.V, status);

@@ -402,3 +402,20 @@ def test_two_scorings_at_once_on_two_streams():
     for g in got:
         for a, b in zip(g, want):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,V,d,K,dtype", [(8193, 300, 24, 3, BF), (17000, 260, 32, 20, BF), (16391, 700, 40, 40, FP)])
+def test_more_rows_than_one_product_takes(T, V, d, K, dtype):
+    x, w, ids, logits = _inputs(T, V, d, K, dtype, seed=12)
+    ids[::5, 1:] = -1
+    ids[8190:8195] = -1
+    for red in ("mean", "sum", "none"):
+        got = _run(x, w, ids, logits, 1.5, red)
+        _check(x, w, ids, logits, 1.5, red, *got)
+    # rows do not see each other
+    for a, b in ((0, 100), (8100, 8300), (T - 50, T)):
+        part = _run(x[a:b], w, ids[a:b], logits[a:b], 1.5, "none")
+        assert torch.equal(part[0], got[0][a:b])
+    xo = torch.zeros(T, d + 3, device=DEV, dtype=dtype)[:, 3:]            # rows off 16 bytes
+    xo.copy_(x)
+    assert torch.equal(_run(xo, w, ids, logits, 1.5, "none")[0], got[0])

@@ -156,3 +156,11 @@ def test_a_head_with_a_bias_is_refused():
         model.log_probs(idx, idx)
     with pytest.raises(ValueError):
         model.distillation_loss(idx, idx[..., None], torch.zeros(1, 2, 1))
+
+
+def test_distillation_takes_8192_rows_at_a_time():
+    """16 bytes for 128 logits of those rows, a sum for four rows of all, whatever the number of tokens."""
+    lib = _lib.load()
+    V = 131072
+    for T in (8192, 65536, 1 << 20):
+        assert lib.swx_distill_fwd_workspace_bytes(_distill(T, V, 64)) <= 8192 * V / 8 + 4 * T + 4096
