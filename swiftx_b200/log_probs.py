@@ -94,7 +94,7 @@ class LinearLogProbsFn(torch.autograd.Function):
         return dx, dw, None, None, None, None, None
 
 
-def _check_top(name, top_k, vocab):
+def check_top(name, top_k, vocab):
     if not 0 <= top_k <= min(vocab, _lib.SWX_MAX_TOP):
         raise ValueError(f"{name}: top_k of 0 to {min(vocab, _lib.SWX_MAX_TOP)} expected, got {top_k}")
 
@@ -115,7 +115,7 @@ def linear_log_probs(x, weight, targets, top_k=0, temperature=1.0, ignore_index=
     each 16 terms, which the loss does not (sums that lose nothing, as of one-hot rows, are too large by as much, 9e-7 at a width of 1024).  fp32 operands keep fp32 accuracy and have to be finite.  A target outside [0, vocab) other than
     ignore_index gives NaN, and so does a row with a NaN or +inf logit, or with nothing but -inf.  Dual numbers are refused, torch.jit.trace records a Python operator.  Deterministic."""
     x = check_head("linear_log_probs", x, weight, targets, weight16)
-    _check_top("linear_log_probs", top_k, weight.shape[0])
+    check_top("linear_log_probs", top_k, weight.shape[0])
     check_temperature("linear_log_probs", temperature)
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     t1 = targets if targets.dim() == 1 else targets.reshape(-1)
@@ -143,7 +143,7 @@ def token_log_probs(logits, targets=None, top_k=0, temperature=1.0, ignore_index
     if targets is not None and (targets.dtype != torch.int64 or targets.shape != logits.shape[:-1] or targets.device != logits.device):
         raise ValueError(f"token_log_probs: int64 targets of shape {tuple(logits.shape[:-1])} on {logits.device} expected, got "
                          f"{targets.dtype} {tuple(targets.shape)} on {targets.device}")
-    _check_top("token_log_probs", top_k, logits.shape[-1])
+    check_top("token_log_probs", top_k, logits.shape[-1])
     check_temperature("token_log_probs", temperature)
     if _lib.needs_node(logits):
         if torch.jit.is_tracing():

@@ -36,7 +36,7 @@ from . import embedding as embedding_kernels
 from . import norm as norm_kernels
 from .conv import causal_conv1d_fn, conv1d_backward, conv1d_forward
 from .decode import decode_conv_step, decode_layer_step, decode_ssm_step
-from .log_probs import LogProbs, linear_log_probs, token_log_probs
+from .log_probs import LogProbs, check_top, linear_log_probs, token_log_probs
 from .loss import linear_cross_entropy, linear_distillation
 from .selective_scan import scan_backward, scan_forward, selective_scan_fn
 
@@ -601,6 +601,10 @@ class SiftLM(nn.Module):
         step from one CUDA graph (GraphedStep).  log_probs=K (0 or more): also returns the
         ``LogProbs`` of the new tokens (b, max_new_tokens) with their K top alternatives, under
         the model's own softmax (before temperature and top_k)."""
+        if log_probs is not None:               # refused before the prompt is consumed
+            check_top("SiftLM.generate", log_probs, self.lm_head.weight.shape[0])
+            if not self.lm_head.weight.is_cuda:
+                raise RuntimeError("SiftLM.generate: log_probs runs on CUDA only (no CPU path)")
         if graphed:
             stepper = GraphedStep(self, idx.shape[0], idx.device)
             advance = lambda tok: stepper(tok).clone()  # noqa: E731

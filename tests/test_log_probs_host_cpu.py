@@ -164,3 +164,15 @@ def test_distillation_takes_8192_rows_at_a_time():
     V = 131072
     for T in (8192, 65536, 1 << 20):
         assert lib.swx_distill_fwd_workspace_bytes(_distill(T, V, 64)) <= 8192 * V / 8 + 4 * T + 4096
+
+
+@pytest.mark.parametrize("k,error", [(21, ValueError), (-1, ValueError), (1 << 40, ValueError), (3, RuntimeError)])
+def test_generation_refuses_before_it_consumes_the_prompt(k, error, monkeypatch):
+    model = SiftLM(SiftConfig(vocab_size=20, d_model=8, n_layers=1))
+    steps = []
+    monkeypatch.setattr(SiftLM, "step", lambda *a: steps.append(a) or torch.zeros(1, 20))
+    for new in (0, 2):
+        with pytest.raises(error):
+            model.generate(torch.zeros(1, 5, dtype=torch.int64), new, log_probs=k)
+    assert not steps
+    assert model.generate(torch.zeros(1, 5, dtype=torch.int64), 2).shape == (1, 7)
