@@ -77,10 +77,15 @@ def _args(x, w, targets, ignore_index, reduction):
     return a
 
 
-def _workspace(lib, name, a, like):
+def _bytes(lib, name, a):
     n = getattr(lib, name)(a)
     if n < 0:
         _lib.check(-n, name)
+    return n
+
+
+def _workspace(lib, name, a, like):
+    n = _bytes(lib, name, a)
     ws = like.new_empty(n // 4 + 1)
     a.workspace, a.workspace_bytes = ws.data_ptr(), n
     return ws
@@ -183,7 +188,7 @@ def _distill_forward(x, w, ids, logits, temperature, reduction):
         a.teacher_ids, a.ids_sr = ids.data_ptr(), ids.stride(0)
         a.teacher_logits, a.tl_sr = logits.data_ptr(), logits.stride(0)
         a.loss, a.count = loss.data_ptr(), count.data_ptr()
-        a.saved_bytes = lib.swx_distill_saved_bytes(a)
+        a.saved_bytes = _bytes(lib, "swx_distill_saved_bytes", a)
         saved = x.new_empty(a.saved_bytes, dtype=torch.uint8)
         a.saved = saved.data_ptr()
         ws = _workspace(lib, "swx_distill_fwd_workspace_bytes", a, loss)  # noqa: F841

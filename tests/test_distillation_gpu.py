@@ -419,3 +419,12 @@ def test_more_rows_than_one_product_takes(T, V, d, K, dtype):
     xo = torch.zeros(T, d + 3, device=DEV, dtype=dtype)[:, 3:]            # rows off 16 bytes
     xo.copy_(x)
     assert torch.equal(_run(xo, w, ids, logits, 1.5, "none")[0], got[0])
+
+
+def test_a_width_that_is_not_supported_is_named():
+    x, w = torch.zeros(2, 65544, device=DEV, dtype=BF), torch.zeros(3, 65544, device=DEV, dtype=BF)
+    ids, logits = torch.zeros(2, 1, device=DEV, dtype=torch.int64), torch.zeros(2, 1, device=DEV)
+    with pytest.raises(ValueError, match="swx_distill"):
+        linear_distillation(x, w, ids, logits)
+    with pytest.raises(ValueError, match="swx_logprob"):
+        linear_log_probs(x, w, ids[:, 0])
