@@ -561,3 +561,18 @@ def test_transforms():
     x2, w2, _ = _inputs(50, 90, 24, FP, seed=1)
     for a, b in zip(f(x2, w2), linear_log_probs(x2, w2, y, top_k=3)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("T,V,d,dtype,top", [(8700, 6001, 521, BF, 40), (16500, 4500, 264, FP, 9)])
+def test_norms_of_the_words_over_several_products(T, V, d, dtype, top):
+    """A teacher's batch: the bound of the candidates comes from the longest word, here the last one, read once for all rows."""
+    assert T > 8192 and T * (top + 4) > V and T * (top + 4) * d * (4 if dtype == FP else 2) > 64 << 20
+    x, w, y = _inputs(T, V, d, dtype, seed=T)
+    w[-1] *= 2
+    with torch.no_grad():
+        out = linear_log_probs(x, w, y, top_k=top)
+        _check_forward(out, x, w, y, 1.0, top)
+        for a, b in ((8192, T), (8100, 8300)):                            # other rows in the same and in other products
+            part = linear_log_probs(x[a:b], w, y[a:b], top_k=top)
+            assert torch.equal(part.top_ids, out.top_ids[a:b]) and torch.equal(part.log_probs, out.log_probs[a:b])
+    assert _lib.load().swx_device_wait_status() == _lib.SWX_OK
