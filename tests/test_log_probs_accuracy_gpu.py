@@ -299,3 +299,34 @@ def test_gradients_of_wide_bf16_rows():
     want = torch.autograd.grad(torch.log_softmax(xd @ wd.t(), 1).gather(1, y[:, None]).sum(), (xd, wd))
     for a, b in zip(got, want):
         assert float((a.double() - b).norm()) <= 2.0 ** -7 * float(b.norm())
+
+
+@pytest.mark.parametrize("T,V,d,dtype,temp", [(300, 5001, 1024, BF, 1.0), (8, 5001, 1024, BF, 1.0), (1, 50001, 1024, BF, 1.0), (300, 300, 256, BF, 0.7), (200, 2000, 1024, FP, 1.0),
+                                              (600, 5001, 2048, BF, 0.5)])
+def test_values_in_the_mean_square(T, V, d, dtype, temp):
+    """With n additions of a sum: the mean cut is made up for to 0.06 2^-24 n of a logit's distance from the mean logit, each logit is rounded by
+    0.2 2^-24 n of the logits' standard deviation in the mean square (measured: 0.13 to 0.18), and a value by 2^-23 of 1 and itself."""
+    g = torch.Generator(device=DEV).manual_seed(T)
+    x = torch.randn(T, d, generator=g, device=DEV).to(dtype)
+    w = (torch.randn(V, d, generator=g, device=DEV) * 2 / d ** 0.5).to(dtype)
+    y = torch.randint(0, V, (T,), generator=g, device=DEV)
+    z = x.double() @ w.double().t() / temp
+    l = torch.log_softmax(z, 1)
+    p = l.exp()
+    H = -(p * l).sum(1)
+    mean = (p * z).sum(1, keepdim=True)
+    n = 4 * _cut(d, dtype)                                                # 2^-24 for each addition
+    rms = lambda t: float(t.square().mean().sqrt())  # noqa: E731
+    rounded = 0.2 * n * float(z.std()) * 2 ** 0.5
+    out = linear_log_probs(x, w, y, top_k=20, temperature=temp)
+    lp, zy = l.gather(1, y[:, None]), z.gather(1, y[:, None])
+    bound = 0.06 * n * rms(zy - mean) + rounded + 2.0 ** -23 * rms(1 + lp.abs())
+    assert rms(out.log_probs.double() - lp[:, 0]) <= bound
+    ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :20]
+    assert torch.equal(out.top_ids, ids)
+    vals = l.gather(1, ids)
+    bound = 0.06 * n * rms(z.gather(1, ids) - mean) + rounded + 2.0 ** -23 * rms(1 + vals.abs())
+    assert rms(out.top_log_probs.double() - vals) <= bound
+    var = (p * (z - mean).square()).sum(1)
+    bound = 0.06 * n * rms(var) + rounded * rms((p * (l + H[:, None])).square().sum(1).sqrt()) + 2.0 ** -23 * rms(1 + H)
+    assert rms(out.entropy.double() - H) <= bound
