@@ -292,7 +292,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
     __shared__ int count[2], ncand, nlist, nexact, owners[THREADS];
     __shared__ uint32_t scratch[THREADS + 1];
     __shared__ Score part[THREADS / 32];
-    __shared__ float norms[THREADS / 32];
+    __shared__ float norms[THREADS / 32], logsum;
     __shared__ float2 dots[sizeof(T) == 2 ? THREADS / 32 * score_block(THREADS) : 1];
     const int64_t row = blockIdx.x;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -322,7 +322,10 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
         if (lane == 0) norms[warp] = xx;
     }
     const Score a = score_join_row<THREADS>(p.score + row * p.np, p.np, p.k2, part);
-    if (threadIdx.x == 0) score_finish(p, row, a);
+    if (threadIdx.x == 0) {
+        score_finish(p, row, a);
+        logsum = logf(a.s);
+    }
     if (p.target[row] == p.ignore) {                                 // a token that does not count
         for (int i = threadIdx.x; i < p.top; i += THREADS) {
             p.top_log_probs[row * p.top + i] = 0.f;
@@ -424,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 3 : 0) score_top_ker
     const int ne = nexact;
     // the first alternative has the statistics' maximum (its own sum, with other roundings, would put its probability above 1, by a part of
     // |z| / temperature), and the others their distance from the first
-    const float ls = logf(a.s);
+    const float ls = logsum;
     auto write = [&](auto z) {
         for (int i = threadIdx.x; i < p.top; i += THREADS) {
             p.top_log_probs[row * p.top + i] = (float)((z(kept[i]) - z(kept[0])) * p.exact_k2) * LN2 - ls;
