@@ -472,8 +472,13 @@ int swx_xent_bwd(const swx_xent_args* args, void* stream);
  * Operands as for swx_xent_args.  A target equal to ignore_index: zeros, and -1 for each top_ids; one
  * outside [0, vocab): its log probability, and the gradients that it enters, NaN.  A row with a NaN or +inf
  * logit, or with nothing but -inf, has NaN values and gradients.  The
- * statistics are fp32; the alternatives are ordered by products in fp64 of the operands, so that
- * neither their order nor their ties depend on the rounding of sums.
+ * statistics are fp32 and relative to the row's largest logit: log probabilities are at most 0 and entropies at least 0
+ * at any temperature.  The alternatives are ordered by products of the operands good to 2^-45 of their magnitudes
+ * (fp32 operands: summed in fp64), so that rounding changes neither their order nor their ties, among the top_k + 4
+ * or more words with the largest fp32 products (where more words than that differ by a rounding of those, others of
+ * them may be missing); their l are the first one's, of the statistics' largest logit, and the distances from it.  The
+ * tensor cores' additions cut off: the exponents' scale makes up for the mean of that, 0.23 2^-24 of the logits for each 16
+ * terms (8192 at a time), which swx_xent_fwd does not; where a sum lost nothing its logit is too large by as much.
  * Forward writes row_max (the largest z) and row_sum (the sum of exp((z - row_max) / temperature); tokens values, both or
  * neither) for the backward.
  * Backward: d_log_probs, d_entropy (tokens values; either may be NULL: zero), entropy as the forward

@@ -132,8 +132,9 @@ double few_additions(int64_t d) {
 static int few_smem(int64_t d) { return 8 * (int)(4 * ((d + 31) / 32) + 4) * 16; }
 
 // CTAs of the kernel for these sizes (each leaves one statistic of a token); 0: not taken.
-// bf16 rows up to 8 tokens whose values fit in shared memory beside other CTAs': 1 and 8 tokens of 50001 x 1024 take 24 and 27 us (the
-// whole call, the weight out of the L2), 29 on 256-row tiles.  A vocabulary of 2048 and less is a few tiles there.
+// bf16 rows up to 8 tokens whose values fit in shared memory beside other CTAs': 1 and 8 tokens of 50001 x 1024 take 24 and 28 us without
+// alternatives and 32 and 34 with 5 (both kernels in a graph, the weight not in the L2; called eagerly 3 more), 9 tokens on 256-row
+// tiles 34 and 43.  A vocabulary of 2048 and less is a few tiles there.
 int score_few_ctas(const HeadOps& o) {
     if (o.dtype != SWX_DTYPE_BF16 || o.T > 8 || o.V <= 2048 || few_smem(o.d) > 72 * 1024) return 0;
     const int per_sm = std::min(SF_PER_SM, (200 * 1024) / (few_smem(o.d) + 6 * 1024));

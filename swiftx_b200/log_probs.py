@@ -104,16 +104,19 @@ def linear_log_probs(x, weight, targets, top_k=0, temperature=1.0, ignore_index=
     softmax, and its top_k largest alternatives, without the logits (CUDA only).  Returns ``LogProbs``.
 
     x (..., d), weight (vocab, d), targets (...) int64, weight16 and autocast as for ``linear_cross_entropy``; top_k up to
-    128.  log_probs and entropy are differentiable in x and weight (a gradient of one alone may be asked for);
+    128.  log_probs (at most 0) and entropy are differentiable in x and weight (a gradient of one alone may be asked for);
     the alternatives are not.  Ignored tokens: zeros, ids of -1 and no gradient, whatever x holds there as long as it is
-    finite.  Alternatives are in falling order, the lowest word first among equals; they are ordered by fp64
-    products of the operands, so that rounding changes neither their order nor their ties (among the top_k + 4 or more words
-    with the largest fp32 products: where more words than that differ by a rounding of those, others of them may be missing).
+    finite.  Alternatives are in falling order, the lowest word first among equals; they are ordered by products of the
+    operands good to 2^-45 of their magnitudes (fp32 operands: summed in fp64), so that rounding changes neither
+    their order nor their ties (among the top_k + 4 or more words with the largest fp32 products: where more words than that
+    differ by a rounding of those, others of them may be missing).
 
-    bf16 operands: products summed in fp32 in the tensor cores (8192 terms at a time), the logits' gradient rounded to bf16 once
-    for its products.  The tensor cores' additions cut off; the exponents' scale makes up for the mean of that, 2^-26 of the logits for
-    each 16 terms, which the loss does not (sums that lose nothing, as of one-hot rows, are too large by as much, 9e-7 at a width of 1024).  fp32 operands keep fp32 accuracy and have to be finite.  A target outside [0, vocab) other than
-    ignore_index gives NaN, and so does a row with a NaN or +inf logit, or with nothing but -inf.  Dual numbers are refused, torch.jit.trace records a Python operator.  Deterministic."""
+    bf16 operands: products summed in fp32 in the tensor cores (8192 terms at a time), the logits' gradient rounded to bf16
+    once for its products.  The tensor cores' additions cut off; the exponents' scale makes up for the mean of that,
+    0.23 2^-24 of the logits for each 16 terms, which the loss does not do (a sum that loses nothing, as a one-hot row's, comes out too
+    large by as much, 9e-7 at a width of 1024).  fp32 operands keep fp32 accuracy and have to be finite.  A target outside
+    [0, vocab) other than ignore_index gives NaN, and so does a row with a NaN or +inf logit, or with nothing but -inf.  Dual
+    numbers are refused, torch.jit.trace records a Python operator.  Deterministic."""
     x = check_head("linear_log_probs", x, weight, targets, weight16)
     check_top("linear_log_probs", top_k, weight.shape[0])
     check_temperature("linear_log_probs", temperature)
