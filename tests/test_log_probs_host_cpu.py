@@ -176,3 +176,15 @@ def test_generation_refuses_before_it_consumes_the_prompt(k, error, monkeypatch)
             model.generate(torch.zeros(1, 5, dtype=torch.int64), new, log_probs=k)
     assert not steps
     assert model.generate(torch.zeros(1, 5, dtype=torch.int64), 2).shape == (1, 7)
+
+
+def test_few_rows_backward_has_room_for_its_statistics():
+    """Up to 8 bf16 rows of a large vocabulary: statistics of 128 logits each, which the forward's other products do not give."""
+    lib = _lib.load()
+    a = _score(T=8, V=5001, d=64)
+    b = _distill(T=8, V=5001, d=64)                                              # the same products without them
+    assert lib.swx_logprob_bwd_workspace_bytes(a) - lib.swx_distill_bwd_workspace_bytes(b) >= 8 * 2 * 20 * 16 + 5 * 8 * 4
+    assert lib.swx_logprob_bwd_workspace_bytes(_score(T=9, V=5001, d=64)) == lib.swx_distill_bwd_workspace_bytes(_distill(T=9, V=5001, d=64))
+    a.targets = a.row_max = a.row_sum = a.dx = a.workspace = 4096
+    a.workspace_bytes = lib.swx_logprob_bwd_workspace_bytes(a) - 1
+    assert lib.swx_logprob_bwd(a, None) == INVALID
